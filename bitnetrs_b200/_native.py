@@ -68,6 +68,13 @@ class Weights(C.Structure):
     ]
 
 
+class KvPages(C.Structure):
+    """bitnet_cuda_kv_pages."""
+
+    _fields_ = [("pool", vp), ("page_table", vp), ("pages", sz), ("seqs", sz), ("pages_per_seq", sz),
+                ("kv_heads", sz), ("head_dim", sz), ("kv_dtype", C.c_int32)]
+
+
 # name: (restype, [argtypes])
 _CUDA_SIGS = {
     "bitnet_cuda_create": (i32, [u32, C.POINTER(vp)]),
@@ -131,6 +138,16 @@ _CUDA_SIGS = {
     "bitnet_cuda_model_kernel_times": (i32, [vp, vp, vp]),
     "bitnet_cuda_model_set_fused_decode": (i32, [vp, i32]),
     "bitnet_cuda_kernel_launches": (u64, [vp]),
+    "bitnet_cuda_kv_block_bytes": (i32, [i32, sz, C.POINTER(sz)]),
+    "bitnet_cuda_kv_layer_pages": (i32, [vp, sz, C.POINTER(KvPages)]),
+    "bitnet_cuda_kv_store_device": (i32, [vp, C.POINTER(KvPages), vp, sz, vp, sz, i32, sz, vp, vp, vp, vp, sz, vp,
+                                          vp]),
+    "bitnet_cuda_kv_load_device": (i32, [vp, C.POINTER(KvPages), sz, vp, vp, vp, sz, vp, sz, i32, vp, vp]),
+    "bitnet_cuda_kv_attention_workspace": (i32, [C.POINTER(KvPages), sz, C.POINTER(sz)]),
+    "bitnet_cuda_kv_attention_device": (i32, [vp, C.POINTER(KvPages), vp, sz, i32, sz, sz, vp, vp, sz, vp, sz, vp, vp,
+                                              sz, vp, vp]),
+    "bitnet_cuda_kv_prompt_attention_device": (i32, [vp, C.POINTER(KvPages), vp, sz, i32, sz, sz, sz, vp, vp, vp, sz,
+                                                     vp, sz, vp, vp, sz, vp, vp]),
 }
 
 _SYNTH_SIGS = {

@@ -159,6 +159,7 @@ void launch_rope_apply(const float* qk, int nh, int nkv, int hd, const float* co
 struct KvGeom {
   void* pool = nullptr;       // [layers][pages][kv_heads][2][16][hd]
   int bf16 = 1;               // element type
+  int quant = 0;              // BITNET_KV_I8 or BITNET_KV_I4: blocks of codes instead (kvq.cuh; bf16 is then 0)
   int pages = 0, kv_heads = 0, hd = 0, layers = 0;
   int max_pages_per_seq = 0;  // page table row length
 };
@@ -236,6 +237,9 @@ void launch_flash_decode_mma(const float* q, int T, int nh, const int32_t* tok_p
 // Fill positions [0, n) of sequence `seq` (all layers) with seeded N(0,1).
 void launch_kv_fill_random(const KvGeom& kv, const int32_t* page_row, int n, uint64_t seed, uint32_t seq,
                            cudaStream_t st);
+// The same draws of one layer as f32 rows [n][kv_heads*hd] of K and of V (for the quantised cache).
+void launch_kv_draw_rows(int kv_heads, int hd, int layer, int n, uint64_t seed, uint32_t seq, float* k, float* v,
+                         cudaStream_t st);
 // Copy positions [0,n) between a host-layout staging buffer [layer][pos][kvh*hd] (f32) and the cache.
 void launch_kv_copy(const KvGeom& kv, const int32_t* page_row, int n, float* k_stage, float* v_stage, bool to_cache,
                     cudaStream_t st);

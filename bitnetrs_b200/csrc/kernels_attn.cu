@@ -908,11 +908,24 @@ __device__ __forceinline__ uint64_t mix64(uint64_t z) {
   return z ^ (z >> 31);
 }
 
+// Same draws as synth_kv_normal: single-precision Box-Muller on one 64-bit
+// draw per element pair (cosine branch -> even element, sine -> odd).
+__device__ __forceinline__ float2 kv_draw_pair(uint64_t seed, uint32_t seq, int layer, int kind, int kvh, int pos,
+                                               int hd, int j) {
+  uint64_t key = mix64(seed ^ mix64(((uint64_t)seq << 40) ^ ((uint64_t)layer << 24) ^ ((uint64_t)kind << 20) ^
+                                     ((uint64_t)kvh << 16) ^ 0x5eedULL));
+  uint64_t pair = ((uint64_t)pos * hd) / 2 + j;
+  uint64_t a = mix64(key + pair * 0x9e3779b97f4a7c15ULL);
+  float u1 = (float)((a >> 40) + 1) * (1.0f / 16777216.0f);
+  float u2 = (float)(a & 0xffffffu) * (1.0f / 16777216.0f);
+  float r = sqrtf(__fmul_rn(-2.0f, logf(u1)));
+  float t = __fmul_rn(6.28318530717958647692f, u2);
+  return make_float2(__fmul_rn(r, cosf(t)), __fmul_rn(r, sinf(t)));
+}
+
 __global__ void kv_fill_random_kernel(KvGeom g, const int32_t* __restrict__ page_row, int n, uint64_t seed,
                                       uint32_t seq) {
   // One block per (position, layer); threads over (kv_head, kind, element pair).
-  // Same draws as synth_kv_normal: single-precision Box-Muller on one 64-bit
-  // draw per element pair (cosine branch -> even element, sine -> odd).
   const int layer = blockIdx.y, pos = blockIdx.x;
   if (pos >= n) return;
   const int page = page_row[pos / kPage], slot = pos % kPage;
@@ -920,18 +933,30 @@ __global__ void kv_fill_random_kernel(KvGeom g, const int32_t* __restrict__ page
   const int per = g.kv_heads * 2 * half;
   for (int i = threadIdx.x; i < per; i += blockDim.x) {
     int kvh = i / (2 * half), kind = (i / half) % 2, j = i % half;
-    uint64_t key = mix64(seed ^ mix64(((uint64_t)seq << 40) ^ ((uint64_t)layer << 24) ^ ((uint64_t)kind << 20) ^
-                                       ((uint64_t)kvh << 16) ^ 0x5eedULL));
-    uint64_t pair = ((uint64_t)pos * g.hd) / 2 + j;
-    uint64_t a = mix64(key + pair * 0x9e3779b97f4a7c15ULL);
-    float u1 = (float)((a >> 40) + 1) * (1.0f / 16777216.0f);
-    float u2 = (float)(a & 0xffffffu) * (1.0f / 16777216.0f);
-    float r = sqrtf(__fmul_rn(-2.0f, logf(u1)));
-    float t = __fmul_rn(6.28318530717958647692f, u2);
+    const float2 x = kv_draw_pair(seed, seq, layer, kind, kvh, pos, g.hd, j);
     size_t off = kv_off(g, layer, page, kvh, kind, slot) + 2 * j;
-    kv_store(g, off, __fmul_rn(r, cosf(t)));
-    kv_store(g, off + 1, __fmul_rn(r, sinf(t)));
+    kv_store(g, off, x.x);
+    kv_store(g, off + 1, x.y);
   }
+}
+
+// The same draws of one layer as rows [n][kv_heads*hd] of K and of V.
+__global__ void kv_draw_rows_kernel(int kv_heads, int hd, int layer, uint64_t seed, uint32_t seq,
+                                    float* __restrict__ k, float* __restrict__ v) {
+  const int pos = blockIdx.x, half = hd / 2;
+  for (int i = threadIdx.x; i < kv_heads * 2 * half; i += blockDim.x) {
+    int kvh = i / (2 * half), kind = (i / half) % 2, j = i % half;
+    const float2 x = kv_draw_pair(seed, seq, layer, kind, kvh, pos, hd, j);
+    float* row = (kind ? v : k) + (size_t)pos * kv_heads * hd + kvh * hd + 2 * j;
+    row[0] = x.x;
+    row[1] = x.y;
+  }
+}
+void launch_kv_draw_rows(int kv_heads, int hd, int layer, int n, uint64_t seed, uint32_t seq, float* k, float* v,
+                         cudaStream_t st) {
+  if (n <= 0) return;
+  kv_draw_rows_kernel<<<n, 256, 0, st>>>(kv_heads, hd, layer, seed, seq, k, v);
+  count_launch();
 }
 
 void launch_kv_fill_random(const KvGeom& kv, const int32_t* page_row, int n, uint64_t seed, uint32_t seq,

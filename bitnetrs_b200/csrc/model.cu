@@ -16,6 +16,7 @@
 #include <cstring>
 
 #include "internal.h"
+#include "kvq.cuh"
 #include "tp.cuh"
 
 using namespace bitnet;
@@ -219,7 +220,8 @@ constexpr int kExactMaxTokens = 1024;
 constexpr int kSmallStepTokens = 16;
 constexpr size_t kExactMaxSmem = 200 * 1024;
 
-// Kernel choice (bitnet_cuda_model_set_numerics):
+// Kernel choice (bitnet_cuda_model_set_numerics).  A quantised cache has its
+// own store and attention kernels (kvq.cuh) in every mode; for the others:
 //  - attention feeds the next int8 quantisation, so outside FAST mode it
 //    always runs in the reference's operation order;
 //  - the lm_head feeds nothing back: AUTO runs the tensor-core kernel for
@@ -436,14 +438,47 @@ void run_forward(bitnet_cuda_model* m, bitnet_cuda_kv* kv, int T, int n_out, int
       launch_ternary_matmul(Lw.wqkv, nqkv, H, m->xq, m->ldq, m->amax, m->rowsum, T, sqkv, Epi::Store, m->qkv, nqkv,
                             nullptr, st, m->status);
     });
+    const KvqView kq = kv->g.quant ? kvq_layer(kv->g, kv->d_table, kv->max_seqs, l) : KvqView{};
     timed(m, kRopeKv, st, [&] {
+      if (kv->g.quant) {
+        KvqStore s;
+        s.q = m->qkv;
+        s.k = m->qkv + qd;
+        s.v = m->qkv + qd + kvd;
+        s.ldq = s.ldk = s.ldv = nqkv;
+        s.nh = m->nh;
+        s.q_out = m->qrot;
+        s.rows = T;
+        s.row_seq = m->tok_seq;
+        s.row_pos = m->tok_pos;
+        s.rope_cos = m->rope_cos;
+        s.rope_sin = m->rope_sin;
+        s.rope_len = (int)m->cfg.max_position_embeddings;
+        s.status = m->status;
+        launch_kvq_store(kq, s, st);
+        return;
+      }
       launch_rope_kv_store(m->qkv, nqkv, T, m->nh, m->nkv, m->hd, m->rope_cos, m->rope_sin, m->tok_pos, m->tok_seq,
                            kv->d_table, kv->g, l, m->qrot, st);
     });
     // a tensor-parallel rank writes its heads straight into its all-gather slot
     float* attn_out = m->tp ? m->tp_gath + (size_t)m->tp_rank * T * qd : m->attn;
     timed(m, kAttn, st, [&] {
-      if (use_exact_attention(m, T) && use_x4_attention(m, kv, max_ctx))
+      if (kv->g.quant) {
+        KvqRows r;
+        r.rows = T;
+        r.row_seq = m->tok_seq;
+        r.row_len = m->tok_pos;
+        r.len_bias = 1;  // a token sees its own position too
+        KvqAttend a;
+        a.q = m->qrot;
+        a.out = attn_out;
+        a.ldq = a.ldo = qd;
+        a.nh = m->nh;
+        a.status = m->status;
+        a.space = m->partial.p;
+        launch_kvq_attend(kq, r, a, max_ctx, st);
+      } else if (use_exact_attention(m, T) && use_x4_attention(m, kv, max_ctx))
         launch_attn_x4(m->qrot, T, m->nh, m->tok_pos, m->tok_seq, m->order, kv->d_table, kv->g, kv->tmap, l, max_ctx,
                        attn_out, m->partial.as<float>(), m->ctx->exp_table, m->status, st);
       else if (use_exact_attention(m, T) && use_exact3_attention(m, kv, max_ctx))
@@ -582,6 +617,7 @@ int copy_logits(bitnet_cuda_model* m, int n_out, float* dst, cudaMemcpyKind kind
 
 // Name of the attention kernel run_forward launches for T tokens (same tests).
 const char* attention_kernel_name(const bitnet_cuda_model* m, const bitnet_cuda_kv* kv, int T, int max_ctx) {
+  if (kv->g.quant) return kvq_attend_kernel_name(kvq_layer(kv->g, kv->d_table, kv->max_seqs, 0), m->nh);
   if (use_decode1(m, kv, T, max_ctx)) return "decode1_kernel";
   if (use_exact_attention(m, T) && use_x4_attention(m, kv, max_ctx)) return "attn_qk_softmax_kernel+attn_pv_kernel";
   if (use_exact_attention(m, T) && use_exact3_attention(m, kv, max_ctx)) return "paged_attention_exact3_kernel";
@@ -684,6 +720,7 @@ int ensure_partial(bitnet_cuda_model* m, const bitnet_cuda_kv* kv, int T, int ma
                       : (use_mma_attention(m, kv, T) ? flash_decode_mma_partial_floats(T, m->nh, max_ctx)
                                                      : paged_attention_partial_floats(T, m->nh, m->hd, max_ctx));
   size_t bytes = std::max<size_t>(floats, 16) * sizeof(float);
+  if (kv->g.quant) bytes = kvq_attend_space(m->nh, m->nkv, m->hd);
   if (bytes <= m->partial.cap) return BITNET_OK;
   // captured graphs hold the old address
   BN_TRY(model_wait(m, m->ctx->stream));
@@ -1006,12 +1043,17 @@ int bitnet_cuda_kv_create(bitnet_cuda_model* m, uint32_t num_pages, uint32_t max
   if (!out || !m) return shape_error("non-null arguments", "null");
   *out = nullptr;
   if (num_pages == 0 || max_seqs == 0) return shape_error("num_pages > 0 and max_seqs > 0", "0");
-  if (kv_dtype != BITNET_KV_F32 && kv_dtype != BITNET_KV_BF16) return config_error("kv_dtype must be F32 or BF16");
+  const bool quant = kv_dtype == BITNET_KV_I8 || kv_dtype == BITNET_KV_I4;
+  if (kv_dtype != BITNET_KV_F32 && kv_dtype != BITNET_KV_BF16 && !quant)
+    return config_error("kv_dtype must be F32, BF16, I8 or I4");
+  if (quant && (m->hd % 2 != 0 || m->hd > kKvqMaxHd))
+    return config_error("a quantised cache takes an even head_dim of at most " + sz(kKvqMaxHd) + ", got " + sz(m->hd));
   std::lock_guard<std::mutex> lk(m->ctx->mu);
   cudaSetDevice(m->ctx->device);
   auto* kv = new bitnet_cuda_kv();
   kv->model = m;
   kv->g.bf16 = kv_dtype == BITNET_KV_BF16;
+  kv->g.quant = quant ? kv_dtype : 0;
   kv->g.pages = (int)num_pages;
   kv->g.kv_heads = m->nkv;
   kv->g.hd = m->hd;
@@ -1019,7 +1061,8 @@ int bitnet_cuda_kv_create(bitnet_cuda_model* m, uint32_t num_pages, uint32_t max
   kv->g.max_pages_per_seq = (int)ceil_div(m->cfg.max_position_embeddings, kPage);
   kv->max_seqs = (int)max_seqs;
   size_t elem = kv->g.bf16 ? 2 : 4;
-  size_t bytes = (size_t)m->L * num_pages * m->nkv * 2 * kPage * m->hd * elem;
+  const size_t block = quant ? (size_t)kvq_block_bytes(m->hd, kv_dtype == BITNET_KV_I4) : 2 * kPage * m->hd * elem;
+  size_t bytes = (size_t)m->L * num_pages * m->nkv * block;
   cudaError_t e = cudaMalloc(&kv->g.pool, bytes);
   if (e != cudaSuccess) {
     delete kv;
@@ -1084,11 +1127,61 @@ int bitnet_cuda_kv_free_pages(bitnet_cuda_kv* kv, size_t* n) {
   return BITNET_OK;
 }
 
+int bitnet_cuda_kv_layer_pages(bitnet_cuda_kv* kv, size_t layer, bitnet_cuda_kv_pages* out) {
+  if (!kv || !out) return shape_error("non-null kv and out", "null");
+  if (!kv->g.quant) return config_error("the cache's kv_dtype must be I8 or I4");
+  if (layer >= (size_t)kv->g.layers) return shape_error("layer < " + sz(kv->g.layers), sz(layer));
+  const KvqView c = kvq_layer(kv->g, kv->d_table, kv->max_seqs, (int)layer);
+  out->pool = c.pool;
+  out->page_table = c.table;
+  out->pages = c.pages;
+  out->seqs = c.seqs;
+  out->pages_per_seq = c.per_seq;
+  out->kv_heads = c.kv_heads;
+  out->head_dim = c.hd;
+  out->kv_dtype = kv->g.quant;
+  return BITNET_OK;
+}
+
 int bitnet_cuda_kv_seq_reserve(bitnet_cuda_kv* kv, uint32_t seq, size_t len) {
   if (seq >= (uint32_t)kv->max_seqs) return shape_error("seq < max_seqs", sz(seq));
   std::lock_guard<std::mutex> lk(kv->model->ctx->mu);
   cudaSetDevice(kv->model->ctx->device);
   return kv_reserve(kv, seq, len, kv->model->ctx->stream);
+}
+
+// Positions [0, n) of one sequence of a quantised cache: quantised from, or read
+// back to, rows [layer][pos][kvd] of f32.
+static int kvq_seq_copy(bitnet_cuda_kv* kv, uint32_t seq, size_t n, const float* k, float* kout, const float* v,
+                        float* vout, bool to_cache) {
+  bitnet_cuda_model* m = kv->model;
+  cudaStream_t st = m->ctx->stream;
+  const size_t rows = n * m->kvd;  // elements of one layer
+  DevBuf ks, vs;
+  BN_TRY(ks.ensure(rows * 4));
+  BN_TRY(vs.ensure(rows * 4));
+  for (int l = 0; l < m->L; ++l) {
+    const KvqView c = kvq_layer(kv->g, kv->d_table + (size_t)seq * kv->g.max_pages_per_seq, 1, l);
+    if (to_cache) {
+      BN_CUDA(cudaMemcpyAsync(ks.p, k + l * rows, rows * 4, cudaMemcpyHostToDevice, st));
+      BN_CUDA(cudaMemcpyAsync(vs.p, v + l * rows, rows * 4, cudaMemcpyHostToDevice, st));
+      KvqStore s;
+      s.k = ks.p;
+      s.v = vs.p;
+      s.ldk = s.ldv = m->kvd;
+      s.rows = (int)n;
+      s.status = m->status;
+      launch_kvq_store(c, s, st);
+    } else {
+      launch_kvq_load(c, (int)n, nullptr, nullptr, ks.p, m->kvd, vs.p, m->kvd, 0, m->status, st);
+      BN_CUDA(cudaMemcpyAsync(kout + l * rows, ks.p, rows * 4, cudaMemcpyDeviceToHost, st));
+      BN_CUDA(cudaMemcpyAsync(vout + l * rows, vs.p, rows * 4, cudaMemcpyDeviceToHost, st));
+    }
+  }
+  BN_CUDA(cudaGetLastError());
+  BN_TRY(check_status(m));  // synchronises; a non-finite row is an error here
+  if (to_cache) kv->seq_len[seq] = n;
+  return BITNET_OK;
 }
 
 static int kv_seq_copy(bitnet_cuda_kv* kv, uint32_t seq, size_t n, const float* k, float* kout, const float* v,
@@ -1104,6 +1197,7 @@ static int kv_seq_copy(bitnet_cuda_kv* kv, uint32_t seq, size_t n, const float* 
     if (to_cache) kv->seq_len[seq] = 0;
     return BITNET_OK;
   }
+  if (kv->g.quant) return kvq_seq_copy(kv, seq, n, k, kout, v, vout, to_cache);
   size_t elems = (size_t)m->L * n * m->kvd;
   DevBuf ks, vs;
   BN_TRY(ks.ensure(elems * 4));
@@ -1139,6 +1233,26 @@ int bitnet_cuda_kv_seq_fill_random(bitnet_cuda_kv* kv, uint32_t seq, size_t n, u
   cudaSetDevice(m->ctx->device);
   cudaStream_t st = m->ctx->stream;
   BN_TRY(kv_reserve(kv, seq, n, st));
+  if (kv->g.quant) {
+    const size_t rows = n * m->kvd;
+    DevBuf ks, vs;
+    BN_TRY(ks.ensure(std::max<size_t>(rows, 4) * 4));
+    BN_TRY(vs.ensure(std::max<size_t>(rows, 4) * 4));
+    for (int l = 0; l < m->L; ++l) {
+      launch_kv_draw_rows(m->nkv, m->hd, l, (int)n, seed, seq, ks.as<float>(), vs.as<float>(), st);
+      KvqStore s;
+      s.k = ks.p;
+      s.v = vs.p;
+      s.ldk = s.ldv = m->kvd;
+      s.rows = (int)n;
+      s.status = m->status;
+      launch_kvq_store(kvq_layer(kv->g, kv->d_table + (size_t)seq * kv->g.max_pages_per_seq, 1, l), s, st);
+    }
+    BN_CUDA(cudaGetLastError());
+    BN_TRY(check_status(m));
+    kv->seq_len[seq] = n;
+    return BITNET_OK;
+  }
   launch_kv_fill_random(kv->g, kv->d_table + (size_t)seq * kv->g.max_pages_per_seq, (int)n, seed, seq, st);
   BN_CUDA(cudaGetLastError());
   BN_CUDA(cudaStreamSynchronize(st));

@@ -314,7 +314,8 @@ class BitNetModel:
 
 
 class KVCache:
-    """Paged KV cache: ``num_pages`` pages of 16 positions (all layers) shared by ``max_seqs`` sequences."""
+    """Paged KV cache: ``num_pages`` pages of 16 positions (all layers) shared by ``max_seqs`` sequences.
+    ``kv_dtype`` is KV_F32, KV_BF16, or a quantised type of :mod:`bitnetrs_b200.paged` (KV_I8, KV_I4)."""
 
     def __init__(self, model: BitNetModel, num_pages: int, max_seqs: int = 1, kv_dtype: int = KV_F32):
         self.model = model

@@ -347,9 +347,15 @@ int bitnet_cuda_lm_head_i8_table(const uint16_t* embed_bf16, size_t rows, size_t
 
 #define BITNET_KV_F32 0  /* the reference KVCache element type (model/src/lib.rs:118-169) */
 #define BITNET_KV_BF16 1 /* paged bf16 cache */
+#define BITNET_KV_I8 2   /* paged cache of 8-bit codes with a scale a row and head (see bitnet_cuda_kv_pages) */
+#define BITNET_KV_I4 3   /* paged cache of 4-bit codes with a scale and a zero a row and head */
 
 /* Paged KV cache (replaces KVCache, model/src/lib.rs:118-315): num_pages pages
- * of 16 positions x all layers, shared by up to max_seqs sequences. */
+ * of 16 positions x all layers, shared by up to max_seqs sequences.  The
+ * quantised types (no counterpart in the reference) take an even head_dim of
+ * at most 256; attention over them runs split over the context in f32
+ * accuracy under every numerics mode (the reference's operation order is
+ * defined by its unquantised cache). */
 int bitnet_cuda_kv_create(bitnet_cuda_model* model, uint32_t num_pages, uint32_t max_seqs, int kv_dtype,
                           bitnet_cuda_kv** out);
 void bitnet_cuda_kv_destroy(bitnet_cuda_kv* kv);
@@ -459,6 +465,98 @@ int bitnet_cuda_model_check(bitnet_cuda_model* model);
  * mode, for contexts up to the cache's capacity. */
 int bitnet_cuda_model_attention_kernel(bitnet_cuda_model* model, bitnet_cuda_kv* kv, uint32_t tokens, char* name,
                                        size_t name_len);
+
+/* ===================================================================== */
+/* Quantised paged KV cache on the device (no counterpart in the reference) */
+/* ===================================================================== */
+
+/* A paged cache of quantised keys and values in the caller's device memory,
+ * or one layer of a model's (bitnet_cuda_kv_layer_pages).  A page holds 16
+ * positions; page_table[s * pages_per_seq + j] names the page of positions
+ * [16j, 16j + 16) of sequence s.  The pool is [pages][kv_heads] blocks of
+ * bitnet_cuda_kv_block_bytes, each:
+ *   K codes [16][head_dim], V codes [16][head_dim], K parameters, V parameters.
+ * I8: code c in [-127, 127], one byte; parameters scale[16].  A row x has
+ *   scale = max|x| / 127 rounded to f32, c = x / scale to the nearest (ties
+ *   to even), value c * scale.
+ * I4: code c in [0, 15], two a byte (dimension 2j in the low half of byte j);
+ *   parameters scale[16], zero[16].  zero = min x, scale = (max x - zero) / 15,
+ *   both rounded to f32, c = (x - zero) / scale to the nearest (ties to even),
+ *   value zero + c * scale.
+ * Codes are the exact nearest ones.  A row that holds a NaN or an infinity
+ * reads back as NaN.
+ *
+ * The entry points below take device addresses, return without synchronising
+ * and can be captured into a graph.  They leave the calling thread's current
+ * device as it was.  What the host cannot see is checked on the device: a
+ * sequence, position, length or page outside the cache is not accessed, and
+ * sets a bit of *status (device int32, which the caller zeroes and reads):
+ * BITNET_STATUS_NON_FINITE or BITNET_STATUS_BAD_CONTEXT. */
+#define BITNET_STATUS_NON_FINITE 1
+#define BITNET_STATUS_BAD_CONTEXT 4
+typedef struct {
+  void* pool;                /* 16-byte aligned */
+  const int32_t* page_table; /* [seqs][pages_per_seq] */
+  size_t pages, seqs, pages_per_seq;
+  size_t kv_heads, head_dim; /* head_dim even, at most 256 */
+  int32_t kv_dtype;          /* BITNET_KV_I8 or BITNET_KV_I4 */
+} bitnet_cuda_kv_pages;
+
+int bitnet_cuda_kv_block_bytes(int kv_dtype, size_t head_dim, size_t* bytes);
+/* One layer of a model's cache.  The description stays valid as long as the
+ * cache; its page table follows the cache's sequences. */
+int bitnet_cuda_kv_layer_pages(bitnet_cuda_kv* kv, size_t layer, bitnet_cuda_kv_pages* out);
+
+/* Quantise rows of K and V into the cache: row r (kv_heads * head_dim
+ * elements of f32, or bf16 when x_is_bf16 != 0, at k + r * ldk and v + r * ldv)
+ * becomes position row_pos[r] of sequence row_seq[r].  Rows with a negative
+ * position are padding and skipped; two rows of one call must not name the
+ * same position (its slot would then hold a mixture).  With rope_cos and
+ * rope_sin (f32 [rope_len][head_dim / 2], both or neither) K is rotated
+ * first as in bitnet_cuda_rope_embed, in 64 bits. */
+int bitnet_cuda_kv_store_device(bitnet_cuda_ctx* ctx, const bitnet_cuda_kv_pages* cache, const void* k, size_t ldk,
+                                const void* v, size_t ldv, int x_is_bf16, size_t rows, const int32_t* row_seq,
+                                const int32_t* row_pos, const float* rope_cos, const float* rope_sin,
+                                size_t rope_len, int32_t* status, void* stream);
+
+/* Read rows back, to f32 or (out_is_bf16 != 0) bf16: the inverse of the store.
+ * Rows with a negative position are left as they were. */
+int bitnet_cuda_kv_load_device(bitnet_cuda_ctx* ctx, const bitnet_cuda_kv_pages* cache, size_t rows,
+                               const int32_t* row_seq, const int32_t* row_pos, void* k, size_t ldk, void* v,
+                               size_t ldv, int out_is_bf16, int32_t* status, void* stream);
+
+/* Bytes of device memory that one attention call needs as its workspace (16-byte
+ * aligned, contents of no matter before and after).  It depends on the heads
+ * alone.  Calls that may overlap in time, replays of captured graphs among
+ * them, need workspaces of their own. */
+int bitnet_cuda_kv_attention_workspace(const bitnet_cuda_kv_pages* cache, size_t n_heads, size_t* bytes);
+
+/* Attention of single tokens, GQA: row r (n_heads * head_dim elements, rotated)
+ * attends to the first row_len[r] positions of sequence row_seq[r]:
+ *   out = sum_j softmax_j(q . k_j / sqrt(head_dim)) v_j,
+ *   lse[r][h] = log sum_j exp(q . k_j / sqrt(head_dim))   (optional, f32 [rows][n_heads]).
+ * A row of length 0 (or less) gives zeros and -inf.  Several rows may name one
+ * sequence.  No length may exceed max_len (a longer one is cut there and sets
+ * the status).  Scores, softmax and sums are held to f32 accuracy; with bf16
+ * q and out (x_is_bf16 != 0) only the output is rounded.  The context is split
+ * over the GPU by the lengths alone, so equal lengths give equal bits. */
+int bitnet_cuda_kv_attention_device(bitnet_cuda_ctx* ctx, const bitnet_cuda_kv_pages* cache, const void* q, size_t ldq,
+                                    int x_is_bf16, size_t rows, size_t n_heads, const int32_t* row_seq,
+                                    const int32_t* row_len, size_t max_len, void* out, size_t ldo, float* lse,
+                                    void* workspace, size_t workspace_bytes, int32_t* status, void* stream);
+
+/* Causal attention of prompts, or parts of prompts, whose K and V are already in
+ * the cache: rows [cu_rows[i], cu_rows[i + 1]) are the positions starts[i],
+ * starts[i] + 1, ... of sequence seq_ids[i] (device int32 arrays of n_seqs + 1,
+ * n_seqs and n_seqs; cu_rows does not decrease and stays within `rows`), and
+ * each attends to the positions up to its own.  Rows outside every range are
+ * left as they were.  max_len bounds starts[i] + the rows of i.  The rest is as
+ * above. */
+int bitnet_cuda_kv_prompt_attention_device(bitnet_cuda_ctx* ctx, const bitnet_cuda_kv_pages* cache, const void* q,
+                                           size_t ldq, int x_is_bf16, size_t rows, size_t n_heads, size_t n_seqs,
+                                           const int32_t* seq_ids, const int32_t* cu_rows, const int32_t* starts,
+                                           size_t max_len, void* out, size_t ldo, float* lse, void* workspace,
+                                           size_t workspace_bytes, int32_t* status, void* stream);
 
 /* Number of kernels this library launched on the context (all entry points,
  * graph-launched kernels included). */
