@@ -345,7 +345,7 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
   int r = found[0];
   long long base = base_sh;
   const float qscale = __fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)hd));
-  while (at < end) {
+  while (at < end && r < R.rows) {
     int seq = 0;
     const int len = row_context(c, R, r, max_len, &seq, a.status);
     const int pages = len > 0 ? (len + kPage - 1) / kPage : 0;
@@ -460,9 +460,532 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
   }
 }
 
+// ---------------------------------------------------------------------------
+// The tensor-core form, for head sizes of 64, 96 and 128 (I4: 64, 128).
+//
+// One warp multiplies one page at a time: the 16 positions of a page are the M
+// of an m16n8k16 product with fp16 operands and f32 sums, and the N are columns
+// (head, term).  Codes are exact in fp16.  q and the weights are not, so each
+// is the sum of two fp16 terms (22 bits), in neighbouring columns: four heads
+// fill the eight columns, and a lane's pair of sums belongs to one head.
+//   S[pos][head] = K codes . q      A = K, B = q (kept in registers)
+//   O[dim][head] += V codes^T . w   A = V^T, B = w (transposed by movmatrix)
+// The scale of a K row multiplies its score; the scale of a V row its weight
+// before that is split.  With I4 codes c - 8 are multiplied, and the rest of
+// a value, zero + 8 scale, enters as a sum of its own.
+// q is multiplied by a power of two a head so that its largest element is
+// near 2^14, the weights by one a warp so that the largest scale of V seen is
+// near 2^11 (rescaled like the maximum when a larger one comes): the second
+// terms then keep 2^-39 of the largest value.
+//
+// The order of dimensions inside a product is free, so a lane fetches
+// contiguous bytes of a row for its K operand (HD/4 codes of two rows) and its
+// V operand (HD/8 codes of four rows).  They come by cp.async into a ring that
+// only the same lane reads, so a warp waits for its own copies alone.
+// ---------------------------------------------------------------------------
+constexpr int kMmaWarps = 8;
+
+template <int HD, bool I4>
+struct MmaTile {
+  static constexpr int kRow = I4 ? HD / 2 : HD;         // bytes of a row's codes
+  static constexpr int kKBytes = kRow / 4;              // a lane's bytes of one K row
+  static constexpr int kVBytes = kRow / 8;              // a lane's bytes of one V row
+  static constexpr int kKPiece = kKBytes % 16 == 0 ? 16 : kKBytes % 8 == 0 ? 8 : 4;
+  static constexpr int kVPiece = kVBytes % 16 == 0 ? 16 : kVBytes % 8 == 0 ? 8 : 4;
+  static constexpr int kKPieces = kKBytes / kKPiece, kVPieces = kVBytes / kVPiece;
+  static constexpr int kKStage = 2 * kKBytes * 32, kVStage = 4 * kVBytes * 32;
+  static constexpr int kParams = I4 ? 256 : 128;
+  static constexpr int kStage = kKStage + kVStage + kParams;
+  static constexpr int kStages = I4 ? 5 : 3;
+  static constexpr int kKSteps = HD / 16, kMTiles = HD / 16;
+  static constexpr int kPartStride = HD + 4;  // floats a head of a warp's partial result
+};
+
+template <int BYTES>
+__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+  else
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+}
+template <int BYTES>
+__device__ __forceinline__ void lds_piece(uint32_t addr, uint32_t* w) {
+  if constexpr (BYTES == 16)
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr)
+                 : "memory");
+  else if constexpr (BYTES == 8)
+    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
+  else
+    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[0]) : "r"(addr) : "memory");
+}
+__device__ __forceinline__ float lds_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ float f16_lo(uint32_t h) {
+  float r;
+  asm("{ .reg .f16 a, b; mov.b32 {a, b}, %1; cvt.f32.f16 %0, a; }\n" : "=f"(r) : "r"(h));
+  return r;
+}
+__device__ __forceinline__ float f16_hi(uint32_t h) {
+  float r;
+  asm("{ .reg .f16 a, b; mov.b32 {a, b}, %1; cvt.f32.f16 %0, b; }\n" : "=f"(r) : "r"(h));
+  return r;
+}
+__device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("add.rn.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+__device__ __forceinline__ float exp2_approx(float x) {  // within 2^-22
+  float r;
+  asm("ex2.approx.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+  return r;
+}
+// x as two fp16 terms, the larger in the low half.
+__device__ __forceinline__ uint32_t two_terms(float x) {
+  const uint32_t h = pack_f16(x, 0.0f);
+  return pack_f16(f16_lo(h), __fsub_rn(x, f16_lo(h)));
+}
+// Four signed bytes of w as fp16 pairs: elements (0, 2) and (1, 3).  A byte with
+// its sign flipped, below the bits of 1024, is 1152 + c.
+__device__ __forceinline__ void bytes_f16(uint32_t w, uint32_t* even, uint32_t* odd) {
+  *even = add_f16x2((w & 0x00ff00ffu) ^ 0x64806480u, 0xe480e480u);
+  *odd = add_f16x2(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u, 0xe480e480u);
+}
+// Eight nibbles of w, less 8, as fp16 pairs: x[i] = elements (i, i + 4).
+__device__ __forceinline__ void nibbles_f16(uint32_t w, uint32_t* x) {
+  const uint32_t v = w >> 8;
+  x[0] = add_f16x2((w & 0x000f000fu) | 0x64006400u, 0xe408e408u);                          // 1024 + c - 1032
+  x[1] = fma_f16x2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);            // (1024 + 16 c) / 16 - 72
+  x[2] = add_f16x2((v & 0x000f000fu) | 0x64006400u, 0xe408e408u);
+  x[3] = fma_f16x2((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
+}
+
+// The share's place in the line of pages: how long the line is, the row in
+// which the share begins and where that row's pages begin.  Every thread takes
+// a run of rows; a scan over the threads gives each its place.
+struct Place {
+  long long total, base;
+  int row;
+};
+__device__ __forceinline__ int row_pages(const KvqView& c, const KvqRows& R, int r, int max_len, int32_t* status) {
+  int seq;
+  const int len = row_context(c, R, r, max_len, &seq, status);
+  return len > 0 ? (len + kPage - 1) / kPage : 0;
+}
+template <int THREADS>
+__device__ Place find_place(const KvqView& c, const KvqRows& R, int max_len, int per_row, int shares, int min_pages,
+                            int32_t* status, long long* start, long long* end) {
+  __shared__ long long warp_sum[THREADS / 32];
+  __shared__ long long base_sh;
+  __shared__ int row_sh;
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int each = (R.rows + THREADS - 1) / THREADS;
+  const int r0 = min(tid * each, R.rows), r1 = min(r0 + each, R.rows);
+  long long mine = 0;
+  for (int r = r0; r < r1; ++r) mine += row_pages(c, R, r, max_len, status);
+  long long upto = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
+    if (lane >= o) upto += v;
+  }
+  if (lane == 31) warp_sum[warp] = upto;
+  __syncthreads();
+  long long before = 0, total = 0;
+#pragma unroll
+  for (int w = 0; w < THREADS / 32; ++w) {
+    if (w < warp) before += warp_sum[w];
+    total += warp_sum[w];
+  }
+  Place at;
+  at.total = total * per_row;
+  const long long cuts = min((long long)shares, (at.total + min_pages - 1) / min_pages);
+  const bool idle = (long long)blockIdx.x >= cuts;
+  *start = idle ? 0 : at.total * blockIdx.x / cuts;
+  *end = idle ? 0 : at.total * (blockIdx.x + 1) / cuts;
+  long long b = (before + upto - mine) * per_row;
+  if (!idle && b <= *start && *start < b + mine * per_row) {
+    for (int r = r0;; ++r) {
+      const long long n = (long long)row_pages(c, R, r, max_len, status) * per_row;
+      if (*start < b + n) {
+        row_sh = r;
+        base_sh = b;
+        break;
+      }
+      b += n;
+    }
+  }
+  __syncthreads();
+  at.row = row_sh;
+  at.base = base_sh;
+  return at;
+}
+
+template <int HD, bool I4, int NT>
+__global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
+    kvq_attend_mma_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int min_pages, int wide_q) {
+  using T = MmaTile<HD, I4>;
+  extern __shared__ __align__(128) uint8_t ring[];
+  __shared__ float ml[kMmaWarps][kMaxHeads][2];
+  pdl_launch_dependents();
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  const Units us = units_of(a.nh, c.kv_heads);
+  const int shares = gridDim.x, share = blockIdx.x;
+  ShareMeta* meta = (ShareMeta*)a.space;
+  for (int r = share; r < R.rows; r += shares) {
+    int seq;
+    if (row_context(c, R, r, max_len, &seq, a.status) == 0) write_empty_row(a, HD, r);
+  }
+  long long at, end;
+  const Place place = find_place<kMmaWarps * 32>(c, R, max_len, us.per_row, shares, min_pages, a.status, &at, &end);
+  ShareMeta note{-1, 0, 0, 0};
+  int r = place.row;
+  long long base = place.base;
+  uint8_t* const mine = ring + warp * (T::kStages * T::kStage);
+  const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
+  const float qscale = __fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)HD));
+
+  while (at < end && r < R.rows) {
+    int seq = 0;
+    const int len = row_context(c, R, r, max_len, &seq, a.status);
+    const int pages = len > 0 ? (len + kPage - 1) / kPage : 0;
+    if (at >= base + (long long)pages * us.per_row) {
+      base += (long long)pages * us.per_row;
+      ++r;
+      continue;
+    }
+    const int u = (int)((at - base) / pages), first_page = (int)((at - base) % pages);
+    const int n_pages = (int)min((long long)(pages - first_page), end - at);
+    int kvh, h0, heads;
+    unit_heads(us, a.nh, c.kv_heads, u, &kvh, &h0, &heads);
+    const int my_pages = n_pages > warp ? (n_pages - warp + kMmaWarps - 1) / kMmaWarps : 0;
+    const int32_t* row_table = c.table + (size_t)seq * c.per_seq + first_page + warp;
+
+    // one page's copies; lane l of the ids holds page (block of 32) + l
+    int ids = 0;
+    auto fetch = [&](int i) {
+      if (i < my_pages) {
+        if ((i & 31) == 0) {
+          ids = i + lane < my_pages ? row_table[(i + lane) * kMmaWarps] : 0;
+          if ((unsigned)ids >= (unsigned)c.pages) {
+            atomicOr(a.status, kStatusBadContext);
+            ids = 0;
+          }
+        }
+        const int page = __shfl_sync(0xffffffffu, ids, i & 31);
+        const uint8_t* block = c.pool + ((size_t)page * c.kv_heads + kvh) * (2 * kPage * T::kRow + T::kParams);
+        const uint32_t dst = mine_s + (i % T::kStages) * T::kStage;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int j = 0; j < T::kKPieces; ++j)
+            cp_async<T::kKPiece>(dst + ((h * T::kKPieces + j) * 32 + lane) * T::kKPiece,
+                                 block + (g + 8 * h) * T::kRow + t * T::kKBytes + j * T::kKPiece);
+#pragma unroll
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+          for (int j = 0; j < T::kVPieces; ++j)
+            cp_async<T::kVPiece>(dst + T::kKStage + ((h * T::kVPieces + j) * 32 + lane) * T::kVPiece,
+                                 block + (kPage + 2 * t + (h & 1) + (h >> 1) * 8) * T::kRow + g * T::kVBytes +
+                                     j * T::kVPiece);
+        cp_async<T::kParams / 32>(dst + T::kKStage + T::kVStage + lane * (T::kParams / 32),
+                                  block + 2 * kPage * T::kRow + lane * (T::kParams / 32));
+      }
+      cp_async_commit();  // an empty group keeps the count of groups in step
+    };
+#pragma unroll
+    for (int i = 0; i < T::kStages - 1; ++i) fetch(i);
+
+    // q: this lane's columns are head g / 2 of each tile of four, term g % 2
+    uint32_t qf[NT][T::kKSteps][2];
+    float qs[NT], qsum[NT];  // of the heads whose sums this lane holds (t of each tile)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      float x[HD / 4];
+      const int h = nt * 4 + (g >> 1);
+      const size_t src = (size_t)r * a.ldq + (size_t)(h0 + min(h, heads - 1)) * HD + t * (HD / 4);
+      if (wide_q) {
+#pragma unroll
+        for (int i = 0; i < HD / 16; ++i) {
+          const float4 v = *(const float4*)((const float*)a.q + src + 4 * i);
+          x[4 * i] = v.x;
+          x[4 * i + 1] = v.y;
+          x[4 * i + 2] = v.z;
+          x[4 * i + 3] = v.w;
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < HD / 4; ++i) x[i] = load_elem(a.q, src + i, a.bf16);
+      }
+      float top = 0.0f, sum = 0.0f;
+      bool odd_one = false;
+#pragma unroll
+      for (int i = 0; i < HD / 4; ++i) {
+        top = fmaxf(top, fabsf(x[i]));
+        sum = __fadd_rn(sum, x[i]);
+        odd_one |= !isfinite(x[i]);
+      }
+#pragma unroll
+      for (int o = 1; o < 4; o <<= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+      }
+      // 2^14 / 2^floor(log2 top), the exponent kept within what a float and its inverse can hold
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
+      const float up = __uint_as_float((uint32_t)(268 - e) << 23), down = __uint_as_float((uint32_t)(e - 14) << 23);
+      const bool lo = g & 1;
+#pragma unroll
+      for (int s = 0; s < T::kKSteps; ++s) {
+        // the lane's elements of this step, in the order in which the codes are widened
+        const int d = I4 ? 8 * (s / 2) : 4 * s, b = I4 ? 2 * (s % 2) : 0, skip = I4 ? 4 : 2;
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t p = two_terms(__fmul_rn(x[d + b + k], up)), q = two_terms(__fmul_rn(x[d + b + k + skip], up));
+          qf[nt][s][k] = __byte_perm(p, q, lo ? 0x7632 : 0x5410);
+        }
+      }
+      // a q that is not finite makes its head NaN
+      const float f = __any_sync(0xfu << (lane & ~3), odd_one) ? __int_as_float(0x7fc00000) : __fmul_rn(qscale, down);
+      qs[nt] = __shfl_sync(0xffffffffu, f, 8 * t);
+      qsum[nt] = __shfl_sync(0xffffffffu, __fmul_rn(sum, up), 8 * t);
+    }
+
+    float m[NT], l[NT], zsum[NT], o[NT][T::kMTiles][4];
+    float vf = __uint_as_float(247u << 23);  // the weights' power of two
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      m[nt] = -INFINITY;
+      l[nt] = zsum[nt] = 0.0f;
+#pragma unroll
+      for (int i = 0; i < T::kMTiles; ++i)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.0f;
+    }
+
+    for (int i = 0; i < my_pages; ++i) {
+      cp_async_wait<T::kStages - 2>();
+      __syncwarp();  // the parameters come from other lanes' copies; the stage before is free
+      fetch(i + T::kStages - 1);
+      const uint32_t src = mine_s + (i % T::kStages) * T::kStage;
+      const uint32_t par = src + T::kKStage + T::kVStage;
+      const int left = len - (first_page + warp + i * kMmaWarps) * kPage;  // live positions from this page on
+      // scores
+      float sc[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
+      uint32_t kw[2][T::kKBytes / 4];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int j = 0; j < T::kKPieces; ++j)
+          lds_piece<T::kKPiece>(src + ((h * T::kKPieces + j) * 32 + lane) * T::kKPiece, kw[h] + j * (T::kKPiece / 4));
+#pragma unroll
+      for (int w = 0; w < T::kKBytes / 4; ++w) {
+        if constexpr (I4) {
+          uint32_t x[4], y[4];
+          nibbles_f16(kw[0][w], x);
+          nibbles_f16(kw[1][w], y);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16(sc[nt], x[0], y[0], x[1], y[1], qf[nt][2 * w][0], qf[nt][2 * w][1]);
+            mma_f16(sc[nt], x[2], y[2], x[3], y[3], qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+          }
+        } else {
+          uint32_t x[2], y[2];
+          bytes_f16(kw[0][w], &x[0], &x[1]);
+          bytes_f16(kw[1][w], &y[0], &y[1]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(sc[nt], x[0], y[0], x[1], y[1], qf[nt][w][0], qf[nt][w][1]);
+        }
+      }
+      const bool live0 = g < left, live1 = g + 8 < left;
+      const float ks0 = lds_f32(par + g * 4), ks1 = lds_f32(par + g * 4 + 32);
+      const int vpar = I4 ? 128 : 64;
+      // behind the context the bytes may be anything: no scale of theirs is used
+      const float vs0 = live0 ? lds_f32(par + vpar + g * 4) : 0.0f, vs1 = live1 ? lds_f32(par + vpar + g * 4 + 32) : 0.0f;
+      float kz0 = 0.0f, kz1 = 0.0f, vz0 = 0.0f, vz1 = 0.0f;
+      if constexpr (I4) {
+        kz0 = __fmaf_rn(8.0f, ks0, lds_f32(par + 64 + g * 4));
+        kz1 = __fmaf_rn(8.0f, ks1, lds_f32(par + 64 + g * 4 + 32));
+        vz0 = live0 ? __fmaf_rn(8.0f, vs0, lds_f32(par + 192 + g * 4)) : 0.0f;
+        vz1 = live1 ? __fmaf_rn(8.0f, vs1, lds_f32(par + 192 + g * 4 + 32)) : 0.0f;
+      }
+      // a scale of V above what the weights' power of two allows
+      float vtop = fmaxf(vs0, vs1);
+      if (__any_sync(0xffffffffu, __fmul_rn(vtop, vf) > 32768.0f)) {
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, b));
+        const int e = min(max((int)(__float_as_uint(vtop) >> 23), 18), 255);
+        const float nf = __uint_as_float((uint32_t)(265 - e) << 23);
+        const float f = __fdiv_rn(nf, vf);
+        vf = nf;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < T::kMTiles; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[nt][k][j] = __fmul_rn(o[nt][k][j], f);
+      }
+      uint32_t wb[NT][2];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt) {
+        float s0 = __fmul_rn(__fadd_rn(sc[nt][0], sc[nt][1]), ks0), s1 = __fmul_rn(__fadd_rn(sc[nt][2], sc[nt][3]), ks1);
+        if constexpr (I4) {
+          s0 = __fmaf_rn(qsum[nt], kz0, s0);
+          s1 = __fmaf_rn(qsum[nt], kz1, s1);
+        }
+        s0 = live0 ? __fmul_rn(s0, qs[nt]) : -INFINITY;
+        s1 = live1 ? __fmul_rn(s1, qs[nt]) : -INFINITY;
+        float top = fmaxf(s0, s1);
+#pragma unroll
+        for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+        if (__any_sync(0xffffffffu, top > m[nt])) {
+          const float mn = fmaxf(m[nt], top), keep = exp2_approx(__fsub_rn(m[nt], mn));
+          m[nt] = mn;
+          l[nt] = __fmul_rn(l[nt], keep);
+          zsum[nt] = __fmul_rn(zsum[nt], keep);
+#pragma unroll
+          for (int k = 0; k < T::kMTiles; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[nt][k][j] = __fmul_rn(o[nt][k][j], keep);
+        }
+        const float w0 = live0 ? exp2_approx(__fsub_rn(s0, m[nt])) : 0.0f;
+        const float w1 = live1 ? exp2_approx(__fsub_rn(s1, m[nt])) : 0.0f;
+        l[nt] = __fadd_rn(l[nt], __fadd_rn(w0, w1));
+        if constexpr (I4) zsum[nt] = __fmaf_rn(w0, vz0, __fmaf_rn(w1, vz1, zsum[nt]));
+        wb[nt][0] = transpose8x8(two_terms(__fmul_rn(w0, __fmul_rn(vs0, vf))));
+        wb[nt][1] = transpose8x8(two_terms(__fmul_rn(w1, __fmul_rn(vs1, vf))));
+      }
+      // output
+      uint32_t vw[4][T::kVBytes / 4];
+#pragma unroll
+      for (int h = 0; h < 4; ++h)
+#pragma unroll
+        for (int j = 0; j < T::kVPieces; ++j)
+          lds_piece<T::kVPiece>(src + T::kKStage + ((h * T::kVPieces + j) * 32 + lane) * T::kVPiece,
+                                vw[h] + j * (T::kVPiece / 4));
+#pragma unroll
+      for (int w = 0; w < T::kVBytes / 4; ++w) {
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          // the halves of two rows' words, so that a widened pair is one dimension at two positions
+          const uint32_t lo = __byte_perm(vw[0][w], vw[1][w], half ? 0x7632 : 0x5410);
+          const uint32_t hi = __byte_perm(vw[2][w], vw[3][w], half ? 0x7632 : 0x5410);
+          if constexpr (I4) {
+            uint32_t x[4], y[4];
+            nibbles_f16(lo, x);
+            nibbles_f16(hi, y);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(o[nt][4 * w + 2 * half], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
+              mma_f16(o[nt][4 * w + 2 * half + 1], x[2], x[3], y[2], y[3], wb[nt][0], wb[nt][1]);
+            }
+          } else {
+            uint32_t x[2], y[2];
+            bytes_f16(lo, &x[0], &x[1]);
+            bytes_f16(hi, &y[0], &y[1]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + half], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
+          }
+        }
+      }
+    }
+    cp_async_wait<0>();
+
+    // the warp's partial result, in its own ring
+    const float back = __fdiv_rn(1.0f, vf);
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+      for (int b = 4; b < 32; b <<= 1) {
+        l[nt] = __fadd_rn(l[nt], __shfl_xor_sync(0xffffffffu, l[nt], b));
+        if constexpr (I4) zsum[nt] = __fadd_rn(zsum[nt], __shfl_xor_sync(0xffffffffu, zsum[nt], b));
+      }
+      __syncwarp();
+      float* part = (float*)mine + (nt * 4 + t) * T::kPartStride + g * (HD / 8);
+#pragma unroll
+      for (int k = 0; k < T::kMTiles; ++k) {
+        part[2 * k] = __fmaf_rn(__fadd_rn(o[nt][k][0], o[nt][k][1]), back, zsum[nt]);
+        part[2 * k + 1] = __fmaf_rn(__fadd_rn(o[nt][k][2], o[nt][k][3]), back, zsum[nt]);
+      }
+      if (g == 0) {
+        ml[warp][nt * 4 + t][0] = m[nt];
+        ml[warp][nt * 4 + t][1] = l[nt];
+      }
+    }
+    __syncthreads();
+    const bool begins = first_page == 0, ends = first_page + n_pages == pages;
+    float* slot = share_slot(a.space, shares, share, begins && !ends ? 1 : 0, HD, us);
+    for (int i = tid; i < heads * HD; i += kMmaWarps * 32) {
+      const int h = i / HD, d = i % HD;
+      float M = -INFINITY, L = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kMmaWarps; ++w) M = fmaxf(M, ml[w][h][0]);
+#pragma unroll
+      for (int w = 0; w < kMmaWarps; ++w) {
+        if (w >= n_pages) continue;  // a warp without pages
+        const float f = exp2_approx(__fsub_rn(ml[w][h][0], M));
+        L = __fmaf_rn(ml[w][h][1], f, L);
+        sum = __fmaf_rn(((const float*)(ring + w * (T::kStages * T::kStage)))[h * T::kPartStride + d], f, sum);
+      }
+      if (begins && ends) {
+        store_elem(a.out, (size_t)r * a.ldo + (size_t)h0 * HD + i, a.bf16, __fdiv_rn(sum, L));
+        if (a.lse && d == 0) a.lse[(size_t)r * a.nh + h0 + h] = lse_of(M, L);
+      } else {
+        slot[h * (HD + 2) + d] = sum;
+        if (d == 0) {
+          slot[h * (HD + 2) + HD] = M;
+          slot[h * (HD + 2) + HD + 1] = L;
+        }
+      }
+    }
+    if (begins && !ends) {
+      note.row = r;
+      note.unit = u;
+    }
+    if (!begins) note.ends = ends;
+    at += n_pages;
+    __syncthreads();  // the rings are free again
+  }
+  if (tid == 0) meta[share] = note;
+}
+
 // Joins the partial results of the unit that begins in this CTA's share and ends in a later one.
 __global__ void __launch_bounds__(256) kvq_join_kernel(KvqView c, KvqAttend a, int shares) {
-  const ShareMeta* meta = (const ShareMeta*)a.space;
+  pdl_wait();
+  const ShareMeta* meta = (const ShareMeta*)after_wait((uint8_t*)a.space);
   const int share = blockIdx.x, hd = c.hd;
   const ShareMeta own = meta[share];
   if (own.row < 0) return;
@@ -512,15 +1035,51 @@ size_t kvq_attend_space(int nh, int kv_heads, int hd) {
   return (size_t)kAttendCtas * (sizeof(ShareMeta) + 2 * us.heads * (hd + 2) * sizeof(float));
 }
 
+namespace {
+constexpr int kMinPages = kMmaWarps;  // a share has a page for every warp
+
+template <int HD, bool I4, int NT>
+void launch_mma(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, int wide_q, cudaStream_t st) {
+  using T = MmaTile<HD, I4>;
+  constexpr int smem = kMmaWarps * T::kStages * T::kStage;
+  static_assert(T::kStages * T::kStage >= NT * 4 * T::kPartStride * 4, "a warp's ring holds its partial result");
+  auto* kernel = kvq_attend_mma_kernel<HD, I4, NT>;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+  const int shares = NT == 1 ? 296 : 148;
+  kernel<<<shares, kMmaWarps * 32, smem, st>>>(c, r, a, max_len, kMinPages, wide_q);
+  launch_pdl(kvq_join_kernel, dim3(shares), dim3(256), 0, st, c, a, shares);
+  count_launch(2);
+}
+using LaunchMma = void (*)(const KvqView&, const KvqRows&, const KvqAttend&, int, int, cudaStream_t);
+// The tensor-core kernel for a cache and number of heads a unit, or null.
+LaunchMma mma_for(const KvqView& c, int heads) {
+  const bool two = heads > 4;
+  switch (c.hd) {
+    case 64:
+      return c.i4 ? (two ? launch_mma<64, true, 2> : launch_mma<64, true, 1>)
+                  : (two ? launch_mma<64, false, 2> : launch_mma<64, false, 1>);
+    case 96:
+      return c.i4 ? nullptr : (two ? launch_mma<96, false, 2> : launch_mma<96, false, 1>);
+    case 128:
+      return c.i4 ? (two ? launch_mma<128, true, 2> : launch_mma<128, true, 1>)
+                  : (two ? launch_mma<128, false, 2> : launch_mma<128, false, 1>);
+  }
+  return nullptr;
+}
+}  // namespace
+
 const char* kvq_attend_kernel_name(const KvqView& c, int nh) {
-  (void)c;
-  (void)nh;
-  return "kvq_attend_plain_kernel";
+  return mma_for(c, units_of(nh, c.kv_heads).heads) ? "kvq_attend_mma_kernel" : "kvq_attend_plain_kernel";
 }
 
 void launch_kvq_attend(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st) {
   if (r.rows <= 0) return;
   const Units us = units_of(a.nh, c.kv_heads);
+  if (LaunchMma launch = mma_for(c, us.heads)) {
+    const int wide_q = !a.bf16 && (uintptr_t)a.q % 16 == 0 && a.ldq % 4 == 0;
+    launch(c, r, a, max_len, wide_q, st);
+    return;
+  }
   const size_t smem = ((size_t)us.heads * c.hd + kPlainWarps * us.heads * (c.hd + 2)) * sizeof(float);
   kvq_attend_plain_kernel<<<kAttendCtas, kPlainWarps * 32, smem, st>>>(c, r, a, max_len);
   kvq_join_kernel<<<kAttendCtas, 256, 0, st>>>(c, a, kAttendCtas);
