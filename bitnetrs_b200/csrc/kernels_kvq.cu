@@ -274,6 +274,13 @@ __device__ __forceinline__ float* share_slot(void* space, int shares, int share,
   return (float*)((ShareMeta*)space + shares) + ((size_t)share * 2 + slot) * (us.heads * (hd + 2));
 }
 
+// A partial result that a warp of the tensor-core kernel leaves for its CTA's
+// join, behind the shares' slots; rows padded like the ring's.
+__device__ __forceinline__ float* warp_slot(void* space, int shares, int warp, int hd, const Units& us) {
+  const size_t slots = (size_t)shares * 2 * (us.heads * (hd + 2));
+  return (float*)((ShareMeta*)space + shares) + (slots + 3) / 4 * 4 + (size_t)warp * (us.heads * (hd + 4));
+}
+
 __device__ void write_empty_row(const KvqAttend& a, int hd, int r) {
   for (int i = threadIdx.x; i < a.nh * hd; i += blockDim.x) store_elem(a.out, (size_t)r * a.ldo + i, a.bf16, 0.0f);
   if (a.lse)
@@ -475,15 +482,26 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // a value, zero + 8 scale, enters as a sum of its own.
 // q is multiplied by a power of two a head so that its largest element is
 // near 2^14, the weights by one a warp so that the largest scale of V seen is
-// near 2^11 (rescaled like the maximum when a larger one comes): the second
-// terms then keep 2^-39 of the largest value.
+// near 2^5 and at most 2^9 (rescaled like the sums when a larger one comes; a
+// weight is at most 2^kSlack): a second term then still holds 2^-30 of the
+// largest weight.
 //
-// The order of dimensions inside a product is free, so a lane fetches
-// contiguous bytes of a row for its K operand (HD/4 codes of two rows) and its
-// V operand (HD/8 codes of four rows).  They come by cp.async into a ring that
-// only the same lane reads, so a warp waits for its own copies alone.
+// Here the line of pages is cut into equal shares for the warps, not the
+// CTAs, so that no warp waits for another before its share is done.  The warps
+// of a CTA hold neighbouring shares: at the end the CTA joins the units that
+// its warps cut, and leaves to the join kernel those that CTAs cut.
+//
+// The order of dimensions inside a product is free, so a lane fetches wide
+// pieces of a row for its K operand (HD/4 codes of two rows, the four lanes of
+// a row side by side) and its V operand (HD/8 codes of four rows).  They come
+// by cp.async into a ring that only the same lane reads, so a warp waits for
+// its own copies alone.
 // ---------------------------------------------------------------------------
 constexpr int kMmaWarps = 8;
+constexpr int kMmaShares = 296;  // two CTAs an SM with up to four heads a unit, else one
+// How far a score may exceed the running maximum before the sums are rescaled
+// (log2): rescaling then all but stops after a unit's first pages.
+constexpr float kSlack = 6.0f;
 
 template <int HD, bool I4>
 struct MmaTile {
@@ -492,6 +510,7 @@ struct MmaTile {
   static constexpr int kVBytes = kRow / 8;              // a lane's bytes of one V row
   static constexpr int kKPiece = kKBytes % 16 == 0 ? 16 : kKBytes % 8 == 0 ? 8 : 4;
   static constexpr int kVPiece = kVBytes % 16 == 0 ? 16 : kVBytes % 8 == 0 ? 8 : 4;
+  static constexpr int kKCodes = kKPiece * (I4 ? 2 : 1);  // codes of a K piece
   static constexpr int kKPieces = kKBytes / kKPiece, kVPieces = kVBytes / kVPiece;
   static constexpr int kKStage = 2 * kKBytes * 32, kVStage = 4 * kVBytes * 32;
   static constexpr int kParams = I4 ? 256 : 128;
@@ -592,113 +611,121 @@ __device__ __forceinline__ void nibbles_f16(uint32_t w, uint32_t* x) {
   x[3] = fma_f16x2((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
 }
 
-// The share's place in the line of pages: how long the line is, the row in
-// which the share begins and where that row's pages begin.  Every thread takes
-// a run of rows; a scan over the threads gives each its place.
-struct Place {
-  long long total, base;
-  int row;
+// The line of work as every CTA sees it: thread t of the CTA sums a run of
+// `each` rows, and before[t] is the line up to that run.
+template <int THREADS>
+struct Line {
+  long long before[THREADS + 1];
+  long long warp_sum[THREADS / 32];
 };
 __device__ __forceinline__ int row_pages(const KvqView& c, const KvqRows& R, int r, int max_len, int32_t* status) {
   int seq;
   const int len = row_context(c, R, r, max_len, &seq, status);
   return len > 0 ? (len + kPage - 1) / kPage : 0;
 }
+// A unit weighs its pages and kUnitCost more: what q, the first copies and the
+// result of a unit cost a warp, in pages.
+constexpr int kUnitCost = 2;
 template <int THREADS>
-__device__ Place find_place(const KvqView& c, const KvqRows& R, int max_len, int per_row, int shares, int min_pages,
-                            int32_t* status, long long* start, long long* end) {
-  __shared__ long long warp_sum[THREADS / 32];
-  __shared__ long long base_sh;
-  __shared__ int row_sh;
+__device__ void measure_line(Line<THREADS>& line, const KvqView& c, const KvqRows& R, int max_len, int per_row, int each,
+                             int32_t* status) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int each = (R.rows + THREADS - 1) / THREADS;
   const int r0 = min(tid * each, R.rows), r1 = min(r0 + each, R.rows);
   long long mine = 0;
-  for (int r = r0; r < r1; ++r) mine += row_pages(c, R, r, max_len, status);
+  for (int r = r0; r < r1; ++r) {
+    const int pages = row_pages(c, R, r, max_len, status);
+    if (pages) mine += (long long)(pages + kUnitCost) * per_row;
+  }
   long long upto = mine;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const long long v = __shfl_up_sync(0xffffffffu, upto, o);
     if (lane >= o) upto += v;
   }
-  if (lane == 31) warp_sum[warp] = upto;
+  if (lane == 31) line.warp_sum[warp] = upto;
   __syncthreads();
-  long long before = 0, total = 0;
-#pragma unroll
-  for (int w = 0; w < THREADS / 32; ++w) {
-    if (w < warp) before += warp_sum[w];
-    total += warp_sum[w];
-  }
-  Place at;
-  at.total = total * per_row;
-  const long long cuts = min((long long)shares, (at.total + min_pages - 1) / min_pages);
-  const bool idle = (long long)blockIdx.x >= cuts;
-  *start = idle ? 0 : at.total * blockIdx.x / cuts;
-  *end = idle ? 0 : at.total * (blockIdx.x + 1) / cuts;
-  long long b = (before + upto - mine) * per_row;
-  if (!idle && b <= *start && *start < b + mine * per_row) {
-    for (int r = r0;; ++r) {
-      const long long n = (long long)row_pages(c, R, r, max_len, status) * per_row;
-      if (*start < b + n) {
-        row_sh = r;
-        base_sh = b;
-        break;
-      }
-      b += n;
-    }
-  }
+  long long first = 0;
+  for (int w = 0; w < warp; ++w) first += line.warp_sum[w];
+  line.before[tid + 1] = first + upto;
+  if (tid == 0) line.before[0] = 0;
   __syncthreads();
-  at.row = row_sh;
-  at.base = base_sh;
-  return at;
 }
+
+// What a warp leaves for the CTA's join: the unit that begins in its share and
+// does not end there (in its ring), and the part of an earlier one (in its
+// ring, or in the workspace when the warp went on after it).
+struct WarpNote {
+  int row, unit;        // row < 0: none begins here and ends later
+  int has0, ends0, far0;
+};
 
 template <int HD, bool I4, int NT>
 __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
-    kvq_attend_mma_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int min_pages, int wide_q) {
+    kvq_attend_mma_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int min_weight, int wide_q) {
   using T = MmaTile<HD, I4>;
+  constexpr int kThreads = kMmaWarps * 32;
   extern __shared__ __align__(128) uint8_t ring[];
-  __shared__ float ml[kMmaWarps][kMaxHeads][2];
+  __shared__ Line<kThreads> line;
+  __shared__ float ml[kMmaWarps][2][kMaxHeads][2];  // of a warp's slots 0 and 1
+  __shared__ WarpNote notes[kMmaWarps];
   pdl_launch_dependents();
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const Units us = units_of(a.nh, c.kv_heads);
   const int shares = gridDim.x, share = blockIdx.x;
-  ShareMeta* meta = (ShareMeta*)a.space;
   for (int r = share; r < R.rows; r += shares) {
     int seq;
     if (row_context(c, R, r, max_len, &seq, a.status) == 0) write_empty_row(a, HD, r);
   }
-  long long at, end;
-  const Place place = find_place<kMmaWarps * 32>(c, R, max_len, us.per_row, shares, min_pages, a.status, &at, &end);
-  ShareMeta note{-1, 0, 0, 0};
-  int r = place.row;
-  long long base = place.base;
+  const int each = (R.rows + kThreads - 1) / kThreads;
+  measure_line<kThreads>(line, c, R, max_len, us.per_row, each, a.status);
+  const long long total = line.before[kThreads];
+  const long long cuts = min((long long)shares * kMmaWarps, (total + min_weight - 1) / min_weight);
+  const long long mine_at = (long long)share * kMmaWarps + warp;
+  long long at = mine_at < cuts ? total * mine_at / cuts : 0;
+  const long long end = mine_at < cuts ? total * (mine_at + 1) / cuts : 0;
+  int lo = 0, hi = kThreads;  // before[lo] <= at < before[hi]
+  while (hi - lo > 1) {
+    const int mid = (lo + hi) / 2;
+    if (line.before[mid] <= at)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  int r = lo * each;
+  long long base = line.before[lo];
+  WarpNote note{-1, 0, 0, 0, 0};
   uint8_t* const mine = ring + warp * (T::kStages * T::kStage);
   const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
   const float qscale = __fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)HD));
+  const int lane_k = g * T::kRow + t * T::kKPiece, lane_v = (kPage + 2 * t) * T::kRow + g * T::kVBytes;
+  const int lane_p = 2 * kPage * T::kRow + lane * (T::kParams / 32);
 
   while (at < end && r < R.rows) {
     int seq = 0;
     const int len = row_context(c, R, r, max_len, &seq, a.status);
     const int pages = len > 0 ? (len + kPage - 1) / kPage : 0;
-    if (at >= base + (long long)pages * us.per_row) {
-      base += (long long)pages * us.per_row;
+    const int weight = pages ? pages + kUnitCost : 0;
+    if (at >= base + (long long)weight * us.per_row) {
+      base += (long long)weight * us.per_row;
       ++r;
       continue;
     }
-    const int u = (int)((at - base) / pages), first_page = (int)((at - base) % pages);
-    const int n_pages = (int)min((long long)(pages - first_page), end - at);
+    const int u = (int)((at - base) / weight);
+    const long long first = base + (long long)u * weight + kUnitCost;  // where the unit's pages begin
+    const int p0 = (int)max(at - first, 0LL), p1 = (int)min(end - first, (long long)pages);
+    at = first + pages;
+    if (p1 <= p0) continue;
     int kvh, h0, heads;
     unit_heads(us, a.nh, c.kv_heads, u, &kvh, &h0, &heads);
-    const int my_pages = n_pages > warp ? (n_pages - warp + kMmaWarps - 1) / kMmaWarps : 0;
-    const int32_t* row_table = c.table + (size_t)seq * c.per_seq + first_page + warp;
+    const int n_pages = p1 - p0;
+    const int32_t* row_table = c.table + (size_t)seq * c.per_seq + p0;
 
     // one page's copies; lane l of the ids holds page (block of 32) + l
-    int ids = 0;
+    int ids = 0, fill = 0;
     auto fetch = [&](int i) {
-      if (i < my_pages) {
+      if (i < n_pages) {
         if ((i & 31) == 0) {
-          ids = i + lane < my_pages ? row_table[(i + lane) * kMmaWarps] : 0;
+          ids = i + lane < n_pages ? row_table[i + lane] : 0;
           if ((unsigned)ids >= (unsigned)c.pages) {
             atomicOr(a.status, kStatusBadContext);
             ids = 0;
@@ -706,25 +733,26 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
         }
         const int page = __shfl_sync(0xffffffffu, ids, i & 31);
         const uint8_t* block = c.pool + ((size_t)page * c.kv_heads + kvh) * (2 * kPage * T::kRow + T::kParams);
-        const uint32_t dst = mine_s + (i % T::kStages) * T::kStage;
+        const uint32_t dst = mine_s + fill * T::kStage;
+        const uint32_t dk = dst + lane * T::kKPiece, dv = dst + T::kKStage + lane * T::kVPiece;
+        const uint8_t *sk = block + lane_k, *sv = block + lane_v;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int j = 0; j < T::kKPieces; ++j)
-            cp_async<T::kKPiece>(dst + ((h * T::kKPieces + j) * 32 + lane) * T::kKPiece,
-                                 block + (g + 8 * h) * T::kRow + t * T::kKBytes + j * T::kKPiece);
+            cp_async<T::kKPiece>(dk + (h * T::kKPieces + j) * 32 * T::kKPiece, sk + 8 * h * T::kRow + 4 * j * T::kKPiece);
 #pragma unroll
         for (int h = 0; h < 4; ++h)
 #pragma unroll
           for (int j = 0; j < T::kVPieces; ++j)
-            cp_async<T::kVPiece>(dst + T::kKStage + ((h * T::kVPieces + j) * 32 + lane) * T::kVPiece,
-                                 block + (kPage + 2 * t + (h & 1) + (h >> 1) * 8) * T::kRow + g * T::kVBytes +
-                                     j * T::kVPiece);
-        cp_async<T::kParams / 32>(dst + T::kKStage + T::kVStage + lane * (T::kParams / 32),
-                                  block + 2 * kPage * T::kRow + lane * (T::kParams / 32));
+            cp_async<T::kVPiece>(dv + (h * T::kVPieces + j) * 32 * T::kVPiece,
+                                 sv + ((h & 1) + (h >> 1) * 8) * T::kRow + j * T::kVPiece);
+        cp_async<T::kParams / 32>(dst + T::kKStage + T::kVStage + lane * (T::kParams / 32), block + lane_p);
+        fill = fill + 1 == T::kStages ? 0 : fill + 1;
       }
       cp_async_commit();  // an empty group keeps the count of groups in step
     };
+    __syncwarp();
 #pragma unroll
     for (int i = 0; i < T::kStages - 1; ++i) fetch(i);
 
@@ -735,19 +763,20 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
     for (int nt = 0; nt < NT; ++nt) {
       float x[HD / 4];
       const int h = nt * 4 + (g >> 1);
-      const size_t src = (size_t)r * a.ldq + (size_t)(h0 + min(h, heads - 1)) * HD + t * (HD / 4);
+      const size_t src = (size_t)r * a.ldq + (size_t)(h0 + min(h, heads - 1)) * HD + t * T::kKCodes;
+      // the lane's codes: kKCodes of every 4 * kKCodes
       if (wide_q) {
 #pragma unroll
-        for (int i = 0; i < HD / 16; ++i) {
-          const float4 v = *(const float4*)((const float*)a.q + src + 4 * i);
-          x[4 * i] = v.x;
-          x[4 * i + 1] = v.y;
-          x[4 * i + 2] = v.z;
-          x[4 * i + 3] = v.w;
+        for (int i = 0; i < HD / 4; i += 4) {
+          const float4 v = *(const float4*)((const float*)a.q + src + i + i / T::kKCodes * (3 * T::kKCodes));
+          x[i] = v.x;
+          x[i + 1] = v.y;
+          x[i + 2] = v.z;
+          x[i + 3] = v.w;
         }
       } else {
 #pragma unroll
-        for (int i = 0; i < HD / 4; ++i) x[i] = load_elem(a.q, src + i, a.bf16);
+        for (int i = 0; i < HD / 4; ++i) x[i] = load_elem(a.q, src + i + i / T::kKCodes * (3 * T::kKCodes), a.bf16);
       }
       float top = 0.0f, sum = 0.0f;
       bool odd_one = false;
@@ -765,7 +794,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
       // 2^14 / 2^floor(log2 top), the exponent kept within what a float and its inverse can hold
       const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
       const float up = __uint_as_float((uint32_t)(268 - e) << 23), down = __uint_as_float((uint32_t)(e - 14) << 23);
-      const bool lo = g & 1;
+      const bool second = g & 1;
 #pragma unroll
       for (int s = 0; s < T::kKSteps; ++s) {
         // the lane's elements of this step, in the order in which the codes are widened
@@ -773,15 +802,17 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
           const uint32_t p = two_terms(__fmul_rn(x[d + b + k], up)), q = two_terms(__fmul_rn(x[d + b + k + skip], up));
-          qf[nt][s][k] = __byte_perm(p, q, lo ? 0x7632 : 0x5410);
+          qf[nt][s][k] = __byte_perm(p, q, second ? 0x7632 : 0x5410);
         }
       }
       // a q that is not finite makes its head NaN
-      const float f = __any_sync(0xfu << (lane & ~3), odd_one) ? __int_as_float(0x7fc00000) : __fmul_rn(qscale, down);
+      const unsigned odd = __ballot_sync(0xffffffffu, odd_one);
+      const float f = (odd >> (lane & ~3)) & 15 ? __int_as_float(0x7fc00000) : __fmul_rn(qscale, down);
       qs[nt] = __shfl_sync(0xffffffffu, f, 8 * t);
       qsum[nt] = __shfl_sync(0xffffffffu, __fmul_rn(sum, up), 8 * t);
     }
 
+    // m: a maximum of the scores at most kSlack (log2) below the true one
     float m[NT], l[NT], zsum[NT], o[NT][T::kMTiles][4];
     float vf = __uint_as_float(247u << 23);  // the weights' power of two
 #pragma unroll
@@ -794,17 +825,21 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
         for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.0f;
     }
 
-    for (int i = 0; i < my_pages; ++i) {
+    int take = 0;
+    for (int i = 0; i < n_pages; ++i) {
       cp_async_wait<T::kStages - 2>();
       __syncwarp();  // the parameters come from other lanes' copies; the stage before is free
       fetch(i + T::kStages - 1);
-      const uint32_t src = mine_s + (i % T::kStages) * T::kStage;
-      const uint32_t par = src + T::kKStage + T::kVStage;
-      const int left = len - (first_page + warp + i * kMmaWarps) * kPage;  // live positions from this page on
-      // scores
-      float sc[NT][4];
+      const uint32_t src = mine_s + take * T::kStage;
+      take = take + 1 == T::kStages ? 0 : take + 1;
+      const uint32_t par = src + T::kKStage + T::kVStage + g * 4;
+      const int left = len - (p0 + i) * kPage;  // live positions from this page on
+      // scores, in two chains of products
+      float sc[NT][2][4];
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.0f;
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int k = 0; k < 4; ++k) sc[nt][0][k] = sc[nt][1][k] = 0.0f;
       uint32_t kw[2][T::kKBytes / 4];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -819,36 +854,36 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
           nibbles_f16(kw[1][w], y);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(sc[nt], x[0], y[0], x[1], y[1], qf[nt][2 * w][0], qf[nt][2 * w][1]);
-            mma_f16(sc[nt], x[2], y[2], x[3], y[3], qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
+            mma_f16(sc[nt][0], x[0], y[0], x[1], y[1], qf[nt][2 * w][0], qf[nt][2 * w][1]);
+            mma_f16(sc[nt][1], x[2], y[2], x[3], y[3], qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
           }
         } else {
           uint32_t x[2], y[2];
           bytes_f16(kw[0][w], &x[0], &x[1]);
           bytes_f16(kw[1][w], &y[0], &y[1]);
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(sc[nt], x[0], y[0], x[1], y[1], qf[nt][w][0], qf[nt][w][1]);
+          for (int nt = 0; nt < NT; ++nt) mma_f16(sc[nt][w & 1], x[0], y[0], x[1], y[1], qf[nt][w][0], qf[nt][w][1]);
         }
       }
       const bool live0 = g < left, live1 = g + 8 < left;
-      const float ks0 = lds_f32(par + g * 4), ks1 = lds_f32(par + g * 4 + 32);
-      const int vpar = I4 ? 128 : 64;
+      const float ks0 = lds_f32(par), ks1 = lds_f32(par + 32);
+      constexpr int vpar = I4 ? 128 : 64;
       // behind the context the bytes may be anything: no scale of theirs is used
-      const float vs0 = live0 ? lds_f32(par + vpar + g * 4) : 0.0f, vs1 = live1 ? lds_f32(par + vpar + g * 4 + 32) : 0.0f;
+      const float vs0 = live0 ? lds_f32(par + vpar) : 0.0f, vs1 = live1 ? lds_f32(par + vpar + 32) : 0.0f;
       float kz0 = 0.0f, kz1 = 0.0f, vz0 = 0.0f, vz1 = 0.0f;
       if constexpr (I4) {
-        kz0 = __fmaf_rn(8.0f, ks0, lds_f32(par + 64 + g * 4));
-        kz1 = __fmaf_rn(8.0f, ks1, lds_f32(par + 64 + g * 4 + 32));
-        vz0 = live0 ? __fmaf_rn(8.0f, vs0, lds_f32(par + 192 + g * 4)) : 0.0f;
-        vz1 = live1 ? __fmaf_rn(8.0f, vs1, lds_f32(par + 192 + g * 4 + 32)) : 0.0f;
+        kz0 = __fmaf_rn(8.0f, ks0, lds_f32(par + 64));
+        kz1 = __fmaf_rn(8.0f, ks1, lds_f32(par + 96));
+        vz0 = live0 ? __fmaf_rn(8.0f, vs0, lds_f32(par + 192)) : 0.0f;
+        vz1 = live1 ? __fmaf_rn(8.0f, vs1, lds_f32(par + 224)) : 0.0f;
       }
       // a scale of V above what the weights' power of two allows
       float vtop = fmaxf(vs0, vs1);
-      if (__any_sync(0xffffffffu, __fmul_rn(vtop, vf) > 32768.0f)) {
+      if (__any_sync(0xffffffffu, __fmul_rn(vtop, vf) > 512.0f)) {
 #pragma unroll
         for (int b = 4; b < 32; b <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, b));
         const int e = min(max((int)(__float_as_uint(vtop) >> 23), 18), 255);
-        const float nf = __uint_as_float((uint32_t)(265 - e) << 23);
+        const float nf = __uint_as_float((uint32_t)(259 - e) << 23);
         const float f = __fdiv_rn(nf, vf);
         vf = nf;
 #pragma unroll
@@ -861,7 +896,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
       uint32_t wb[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float s0 = __fmul_rn(__fadd_rn(sc[nt][0], sc[nt][1]), ks0), s1 = __fmul_rn(__fadd_rn(sc[nt][2], sc[nt][3]), ks1);
+        float s0 = __fmul_rn(__fadd_rn(__fadd_rn(sc[nt][0][0], sc[nt][1][0]), __fadd_rn(sc[nt][0][1], sc[nt][1][1])), ks0);
+        float s1 = __fmul_rn(__fadd_rn(__fadd_rn(sc[nt][0][2], sc[nt][1][2]), __fadd_rn(sc[nt][0][3], sc[nt][1][3])), ks1);
         if constexpr (I4) {
           s0 = __fmaf_rn(qsum[nt], kz0, s0);
           s1 = __fmaf_rn(qsum[nt], kz1, s1);
@@ -869,9 +905,9 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
         s0 = live0 ? __fmul_rn(s0, qs[nt]) : -INFINITY;
         s1 = live1 ? __fmul_rn(s1, qs[nt]) : -INFINITY;
         float top = fmaxf(s0, s1);
+        if (__any_sync(0xffffffffu, top > __fadd_rn(m[nt], kSlack))) {
 #pragma unroll
-        for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
-        if (__any_sync(0xffffffffu, top > m[nt])) {
+          for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
           const float mn = fmaxf(m[nt], top), keep = exp2_approx(__fsub_rn(m[nt], mn));
           m[nt] = mn;
           l[nt] = __fmul_rn(l[nt], keep);
@@ -901,12 +937,12 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           // the halves of two rows' words, so that a widened pair is one dimension at two positions
-          const uint32_t lo = __byte_perm(vw[0][w], vw[1][w], half ? 0x7632 : 0x5410);
-          const uint32_t hi = __byte_perm(vw[2][w], vw[3][w], half ? 0x7632 : 0x5410);
+          const uint32_t p = __byte_perm(vw[0][w], vw[1][w], half ? 0x7632 : 0x5410);
+          const uint32_t q = __byte_perm(vw[2][w], vw[3][w], half ? 0x7632 : 0x5410);
           if constexpr (I4) {
             uint32_t x[4], y[4];
-            nibbles_f16(lo, x);
-            nibbles_f16(hi, y);
+            nibbles_f16(p, x);
+            nibbles_f16(q, y);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               mma_f16(o[nt][4 * w + 2 * half], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
@@ -914,8 +950,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
             }
           } else {
             uint32_t x[2], y[2];
-            bytes_f16(lo, &x[0], &x[1]);
-            bytes_f16(hi, &y[0], &y[1]);
+            bytes_f16(p, &x[0], &x[1]);
+            bytes_f16(q, &y[0], &y[1]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + half], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
           }
@@ -924,62 +960,104 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
     }
     cp_async_wait<0>();
 
-    // the warp's partial result, in its own ring
+    const bool begins = p0 == 0, ends = p1 == pages;
     const float back = __fdiv_rn(1.0f, vf);
+    const int slot = begins && !ends ? 1 : 0;
+    if (!begins) {
+      note.has0 = 1;
+      note.ends0 = ends;
+      note.far0 = at < end;  // the ring is needed again
+    } else if (!ends) {
+      note.row = r;
+      note.unit = u;
+    }
+    __syncwarp();
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      const int h = nt * 4 + t;
 #pragma unroll
       for (int b = 4; b < 32; b <<= 1) {
         l[nt] = __fadd_rn(l[nt], __shfl_xor_sync(0xffffffffu, l[nt], b));
         if constexpr (I4) zsum[nt] = __fadd_rn(zsum[nt], __shfl_xor_sync(0xffffffffu, zsum[nt], b));
       }
-      __syncwarp();
-      float* part = (float*)mine + (nt * 4 + t) * T::kPartStride + g * (HD / 8);
+      if (h >= heads) continue;
+      float x[HD / 8];  // dimensions g * HD / 8 and on
 #pragma unroll
       for (int k = 0; k < T::kMTiles; ++k) {
-        part[2 * k] = __fmaf_rn(__fadd_rn(o[nt][k][0], o[nt][k][1]), back, zsum[nt]);
-        part[2 * k + 1] = __fmaf_rn(__fadd_rn(o[nt][k][2], o[nt][k][3]), back, zsum[nt]);
-      }
-      if (g == 0) {
-        ml[warp][nt * 4 + t][0] = m[nt];
-        ml[warp][nt * 4 + t][1] = l[nt];
-      }
-    }
-    __syncthreads();
-    const bool begins = first_page == 0, ends = first_page + n_pages == pages;
-    float* slot = share_slot(a.space, shares, share, begins && !ends ? 1 : 0, HD, us);
-    for (int i = tid; i < heads * HD; i += kMmaWarps * 32) {
-      const int h = i / HD, d = i % HD;
-      float M = -INFINITY, L = 0.0f, sum = 0.0f;
-#pragma unroll
-      for (int w = 0; w < kMmaWarps; ++w) M = fmaxf(M, ml[w][h][0]);
-#pragma unroll
-      for (int w = 0; w < kMmaWarps; ++w) {
-        if (w >= n_pages) continue;  // a warp without pages
-        const float f = exp2_approx(__fsub_rn(ml[w][h][0], M));
-        L = __fmaf_rn(ml[w][h][1], f, L);
-        sum = __fmaf_rn(((const float*)(ring + w * (T::kStages * T::kStage)))[h * T::kPartStride + d], f, sum);
+        x[2 * k] = __fmaf_rn(__fadd_rn(o[nt][k][0], o[nt][k][1]), back, zsum[nt]);
+        x[2 * k + 1] = __fmaf_rn(__fadd_rn(o[nt][k][2], o[nt][k][3]), back, zsum[nt]);
       }
       if (begins && ends) {
-        store_elem(a.out, (size_t)r * a.ldo + (size_t)h0 * HD + i, a.bf16, __fdiv_rn(sum, L));
-        if (a.lse && d == 0) a.lse[(size_t)r * a.nh + h0 + h] = lse_of(M, L);
+        const float inv = __fdiv_rn(1.0f, l[nt]);
+        const size_t dst = (size_t)r * a.ldo + (size_t)(h0 + h) * HD + g * (HD / 8);
+#pragma unroll
+        for (int k = 0; k < HD / 8; ++k) store_elem(a.out, dst + k, a.bf16, __fmul_rn(x[k], inv));
+        if (a.lse && g == 0) a.lse[(size_t)r * a.nh + h0 + h] = lse_of(m[nt], l[nt]);
       } else {
-        slot[h * (HD + 2) + d] = sum;
-        if (d == 0) {
-          slot[h * (HD + 2) + HD] = M;
-          slot[h * (HD + 2) + HD + 1] = L;
+        float* part = !begins && at < end ? warp_slot(a.space, shares, (int)mine_at, HD, us) : (float*)mine;
+        part += h * T::kPartStride + g * (HD / 8);
+#pragma unroll
+        for (int k = 0; k < HD / 8; k += 4) *(float4*)(part + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+        if (g == 0) {
+          ml[warp][slot][h][0] = m[nt];
+          ml[warp][slot][h][1] = l[nt];
         }
       }
     }
-    if (begins && !ends) {
-      note.row = r;
-      note.unit = u;
-    }
-    if (!begins) note.ends = ends;
-    at += n_pages;
-    __syncthreads();  // the rings are free again
   }
-  if (tid == 0) meta[share] = note;
+  if (lane == 0) notes[warp] = note;
+  __syncthreads();
+
+  // Join what the CTA's warps left.  Chain -1 is what came in from the share
+  // before, chain w the unit that begins in warp w's share.
+  ShareMeta out{-1, 0, 0, 0};
+  for (int chain = -1; chain < kMmaWarps; ++chain) {
+    const bool head = chain < 0;
+    if (head ? !notes[0].has0 : notes[chain].row < 0) continue;
+    const int from = chain + 1;  // the warps whose slot 0 belongs to it: [from, to)
+    int to = from;
+    bool ends = false;
+    while (to < kMmaWarps && !ends) ends = notes[to++].ends0;
+    const int row = head ? -1 : notes[chain].row, unit = head ? 0 : notes[chain].unit;
+    int kvh, h0 = 0, heads = us.heads;
+    if (!head) unit_heads(us, a.nh, c.kv_heads, unit, &kvh, &h0, &heads);
+    float* dst = share_slot(a.space, shares, share, head ? 0 : 1, HD, us);
+    for (int i = tid; i < heads * HD; i += kThreads) {
+      const int h = i / HD, d = i % HD, at_part = h * T::kPartStride + d;
+      float M = head ? -INFINITY : ml[max(chain, 0)][1][h][0];
+      for (int w = from; w < to; ++w) M = fmaxf(M, ml[w][0][h][0]);
+      float L = 0.0f, sum = 0.0f;
+      if (!head) {
+        const float f = exp2_approx(__fsub_rn(ml[chain][1][h][0], M));
+        L = __fmul_rn(ml[chain][1][h][1], f);
+        sum = __fmul_rn(((const float*)(ring + chain * (T::kStages * T::kStage)))[at_part], f);
+      }
+      for (int w = from; w < to; ++w) {
+        const float f = exp2_approx(__fsub_rn(ml[w][0][h][0], M));
+        const float* part = notes[w].far0 ? warp_slot(a.space, shares, share * kMmaWarps + w, HD, us)
+                                          : (const float*)(ring + w * (T::kStages * T::kStage));
+        L = __fmaf_rn(ml[w][0][h][1], f, L);
+        sum = __fmaf_rn(part[at_part], f, sum);
+      }
+      if (!head && ends) {
+        store_elem(a.out, (size_t)row * a.ldo + (size_t)h0 * HD + i, a.bf16, __fdiv_rn(sum, L));
+        if (a.lse && d == 0) a.lse[(size_t)row * a.nh + h0 + h] = lse_of(M, L);
+      } else {
+        dst[h * (HD + 2) + d] = sum;
+        if (d == 0) {
+          dst[h * (HD + 2) + HD] = M;
+          dst[h * (HD + 2) + HD + 1] = L;
+        }
+      }
+    }
+    if (head) {
+      out.ends = ends;
+    } else if (!ends) {
+      out.row = row;
+      out.unit = unit;
+    }
+  }
+  if (tid == 0) ((ShareMeta*)a.space)[share] = out;
 }
 
 // Joins the partial results of the unit that begins in this CTA's share and ends in a later one.
@@ -1032,11 +1110,14 @@ void launch_kvq_load(const KvqView& c, int rows, const int32_t* row_seq, const i
 
 size_t kvq_attend_space(int nh, int kv_heads, int hd) {
   const Units us = units_of(nh, kv_heads);
-  return (size_t)kAttendCtas * (sizeof(ShareMeta) + 2 * us.heads * (hd + 2) * sizeof(float));
+  const size_t plain = (size_t)kAttendCtas * (sizeof(ShareMeta) + 2 * us.heads * (hd + 2) * sizeof(float));
+  const size_t mma = (size_t)kMmaShares * (sizeof(ShareMeta) + 2 * us.heads * (hd + 2) * sizeof(float) +
+                                           kMmaWarps * us.heads * (hd + 4) * sizeof(float)) + 16;
+  return std::max(plain, mma);
 }
 
 namespace {
-constexpr int kMinPages = kMmaWarps;  // a share has a page for every warp
+constexpr int kMinWeight = kUnitCost + 2;  // the least share of a warp
 
 template <int HD, bool I4, int NT>
 void launch_mma(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, int wide_q, cudaStream_t st) {
@@ -1045,8 +1126,8 @@ void launch_mma(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_
   static_assert(T::kStages * T::kStage >= NT * 4 * T::kPartStride * 4, "a warp's ring holds its partial result");
   auto* kernel = kvq_attend_mma_kernel<HD, I4, NT>;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  const int shares = NT == 1 ? 296 : 148;
-  kernel<<<shares, kMmaWarps * 32, smem, st>>>(c, r, a, max_len, kMinPages, wide_q);
+  const int shares = NT == 1 ? kMmaShares : kMmaShares / 2;
+  kernel<<<shares, kMmaWarps * 32, smem, st>>>(c, r, a, max_len, kMinWeight, wide_q);
   launch_pdl(kvq_join_kernel, dim3(shares), dim3(256), 0, st, c, a, shares);
   count_launch(2);
 }
