@@ -3,6 +3,7 @@
 #include "kvq.cuh"
 
 #include <algorithm>
+#include <utility>
 
 namespace bitnet {
 
@@ -470,21 +471,30 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // ---------------------------------------------------------------------------
 // The tensor-core form, for head sizes of 64, 96 and 128 (I4: 64, 128).
 //
-// One warp multiplies one page at a time: the 16 positions of a page are the M
-// of an m16n8k16 product with fp16 operands and f32 sums, and the N are columns
-// (head, term).  Codes are exact in fp16.  q and the weights are not, so each
-// is the sum of two fp16 terms (22 bits), in neighbouring columns: four heads
-// fill the eight columns, and a lane's pair of sums belongs to one head.
-//   S[pos][head] = K codes . q      A = K, B = q (kept in registers)
-//   O[dim][head] += V codes^T . w   A = V^T, B = w (transposed by movmatrix)
-// The scale of a K row multiplies its score; the scale of a V row its weight
-// before that is split.  With I4 codes c - 8 are multiplied, and the rest of
-// a value, zero + 8 scale, enters as a sum of its own.
-// q is multiplied by a power of two a head so that its largest element is
-// near 2^14, the weights by one a warp so that the largest scale of V seen is
-// near 2^5 and at most 2^9 (rescaled like the sums when a larger one comes; a
-// weight is at most 2^kSlack): a second term then still holds 2^-30 of the
-// largest weight.
+// One warp multiplies one page at a time, its 16 positions (scores) or 16
+// dimensions (output) being the M of a product, and four heads its N.
+//   S[pos][head] = K codes . q        m16n8k32, 8-bit integers
+//   O[dim][head] += V codes^T . w     m16n8k16, fp16 with f32 sums
+// Scores: codes go into the product as they lie in memory.  q is held as a
+// 31-bit integer a dimension (relative to the head's largest element) in four
+// balanced digits of base 256, one column each, so that the integer products
+// are exact and a head's four columns, two in each of two products, are the
+// score.  The scale of a K row multiplies it.
+// Output: codes are exact in fp16.  A weight is not, so it is the sum of two
+// fp16 terms (22 bits), in neighbouring columns; a lane's pair of sums belongs
+// to one head.  The scale of a V row multiplies its weight before that is
+// split.  An I4 zero enters scores (times the sum of q) and output as a sum of
+// its own.
+// The weights are multiplied by a power of two a warp so that the largest
+// scale of V seen is near 2^5 and at most 2^9 (rescaled like the sums when a
+// larger one comes; a weight is at most 2^kSlack): a second term then still
+// holds 2^-30 of the largest weight.
+//
+// The order of dimensions inside a product is free, so a lane fetches wide
+// pieces of a row for its K operand (HD/4 codes of two rows, the four lanes of
+// a row side by side) and its V operand (HD/8 codes of four rows).  They come
+// by cp.async into a ring that only the same lane reads, so a warp waits for
+// its own copies alone.
 //
 // Here the line of pages is cut into equal shares for the warps, not the
 // CTAs, so that no warp waits for another before its share is done.  The warps
@@ -516,16 +526,17 @@ struct MmaTile {
   static constexpr int kParams = I4 ? 256 : 128;
   static constexpr int kStage = kKStage + kVStage + kParams;
   static constexpr int kStages = I4 ? 5 : 3;
-  static constexpr int kKSteps = HD / 16, kMTiles = HD / 16;
+  static constexpr int kKSteps = HD / 32, kMTiles = HD / 16;
   static constexpr int kPartStride = HD + 4;  // floats a head of a warp's partial result
 };
 
-template <int BYTES>
+template <int BYTES, int DST, int SRC>
 __device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
   if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;\n" ::"r"(dst), "l"(src) : "memory");
+    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;\n" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
   else
-    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;\n" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+    asm volatile("cp.async.ca.shared.global [%0 + %2], [%1 + %3], %4;\n" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC), "n"(BYTES)
+                 : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
 template <int N>
@@ -555,6 +566,21 @@ __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1,
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// c = product (START) or c += product
+template <bool START>
+__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                       uint32_t b1) {
+  if constexpr (START)
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};\n"
+        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
+  else
+    asm volatile(
+        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
+        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
   uint32_t y;
@@ -596,19 +622,37 @@ __device__ __forceinline__ uint32_t two_terms(float x) {
   const uint32_t h = pack_f16(x, 0.0f);
   return pack_f16(f16_lo(h), __fsub_rn(x, f16_lo(h)));
 }
+// (x & mask) ^ bits, and (x & mask) | bits, in one instruction each
+__device__ __forceinline__ uint32_t and_xor(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;\n" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
+  return r;
+}
+__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
+  return r;
+}
 // Four signed bytes of w as fp16 pairs: elements (0, 2) and (1, 3).  A byte with
 // its sign flipped, below the bits of 1024, is 1152 + c.
 __device__ __forceinline__ void bytes_f16(uint32_t w, uint32_t* even, uint32_t* odd) {
-  *even = add_f16x2((w & 0x00ff00ffu) ^ 0x64806480u, 0xe480e480u);
-  *odd = add_f16x2(((w >> 8) & 0x00ff00ffu) ^ 0x64806480u, 0xe480e480u);
+  *even = add_f16x2(and_xor(w, 0x00ff00ffu, 0x64806480u), 0xe480e480u);
+  *odd = add_f16x2(and_xor(w >> 8, 0x00ff00ffu, 0x64806480u), 0xe480e480u);
 }
-// Eight nibbles of w, less 8, as fp16 pairs: x[i] = elements (i, i + 4).
+// Eight nibbles of w as fp16 pairs: x[i] = elements (i, i + 4).
 __device__ __forceinline__ void nibbles_f16(uint32_t w, uint32_t* x) {
   const uint32_t v = w >> 8;
-  x[0] = add_f16x2((w & 0x000f000fu) | 0x64006400u, 0xe408e408u);                          // 1024 + c - 1032
-  x[1] = fma_f16x2((w & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);            // (1024 + 16 c) / 16 - 72
-  x[2] = add_f16x2((v & 0x000f000fu) | 0x64006400u, 0xe408e408u);
-  x[3] = fma_f16x2((v & 0x00f000f0u) | 0x64006400u, 0x2c002c00u, 0xd480d480u);
+  x[0] = add_f16x2(and_or(w, 0x000f000fu, 0x64006400u), 0xe400e400u);               // 1024 + c - 1024
+  x[1] = fma_f16x2(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd400d400u);  // (1024 + 16 c) / 16 - 64
+  x[2] = add_f16x2(and_or(v, 0x000f000fu, 0x64006400u), 0xe400e400u);
+  x[3] = fma_f16x2(and_or(v, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd400d400u);
+}
+// x as balanced base-256 digits, the least in the lowest byte (|x| <= 2^30).
+__device__ __forceinline__ uint32_t digits(int x) { return ((uint32_t)x + 0x80808080u) ^ 0x80808080u; }
+// Byte `i` of four words.
+__device__ __forceinline__ uint32_t gather_byte(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i) {
+  const uint32_t sel = (uint32_t)(i | ((i + 4) << 4));
+  return __byte_perm(__byte_perm(a, b, sel), __byte_perm(c, d, sel), 0x5410);
 }
 
 // The line of work as every CTA sees it: thread t of the CTA sums a run of
@@ -659,6 +703,21 @@ struct WarpNote {
   int has0, ends0, far0;
 };
 
+// A lane's copies of one page's block: K rows g and g + 8, V rows 2t, 2t + 1,
+// 2t + 8 and 2t + 9 in pieces, and its part of the parameters.
+template <class T, size_t... IK, size_t... IV>
+__device__ __forceinline__ void copy_page(uint32_t dst, const uint8_t* block, int lane, int lane_k, int lane_v,
+                                          std::index_sequence<IK...>, std::index_sequence<IV...>) {
+  const uint32_t dk = dst + lane * T::kKPiece, dv = dst + lane * T::kVPiece;
+  const uint8_t *sk = block + lane_k, *sv = block + lane_v;
+  (cp_async<T::kKPiece, (int)IK * 32 * T::kKPiece,
+            8 * ((int)IK / T::kKPieces) * T::kRow + 4 * ((int)IK % T::kKPieces) * T::kKPiece>(dk, sk), ...);
+  (cp_async<T::kVPiece, T::kKStage + (int)IV * 32 * T::kVPiece,
+            (((int)IV / T::kVPieces) % 2 + ((int)IV / T::kVPieces) / 2 * 8) * T::kRow + (int)IV % T::kVPieces * T::kVPiece>(dv, sv), ...);
+  cp_async<T::kParams / 32, T::kKStage + T::kVStage, 2 * kPage * T::kRow>(dst + lane * (T::kParams / 32),
+                                                                          block + lane * (T::kParams / 32));
+}
+
 template <int HD, bool I4, int NT>
 __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
     kvq_attend_mma_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int min_weight, int wide_q) {
@@ -698,7 +757,6 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
   const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
   const float qscale = __fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)HD));
   const int lane_k = g * T::kRow + t * T::kKPiece, lane_v = (kPage + 2 * t) * T::kRow + g * T::kVBytes;
-  const int lane_p = 2 * kPage * T::kRow + lane * (T::kParams / 32);
 
   while (at < end && r < R.rows) {
     int seq = 0;
@@ -734,20 +792,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
         const int page = __shfl_sync(0xffffffffu, ids, i & 31);
         const uint8_t* block = c.pool + ((size_t)page * c.kv_heads + kvh) * (2 * kPage * T::kRow + T::kParams);
         const uint32_t dst = mine_s + fill * T::kStage;
-        const uint32_t dk = dst + lane * T::kKPiece, dv = dst + T::kKStage + lane * T::kVPiece;
-        const uint8_t *sk = block + lane_k, *sv = block + lane_v;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < T::kKPieces; ++j)
-            cp_async<T::kKPiece>(dk + (h * T::kKPieces + j) * 32 * T::kKPiece, sk + 8 * h * T::kRow + 4 * j * T::kKPiece);
-#pragma unroll
-        for (int h = 0; h < 4; ++h)
-#pragma unroll
-          for (int j = 0; j < T::kVPieces; ++j)
-            cp_async<T::kVPiece>(dv + (h * T::kVPieces + j) * 32 * T::kVPiece,
-                                 sv + ((h & 1) + (h >> 1) * 8) * T::kRow + j * T::kVPiece);
-        cp_async<T::kParams / 32>(dst + T::kKStage + T::kVStage + lane * (T::kParams / 32), block + lane_p);
+        copy_page<T>(dst, block, lane, lane_k, lane_v, std::make_index_sequence<2 * T::kKPieces>{},
+                     std::make_index_sequence<4 * T::kVPieces>{});
         fill = fill + 1 == T::kStages ? 0 : fill + 1;
       }
       cp_async_commit();  // an empty group keeps the count of groups in step
@@ -756,8 +802,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
 #pragma unroll
     for (int i = 0; i < T::kStages - 1; ++i) fetch(i);
 
-    // q: this lane's columns are head g / 2 of each tile of four, term g % 2
-    uint32_t qf[NT][T::kKSteps][2];
+    // q: this lane's columns are head g / 2 of each tile of four, digits 3 - g % 2 and 1 - g % 2
+    uint32_t qf[NT][T::kKSteps][2][2];
     float qs[NT], qsum[NT];  // of the heads whose sums this lane holds (t of each tile)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -778,38 +824,39 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
 #pragma unroll
         for (int i = 0; i < HD / 4; ++i) x[i] = load_elem(a.q, src + i + i / T::kKCodes * (3 * T::kKCodes), a.bf16);
       }
-      float top = 0.0f, sum = 0.0f;
-      bool odd_one = false;
+      float top = 0.0f, sum = 0.0f, zero = 0.0f;
 #pragma unroll
       for (int i = 0; i < HD / 4; ++i) {
         top = fmaxf(top, fabsf(x[i]));
-        sum = __fadd_rn(sum, x[i]);
-        odd_one |= !isfinite(x[i]);
+        if constexpr (I4) sum = __fadd_rn(sum, x[i]);
+        zero = __fmaf_rn(x[i], 0.0f, zero);  // NaN when an element is not finite
       }
 #pragma unroll
       for (int o = 1; o < 4; o <<= 1) {
         top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+        if constexpr (I4) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
+        zero = __fadd_rn(zero, __shfl_xor_sync(0xffffffffu, zero, o));
       }
-      // 2^14 / 2^floor(log2 top), the exponent kept within what a float and its inverse can hold
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
-      const float up = __uint_as_float((uint32_t)(268 - e) << 23), down = __uint_as_float((uint32_t)(e - 14) << 23);
-      const bool second = g & 1;
+      // 2^29 / 2^floor(log2 top), the exponents kept within what a float and its inverse can hold
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 30), 254);
+      const float up = __uint_as_float((uint32_t)(283 - e) << 23), down = __uint_as_float((uint32_t)(e - 29) << 23);
+      const int d3 = 3 - (g & 1), d1 = 1 - (g & 1);
 #pragma unroll
-      for (int s = 0; s < T::kKSteps; ++s) {
-        // the lane's elements of this step, in the order in which the codes are widened
-        const int d = I4 ? 8 * (s / 2) : 4 * s, b = I4 ? 2 * (s % 2) : 0, skip = I4 ? 4 : 2;
+      for (int s = 0; s < T::kKSteps; ++s)
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const uint32_t p = two_terms(__fmul_rn(x[d + b + k], up)), q = two_terms(__fmul_rn(x[d + b + k + skip], up));
-          qf[nt][s][k] = __byte_perm(p, q, second ? 0x7632 : 0x5410);
+          // the lane's elements of this half step, in the order in which the codes lie in a word
+          const int d = I4 ? 8 * s + k : 8 * s + 4 * k, skip = I4 ? 2 : 1;
+          uint32_t w[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = digits(__float2int_rn(__fmul_rn(x[d + j * skip], up)));
+          qf[nt][s][0][k] = gather_byte(w[0], w[1], w[2], w[3], d3);
+          qf[nt][s][1][k] = gather_byte(w[0], w[1], w[2], w[3], d1);
         }
-      }
       // a q that is not finite makes its head NaN
-      const unsigned odd = __ballot_sync(0xffffffffu, odd_one);
-      const float f = (odd >> (lane & ~3)) & 15 ? __int_as_float(0x7fc00000) : __fmul_rn(qscale, down);
+      const float f = __fadd_rn(__fmul_rn(qscale, down), zero);
       qs[nt] = __shfl_sync(0xffffffffu, f, 8 * t);
-      qsum[nt] = __shfl_sync(0xffffffffu, __fmul_rn(sum, up), 8 * t);
+      qsum[nt] = I4 ? __shfl_sync(0xffffffffu, __fmul_rn(sum, up), 8 * t) : 0.0f;
     }
 
     // m: a maximum of the scores at most kSlack (log2) below the true one
@@ -834,12 +881,8 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
       take = take + 1 == T::kStages ? 0 : take + 1;
       const uint32_t par = src + T::kKStage + T::kVStage + g * 4;
       const int left = len - (p0 + i) * kPage;  // live positions from this page on
-      // scores, in two chains of products
-      float sc[NT][2][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int k = 0; k < 4; ++k) sc[nt][0][k] = sc[nt][1][k] = 0.0f;
+      // scores
+      int sc[NT][2][4];
       uint32_t kw[2][T::kKBytes / 4];
 #pragma unroll
       for (int h = 0; h < 2; ++h)
@@ -847,23 +890,28 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
         for (int j = 0; j < T::kKPieces; ++j)
           lds_piece<T::kKPiece>(src + ((h * T::kKPieces + j) * 32 + lane) * T::kKPiece, kw[h] + j * (T::kKPiece / 4));
 #pragma unroll
-      for (int w = 0; w < T::kKBytes / 4; ++w) {
+      for (int s = 0; s < T::kKSteps; ++s) {
+        uint32_t x[2], y[2];  // rows g and g + 8
         if constexpr (I4) {
-          uint32_t x[4], y[4];
-          nibbles_f16(kw[0][w], x);
-          nibbles_f16(kw[1][w], y);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(sc[nt][0], x[0], y[0], x[1], y[1], qf[nt][2 * w][0], qf[nt][2 * w][1]);
-            mma_f16(sc[nt][1], x[2], y[2], x[3], y[3], qf[nt][2 * w + 1][0], qf[nt][2 * w + 1][1]);
-          }
+          x[0] = kw[0][s] & 0x0f0f0f0fu;
+          x[1] = (kw[0][s] >> 4) & 0x0f0f0f0fu;
+          y[0] = kw[1][s] & 0x0f0f0f0fu;
+          y[1] = (kw[1][s] >> 4) & 0x0f0f0f0fu;
         } else {
-          uint32_t x[2], y[2];
-          bytes_f16(kw[0][w], &x[0], &x[1]);
-          bytes_f16(kw[1][w], &y[0], &y[1]);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(sc[nt][w & 1], x[0], y[0], x[1], y[1], qf[nt][w][0], qf[nt][w][1]);
+          x[0] = kw[0][2 * s];
+          x[1] = kw[0][2 * s + 1];
+          y[0] = kw[1][2 * s];
+          y[1] = kw[1][2 * s + 1];
         }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            if (s == 0)
+              mma_s8<true>(sc[nt][j], x[0], y[0], x[1], y[1], qf[nt][s][j][0], qf[nt][s][j][1]);
+            else
+              mma_s8<false>(sc[nt][j], x[0], y[0], x[1], y[1], qf[nt][s][j][0], qf[nt][s][j][1]);
+          }
       }
       const bool live0 = g < left, live1 = g + 8 < left;
       const float ks0 = lds_f32(par), ks1 = lds_f32(par + 32);
@@ -872,10 +920,10 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
       const float vs0 = live0 ? lds_f32(par + vpar) : 0.0f, vs1 = live1 ? lds_f32(par + vpar + 32) : 0.0f;
       float kz0 = 0.0f, kz1 = 0.0f, vz0 = 0.0f, vz1 = 0.0f;
       if constexpr (I4) {
-        kz0 = __fmaf_rn(8.0f, ks0, lds_f32(par + 64));
-        kz1 = __fmaf_rn(8.0f, ks1, lds_f32(par + 96));
-        vz0 = live0 ? __fmaf_rn(8.0f, vs0, lds_f32(par + 192)) : 0.0f;
-        vz1 = live1 ? __fmaf_rn(8.0f, vs1, lds_f32(par + 224)) : 0.0f;
+        kz0 = lds_f32(par + 64);
+        kz1 = lds_f32(par + 96);
+        vz0 = live0 ? lds_f32(par + 192) : 0.0f;
+        vz1 = live1 ? lds_f32(par + 224) : 0.0f;
       }
       // a scale of V above what the weights' power of two allows
       float vtop = fmaxf(vs0, vs1);
@@ -896,8 +944,11 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
       uint32_t wb[NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
-        float s0 = __fmul_rn(__fadd_rn(__fadd_rn(sc[nt][0][0], sc[nt][1][0]), __fadd_rn(sc[nt][0][1], sc[nt][1][1])), ks0);
-        float s1 = __fmul_rn(__fadd_rn(__fadd_rn(sc[nt][0][2], sc[nt][1][2]), __fadd_rn(sc[nt][0][3], sc[nt][1][3])), ks1);
+        // digits 3 and 2, 1 and 0: sums of at most 2^29
+        float s0 = __fmaf_rn((float)(sc[nt][0][0] * 256 + sc[nt][0][1]), 65536.0f, (float)(sc[nt][1][0] * 256 + sc[nt][1][1]));
+        float s1 = __fmaf_rn((float)(sc[nt][0][2] * 256 + sc[nt][0][3]), 65536.0f, (float)(sc[nt][1][2] * 256 + sc[nt][1][3]));
+        s0 = __fmul_rn(s0, ks0);
+        s1 = __fmul_rn(s1, ks1);
         if constexpr (I4) {
           s0 = __fmaf_rn(qsum[nt], kz0, s0);
           s1 = __fmaf_rn(qsum[nt], kz1, s1);
