@@ -1,9 +1,9 @@
 // kernels_kvq.cu — the quantised paged key-value cache: rows quantised into
 // their slots, rows read back, and GQA attention split over the context.
+#include "async.cuh"
 #include "kvq.cuh"
 
 #include <algorithm>
-#include <utility>
 
 namespace bitnet {
 
@@ -490,11 +490,17 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // larger one comes; a weight is at most 2^kSlack): a second term then still
 // holds 2^-30 of the largest weight.
 //
-// The order of dimensions inside a product is free, so a lane fetches wide
+// The order of dimensions inside a product is free, so a lane reads wide
 // pieces of a row for its K operand (HD/4 codes of two rows, the four lanes of
-// a row side by side) and its V operand (HD/8 codes of four rows).  They come
-// by cp.async into a ring that only the same lane reads, so a warp waits for
-// its own copies alone.
+// a row side by side) and its V operand (HD/8 codes of four rows).
+//
+// Each warp has a ring of pages of its own in shared memory.  One lane fetches
+// a page with two copies of the asynchronous copy engine, the codes as a tile
+// of 128-byte lines with their 16-byte pieces exchanged (128-byte swizzle), so
+// that the reads above meet no bank twice, and the parameters as they are.
+// Measured on a batch of 256 contexts of 128 to 4096 (I8), with the same bytes
+// asked for ahead: copies by each lane (cp.async) stop at 4.0 TB/s, since a
+// load that goes through L1 needs an entry there until it lands.
 //
 // Here the line of pages is cut into equal shares for the warps, not the
 // CTAs, so that no warp waits for another before its share is done.  The warps
@@ -519,50 +525,58 @@ struct MmaTile {
   static constexpr int kKBytes = kRow / 4;              // a lane's bytes of one K row
   static constexpr int kVBytes = kRow / 8;              // a lane's bytes of one V row
   static constexpr int kKPiece = kKBytes % 16 == 0 ? 16 : kKBytes % 8 == 0 ? 8 : 4;
-  static constexpr int kVPiece = kVBytes % 16 == 0 ? 16 : kVBytes % 8 == 0 ? 8 : 4;
+  static constexpr int kVPiece = kVBytes % 16 == 0 ? 16 : kVBytes % 8 == 0 ? 8 : kVBytes % 4 == 0 ? 4 : 2;
   static constexpr int kKCodes = kKPiece * (I4 ? 2 : 1);  // codes of a K piece
   static constexpr int kKPieces = kKBytes / kKPiece, kVPieces = kVBytes / kVPiece;
-  static constexpr int kKStage = 2 * kKBytes * 32, kVStage = 4 * kVBytes * 32;
+  static constexpr int kVWords = kVPiece >= 4 ? kVBytes / 4 : kVPieces;  // registers of a V row
+  static constexpr int kCodes = 2 * kPage * kRow;         // bytes of a page's codes
+  static constexpr int kTile = (kCodes + 1023) / 1024 * 1024;
   static constexpr int kParams = I4 ? 256 : 128;
-  static constexpr int kStage = kKStage + kVStage + kParams;
-  static constexpr int kStages = I4 ? 5 : 3;
+  static constexpr int kStages = kTile <= 1024 ? 8 : kTile <= 2048 ? 5 : 3;
+  static constexpr int kRing = kStages * kTile;                  // a warp's tiles
+  static constexpr int kSmem = kMmaWarps * kStages * (kTile + kParams);
   static constexpr int kKSteps = HD / 32, kMTiles = HD / 16;
   static constexpr int kPartStride = HD + 4;  // floats a head of a warp's partial result
 };
 
-template <int BYTES, int DST, int SRC>
-__device__ __forceinline__ void cp_async(uint32_t dst, const void* src) {
-  if constexpr (BYTES == 16)
-    asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;\n" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC) : "memory");
-  else
-    asm volatile("cp.async.ca.shared.global [%0 + %2], [%1 + %3], %4;\n" ::"r"(dst), "l"(src), "n"(DST), "n"(SRC), "n"(BYTES)
-                 : "memory");
+// Where byte x of a tile lies: 16-byte pieces of a 128-byte line are exchanged by the line's number.
+__device__ __forceinline__ int swizzled(int x) { return x ^ ((x >> 3) & 0x70); }
+
+// A tile of one block's codes, lines of 128 bytes, swizzled as above.
+__device__ __forceinline__ void tma_codes(uint32_t dst, const CUtensorMap* map, int block, uint32_t bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
+      " [%0], [%1, {%2, %2, %3}], [%4];\n" ::"r"(dst),
+      "l"((uint64_t)map), "r"(0), "r"(block), "r"(bar)
+      : "memory");
 }
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;\n" ::: "memory"); }
-template <int N>
-__device__ __forceinline__ void cp_async_wait() {
-  asm volatile("cp.async.wait_group %0;\n" ::"n"(N) : "memory");
+__device__ __forceinline__ void tma_bytes(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
+  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
+               "l"((uint64_t)src), "r"(bytes), "r"(bar)
+               : "memory");
 }
 template <int BYTES>
-__device__ __forceinline__ void lds_piece(uint32_t addr, uint32_t* w) {
-  if constexpr (BYTES == 16)
-    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];\n"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                 : "r"(addr)
-                 : "memory");
-  else if constexpr (BYTES == 8)
-    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(addr) : "memory");
-  else
-    asm volatile("ld.shared.u32 %0, [%1];\n" : "=r"(w[0]) : "r"(addr) : "memory");
+__device__ __forceinline__ void lds_piece(const uint8_t* p, uint32_t* w) {
+  if constexpr (BYTES == 16) {
+    const uint4 v = *(const uint4*)p;
+    w[0] = v.x;
+    w[1] = v.y;
+    w[2] = v.z;
+    w[3] = v.w;
+  } else if constexpr (BYTES == 8) {
+    const uint2 v = *(const uint2*)p;
+    w[0] = v.x;
+    w[1] = v.y;
+  } else if constexpr (BYTES == 4) {
+    w[0] = *(const uint32_t*)p;
+  } else {
+    w[0] = *(const uint16_t*)p;
+  }
 }
-__device__ __forceinline__ float lds_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared.f32 %0, [%1];\n" : "=f"(v) : "r"(addr) : "memory");
-  return v;
-}
+// c += product, fp16
 __device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -572,12 +586,12 @@ template <bool START>
 __device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                        uint32_t b1) {
   if constexpr (START)
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};\n"
         : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
   else
-    asm volatile(
+    asm(
         "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
         : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
@@ -703,27 +717,15 @@ struct WarpNote {
   int has0, ends0, far0;
 };
 
-// A lane's copies of one page's block: K rows g and g + 8, V rows 2t, 2t + 1,
-// 2t + 8 and 2t + 9 in pieces, and its part of the parameters.
-template <class T, size_t... IK, size_t... IV>
-__device__ __forceinline__ void copy_page(uint32_t dst, const uint8_t* block, int lane, int lane_k, int lane_v,
-                                          std::index_sequence<IK...>, std::index_sequence<IV...>) {
-  const uint32_t dk = dst + lane * T::kKPiece, dv = dst + lane * T::kVPiece;
-  const uint8_t *sk = block + lane_k, *sv = block + lane_v;
-  (cp_async<T::kKPiece, (int)IK * 32 * T::kKPiece,
-            8 * ((int)IK / T::kKPieces) * T::kRow + 4 * ((int)IK % T::kKPieces) * T::kKPiece>(dk, sk), ...);
-  (cp_async<T::kVPiece, T::kKStage + (int)IV * 32 * T::kVPiece,
-            (((int)IV / T::kVPieces) % 2 + ((int)IV / T::kVPieces) / 2 * 8) * T::kRow + (int)IV % T::kVPieces * T::kVPiece>(dv, sv), ...);
-  cp_async<T::kParams / 32, T::kKStage + T::kVStage, 2 * kPage * T::kRow>(dst + lane * (T::kParams / 32),
-                                                                          block + lane * (T::kParams / 32));
-}
-
 template <int HD, bool I4, int NT>
 __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
-    kvq_attend_mma_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int min_weight, int wide_q) {
+    kvq_attend_mma_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int min_weight, int wide_q,
+                          const __grid_constant__ CUtensorMap tmap) {
   using T = MmaTile<HD, I4>;
   constexpr int kThreads = kMmaWarps * 32;
-  extern __shared__ __align__(128) uint8_t ring[];
+  extern __shared__ __align__(1024) uint8_t ring[];
+  __shared__ __align__(8) uint64_t full[kMmaWarps][T::kStages];
+  __shared__ int gave_up;
   __shared__ Line<kThreads> line;
   __shared__ float ml[kMmaWarps][2][kMaxHeads][2];  // of a warp's slots 0 and 1
   __shared__ WarpNote notes[kMmaWarps];
@@ -735,6 +737,11 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
     int seq;
     if (row_context(c, R, r, max_len, &seq, a.status) == 0) write_empty_row(a, HD, r);
   }
+  if (lane == 0) {
+    for (int i = 0; i < T::kStages; ++i) mbar_init(smem_u32(&full[warp][i]), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+  }
+  if (tid == 0) gave_up = 0;
   const int each = (R.rows + kThreads - 1) / kThreads;
   measure_line<kThreads>(line, c, R, max_len, us.per_row, each, a.status);
   const long long total = line.before[kThreads];
@@ -753,10 +760,23 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
   int r = lo * each;
   long long base = line.before[lo];
   WarpNote note{-1, 0, 0, 0, 0};
-  uint8_t* const mine = ring + warp * (T::kStages * T::kStage);
-  const uint32_t mine_s = (uint32_t)__cvta_generic_to_shared(mine);
+  uint8_t* const mine = ring + warp * T::kRing;
+  uint8_t* const params = ring + kMmaWarps * T::kRing + warp * (T::kStages * T::kParams);
+  const uint32_t mine_s = smem_u32(mine), params_s = smem_u32(params), bar_s = smem_u32(&full[warp][0]);
   const float qscale = __fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)HD));
-  const int lane_k = g * T::kRow + t * T::kKPiece, lane_v = (kPage + 2 * t) * T::kRow + g * T::kVBytes;
+  // this lane's pieces in a tile
+  int at_k[2][T::kKPieces], at_v[4][T::kVPieces];
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int j = 0; j < T::kKPieces; ++j) at_k[h][j] = swizzled((g + 8 * h) * T::kRow + (4 * j + t) * T::kKPiece);
+#pragma unroll
+  for (int h = 0; h < 4; ++h)
+#pragma unroll
+    for (int j = 0; j < T::kVPieces; ++j)
+      at_v[h][j] = swizzled((kPage + 2 * t + (h & 1) + (h >> 1) * 8) * T::kRow + g * T::kVBytes + j * T::kVPiece);
+  int fill = 0, take = 0;      // stages, the next to fetch into and the next to use
+  uint32_t parity = 0;         // of the copies that `take` waits for
 
   while (at < end && r < R.rows) {
     int seq = 0;
@@ -779,28 +799,29 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
     const int32_t* row_table = c.table + (size_t)seq * c.per_seq + p0;
 
     // one page's copies; lane l of the ids holds page (block of 32) + l
-    int ids = 0, fill = 0;
+    int ids = 0;
     auto fetch = [&](int i) {
-      if (i < n_pages) {
-        if ((i & 31) == 0) {
-          ids = i + lane < n_pages ? row_table[i + lane] : 0;
-          if ((unsigned)ids >= (unsigned)c.pages) {
-            atomicOr(a.status, kStatusBadContext);
-            ids = 0;
-          }
+      if (i >= n_pages) return;
+      if ((i & 31) == 0) {
+        ids = i + lane < n_pages ? row_table[i + lane] : 0;
+        if ((unsigned)ids >= (unsigned)c.pages) {
+          atomicOr(a.status, kStatusBadContext);
+          ids = 0;
         }
-        const int page = __shfl_sync(0xffffffffu, ids, i & 31);
-        const uint8_t* block = c.pool + ((size_t)page * c.kv_heads + kvh) * (2 * kPage * T::kRow + T::kParams);
-        const uint32_t dst = mine_s + fill * T::kStage;
-        copy_page<T>(dst, block, lane, lane_k, lane_v, std::make_index_sequence<2 * T::kKPieces>{},
-                     std::make_index_sequence<4 * T::kVPieces>{});
-        fill = fill + 1 == T::kStages ? 0 : fill + 1;
       }
-      cp_async_commit();  // an empty group keeps the count of groups in step
+      const int block = __shfl_sync(0xffffffffu, ids, i & 31) * c.kv_heads + kvh;
+      if (lane == 0) {
+        const uint32_t bar = bar_s + fill * 8;
+        mbar_expect_tx(bar, T::kCodes + T::kParams);
+        tma_codes(mine_s + fill * T::kTile, &tmap, block, bar);
+        tma_bytes(params_s + fill * T::kParams, c.pool + (size_t)block * (T::kCodes + T::kParams) + T::kCodes,
+                  T::kParams, bar);
+      }
+      fill = fill + 1 == T::kStages ? 0 : fill + 1;
     };
     __syncwarp();
-#pragma unroll
-    for (int i = 0; i < T::kStages - 1; ++i) fetch(i);
+#pragma unroll 1
+    for (int i = 0; i < T::kStages; ++i) fetch(i);
 
     // q: this lane's columns are head g / 2 of each tile of four, digits 3 - g % 2 and 1 - g % 2
     uint32_t qf[NT][T::kKSteps][2][2];
@@ -872,14 +893,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
         for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.0f;
     }
 
-    int take = 0;
     for (int i = 0; i < n_pages; ++i) {
-      cp_async_wait<T::kStages - 2>();
-      __syncwarp();  // the parameters come from other lanes' copies; the stage before is free
-      fetch(i + T::kStages - 1);
-      const uint32_t src = mine_s + take * T::kStage;
-      take = take + 1 == T::kStages ? 0 : take + 1;
-      const uint32_t par = src + T::kKStage + T::kVStage + g * 4;
+      if (!mbar_wait(bar_s + take * 8, parity, &gave_up)) {
+        give_up(&gave_up, a.status);
+        at = end;  // nothing more is asked for
+        break;
+      }
+      const uint8_t* src = mine + take * T::kTile;
+      const float* par = (const float*)(params + take * T::kParams) + g;
       const int left = len - (p0 + i) * kPage;  // live positions from this page on
       // scores
       int sc[NT][2][4];
@@ -888,7 +909,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
       for (int h = 0; h < 2; ++h)
 #pragma unroll
         for (int j = 0; j < T::kKPieces; ++j)
-          lds_piece<T::kKPiece>(src + ((h * T::kKPieces + j) * 32 + lane) * T::kKPiece, kw[h] + j * (T::kKPiece / 4));
+          lds_piece<T::kKPiece>(src + at_k[h][j], kw[h] + j * (T::kKPiece / 4));
 #pragma unroll
       for (int s = 0; s < T::kKSteps; ++s) {
         uint32_t x[2], y[2];  // rows g and g + 8
@@ -914,16 +935,16 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
           }
       }
       const bool live0 = g < left, live1 = g + 8 < left;
-      const float ks0 = lds_f32(par), ks1 = lds_f32(par + 32);
-      constexpr int vpar = I4 ? 128 : 64;
+      const float ks0 = par[0], ks1 = par[8];
+      constexpr int vpar = I4 ? 32 : 16;
       // behind the context the bytes may be anything: no scale of theirs is used
-      const float vs0 = live0 ? lds_f32(par + vpar) : 0.0f, vs1 = live1 ? lds_f32(par + vpar + 32) : 0.0f;
+      const float vs0 = live0 ? par[vpar] : 0.0f, vs1 = live1 ? par[vpar + 8] : 0.0f;
       float kz0 = 0.0f, kz1 = 0.0f, vz0 = 0.0f, vz1 = 0.0f;
       if constexpr (I4) {
-        kz0 = lds_f32(par + 64);
-        kz1 = lds_f32(par + 96);
-        vz0 = live0 ? lds_f32(par + 192) : 0.0f;
-        vz1 = live1 ? lds_f32(par + 224) : 0.0f;
+        kz0 = par[16];
+        kz1 = par[24];
+        vz0 = live0 ? par[48] : 0.0f;
+        vz1 = live1 ? par[56] : 0.0f;
       }
       // a scale of V above what the weights' power of two allows
       float vtop = fmaxf(vs0, vs1);
@@ -976,40 +997,52 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
         wb[nt][1] = transpose8x8(two_terms(__fmul_rn(w1, __fmul_rn(vs1, vf))));
       }
       // output
-      uint32_t vw[4][T::kVBytes / 4];
+      uint32_t vw[4][T::kVWords];
 #pragma unroll
       for (int h = 0; h < 4; ++h)
 #pragma unroll
         for (int j = 0; j < T::kVPieces; ++j)
-          lds_piece<T::kVPiece>(src + T::kKStage + ((h * T::kVPieces + j) * 32 + lane) * T::kVPiece,
-                                vw[h] + j * (T::kVPiece / 4));
+          lds_piece<T::kVPiece>(src + at_v[h][j], vw[h] + j * (T::kVPiece >= 4 ? T::kVPiece / 4 : 1));
 #pragma unroll
-      for (int w = 0; w < T::kVBytes / 4; ++w) {
+      for (int w = 0; w < T::kVBytes / 2; ++w) {
+        // two bytes each of two rows, so that a widened pair is one dimension at two positions
+        const int word = T::kVPiece >= 4 ? w / 2 : w, sel = T::kVPiece >= 4 && w % 2 ? 0x7632 : 0x5410;
+        const uint32_t p = __byte_perm(vw[0][word], vw[1][word], sel), q = __byte_perm(vw[2][word], vw[3][word], sel);
+        if constexpr (I4) {
+          uint32_t x[4], y[4];
+          nibbles_f16(p, x);
+          nibbles_f16(q, y);
 #pragma unroll
-        for (int half = 0; half < 2; ++half) {
-          // the halves of two rows' words, so that a widened pair is one dimension at two positions
-          const uint32_t p = __byte_perm(vw[0][w], vw[1][w], half ? 0x7632 : 0x5410);
-          const uint32_t q = __byte_perm(vw[2][w], vw[3][w], half ? 0x7632 : 0x5410);
-          if constexpr (I4) {
-            uint32_t x[4], y[4];
-            nibbles_f16(p, x);
-            nibbles_f16(q, y);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(o[nt][4 * w + 2 * half], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
-              mma_f16(o[nt][4 * w + 2 * half + 1], x[2], x[3], y[2], y[3], wb[nt][0], wb[nt][1]);
-            }
-          } else {
-            uint32_t x[2], y[2];
-            bytes_f16(p, &x[0], &x[1]);
-            bytes_f16(q, &y[0], &y[1]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][2 * w + half], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            mma_f16(o[nt][2 * w], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
+            mma_f16(o[nt][2 * w + 1], x[2], x[3], y[2], y[3], wb[nt][0], wb[nt][1]);
           }
+        } else {
+          uint32_t x[2], y[2];
+          bytes_f16(p, &x[0], &x[1]);
+          bytes_f16(q, &y[0], &y[1]);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][w], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
         }
       }
+      __syncwarp();  // every lane has read the stage
+      fetch(i + T::kStages);
+      if (++take == T::kStages) {
+        take = 0;
+        parity ^= 1;
+      }
     }
-    cp_async_wait<0>();
+    if (gave_up) {
+      // copies still in flight land (or the wait for each runs out) before the CTA may go
+      while (take != fill) {
+        mbar_wait(bar_s + take * 8, parity, nullptr);
+        if (++take == T::kStages) {
+          take = 0;
+          parity ^= 1;
+        }
+      }
+      break;
+    }
 
     const bool begins = p0 == 0, ends = p1 == pages;
     const float back = __fdiv_rn(1.0f, vf);
@@ -1059,86 +1092,134 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
   if (lane == 0) notes[warp] = note;
   __syncthreads();
 
-  // Join what the CTA's warps left.  Chain -1 is what came in from the share
-  // before, chain w the unit that begins in warp w's share.
-  ShareMeta out{-1, 0, 0, 0};
-  for (int chain = -1; chain < kMmaWarps; ++chain) {
+  // Join what the CTA's warps left.  Chain w is the unit that begins in warp
+  // w's share and ends later, chain -1 what came in from the share before; a
+  // warp joins one head of one chain at a time.
+  if (tid == 0) {
+    ShareMeta out{-1, 0, 0, 0};
+    for (int w = 0; w < kMmaWarps; ++w) {
+      if (notes[w].ends0) {
+        out.row = -1;  // what was open has ended
+        out.ends |= notes[0].has0;
+      }
+      if (notes[w].row >= 0) {
+        out.row = notes[w].row;
+        out.unit = notes[w].unit;
+      }
+    }
+    ((ShareMeta*)a.space)[share] = out;
+  }
+  for (int job = warp; job < (kMmaWarps + 1) * us.heads; job += kMmaWarps) {
+    const int chain = job / us.heads - 1, h = job % us.heads;
     const bool head = chain < 0;
     if (head ? !notes[0].has0 : notes[chain].row < 0) continue;
     const int from = chain + 1;  // the warps whose slot 0 belongs to it: [from, to)
     int to = from;
     bool ends = false;
     while (to < kMmaWarps && !ends) ends = notes[to++].ends0;
-    const int row = head ? -1 : notes[chain].row, unit = head ? 0 : notes[chain].unit;
     int kvh, h0 = 0, heads = us.heads;
-    if (!head) unit_heads(us, a.nh, c.kv_heads, unit, &kvh, &h0, &heads);
-    float* dst = share_slot(a.space, shares, share, head ? 0 : 1, HD, us);
-    for (int i = tid; i < heads * HD; i += kThreads) {
-      const int h = i / HD, d = i % HD, at_part = h * T::kPartStride + d;
-      float M = head ? -INFINITY : ml[max(chain, 0)][1][h][0];
-      for (int w = from; w < to; ++w) M = fmaxf(M, ml[w][0][h][0]);
-      float L = 0.0f, sum = 0.0f;
-      if (!head) {
-        const float f = exp2_approx(__fsub_rn(ml[chain][1][h][0], M));
-        L = __fmul_rn(ml[chain][1][h][1], f);
-        sum = __fmul_rn(((const float*)(ring + chain * (T::kStages * T::kStage)))[at_part], f);
-      }
-      for (int w = from; w < to; ++w) {
-        const float f = exp2_approx(__fsub_rn(ml[w][0][h][0], M));
-        const float* part = notes[w].far0 ? warp_slot(a.space, shares, share * kMmaWarps + w, HD, us)
-                                          : (const float*)(ring + w * (T::kStages * T::kStage));
-        L = __fmaf_rn(ml[w][0][h][1], f, L);
-        sum = __fmaf_rn(part[at_part], f, sum);
-      }
-      if (!head && ends) {
-        store_elem(a.out, (size_t)row * a.ldo + (size_t)h0 * HD + i, a.bf16, __fdiv_rn(sum, L));
-        if (a.lse && d == 0) a.lse[(size_t)row * a.nh + h0 + h] = lse_of(M, L);
-      } else {
-        dst[h * (HD + 2) + d] = sum;
-        if (d == 0) {
-          dst[h * (HD + 2) + HD] = M;
-          dst[h * (HD + 2) + HD + 1] = L;
-        }
+    if (!head) unit_heads(us, a.nh, c.kv_heads, notes[chain].unit, &kvh, &h0, &heads);
+    if (h >= heads) continue;
+    // piece 0 is the chain's own (none for the head), piece 1 + i warp from + i's slot 0
+    float M = head ? -INFINITY : ml[chain][1][h][0];
+    for (int w = from; w < to; ++w) M = fmaxf(M, ml[w][0][h][0]);
+    float L = 0.0f, sum[HD / 32], f[kMmaWarps + 1];
+    const float* part[kMmaWarps + 1];
+#pragma unroll
+    for (int i = 0; i <= kMmaWarps; ++i) {
+      const int w = from + i - 1;
+      const bool there = i ? w < to : !head;
+      part[i] = nullptr;
+      f[i] = 0.0f;
+      if (there) {
+        const float* v = ml[w][i ? 0 : 1][h];
+        f[i] = exp2_approx(__fsub_rn(v[0], M));
+        L = __fmaf_rn(v[1], f[i], L);
+        part[i] = (i && notes[w].far0 ? warp_slot(a.space, shares, share * kMmaWarps + w, HD, us)
+                                      : (const float*)(ring + w * T::kRing)) + h * T::kPartStride;
       }
     }
-    if (head) {
-      out.ends = ends;
-    } else if (!ends) {
-      out.row = row;
-      out.unit = unit;
+#pragma unroll
+    for (int k = 0; k < HD / 32; ++k) sum[k] = 0.0f;
+#pragma unroll
+    for (int i = 0; i <= kMmaWarps; ++i)
+      if (part[i])
+#pragma unroll
+        for (int k = 0; k < HD / 32; ++k) sum[k] = __fmaf_rn(part[i][lane + 32 * k], f[i], sum[k]);
+    if (!head && ends) {
+      const float inv = __fdiv_rn(1.0f, L);
+      const size_t row = notes[chain].row;
+#pragma unroll
+      for (int k = 0; k < HD / 32; ++k)
+        store_elem(a.out, row * a.ldo + (size_t)(h0 + h) * HD + lane + 32 * k, a.bf16, __fmul_rn(sum[k], inv));
+      if (a.lse && lane == 0) a.lse[row * a.nh + h0 + h] = lse_of(M, L);
+    } else {
+      float* dst = share_slot(a.space, shares, share, head ? 0 : 1, HD, us) + h * (HD + 2);
+#pragma unroll
+      for (int k = 0; k < HD / 32; ++k) dst[lane + 32 * k] = sum[k];
+      if (lane == 0) {
+        dst[HD] = M;
+        dst[HD + 1] = L;
+      }
     }
   }
-  if (tid == 0) ((ShareMeta*)a.space)[share] = out;
 }
 
-// Joins the partial results of the unit that begins in this CTA's share and ends in a later one.
-__global__ void __launch_bounds__(256) kvq_join_kernel(KvqView c, KvqAttend a, int shares) {
+// Joins the partial results of the unit that begins in this CTA's share and ends
+// in a later one, one head a CTA (blockIdx.y): the factors of all pieces
+// first, by all threads at once, then the sums, each group of threads over a
+// share of the pieces.
+constexpr int kJoinThreads = 256;
+__global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(KvqView c, KvqAttend a, int shares) {
+  __shared__ float factor[kAttendCtas];
+  __shared__ float red[kJoinThreads / 32];
+  __shared__ float sums[kJoinThreads];
+  __shared__ int last_sh;
   pdl_wait();
   const ShareMeta* meta = (const ShareMeta*)after_wait((uint8_t*)a.space);
-  const int share = blockIdx.x, hd = c.hd;
+  const int share = blockIdx.x, h = blockIdx.y, hd = c.hd, tid = threadIdx.x;
   const ShareMeta own = meta[share];
   if (own.row < 0) return;
   const Units us = units_of(a.nh, c.kv_heads);
   int kvh, h0, heads;
   unit_heads(us, a.nh, c.kv_heads, own.unit, &kvh, &h0, &heads);
-  int last = share + 1;
-  while (last < shares - 1 && !meta[last].ends) ++last;
-  for (int i = threadIdx.x; i < heads * hd; i += blockDim.x) {
-    const int h = i / hd, d = i % hd;
-    const float* p = share_slot(a.space, shares, share, 1, hd, us) + h * (hd + 2);
-    float M = p[hd], L = p[hd + 1], o = p[d];
-    for (int s = share + 1; s <= last; ++s) {
-      p = share_slot(a.space, shares, s, 0, hd, us) + h * (hd + 2);
-      const float m = p[hd], l = p[hd + 1];
-      if (l == 0.0f) continue;
-      const float mn = fmaxf(M, m), f = exp2f(__fsub_rn(M, mn)), g = exp2f(__fsub_rn(m, mn));
-      L = __fmaf_rn(L, L == 0.0f ? 0.0f : f, __fmul_rn(l, g));
-      o = __fmaf_rn(o, L == 0.0f ? 0.0f : f, __fmul_rn(p[d], g));
-      M = mn;
+  if (h >= heads) return;
+  if (tid == 0) last_sh = shares - 1;
+  __syncthreads();
+  for (int s = share + 1 + tid; s < shares; s += kJoinThreads)
+    if (meta[s].ends) {
+      atomicMin(&last_sh, s);
+      break;
     }
-    store_elem(a.out, (size_t)own.row * a.ldo + (size_t)h0 * hd + i, a.bf16, __fdiv_rn(o, L));
-    if (a.lse && d == 0) a.lse[(size_t)own.row * a.nh + h0 + h] = lse_of(M, L);
+  __syncthreads();
+  const int n = last_sh - share + 1;  // pieces: slot 1 of this share, slot 0 of the later ones
+  auto piece = [&](int i) { return share_slot(a.space, shares, share + i, i == 0, hd, us) + h * (hd + 2); };
+  float M = -INFINITY;
+  for (int i = tid; i < n; i += kJoinThreads) M = fmaxf(M, piece(i)[hd]);
+  M = block_reduce(M, [](float x, float y) { return fmaxf(x, y); }, red);
+  float L = 0.0f;
+  for (int i = tid; i < n; i += kJoinThreads) {
+    const float* p = piece(i);
+    const float f = p[hd + 1] == 0.0f ? 0.0f : exp2_approx(__fsub_rn(p[hd], M));
+    factor[i] = f;
+    L = __fmaf_rn(p[hd + 1], f, L);
   }
+  __syncthreads();
+  L = block_reduce(L, [](float x, float y) { return __fadd_rn(x, y); }, red);
+  // threads over dimensions, and groups of threads over the pieces
+  static_assert(kJoinThreads >= kKvqMaxHd, "a thread a dimension");
+  const int groups = kJoinThreads / hd, d = tid % hd, grp = tid / hd;
+  float o = 0.0f;
+  if (grp < groups)
+#pragma unroll 8
+    for (int i = grp; i < n; i += groups) o = __fmaf_rn(piece(i)[d], factor[i], o);
+  sums[tid] = o;
+  __syncthreads();
+  if (tid < hd) {
+    for (int k = 1; k < groups; ++k) o = __fadd_rn(o, sums[k * hd + tid]);
+    store_elem(a.out, (size_t)own.row * a.ldo + (size_t)(h0 + h) * hd + d, a.bf16, __fdiv_rn(o, L));
+  }
+  if (a.lse && tid == 0) a.lse[(size_t)own.row * a.nh + h0 + h] = lse_of(M, L);
 }
 
 }  // namespace
@@ -1170,31 +1251,50 @@ size_t kvq_attend_space(int nh, int kv_heads, int hd) {
 namespace {
 constexpr int kMinWeight = kUnitCost + 2;  // the least share of a warp
 
-template <int HD, bool I4, int NT>
-void launch_mma(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, int wide_q, cudaStream_t st) {
-  using T = MmaTile<HD, I4>;
-  constexpr int smem = kMmaWarps * T::kStages * T::kStage;
-  static_assert(T::kStages * T::kStage >= NT * 4 * T::kPartStride * 4, "a warp's ring holds its partial result");
-  auto* kernel = kvq_attend_mma_kernel<HD, I4, NT>;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-  const int shares = NT == 1 ? kMmaShares : kMmaShares / 2;
-  kernel<<<shares, kMmaWarps * 32, smem, st>>>(c, r, a, max_len, kMinWeight, wide_q);
-  launch_pdl(kvq_join_kernel, dim3(shares), dim3(256), 0, st, c, a, shares);
-  count_launch(2);
+// The codes of every block as a tensor of 128-byte lines: [blocks][lines][128].
+template <class T>
+bool codes_map(const KvqView& c, CUtensorMap* map) {
+  const cuuint64_t dims[3] = {128, T::kCodes / 128, (cuuint64_t)c.pages * c.kv_heads};
+  const cuuint64_t strides[2] = {128, T::kCodes + T::kParams};
+  const cuuint32_t box[3] = {128, T::kCodes / 128, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c.pool, dims, strides, box, estr,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
-using LaunchMma = void (*)(const KvqView&, const KvqRows&, const KvqAttend&, int, int, cudaStream_t);
+
+template <int HD, bool I4, int NT>
+bool launch_mma(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, int wide_q, cudaStream_t st) {
+  using T = MmaTile<HD, I4>;
+  static_assert(T::kRing >= NT * 4 * T::kPartStride * 4, "a warp's ring holds its partial result");
+  CUtensorMap map;
+  if (!codes_map<T>(c, &map)) return false;
+  auto* kernel = kvq_attend_mma_kernel<HD, I4, NT>;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
+  const int shares = NT == 1 ? kMmaShares : kMmaShares / 2;
+  kernel<<<shares, kMmaWarps * 32, T::kSmem, st>>>(c, r, a, max_len, kMinWeight, wide_q, map);
+  launch_pdl(kvq_join_kernel, dim3(shares, units_of(a.nh, c.kv_heads).heads), dim3(kJoinThreads), 0, st, c, a, shares);
+  count_launch(2);
+  return true;
+}
+using LaunchMma = bool (*)(const KvqView&, const KvqRows&, const KvqAttend&, int, int, cudaStream_t);
 // The tensor-core kernel for a cache and number of heads a unit, or null.
+template <int HD>
+LaunchMma mma_of(bool i4, bool two) {
+  return i4 ? (two ? launch_mma<HD, true, 2> : launch_mma<HD, true, 1>)
+            : (two ? launch_mma<HD, false, 2> : launch_mma<HD, false, 1>);
+}
 LaunchMma mma_for(const KvqView& c, int heads) {
-  const bool two = heads > 4;
+  if ((size_t)c.pages * c.kv_heads >= (1ull << 31) || !tensor_map_encoder()) return nullptr;
   switch (c.hd) {
+    case 32:
+      return mma_of<32>(c.i4, heads > 4);
     case 64:
-      return c.i4 ? (two ? launch_mma<64, true, 2> : launch_mma<64, true, 1>)
-                  : (two ? launch_mma<64, false, 2> : launch_mma<64, false, 1>);
+      return mma_of<64>(c.i4, heads > 4);
     case 96:
-      return c.i4 ? nullptr : (two ? launch_mma<96, false, 2> : launch_mma<96, false, 1>);
+      return mma_of<96>(c.i4, heads > 4);
     case 128:
-      return c.i4 ? (two ? launch_mma<128, true, 2> : launch_mma<128, true, 1>)
-                  : (two ? launch_mma<128, false, 2> : launch_mma<128, false, 1>);
+      return mma_of<128>(c.i4, heads > 4);
   }
   return nullptr;
 }
@@ -1209,12 +1309,11 @@ void launch_kvq_attend(const KvqView& c, const KvqRows& r, const KvqAttend& a, i
   const Units us = units_of(a.nh, c.kv_heads);
   if (LaunchMma launch = mma_for(c, us.heads)) {
     const int wide_q = !a.bf16 && (uintptr_t)a.q % 16 == 0 && a.ldq % 4 == 0;
-    launch(c, r, a, max_len, wide_q, st);
-    return;
+    if (launch(c, r, a, max_len, wide_q, st)) return;
   }
   const size_t smem = ((size_t)us.heads * c.hd + kPlainWarps * us.heads * (c.hd + 2)) * sizeof(float);
   kvq_attend_plain_kernel<<<kAttendCtas, kPlainWarps * 32, smem, st>>>(c, r, a, max_len);
-  kvq_join_kernel<<<kAttendCtas, 256, 0, st>>>(c, a, kAttendCtas);
+  kvq_join_kernel<<<dim3(kAttendCtas, us.heads), kJoinThreads, 0, st>>>(c, a, kAttendCtas);
   count_launch(2);
 }
 
