@@ -471,7 +471,7 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // ---------------------------------------------------------------------------
 // The tensor-core form, for head sizes of 64, 96 and 128 (I4: 64, 128).
 //
-// One warp multiplies one page at a time, its 16 positions (scores) or 16
+// One warp multiplies a page (two of them in turn), its 16 positions (scores) or 16
 // dimensions (output) being the M of a product, and four heads its N.
 //   S[pos][head] = K codes . q        m16n8k32, 8-bit integers
 //   O[dim][head] += V codes^T . w     m16n8k16, fp16 with f32 sums
@@ -513,13 +513,13 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // by cp.async into a ring that only the same lane reads, so a warp waits for
 // its own copies alone.
 // ---------------------------------------------------------------------------
-constexpr int kMmaWarps = 8;
+constexpr int kMmaMaxWarps = 8;
 constexpr int kMmaShares = 296;  // two CTAs an SM with up to four heads a unit, else one
 // How far a score may exceed the running maximum before the sums are rescaled
 // (log2): rescaling then all but stops after a unit's first pages.
 constexpr float kSlack = 6.0f;
 
-template <int HD, bool I4>
+template <int HD, bool I4, int NT>
 struct MmaTile {
   static constexpr int kRow = I4 ? HD / 2 : HD;         // bytes of a row's codes
   static constexpr int kKBytes = kRow / 4;              // a lane's bytes of one K row
@@ -532,9 +532,12 @@ struct MmaTile {
   static constexpr int kCodes = 2 * kPage * kRow;         // bytes of a page's codes
   static constexpr int kTile = (kCodes + 1023) / 1024 * 1024;
   static constexpr int kParams = I4 ? 256 : 128;
-  static constexpr int kStages = kTile <= 1024 ? 8 : kTile <= 2048 ? 5 : 3;
-  static constexpr int kRing = kStages * kTile;                  // a warp's tiles
-  static constexpr int kSmem = kMmaWarps * kStages * (kTile + kParams);
+  // Warps a CTA and stages (of two pages) a warp: what shared memory holds
+  // twice an SM (once with NT = 2).
+  static constexpr int kWarps = NT == 1 && kTile > 3 * 1024 ? 6 : kMmaMaxWarps;
+  static constexpr int kStages = NT == 2 ? 3 : kTile <= 1024 ? 4 : kRow == 64 && !I4 ? 3 : 2;
+  static constexpr int kRing = kStages * 2 * kTile;  // a warp's tiles
+  static constexpr int kSmem = kWarps * kStages * 2 * (kTile + kParams);
   static constexpr int kKSteps = HD / 32, kMTiles = HD / 16;
   static constexpr int kPartStride = HD + 4;  // floats a head of a warp's partial result
 };
@@ -626,9 +629,9 @@ __device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c
   asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(r) : "r"(a), "r"(b), "r"(c));
   return r;
 }
-__device__ __forceinline__ float exp2_approx(float x) {  // within 2^-22
+__device__ __forceinline__ float exp2_approx(float x) {  // within 2^-22; results below 2^-126 are 0
   float r;
-  asm("ex2.approx.f32 %0, %1;\n" : "=f"(r) : "f"(x));
+  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
   return r;
 }
 // x as two fp16 terms, the larger in the low half.
@@ -718,11 +721,11 @@ struct WarpNote {
 };
 
 template <int HD, bool I4, int NT>
-__global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
+__global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 : 1)
     kvq_attend_mma_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int min_weight, int wide_q,
                           const __grid_constant__ CUtensorMap tmap) {
-  using T = MmaTile<HD, I4>;
-  constexpr int kThreads = kMmaWarps * 32;
+  using T = MmaTile<HD, I4, NT>;
+  constexpr int kMmaWarps = T::kWarps, kThreads = kMmaWarps * 32;
   extern __shared__ __align__(1024) uint8_t ring[];
   __shared__ __align__(8) uint64_t full[kMmaWarps][T::kStages];
   __shared__ int gave_up;
@@ -761,7 +764,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
   long long base = line.before[lo];
   WarpNote note{-1, 0, 0, 0, 0};
   uint8_t* const mine = ring + warp * T::kRing;
-  uint8_t* const params = ring + kMmaWarps * T::kRing + warp * (T::kStages * T::kParams);
+  uint8_t* const params = ring + kMmaWarps * T::kRing + warp * (T::kStages * 2 * T::kParams);
   const uint32_t mine_s = smem_u32(mine), params_s = smem_u32(params), bar_s = smem_u32(&full[warp][0]);
   const float qscale = __fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)HD));
   // this lane's pieces in a tile
@@ -798,7 +801,7 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
     const int n_pages = p1 - p0;
     const int32_t* row_table = c.table + (size_t)seq * c.per_seq + p0;
 
-    // one page's copies; lane l of the ids holds page (block of 32) + l
+    // the copies of pages i and i + 1; lane l of the ids holds page (block of 32) + l
     int ids = 0;
     auto fetch = [&](int i) {
       if (i >= n_pages) return;
@@ -809,19 +812,26 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
           ids = 0;
         }
       }
-      const int block = __shfl_sync(0xffffffffu, ids, i & 31) * c.kv_heads + kvh;
+      const int first_block = __shfl_sync(0xffffffffu, ids, i & 31) * c.kv_heads + kvh;
+      const int second_block = __shfl_sync(0xffffffffu, ids, (i + 1) & 31) * c.kv_heads + kvh;
       if (lane == 0) {
-        const uint32_t bar = bar_s + fill * 8;
-        mbar_expect_tx(bar, T::kCodes + T::kParams);
-        tma_codes(mine_s + fill * T::kTile, &tmap, block, bar);
-        tma_bytes(params_s + fill * T::kParams, c.pool + (size_t)block * (T::kCodes + T::kParams) + T::kCodes,
-                  T::kParams, bar);
+        const uint32_t bar = bar_s + fill * 8, tile = mine_s + fill * (2 * T::kTile);
+        const uint32_t par = params_s + fill * (2 * T::kParams);
+        const bool both = i + 1 < n_pages;
+        mbar_expect_tx(bar, (T::kCodes + T::kParams) << both);
+        tma_codes(tile, &tmap, first_block, bar);
+        tma_bytes(par, c.pool + (size_t)first_block * (T::kCodes + T::kParams) + T::kCodes, T::kParams, bar);
+        if (both) {
+          tma_codes(tile + T::kTile, &tmap, second_block, bar);
+          tma_bytes(par + T::kParams, c.pool + (size_t)second_block * (T::kCodes + T::kParams) + T::kCodes,
+                    T::kParams, bar);
+        }
       }
       fill = fill + 1 == T::kStages ? 0 : fill + 1;
     };
     __syncwarp();
 #pragma unroll 1
-    for (int i = 0; i < T::kStages; ++i) fetch(i);
+    for (int i = 0; i < T::kStages; ++i) fetch(2 * i);
 
     // q: this lane's columns are head g / 2 of each tile of four, digits 3 - g % 2 and 1 - g % 2
     uint32_t qf[NT][T::kKSteps][2][2];
@@ -880,12 +890,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
       qsum[nt] = I4 ? __shfl_sync(0xffffffffu, __fmul_rn(sum, up), 8 * t) : 0.0f;
     }
 
-    // m: a maximum of the scores at most kSlack (log2) below the true one
-    float m[NT], l[NT], zsum[NT], o[NT][T::kMTiles][4];
+    // Scores stay in the units of the integer products times their scales;
+    // qs (> 0) takes them to log2.  m is a maximum of theirs that lies at most
+    // kSlack / qs below the true one, mq = m * qs.
+    float m[NT], mq[NT], limit[NT], l[NT], zsum[NT], o[NT][T::kMTiles][4];
     float vf = __uint_as_float(247u << 23);  // the weights' power of two
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-      m[nt] = -INFINITY;
+      m[nt] = mq[nt] = limit[nt] = -INFINITY;
       l[nt] = zsum[nt] = 0.0f;
 #pragma unroll
       for (int i = 0; i < T::kMTiles; ++i)
@@ -893,140 +905,153 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
         for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.0f;
     }
 
-    for (int i = 0; i < n_pages; ++i) {
+    for (int i = 0; i < n_pages; i += 2) {
       if (!mbar_wait(bar_s + take * 8, parity, &gave_up)) {
         give_up(&gave_up, a.status);
         at = end;  // nothing more is asked for
         break;
       }
-      const uint8_t* src = mine + take * T::kTile;
-      const float* par = (const float*)(params + take * T::kParams) + g;
-      const int left = len - (p0 + i) * kPage;  // live positions from this page on
-      // scores
-      int sc[NT][2][4];
-      uint32_t kw[2][T::kKBytes / 4];
+      const uint8_t* src = mine + take * (2 * T::kTile);
+      const float* par = (const float*)(params + take * (2 * T::kParams)) + g;
+      // live positions from the first page on; with an odd number of pages the
+      // second tile of the last pair holds what was there before
+      const int left = min(len - (p0 + i) * kPage, (n_pages - i) * kPage);
+      constexpr int kParFloats = T::kParams / 4, vpar = I4 ? 32 : 16;
+      float raw[2][NT][2], vs[2][2], vz[2][2];  // [page][..][slot g or g + 8]
+      bool again = false;
+      float vtop = 0.0f;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
+      for (int pg = 0; pg < 2; ++pg) {
+        // scores
+        int sc[NT][2][4];
+        uint32_t kw[2][T::kKBytes / 4];
 #pragma unroll
-        for (int j = 0; j < T::kKPieces; ++j)
-          lds_piece<T::kKPiece>(src + at_k[h][j], kw[h] + j * (T::kKPiece / 4));
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int s = 0; s < T::kKSteps; ++s) {
-        uint32_t x[2], y[2];  // rows g and g + 8
-        if constexpr (I4) {
-          x[0] = kw[0][s] & 0x0f0f0f0fu;
-          x[1] = (kw[0][s] >> 4) & 0x0f0f0f0fu;
-          y[0] = kw[1][s] & 0x0f0f0f0fu;
-          y[1] = (kw[1][s] >> 4) & 0x0f0f0f0fu;
-        } else {
-          x[0] = kw[0][2 * s];
-          x[1] = kw[0][2 * s + 1];
-          y[0] = kw[1][2 * s];
-          y[1] = kw[1][2 * s + 1];
+          for (int j = 0; j < T::kKPieces; ++j)
+            lds_piece<T::kKPiece>(src + pg * T::kTile + at_k[h][j], kw[h] + j * (T::kKPiece / 4));
+#pragma unroll
+        for (int s = 0; s < T::kKSteps; ++s) {
+          uint32_t x[2], y[2];  // rows g and g + 8
+          if constexpr (I4) {
+            x[0] = kw[0][s] & 0x0f0f0f0fu;
+            x[1] = (kw[0][s] >> 4) & 0x0f0f0f0fu;
+            y[0] = kw[1][s] & 0x0f0f0f0fu;
+            y[1] = (kw[1][s] >> 4) & 0x0f0f0f0fu;
+          } else {
+            x[0] = kw[0][2 * s];
+            x[1] = kw[0][2 * s + 1];
+            y[0] = kw[1][2 * s];
+            y[1] = kw[1][2 * s + 1];
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              if (s == 0)
+                mma_s8<true>(sc[nt][j], x[0], y[0], x[1], y[1], qf[nt][s][j][0], qf[nt][s][j][1]);
+              else
+                mma_s8<false>(sc[nt][j], x[0], y[0], x[1], y[1], qf[nt][s][j][0], qf[nt][s][j][1]);
+            }
         }
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
+        for (int k = 0; k < 2; ++k) {
+          const bool live = pg * kPage + 8 * k + g < left;
+          const float* pp = par + pg * kParFloats + 8 * k;
+          const float ks = pp[0], kz = I4 ? pp[16] : 0.0f;
+          // behind the context the bytes may be anything: no scale of theirs is used
+          vs[pg][k] = live ? pp[vpar] : 0.0f;
+          vz[pg][k] = I4 && live ? pp[vpar + 16] : 0.0f;
+          vtop = fmaxf(vtop, vs[pg][k]);
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            if (s == 0)
-              mma_s8<true>(sc[nt][j], x[0], y[0], x[1], y[1], qf[nt][s][j][0], qf[nt][s][j][1]);
-            else
-              mma_s8<false>(sc[nt][j], x[0], y[0], x[1], y[1], qf[nt][s][j][0], qf[nt][s][j][1]);
+          for (int nt = 0; nt < NT; ++nt) {
+            // digits 3 and 2, 1 and 0: sums of at most 2^29
+            float x = __fmaf_rn((float)(sc[nt][0][2 * k] * 256 + sc[nt][0][2 * k + 1]), 65536.0f,
+                                (float)(sc[nt][1][2 * k] * 256 + sc[nt][1][2 * k + 1]));
+            x = I4 ? __fmaf_rn(qsum[nt], kz, __fmul_rn(x, ks)) : __fmul_rn(x, ks);
+            raw[pg][nt][k] = live ? x : -INFINITY;
+            again |= raw[pg][nt][k] > limit[nt];
           }
+        }
       }
-      const bool live0 = g < left, live1 = g + 8 < left;
-      const float ks0 = par[0], ks1 = par[8];
-      constexpr int vpar = I4 ? 32 : 16;
-      // behind the context the bytes may be anything: no scale of theirs is used
-      const float vs0 = live0 ? par[vpar] : 0.0f, vs1 = live1 ? par[vpar + 8] : 0.0f;
-      float kz0 = 0.0f, kz1 = 0.0f, vz0 = 0.0f, vz1 = 0.0f;
-      if constexpr (I4) {
-        kz0 = par[16];
-        kz1 = par[24];
-        vz0 = live0 ? par[48] : 0.0f;
-        vz1 = live1 ? par[56] : 0.0f;
-      }
-      // a scale of V above what the weights' power of two allows
-      float vtop = fmaxf(vs0, vs1);
-      if (__any_sync(0xffffffffu, __fmul_rn(vtop, vf) > 512.0f)) {
+      // a score above the slack, or a scale of V above what the weights' power of two allows
+      again |= __fmul_rn(vtop, vf) > 512.0f;
+      if (__any_sync(0xffffffffu, again)) {
 #pragma unroll
         for (int b = 4; b < 32; b <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, b));
-        const int e = min(max((int)(__float_as_uint(vtop) >> 23), 18), 255);
-        const float nf = __uint_as_float((uint32_t)(259 - e) << 23);
-        const float f = __fdiv_rn(nf, vf);
-        vf = nf;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < T::kMTiles; ++k)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[nt][k][j] = __fmul_rn(o[nt][k][j], f);
-      }
-      uint32_t wb[NT][2];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        // digits 3 and 2, 1 and 0: sums of at most 2^29
-        float s0 = __fmaf_rn((float)(sc[nt][0][0] * 256 + sc[nt][0][1]), 65536.0f, (float)(sc[nt][1][0] * 256 + sc[nt][1][1]));
-        float s1 = __fmaf_rn((float)(sc[nt][0][2] * 256 + sc[nt][0][3]), 65536.0f, (float)(sc[nt][1][2] * 256 + sc[nt][1][3]));
-        s0 = __fmul_rn(s0, ks0);
-        s1 = __fmul_rn(s1, ks1);
-        if constexpr (I4) {
-          s0 = __fmaf_rn(qsum[nt], kz0, s0);
-          s1 = __fmaf_rn(qsum[nt], kz1, s1);
+        float f = 1.0f;
+        if (__fmul_rn(vtop, vf) > 512.0f) {
+          const int e = min(max((int)(__float_as_uint(vtop) >> 23), 18), 255);
+          const float nf = __uint_as_float((uint32_t)(259 - e) << 23);
+          f = __fdiv_rn(nf, vf);
+          vf = nf;
         }
-        s0 = live0 ? __fmul_rn(s0, qs[nt]) : -INFINITY;
-        s1 = live1 ? __fmul_rn(s1, qs[nt]) : -INFINITY;
-        float top = fmaxf(s0, s1);
-        if (__any_sync(0xffffffffu, top > __fadd_rn(m[nt], kSlack))) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+          float top = fmaxf(fmaxf(raw[0][nt][0], raw[0][nt][1]), fmaxf(raw[1][nt][0], raw[1][nt][1]));
 #pragma unroll
           for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
-          const float mn = fmaxf(m[nt], top), keep = exp2_approx(__fsub_rn(m[nt], mn));
-          m[nt] = mn;
+          float keep = 1.0f;
+          if (top > m[nt]) {
+            m[nt] = top;
+            const float nq = __fmul_rn(top, qs[nt]);
+            keep = exp2_approx(__fsub_rn(mq[nt], nq));
+            mq[nt] = nq;
+            limit[nt] = __fadd_rn(top, __fdiv_rn(kSlack, qs[nt]));
+          }
           l[nt] = __fmul_rn(l[nt], keep);
           zsum[nt] = __fmul_rn(zsum[nt], keep);
+          keep = __fmul_rn(keep, f);
 #pragma unroll
           for (int k = 0; k < T::kMTiles; ++k)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[nt][k][j] = __fmul_rn(o[nt][k][j], keep);
         }
-        const float w0 = live0 ? exp2_approx(__fsub_rn(s0, m[nt])) : 0.0f;
-        const float w1 = live1 ? exp2_approx(__fsub_rn(s1, m[nt])) : 0.0f;
-        l[nt] = __fadd_rn(l[nt], __fadd_rn(w0, w1));
-        if constexpr (I4) zsum[nt] = __fmaf_rn(w0, vz0, __fmaf_rn(w1, vz1, zsum[nt]));
-        wb[nt][0] = transpose8x8(two_terms(__fmul_rn(w0, __fmul_rn(vs0, vf))));
-        wb[nt][1] = transpose8x8(two_terms(__fmul_rn(w1, __fmul_rn(vs1, vf))));
       }
-      // output
-      uint32_t vw[4][T::kVWords];
 #pragma unroll
-      for (int h = 0; h < 4; ++h)
+      for (int pg = 0; pg < 2; ++pg) {
+        uint32_t wb[NT][2];
 #pragma unroll
-        for (int j = 0; j < T::kVPieces; ++j)
-          lds_piece<T::kVPiece>(src + at_v[h][j], vw[h] + j * (T::kVPiece >= 4 ? T::kVPiece / 4 : 1));
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-      for (int w = 0; w < T::kVBytes / 2; ++w) {
-        // two bytes each of two rows, so that a widened pair is one dimension at two positions
-        const int word = T::kVPiece >= 4 ? w / 2 : w, sel = T::kVPiece >= 4 && w % 2 ? 0x7632 : 0x5410;
-        const uint32_t p = __byte_perm(vw[0][word], vw[1][word], sel), q = __byte_perm(vw[2][word], vw[3][word], sel);
-        if constexpr (I4) {
-          uint32_t x[4], y[4];
-          nibbles_f16(p, x);
-          nibbles_f16(q, y);
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            mma_f16(o[nt][2 * w], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
-            mma_f16(o[nt][2 * w + 1], x[2], x[3], y[2], y[3], wb[nt][0], wb[nt][1]);
+          for (int k = 0; k < 2; ++k) {
+            const float w = exp2_approx(__fmaf_rn(raw[pg][nt][k], qs[nt], -mq[nt]));  // 0 behind the context
+            l[nt] = __fadd_rn(l[nt], w);
+            if constexpr (I4) zsum[nt] = __fmaf_rn(w, vz[pg][k], zsum[nt]);
+            wb[nt][k] = transpose8x8(two_terms(__fmul_rn(w, __fmul_rn(vs[pg][k], vf))));
           }
-        } else {
-          uint32_t x[2], y[2];
-          bytes_f16(p, &x[0], &x[1]);
-          bytes_f16(q, &y[0], &y[1]);
+        // output
+        uint32_t vw[4][T::kVWords];
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][w], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
+        for (int h = 0; h < 4; ++h)
+#pragma unroll
+          for (int j = 0; j < T::kVPieces; ++j)
+            lds_piece<T::kVPiece>(src + pg * T::kTile + at_v[h][j], vw[h] + j * (T::kVPiece >= 4 ? T::kVPiece / 4 : 1));
+#pragma unroll
+        for (int w = 0; w < T::kVBytes / 2; ++w) {
+          // two bytes each of two rows, so that a widened pair is one dimension at two positions
+          const int word = T::kVPiece >= 4 ? w / 2 : w, sel = T::kVPiece >= 4 && w % 2 ? 0x7632 : 0x5410;
+          const uint32_t p = __byte_perm(vw[0][word], vw[1][word], sel), q = __byte_perm(vw[2][word], vw[3][word], sel);
+          if constexpr (I4) {
+            uint32_t x[4], y[4];
+            nibbles_f16(p, x);
+            nibbles_f16(q, y);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+              mma_f16(o[nt][2 * w], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
+              mma_f16(o[nt][2 * w + 1], x[2], x[3], y[2], y[3], wb[nt][0], wb[nt][1]);
+            }
+          } else {
+            uint32_t x[2], y[2];
+            bytes_f16(p, &x[0], &x[1]);
+            bytes_f16(q, &y[0], &y[1]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][w], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
+          }
         }
       }
       __syncwarp();  // every lane has read the stage
-      fetch(i + T::kStages);
+      fetch(i + 2 * T::kStages);
       if (++take == T::kStages) {
         take = 0;
         parity ^= 1;
@@ -1076,14 +1101,14 @@ __global__ void __launch_bounds__(kMmaWarps * 32, NT == 1 ? 2 : 1)
         const size_t dst = (size_t)r * a.ldo + (size_t)(h0 + h) * HD + g * (HD / 8);
 #pragma unroll
         for (int k = 0; k < HD / 8; ++k) store_elem(a.out, dst + k, a.bf16, __fmul_rn(x[k], inv));
-        if (a.lse && g == 0) a.lse[(size_t)r * a.nh + h0 + h] = lse_of(m[nt], l[nt]);
+        if (a.lse && g == 0) a.lse[(size_t)r * a.nh + h0 + h] = lse_of(mq[nt], l[nt]);
       } else {
         float* part = !begins && at < end ? warp_slot(a.space, shares, (int)mine_at, HD, us) : (float*)mine;
         part += h * T::kPartStride + g * (HD / 8);
 #pragma unroll
         for (int k = 0; k < HD / 8; k += 4) *(float4*)(part + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
         if (g == 0) {
-          ml[warp][slot][h][0] = m[nt];
+          ml[warp][slot][h][0] = mq[nt];
           ml[warp][slot][h][1] = l[nt];
         }
       }
@@ -1244,7 +1269,7 @@ size_t kvq_attend_space(int nh, int kv_heads, int hd) {
   const Units us = units_of(nh, kv_heads);
   const size_t plain = (size_t)kAttendCtas * (sizeof(ShareMeta) + 2 * us.heads * (hd + 2) * sizeof(float));
   const size_t mma = (size_t)kMmaShares * (sizeof(ShareMeta) + 2 * us.heads * (hd + 2) * sizeof(float) +
-                                           kMmaWarps * us.heads * (hd + 4) * sizeof(float)) + 16;
+                                           kMmaMaxWarps * us.heads * (hd + 4) * sizeof(float)) + 16;
   return std::max(plain, mma);
 }
 
@@ -1265,14 +1290,14 @@ bool codes_map(const KvqView& c, CUtensorMap* map) {
 
 template <int HD, bool I4, int NT>
 bool launch_mma(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, int wide_q, cudaStream_t st) {
-  using T = MmaTile<HD, I4>;
+  using T = MmaTile<HD, I4, NT>;
   static_assert(T::kRing >= NT * 4 * T::kPartStride * 4, "a warp's ring holds its partial result");
   CUtensorMap map;
   if (!codes_map<T>(c, &map)) return false;
   auto* kernel = kvq_attend_mma_kernel<HD, I4, NT>;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
   const int shares = NT == 1 ? kMmaShares : kMmaShares / 2;
-  kernel<<<shares, kMmaWarps * 32, T::kSmem, st>>>(c, r, a, max_len, kMinWeight, wide_q, map);
+  kernel<<<shares, T::kWarps * 32, T::kSmem, st>>>(c, r, a, max_len, kMinWeight, wide_q, map);
   launch_pdl(kvq_join_kernel, dim3(shares, units_of(a.nh, c.kv_heads).heads), dim3(kJoinThreads), 0, st, c, a, shares);
   count_launch(2);
   return true;
