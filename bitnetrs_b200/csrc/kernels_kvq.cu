@@ -490,14 +490,11 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // larger one comes; a weight is at most 2^kSlack): a second term then still
 // holds 2^-30 of the largest weight.
 //
-// The order of dimensions inside a product is free, so a lane reads wide
-// pieces of a row for its K operand (HD/4 codes of two rows, the four lanes of
-// a row side by side) and its V operand (HD/8 codes of four rows).
-//
 // Each warp has a ring of pages of its own in shared memory.  One lane fetches
 // a page with two copies of the asynchronous copy engine, the codes as a tile
 // of 128-byte lines with their 16-byte pieces exchanged (128-byte swizzle), so
-// that the reads above meet no bank twice, and the parameters as they are.
+// that loads of 8 rows x 16 bytes meet no bank twice, and the parameters as
+// they are.
 // Measured on a batch of 256 contexts of 128 to 4096 (I8), with the same bytes
 // asked for ahead: copies by each lane (cp.async) stop at 4.0 TB/s, since a
 // load that goes through L1 needs an entry there until it lands.
@@ -522,13 +519,7 @@ constexpr float kSlack = 6.0f;
 template <int HD, bool I4, int NT>
 struct MmaTile {
   static constexpr int kRow = I4 ? HD / 2 : HD;         // bytes of a row's codes
-  static constexpr int kKBytes = kRow / 4;              // a lane's bytes of one K row
-  static constexpr int kVBytes = kRow / 8;              // a lane's bytes of one V row
-  static constexpr int kKPiece = kKBytes % 16 == 0 ? 16 : kKBytes % 8 == 0 ? 8 : 4;
-  static constexpr int kVPiece = kVBytes % 16 == 0 ? 16 : kVBytes % 8 == 0 ? 8 : kVBytes % 4 == 0 ? 4 : 2;
-  static constexpr int kKCodes = kKPiece * (I4 ? 2 : 1);  // codes of a K piece
-  static constexpr int kKPieces = kKBytes / kKPiece, kVPieces = kVBytes / kVPiece;
-  static constexpr int kVWords = kVPiece >= 4 ? kVBytes / 4 : kVPieces;  // registers of a V row
+  static constexpr int kChunks = kRow / 16;             // 16-byte pieces of a row
   static constexpr int kCodes = 2 * kPage * kRow;         // bytes of a page's codes
   static constexpr int kTile = (kCodes + 1023) / 1024 * 1024;
   static constexpr int kParams = I4 ? 256 : 128;
@@ -558,22 +549,33 @@ __device__ __forceinline__ void tma_bytes(uint32_t dst, const void* src, uint32_
                "l"((uint64_t)src), "r"(bytes), "r"(bar)
                : "memory");
 }
-template <int BYTES>
-__device__ __forceinline__ void lds_piece(const uint8_t* p, uint32_t* w) {
-  if constexpr (BYTES == 16) {
-    const uint4 v = *(const uint4*)p;
-    w[0] = v.x;
-    w[1] = v.y;
-    w[2] = v.z;
-    w[3] = v.w;
-  } else if constexpr (BYTES == 8) {
-    const uint2 v = *(const uint2*)p;
-    w[0] = v.x;
-    w[1] = v.y;
-  } else if constexpr (BYTES == 4) {
-    w[0] = *(const uint32_t*)p;
-  } else {
-    w[0] = *(const uint16_t*)p;
+// N (2 or 4) matrices of 8 rows x 16 bytes, whose row addresses the lanes
+// 8 i .. 8 i + 7 hold for matrix i.  A lane gets bytes 4t .. 4t + 3 of row g;
+// transposed (as 16-bit elements) bytes 2g, 2g + 1 of rows 2t and 2t + 1.
+template <int N, bool TRANS>
+__device__ __forceinline__ void load_matrices(uint32_t addr, uint32_t* w) {
+  if constexpr (N == 4 && TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr));
+  else if constexpr (N == 4)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
+                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                 : "r"(addr));
+  else if constexpr (TRANS)
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+  else
+    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
+}
+// All pieces of 16 rows: w[2 c + h] is piece c of rows 8 h .. 8 h + 7.
+template <int CHUNKS, bool TRANS>
+__device__ __forceinline__ void load_rows(uint32_t tile, const int* at, uint32_t* w) {
+#pragma unroll
+  for (int c = 0; c < CHUNKS; c += 2) {
+    if (c + 1 < CHUNKS)
+      load_matrices<4, TRANS>(tile + at[c / 2], w + 2 * c);
+    else
+      load_matrices<2, TRANS>(tile + at[c / 2], w + 2 * c);
   }
 }
 // c += product, fp16
@@ -767,17 +769,14 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
   uint8_t* const params = ring + kMmaWarps * T::kRing + warp * (T::kStages * 2 * T::kParams);
   const uint32_t mine_s = smem_u32(mine), params_s = smem_u32(params), bar_s = smem_u32(&full[warp][0]);
   const float qscale = __fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)HD));
-  // this lane's pieces in a tile
-  int at_k[2][T::kKPieces], at_v[4][T::kVPieces];
+  // the rows that this lane names for the loads of K and V
+  int at_k[(T::kChunks + 1) / 2], at_v[(T::kChunks + 1) / 2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int j = 0; j < T::kKPieces; ++j) at_k[h][j] = swizzled((g + 8 * h) * T::kRow + (4 * j + t) * T::kKPiece);
-#pragma unroll
-  for (int h = 0; h < 4; ++h)
-#pragma unroll
-    for (int j = 0; j < T::kVPieces; ++j)
-      at_v[h][j] = swizzled((kPage + 2 * t + (h & 1) + (h >> 1) * 8) * T::kRow + g * T::kVBytes + j * T::kVPiece);
+  for (int c = 0; c < T::kChunks; c += 2) {
+    const int row = lane & 15, piece = min(c + (lane >> 4), T::kChunks - 1);
+    at_k[c / 2] = swizzled(row * T::kRow + piece * 16);
+    at_v[c / 2] = swizzled((kPage + row) * T::kRow + piece * 16);
+  }
   int fill = 0, take = 0;      // stages, the next to fetch into and the next to use
   uint32_t parity = 0;         // of the copies that `take` waits for
 
@@ -838,22 +837,23 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
     float qs[NT], qsum[NT];  // of the heads whose sums this lane holds (t of each tile)
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      // of every 32 dimensions a lane's K codes are (I8) 4t .. 4t + 3 and 16 more, (I4) 8t .. 8t + 7
       float x[HD / 4];
       const int h = nt * 4 + (g >> 1);
-      const size_t src = (size_t)r * a.ldq + (size_t)(h0 + min(h, heads - 1)) * HD + t * T::kKCodes;
-      // the lane's codes: kKCodes of every 4 * kKCodes
-      if (wide_q) {
+      const size_t src = (size_t)r * a.ldq + (size_t)(h0 + min(h, heads - 1)) * HD + t * (I4 ? 8 : 4);
 #pragma unroll
-        for (int i = 0; i < HD / 4; i += 4) {
-          const float4 v = *(const float4*)((const float*)a.q + src + i + i / T::kKCodes * (3 * T::kKCodes));
+      for (int i = 0; i < HD / 4; i += 4) {
+        const size_t at_q = src + i / 8 * 32 + i % 8 * (I4 ? 1 : 4);
+        if (wide_q) {
+          const float4 v = *(const float4*)((const float*)a.q + at_q);
           x[i] = v.x;
           x[i + 1] = v.y;
           x[i + 2] = v.z;
           x[i + 3] = v.w;
-        }
-      } else {
+        } else {
 #pragma unroll
-        for (int i = 0; i < HD / 4; ++i) x[i] = load_elem(a.q, src + i + i / T::kKCodes * (3 * T::kKCodes), a.bf16);
+          for (int j = 0; j < 4; ++j) x[i + j] = load_elem(a.q, at_q + j, a.bf16);
+        }
       }
       float top = 0.0f, sum = 0.0f, zero = 0.0f;
 #pragma unroll
@@ -911,38 +911,32 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
         at = end;  // nothing more is asked for
         break;
       }
-      const uint8_t* src = mine + take * (2 * T::kTile);
+      const uint32_t src = mine_s + take * (2 * T::kTile);
       const float* par = (const float*)(params + take * (2 * T::kParams)) + g;
       // live positions from the first page on; with an odd number of pages the
       // second tile of the last pair holds what was there before
       const int left = min(len - (p0 + i) * kPage, (n_pages - i) * kPage);
       constexpr int kParFloats = T::kParams / 4, vpar = I4 ? 32 : 16;
       float raw[2][NT][2], vs[2][2], vz[2][2];  // [page][..][slot g or g + 8]
-      bool again = false;
-      float vtop = 0.0f;
 #pragma unroll
       for (int pg = 0; pg < 2; ++pg) {
         // scores
         int sc[NT][2][4];
-        uint32_t kw[2][T::kKBytes / 4];
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int j = 0; j < T::kKPieces; ++j)
-            lds_piece<T::kKPiece>(src + pg * T::kTile + at_k[h][j], kw[h] + j * (T::kKPiece / 4));
+        uint32_t kw[2 * T::kChunks];
+        load_rows<T::kChunks, false>(src + pg * T::kTile, at_k, kw);
 #pragma unroll
         for (int s = 0; s < T::kKSteps; ++s) {
           uint32_t x[2], y[2];  // rows g and g + 8
           if constexpr (I4) {
-            x[0] = kw[0][s] & 0x0f0f0f0fu;
-            x[1] = (kw[0][s] >> 4) & 0x0f0f0f0fu;
-            y[0] = kw[1][s] & 0x0f0f0f0fu;
-            y[1] = (kw[1][s] >> 4) & 0x0f0f0f0fu;
+            x[0] = kw[2 * s] & 0x0f0f0f0fu;
+            x[1] = (kw[2 * s] >> 4) & 0x0f0f0f0fu;
+            y[0] = kw[2 * s + 1] & 0x0f0f0f0fu;
+            y[1] = (kw[2 * s + 1] >> 4) & 0x0f0f0f0fu;
           } else {
-            x[0] = kw[0][2 * s];
-            x[1] = kw[0][2 * s + 1];
-            y[0] = kw[1][2 * s];
-            y[1] = kw[1][2 * s + 1];
+            x[0] = kw[4 * s];
+            y[0] = kw[4 * s + 1];
+            x[1] = kw[4 * s + 2];
+            y[1] = kw[4 * s + 3];
           }
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
@@ -956,24 +950,35 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const bool live = pg * kPage + 8 * k + g < left;
           const float* pp = par + pg * kParFloats + 8 * k;
           const float ks = pp[0], kz = I4 ? pp[16] : 0.0f;
-          // behind the context the bytes may be anything: no scale of theirs is used
-          vs[pg][k] = live ? pp[vpar] : 0.0f;
-          vz[pg][k] = I4 && live ? pp[vpar + 16] : 0.0f;
-          vtop = fmaxf(vtop, vs[pg][k]);
+          vs[pg][k] = pp[vpar];
+          vz[pg][k] = I4 ? pp[vpar + 16] : 0.0f;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             // digits 3 and 2, 1 and 0: sums of at most 2^29
-            float x = __fmaf_rn((float)(sc[nt][0][2 * k] * 256 + sc[nt][0][2 * k + 1]), 65536.0f,
-                                (float)(sc[nt][1][2 * k] * 256 + sc[nt][1][2 * k + 1]));
-            x = I4 ? __fmaf_rn(qsum[nt], kz, __fmul_rn(x, ks)) : __fmul_rn(x, ks);
-            raw[pg][nt][k] = live ? x : -INFINITY;
-            again |= raw[pg][nt][k] > limit[nt];
+            const float x = __fmaf_rn((float)(sc[nt][0][2 * k] * 256 + sc[nt][0][2 * k + 1]), 65536.0f,
+                                      (float)(sc[nt][1][2 * k] * 256 + sc[nt][1][2 * k + 1]));
+            raw[pg][nt][k] = I4 ? __fmaf_rn(qsum[nt], kz, __fmul_rn(x, ks)) : __fmul_rn(x, ks);
           }
         }
       }
+      if (left < 2 * kPage) {  // behind the context the bytes may be anything: no scale of theirs is used
+#pragma unroll
+        for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+          for (int k = 0; k < 2; ++k)
+            if (pg * kPage + 8 * k + g >= left) {
+              vs[pg][k] = vz[pg][k] = 0.0f;
+#pragma unroll
+              for (int nt = 0; nt < NT; ++nt) raw[pg][nt][k] = -INFINITY;
+            }
+      }
+      float vtop = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
+      bool again = false;
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+        again |= fmaxf(fmaxf(raw[0][nt][0], raw[0][nt][1]), fmaxf(raw[1][nt][0], raw[1][nt][1])) > limit[nt];
       // a score above the slack, or a scale of V above what the weights' power of two allows
       again |= __fmul_rn(vtop, vf) > 512.0f;
       if (__any_sync(0xffffffffu, again)) {
@@ -1021,21 +1026,16 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
             wb[nt][k] = transpose8x8(two_terms(__fmul_rn(w, __fmul_rn(vs[pg][k], vf))));
           }
         // output
-        uint32_t vw[4][T::kVWords];
+        // a register of V holds two bytes each of two positions, so that a widened pair is one dimension at two
+        // positions: of dimensions 2g, 2g + 1 of every 16 (I8), or 4g .. 4g + 3 of every 32 (I4)
+        uint32_t vw[2 * T::kChunks];
+        load_rows<T::kChunks, true>(src + pg * T::kTile, at_v, vw);
 #pragma unroll
-        for (int h = 0; h < 4; ++h)
-#pragma unroll
-          for (int j = 0; j < T::kVPieces; ++j)
-            lds_piece<T::kVPiece>(src + pg * T::kTile + at_v[h][j], vw[h] + j * (T::kVPiece >= 4 ? T::kVPiece / 4 : 1));
-#pragma unroll
-        for (int w = 0; w < T::kVBytes / 2; ++w) {
-          // two bytes each of two rows, so that a widened pair is one dimension at two positions
-          const int word = T::kVPiece >= 4 ? w / 2 : w, sel = T::kVPiece >= 4 && w % 2 ? 0x7632 : 0x5410;
-          const uint32_t p = __byte_perm(vw[0][word], vw[1][word], sel), q = __byte_perm(vw[2][word], vw[3][word], sel);
+        for (int w = 0; w < T::kChunks; ++w) {
           if constexpr (I4) {
             uint32_t x[4], y[4];
-            nibbles_f16(p, x);
-            nibbles_f16(q, y);
+            nibbles_f16(vw[2 * w], x);
+            nibbles_f16(vw[2 * w + 1], y);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
               mma_f16(o[nt][2 * w], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
@@ -1043,8 +1043,8 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
             }
           } else {
             uint32_t x[2], y[2];
-            bytes_f16(p, &x[0], &x[1]);
-            bytes_f16(q, &y[0], &y[1]);
+            bytes_f16(vw[2 * w], &x[0], &x[1]);
+            bytes_f16(vw[2 * w + 1], &y[0], &y[1]);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][w], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
           }
@@ -1090,7 +1090,9 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
         if constexpr (I4) zsum[nt] = __fadd_rn(zsum[nt], __shfl_xor_sync(0xffffffffu, zsum[nt], b));
       }
       if (h >= heads) continue;
-      float x[HD / 8];  // dimensions g * HD / 8 and on
+      // the lane's dimensions: kRun from g * kRun of every 8 * kRun
+      constexpr int kRun = I4 ? 4 : 2;
+      float x[HD / 8];
 #pragma unroll
       for (int k = 0; k < T::kMTiles; ++k) {
         x[2 * k] = __fmaf_rn(__fadd_rn(o[nt][k][0], o[nt][k][1]), back, zsum[nt]);
@@ -1098,15 +1100,22 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
       }
       if (begins && ends) {
         const float inv = __fdiv_rn(1.0f, l[nt]);
-        const size_t dst = (size_t)r * a.ldo + (size_t)(h0 + h) * HD + g * (HD / 8);
+        const size_t dst = (size_t)r * a.ldo + (size_t)(h0 + h) * HD + g * kRun;
 #pragma unroll
-        for (int k = 0; k < HD / 8; ++k) store_elem(a.out, dst + k, a.bf16, __fmul_rn(x[k], inv));
+        for (int k = 0; k < HD / 8; ++k)
+          store_elem(a.out, dst + k / kRun * (8 * kRun) + k % kRun, a.bf16, __fmul_rn(x[k], inv));
         if (a.lse && g == 0) a.lse[(size_t)r * a.nh + h0 + h] = lse_of(mq[nt], l[nt]);
       } else {
         float* part = !begins && at < end ? warp_slot(a.space, shares, (int)mine_at, HD, us) : (float*)mine;
-        part += h * T::kPartStride + g * (HD / 8);
+        part += h * T::kPartStride + g * kRun;
 #pragma unroll
-        for (int k = 0; k < HD / 8; k += 4) *(float4*)(part + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+        for (int k = 0; k < HD / 8; k += kRun) {
+          float* dst = part + k * 8;
+          if constexpr (I4)
+            *(float4*)dst = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+          else
+            *(float2*)dst = make_float2(x[k], x[k + 1]);
+        }
         if (g == 0) {
           ml[warp][slot][h][0] = mq[nt];
           ml[warp][slot][h][1] = l[nt];
