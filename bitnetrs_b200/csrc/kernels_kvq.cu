@@ -44,22 +44,24 @@ __device__ __forceinline__ void store_elem(void* x, size_t i, int bf16, float v)
   else
     ((float*)x)[i] = v;
 }
-__device__ __forceinline__ double warp_max(double v) {
-#pragma unroll
-  for (int o = 16; o; o >>= 1) v = fmax(v, __shfl_xor_sync(0xffffffffu, v, o));
-  return v;
-}
-
 // ---------------------------------------------------------------------------
-// Store.  One warp quantises one row of one head: the largest magnitude (I8)
-// or the extremes (I4) by a warp reduction, then the code nearest to each
-// element.  The nearest code is exact, ties to even, whatever the scale: the
-// product with the scale's reciprocal may land on the wrong side of a border,
-// so the remainder of that code (one fma, exact at a border) puts it right.
-// Elements are held in 64 bits, in which a rotated element is rounded once.
+// Store.  A group of GROUP lanes (a power of two) quantises one row of one
+// head, N neighbouring elements a lane: the largest magnitude (I8) or the
+// extremes (I4) by a reduction over the group, then the code nearest to each
+// element.
+//
+// The nearest code is exact, ties to even, whatever the scale.  In 32 bits
+// t = x / scale is off by less than 127 * 3 * 2^-24 < 2^-15, so rint(t) is the
+// code unless t lies that close to a border; there the quotient is taken in 64
+// bits, and the remainder of the code it gives (one fma, exact at a border)
+// decides.  A rotated element is held in 64 bits: its two products are exact
+// there and their sum is rounded once.
+//
+// Bound by memory for many rows (the rows read once, the codes written once)
+// and by three dependent loads (position, page, and the row beside them) for few.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ int nearest_code(double x, double scale, double inv, int least, int most) {
-  double c = rint(x * inv);
+__device__ __noinline__ int border_code(double x, double scale, int least, int most) {
+  double c = rint(x / scale);
   const double r = fma(-c, scale, x), h = 0.5 * scale;
   const bool odd = ((int)c & 1) != 0;
   if (r > h || (r == h && odd))
@@ -68,136 +70,281 @@ __device__ __forceinline__ int nearest_code(double x, double scale, double inv, 
     c -= 1.0;
   return min(max((int)c, least), most);
 }
+// `x` is what is divided: an element (I8), or an element less the zero (I4).
+__device__ __forceinline__ int nearest_code(double x, float xf, float scale, float inv, int least, int most) {
+  const float t = __fmul_rn(xf, inv), c = rintf(t);
+  // a scale so small that its reciprocal is not finite, or t, also goes the long way
+  if (!(fabsf(__fsub_rn(t, c)) < 0.4999f)) return border_code(x, scale, least, most);
+  return min(max((int)c, least), most);
+}
 
-constexpr int kStoreWarps = 8;
-constexpr int kStorePairs = kKvqMaxHd / 64;  // pairs of dimensions a lane holds
-
-__global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, KvqStore s) {
-  const int lane = threadIdx.x & 31;
-  const int jobs = 2 * c.kv_heads + (s.q ? s.nh : 0);  // K heads, V heads, q heads of a row
-  const size_t job = (size_t)blockIdx.x * kStoreWarps + (threadIdx.x >> 5);
-  const int row = (int)(job / jobs), what = (int)(job % jobs);
-  if (row >= s.rows) return;
-  const int pos = s.row_pos ? s.row_pos[row] : row;
-  if (pos < 0) return;
-  const int seq = s.row_seq ? s.row_seq[row] : 0;
-  const int kind = what < c.kv_heads ? 0 : 1;
-  const int head = kind ? what - c.kv_heads : what;
-  uint8_t* block = block_of(c, seq, pos, min(head, c.kv_heads - 1));
-  if (!block || (s.rope_cos && pos >= s.rope_len)) {
-    if (lane == 0) atomicOr(s.status, kStatusBadContext);
-    return;
-  }
-  const int hd = c.hd, half = hd / 2;
-  const float* cs = s.rope_cos ? s.rope_cos + (size_t)pos * half : nullptr;
-  const float* sn = s.rope_cos ? s.rope_sin + (size_t)pos * half : nullptr;
-  if (what >= 2 * c.kv_heads) {  // a q head, in the reference's f32 order (rope.rs:414-431)
-    const int h = what - 2 * c.kv_heads;
-    const float* x = s.q + (size_t)row * s.ldq + h * hd;
-    float* o = s.q_out + ((size_t)row * s.nh + h) * hd;
-    for (int p = lane; p < half; p += 32) {
-      const float lo = x[p], hi = x[p + half];
-      o[p] = __fsub_rn(__fmul_rn(lo, cs[p]), __fmul_rn(hi, sn[p]));
-      o[p + half] = __fadd_rn(__fmul_rn(hi, cs[p]), __fmul_rn(lo, sn[p]));
+// N elements from x[i] on, in wide loads where `wide` says that they are aligned.
+template <int N>
+__device__ __forceinline__ void load_run(const void* x, size_t i, int bf16, bool wide, float* v) {
+  if (N == 8 && wide) {
+    if (bf16) {
+      const uint4 w = *(const uint4*)((const uint16_t*)x + i);
+      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+      for (int j = 0; j < N / 2; ++j) {
+        v[2 * j] = bf_lo(u[j]);
+        v[2 * j + 1] = bf_hi(u[j]);
+      }
+    } else {
+      const float4 p = *(const float4*)((const float*)x + i), q = *(const float4*)((const float*)x + i + 4);
+      const float u[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
+#pragma unroll
+      for (int j = 0; j < N; ++j) v[j] = u[j];
     }
-    return;
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) v[j] = load_elem(x, i + j, bf16);
   }
-  const void* src = kind ? s.v : s.k;
-  const size_t at = (size_t)row * (kind ? s.ldv : s.ldk) + (size_t)head * hd;
-  const bool turn = kind == 0 && cs;
-  double x[kStorePairs][2];
-  double top = 0.0, low = INFINITY;  // the largest x (I4) or |x| (I8), the least x
-  if (c.i4) top = -INFINITY;
+}
+
+constexpr int kStoreWarps = 4;
+
+// Lanes a row of one head, and elements a lane: 8 where the head size is a
+// multiple of 16 (a rotation pairs runs of 8 then), else 2.
+struct RowSplit {
+  int group, run;
+};
+inline RowSplit split_row(int hd) {
+  RowSplit s;
+  s.run = hd % 16 == 0 ? 8 : 2;
+  s.group = 1;
+  while (s.group * s.run < hd && s.group < 32) s.group *= 2;
+  return s;
+}
+
+// N elements a lane (8: once over the row; 2: as often as the row needs it).
+template <int N, bool I4, bool ROPE>
+__global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, KvqStore s, int group, int wide) {
+  constexpr int kRuns = N == 8 ? 1 : kKvqMaxHd / 64;
+  const int lane = threadIdx.x & 31, in = lane & (group - 1);
+  const int jobs = 2 * c.kv_heads + (s.q ? s.nh : 0);  // K heads, V heads, q heads of a row
+  const size_t job = ((size_t)blockIdx.x * (kStoreWarps * 32) + threadIdx.x) / group;
+  const size_t row = job / jobs;
+  const int what = (int)(job % jobs);
+  // lanes without a row run on with the group's reductions
+  bool on = row < (size_t)s.rows;
+  const int pos = on ? (s.row_pos ? s.row_pos[row] : (int)row) : -1, seq = on && s.row_seq ? s.row_seq[row] : 0;
+  on = on && pos >= 0;
+  const int hd = c.hd, half = hd / 2;
+  const int kind = what < c.kv_heads ? 0 : 1, head = kind ? what - c.kv_heads : what;
+  const bool is_q = what >= 2 * c.kv_heads;
+  const void* src = is_q ? (const void*)s.q : kind ? s.v : s.k;
+  const size_t at = row * (is_q ? s.ldq : kind ? s.ldv : s.ldk) + (size_t)(is_q ? what - 2 * c.kv_heads : head) * hd;
+  const int bf16 = is_q ? 0 : s.bf16;
+  // the row, asked for before its place is known
+  float x[kRuns][N], w[kRuns][N];  // w: what a rotation pairs x with
+#pragma unroll
+  for (int i = 0; i < kRuns; ++i) {
+    const int d = N * (in + 32 * i);
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[i][j] = w[i][j] = 0.0f;
+    if (!on || d >= hd) continue;
+    load_run<N>(src, at + d, bf16, wide, x[i]);
+    if (ROPE && (kind == 0 || is_q)) {
+      if (N == 8)
+        load_run<N>(src, at + (d < half ? d + half : d - half), bf16, wide, w[i]);
+      else
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[i][j] = load_elem(src, at + (d + j < half ? d + j + half : d + j - half), bf16);
+    }
+  }
+  uint8_t* block = on ? block_of(c, seq, pos, is_q ? 0 : head) : nullptr;
+  if (on && (!block || (ROPE && pos >= s.rope_len))) {
+    if (in == 0) atomicOr(s.status, kStatusBadContext);
+    on = false;
+  }
+  const float* cs = ROPE && on ? s.rope_cos + (size_t)pos * half : nullptr;
+  const float* sn = ROPE && on ? s.rope_sin + (size_t)pos * half : nullptr;
+  if (is_q) {  // in the reference's f32 order (rope.rs:414-431); a whole group, and no reduction below has others in it
+    float* o = s.q_out + (row * s.nh + (what - 2 * c.kv_heads)) * hd;
+    if (on)
+#pragma unroll
+      for (int i = 0; i < kRuns; ++i)
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const int d = N * (in + 32 * i) + j;
+          if (d >= hd) continue;
+          const int p = d < half ? d : d - half;
+          o[d] = d < half ? __fsub_rn(__fmul_rn(x[i][j], cs[p]), __fmul_rn(w[i][j], sn[p]))
+                          : __fadd_rn(__fmul_rn(x[i][j], cs[p]), __fmul_rn(w[i][j], sn[p]));
+        }
+    on = false;
+  }
+  double v[ROPE ? kRuns : 1][N];  // elements in 64 bits, where 32 do not hold them
+  float top = I4 ? -INFINITY : 0.0f, low = INFINITY;  // the largest x (I4) or |x| (I8), the least x
+  double top64 = top, low64 = low;
   bool finite = true;
 #pragma unroll
-  for (int i = 0; i < kStorePairs; ++i)
+  for (int i = 0; i < kRuns; ++i)
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-      const int d = 2 * (lane + 32 * i) + j;
-      x[i][j] = 0.0;
-      if (d >= hd) continue;
-      double v = load_elem(src, at + d, s.bf16);
-      if (turn) {
-        const int p = d < half ? d : d - half;
-        const double w = load_elem(src, at + (d < half ? d + half : p), s.bf16);
-        // each product is exact in 64 bits, the sum is rounded once
-        v = d < half ? __dsub_rn(__dmul_rn(v, cs[p]), __dmul_rn(w, sn[p]))
-                     : __dadd_rn(__dmul_rn(v, cs[p]), __dmul_rn(w, sn[p]));
+    for (int j = 0; j < N; ++j) {
+      const int d = N * (in + 32 * i) + j;
+      if (ROPE) v[i][j] = x[i][j];
+      if (!on || d >= hd) continue;
+      if (ROPE) {
+        if (kind == 0) {
+          const int p = d < half ? d : d - half;
+          const double a = __dmul_rn(x[i][j], cs[p]), b = __dmul_rn(w[i][j], sn[p]);
+          v[i][j] = d < half ? __dsub_rn(a, b) : __dadd_rn(a, b);
+          x[i][j] = (float)v[i][j];
+        }
+        top64 = fmax(top64, I4 ? v[i][j] : fabs(v[i][j]));
+        if (I4) low64 = fmin(low64, v[i][j]);
+      } else {
+        top = fmaxf(top, I4 ? x[i][j] : fabsf(x[i][j]));
+        if (I4) low = fminf(low, x[i][j]);
       }
-      finite &= isfinite(v) != 0;
-      x[i][j] = v;
-      top = fmax(top, c.i4 ? v : fabs(v));
-      low = fmin(low, v);
+      finite &= isfinite(x[i][j]) != 0;
     }
-  finite = __all_sync(0xffffffffu, finite);
-  top = warp_max(top);
   float zero = 0.0f, scale;
-  if (c.i4) {
-    low = -warp_max(-low);
-    zero = __fadd_rn((float)low, 0.0f);  // never -0
-    scale = __fadd_rn((float)((top - (double)zero) / 15.0), 0.0f);
+  int bad = !finite;
+  for (int o = group / 2; o; o >>= 1) {
+    bad |= __shfl_xor_sync(0xffffffffu, bad, o);
+    if (ROPE) {
+      top64 = fmax(top64, __shfl_xor_sync(0xffffffffu, top64, o));
+      if (I4) low64 = fmin(low64, __shfl_xor_sync(0xffffffffu, low64, o));
+    } else {
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (I4) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+    }
+  }
+  if (!on) return;
+  if (!ROPE) {
+    top64 = top;
+    low64 = low;
+  }
+  if (I4) {
+    zero = __fadd_rn((float)low64, 0.0f);  // never -0
+    scale = __fadd_rn((float)((top64 - (double)zero) / 15.0), 0.0f);
   } else {
-    scale = (float)(top / 127.0);
+    scale = ROPE ? (float)(top64 / 127.0) : __fdiv_rn(top, 127.0f);
   }
   // a row that holds a value that is not finite reads back as NaN
-  if (!finite || !isfinite(scale) || !isfinite(zero)) {
+  if (bad || !isfinite(scale) || !isfinite(zero)) {
     scale = __int_as_float(0x7fc00000);
-    if (lane == 0) atomicOr(s.status, kStatusNonFinite);
-    finite = false;
+    if (in == 0) atomicOr(s.status, kStatusNonFinite);
+    bad = 1;
   }
-  const int slot = pos % kPage, rowb = kvq_row_bytes(hd, c.i4);
-  uint8_t* codes = block + (size_t)(kind * kPage + slot) * rowb;
-  const double inv = 1.0 / (double)scale;
+  const int slot = pos % kPage;
+  uint8_t* codes = block + (size_t)(kind * kPage + slot) * kvq_row_bytes(hd, I4);
+  const float inv = __fdiv_rn(1.0f, scale);
 #pragma unroll
-  for (int i = 0; i < kStorePairs; ++i) {
-    const int d = 2 * (lane + 32 * i);
+  for (int i = 0; i < kRuns; ++i) {
+    const int d = N * (in + 32 * i);
     if (d >= hd) continue;
-    int q[2] = {0, 0};
-    if (finite && scale > 0.0f)
+    uint32_t word[2] = {0u, 0u};
+    if (!bad && scale > 0.0f)
 #pragma unroll
-      for (int j = 0; j < 2; ++j)
-        q[j] = nearest_code(x[i][j] - (double)zero, scale, inv, c.i4 ? 0 : -127, c.i4 ? 15 : 127);
-    if (c.i4)
-      codes[d / 2] = (uint8_t)(q[0] | (q[1] << 4));
+      for (int j = 0; j < N; ++j) {
+        const double y = ROPE ? v[i][j] - (double)zero : (double)x[i][j] - (double)zero;
+        const float yf = I4 ? (ROPE ? (float)y : __fsub_rn(x[i][j], zero)) : x[i][j];
+        const uint32_t q = (uint32_t)nearest_code(y, yf, scale, inv, I4 ? 0 : -127, I4 ? 15 : 127);
+        if (I4)
+          word[0] |= q << (4 * j);
+        else
+          word[j / 4] |= (q & 255u) << (8 * (j % 4));
+      }
+    if (N == 8 && I4)
+      *(uint32_t*)(codes + d / 2) = word[0];
+    else if (N == 8)
+      *(uint2*)(codes + d) = make_uint2(word[0], word[1]);
+    else if (I4)
+      codes[d / 2] = (uint8_t)word[0];
     else
-      *(uint16_t*)(codes + d) = (uint16_t)((q[0] & 255) | (q[1] << 8));
+      *(uint16_t*)(codes + d) = (uint16_t)word[0];
   }
-  if (lane == 0) {
-    float* par = block_params(block, hd, c.i4, kind);
+  if (in == 0) {
+    float* par = block_params(block, hd, I4, kind);
     par[slot] = scale;
-    if (c.i4) par[kPage + slot] = zero;
+    if (I4) par[kPage + slot] = zero;
   }
 }
 
 // ---------------------------------------------------------------------------
-// Load.  One warp reads one row of one head.
+// Load.  A warp reads a row of K and V, all heads, the lanes over runs of N
+// elements in the order in which they are written.  kLoadAhead runs a lane are
+// asked for before the first is written.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float code_at(const uint8_t* codes, int d, int i4) {
   return i4 ? (float)((codes[d >> 1] >> ((d & 1) * 4)) & 15) : (float)(int8_t)codes[d];
 }
+constexpr int kLoadAhead = 4;
+template <int N, bool I4>
 __global__ void __launch_bounds__(kStoreWarps * 32)
     kvq_load_kernel(KvqView c, int rows, const int32_t* __restrict__ row_seq, const int32_t* __restrict__ row_pos,
-                    void* __restrict__ k, size_t ldk, void* __restrict__ v, size_t ldv, int bf16, int32_t* status) {
-  const int lane = threadIdx.x & 31;
+                    void* __restrict__ k, size_t ldk, void* __restrict__ v, size_t ldv, int bf16, int wide,
+                    int per_row, int32_t* status) {
+  // per_row warps share a row
+  const int lane = threadIdx.x & 31, hd = c.hd, runs = hd / N, all = 2 * c.kv_heads * runs;
   const size_t job = (size_t)blockIdx.x * kStoreWarps + (threadIdx.x >> 5);
-  const int row = (int)(job / (2 * c.kv_heads)), what = (int)(job % (2 * c.kv_heads));
+  const int row = (int)(job / per_row), part = (int)(job % per_row);
   if (row >= rows) return;
   const int pos = row_pos ? row_pos[row] : row;
   if (pos < 0) return;
-  const int kind = what / c.kv_heads, head = what % c.kv_heads;
-  uint8_t* block = block_of(c, row_seq ? row_seq[row] : 0, pos, head);
-  if (!block) {
+  const uint8_t* first = block_of(c, row_seq ? row_seq[row] : 0, pos, 0);
+  if (!first) {
     if (lane == 0) atomicOr(status, kStatusBadContext);
     return;
   }
-  const int slot = pos % kPage;
-  const uint8_t* codes = block + (size_t)(kind * kPage + slot) * kvq_row_bytes(c.hd, c.i4);
-  const float* par = block_params(block, c.hd, c.i4, kind);
-  const float scale = par[slot], zero = c.i4 ? par[kPage + slot] : 0.0f;
-  void* dst = kind ? v : k;
-  const size_t at = (size_t)row * (kind ? ldv : ldk) + (size_t)head * c.hd;
-  for (int d = lane; d < c.hd; d += 32)
-    store_elem(dst, at + d, bf16, __fmaf_rn(code_at(codes, d, c.i4), scale, zero));
+  const int slot = pos % kPage, rowb = kvq_row_bytes(hd, I4), block_bytes = kvq_block_bytes(hd, I4);
+  for (int r0 = part * 32 + lane; r0 < all; r0 += per_row * 32 * kLoadAhead) {
+    uint32_t w[kLoadAhead][2];
+    float scale[kLoadAhead], zero[kLoadAhead];
+#pragma unroll
+    for (int i = 0; i < kLoadAhead; ++i) {
+      const int r = r0 + i * per_row * 32;
+      if (r >= all) continue;
+      const int which = r / runs, d = r % runs * N, kind = which >= c.kv_heads, head = which - kind * c.kv_heads;
+      const uint8_t* block = first + (size_t)head * block_bytes;
+      const uint8_t* codes = block + (kind * kPage + slot) * rowb;
+      if (N == 8 && I4) {
+        w[i][0] = *(const uint32_t*)(codes + d / 2);
+      } else if (N == 8) {
+        const uint2 u = *(const uint2*)(codes + d);
+        w[i][0] = u.x;
+        w[i][1] = u.y;
+      } else {
+        w[i][0] = I4 ? codes[d / 2] : *(const uint16_t*)(codes + d);
+      }
+      const float* par = block_params((uint8_t*)block, hd, I4, kind);
+      scale[i] = par[slot];
+      zero[i] = I4 ? par[kPage + slot] : 0.0f;
+    }
+#pragma unroll
+    for (int i = 0; i < kLoadAhead; ++i) {
+      const int r = r0 + i * per_row * 32;
+      if (r >= all) continue;
+      const int which = r / runs, d = r % runs * N, kind = which >= c.kv_heads, head = which - kind * c.kv_heads;
+      void* dst = kind ? v : k;
+      const size_t at = (size_t)row * (kind ? ldv : ldk) + (size_t)head * hd + d;
+      float x[N];
+#pragma unroll
+      for (int j = 0; j < N; ++j) {
+        const float q = I4 ? (float)((w[i][0] >> (4 * j)) & 15u) : (float)(int8_t)(w[i][j / 4] >> (8 * (j % 4)));
+        x[j] = __fmaf_rn(q, scale[i], zero[i]);
+      }
+      if (N == 8 && wide && bf16) {
+        uint32_t u[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
+          u[j] = *(const uint32_t*)&p;
+        }
+        *(uint4*)((uint16_t*)dst + at) = make_uint4(u[0], u[1], u[2], u[3]);
+      } else if (N == 8 && wide) {
+        *(float4*)((float*)dst + at) = make_float4(x[0], x[1], x[2], x[3]);
+        *(float4*)((float*)dst + at + 4) = make_float4(x[4 % N], x[5 % N], x[6 % N], x[7 % N]);
+      } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) store_elem(dst, at + j, bf16, x[j]);
+      }
+    }
+  }
 }
 
 // ---------------------------------------------------------------------------
@@ -1258,19 +1405,48 @@ __global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(KvqView c, KvqAt
 
 }  // namespace
 
+namespace {
+// Whether runs of 8 elements of a matrix start on 16 bytes.
+bool aligned_runs(const void* p, size_t ld, int bf16) { return (uintptr_t)p % 16 == 0 && ld % (bf16 ? 8 : 4) == 0; }
+
+template <int N, bool I4, bool ROPE>
+void launch_store(const KvqView& c, const KvqStore& s, int group, int wide, cudaStream_t st) {
+  const size_t jobs = (size_t)s.rows * (2 * c.kv_heads + (s.q ? s.nh : 0));
+  kvq_store_kernel<N, I4, ROPE>
+      <<<(unsigned)ceil_div(jobs * group, kStoreWarps * 32), kStoreWarps * 32, 0, st>>>(c, s, group, wide);
+}
+template <int N>
+void launch_store_of(const KvqView& c, const KvqStore& s, int group, int wide, cudaStream_t st) {
+  if (c.i4)
+    s.rope_cos ? launch_store<N, true, true>(c, s, group, wide, st) : launch_store<N, true, false>(c, s, group, wide, st);
+  else
+    s.rope_cos ? launch_store<N, false, true>(c, s, group, wide, st) : launch_store<N, false, false>(c, s, group, wide, st);
+}
+}  // namespace
+
 void launch_kvq_store(const KvqView& c, const KvqStore& s, cudaStream_t st) {
   if (s.rows <= 0) return;
-  const size_t jobs = (size_t)s.rows * (2 * c.kv_heads + (s.q ? s.nh : 0));
-  kvq_store_kernel<<<(unsigned)ceil_div(jobs, kStoreWarps), kStoreWarps * 32, 0, st>>>(c, s);
+  const RowSplit split = split_row(c.hd);
+  const int wide = aligned_runs(s.k, s.ldk, s.bf16) && aligned_runs(s.v, s.ldv, s.bf16) &&
+                   (!s.q || aligned_runs(s.q, s.ldq, 0));
+  if (split.run == 8)
+    launch_store_of<8>(c, s, split.group, wide, st);
+  else
+    launch_store_of<2>(c, s, split.group, wide, st);
   count_launch();
 }
 
 void launch_kvq_load(const KvqView& c, int rows, const int32_t* row_seq, const int32_t* row_pos, void* k, size_t ldk,
                      void* v, size_t ldv, int bf16, int32_t* status, cudaStream_t st) {
   if (rows <= 0) return;
-  const size_t jobs = (size_t)rows * 2 * c.kv_heads;
-  kvq_load_kernel<<<(unsigned)ceil_div(jobs, kStoreWarps), kStoreWarps * 32, 0, st>>>(c, rows, row_seq, row_pos, k,
-                                                                                      ldk, v, ldv, bf16, status);
+  const int run = split_row(c.hd).run, wide = aligned_runs(k, ldk, bf16) && aligned_runs(v, ldv, bf16);
+  // few rows: more warps to each, so that all runs are asked for at once
+  const int most = (int)ceil_div((size_t)2 * c.kv_heads * (c.hd / run), 32);
+  const int per_row = rows >= 148 * 16 ? (int)ceil_div(most, kLoadAhead) : most;
+  const unsigned blocks = (unsigned)ceil_div((size_t)rows * per_row, kStoreWarps);
+  auto* kernel = run == 8 ? (c.i4 ? kvq_load_kernel<8, true> : kvq_load_kernel<8, false>)
+                          : (c.i4 ? kvq_load_kernel<2, true> : kvq_load_kernel<2, false>);
+  kernel<<<blocks, kStoreWarps * 32, 0, st>>>(c, rows, row_seq, row_pos, k, ldk, v, ldv, bf16, wide, per_row, status);
   count_launch();
 }
 

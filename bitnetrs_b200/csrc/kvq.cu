@@ -71,8 +71,9 @@ int check_words(const void* p, const char* what) {
 int check_ctx(const bitnet_cuda_ctx* ctx) { return ctx ? BITNET_OK : shape_error("non-null context", "null"); }
 
 int check_rows(size_t rows, const KvqView& c) {
-  // one warp a row, kind and head; the grid's first dimension bounds them
-  if (rows > (size_t)INT_MAX / (2 * (size_t)c.kv_heads)) return shape_error("rows * 2 * kv_heads < 2^31", "rows = " + sz(rows));
+  // up to 32 lanes a row, kind and head; the grid's first dimension bounds their blocks
+  if (rows > (size_t)INT_MAX / (2 * (size_t)c.kv_heads))
+    return shape_error("rows * 2 * kv_heads < 2^31", "rows = " + sz(rows));
   return BITNET_OK;
 }
 

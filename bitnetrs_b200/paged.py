@@ -36,6 +36,8 @@ class PagedKV:
         self.backend = backend
         self._lib = N.cuda_lib()
         self._pages = pages
+        self._ref = C.byref(pages)
+        self._kv_width = pages.kv_heads * pages.head_dim
         self._owner = owner  # keeps a model's cache alive
 
     @classmethod
@@ -54,10 +56,6 @@ class PagedKV:
         check(N.cuda_lib().bitnet_cuda_kv_block_bytes(kv_dtype, head_dim, C.byref(n)))
         return n.value
 
-    @property
-    def _kv_width(self) -> int:
-        return self._pages.kv_heads * self._pages.head_dim
-
     def store(self, k: int, v: int, rows: int, row_seq: int, row_pos: int, status: int, *, ldk: Optional[int] = None,
               ldv: Optional[int] = None, bf16: bool = False, rope: Optional[Tuple[int, int, int]] = None,
               stream: int = 0) -> None:
@@ -66,7 +64,7 @@ class PagedKV:
         cos, sin, length = rope if rope is not None else (None, None, 0)
         w = self._kv_width
         check(self._lib.bitnet_cuda_kv_store_device(
-            self.backend.handle, C.byref(self._pages), k, w if ldk is None else ldk, v, w if ldv is None else ldv,
+            self.backend._h, self._ref, k, w if ldk is None else ldk, v, w if ldv is None else ldv,
             int(bf16), rows, row_seq, row_pos, cos, sin, length, status, stream or None))
 
     def load(self, k: int, v: int, rows: int, row_seq: int, row_pos: int, status: int, *, ldk: Optional[int] = None,
@@ -74,13 +72,13 @@ class PagedKV:
         """Read rows back into ``k`` and ``v``."""
         w = self._kv_width
         check(self._lib.bitnet_cuda_kv_load_device(
-            self.backend.handle, C.byref(self._pages), rows, row_seq, row_pos, k, w if ldk is None else ldk, v,
+            self.backend._h, self._ref, rows, row_seq, row_pos, k, w if ldk is None else ldk, v,
             w if ldv is None else ldv, int(bf16), status, stream or None))
 
     def attention_workspace(self, n_heads: int) -> int:
         """Bytes of the workspace that one attention call in flight needs."""
         n = C.c_size_t()
-        check(self._lib.bitnet_cuda_kv_attention_workspace(C.byref(self._pages), n_heads, C.byref(n)))
+        check(self._lib.bitnet_cuda_kv_attention_workspace(self._ref, n_heads, C.byref(n)))
         return n.value
 
     def attention(self, q: int, out: int, rows: int, n_heads: int, row_seq: int, row_len: int, max_len: int,
@@ -89,7 +87,7 @@ class PagedKV:
         """Attention of single tokens: row r sees the first ``row_len[r]`` positions of sequence ``row_seq[r]``."""
         w = n_heads * self._pages.head_dim
         check(self._lib.bitnet_cuda_kv_attention_device(
-            self.backend.handle, C.byref(self._pages), q, w if ldq is None else ldq, int(bf16), rows, n_heads,
+            self.backend._h, self._ref, q, w if ldq is None else ldq, int(bf16), rows, n_heads,
             row_seq, row_len, max_len, out, w if ldo is None else ldo, lse or None, workspace, workspace_bytes, status,
             stream or None))
 
@@ -101,6 +99,6 @@ class PagedKV:
         the positions from ``starts[i]`` of sequence ``seq_ids[i]``."""
         w = n_heads * self._pages.head_dim
         check(self._lib.bitnet_cuda_kv_prompt_attention_device(
-            self.backend.handle, C.byref(self._pages), q, w if ldq is None else ldq, int(bf16), rows, n_heads, n_seqs,
+            self.backend._h, self._ref, q, w if ldq is None else ldq, int(bf16), rows, n_heads, n_seqs,
             seq_ids, cu_rows, starts, max_len, out, w if ldo is None else ldo, lse or None, workspace,
             workspace_bytes, status, stream or None))
