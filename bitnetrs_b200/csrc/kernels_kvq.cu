@@ -4,6 +4,7 @@
 #include "kvq.cuh"
 
 #include <algorithm>
+#include <climits>
 
 namespace bitnet {
 
@@ -81,20 +82,27 @@ __device__ __forceinline__ int nearest_code(double x, float xf, float scale, flo
 // N elements from x[i] on, in wide loads where `wide` says that they are aligned.
 template <int N>
 __device__ __forceinline__ void load_run(const void* x, size_t i, int bf16, bool wide, float* v) {
-  if (N == 8 && wide) {
+  if (N >= 8 && wide) {
     if (bf16) {
-      const uint4 w = *(const uint4*)((const uint16_t*)x + i);
-      const uint32_t u[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-      for (int j = 0; j < N / 2; ++j) {
-        v[2 * j] = bf_lo(u[j]);
-        v[2 * j + 1] = bf_hi(u[j]);
+      for (int j = 0; j < N; j += 8) {
+        const uint4 w = *(const uint4*)((const uint16_t*)x + i + j);
+        const uint32_t u[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          v[(j + 2 * k) % N] = bf_lo(u[k]);
+          v[(j + 2 * k + 1) % N] = bf_hi(u[k]);
+        }
       }
     } else {
-      const float4 p = *(const float4*)((const float*)x + i), q = *(const float4*)((const float*)x + i + 4);
-      const float u[8] = {p.x, p.y, p.z, p.w, q.x, q.y, q.z, q.w};
 #pragma unroll
-      for (int j = 0; j < N; ++j) v[j] = u[j];
+      for (int j = 0; j < N; j += 4) {
+        const float4 p = *(const float4*)((const float*)x + i + j);
+        v[j] = p.x;
+        v[(j + 1) % N] = p.y;
+        v[(j + 2) % N] = p.z;
+        v[(j + 3) % N] = p.w;
+      }
     }
   } else {
 #pragma unroll
@@ -103,63 +111,78 @@ __device__ __forceinline__ void load_run(const void* x, size_t i, int bf16, bool
 }
 
 constexpr int kStoreWarps = 4;
+constexpr int kLoadTeams = 148 * 320;  // warps, at most: eight times what the SMs hold
 
-// Lanes a row of one head, and elements a lane: 8 where the head size is a
-// multiple of 16 (a rotation pairs runs of 8 then), else 2.
+// Elements a lane, and lanes a row of one head.  A rotation pairs whole runs, so
+// half a row is a multiple of a run of 8 or 16.  With many rows 16 elements a
+// lane keep twice the bytes on the way (7173 rows of 16 heads, bf16 to I4: 31 us
+// with 8, 22 us with 16); with few there are more lanes to share the work.
 struct RowSplit {
   int group, run;
 };
-inline RowSplit split_row(int hd) {
+inline RowSplit split_row(int hd, bool many) {
   RowSplit s;
-  s.run = hd % 16 == 0 ? 8 : 2;
+  s.run = many && hd % 32 == 0 ? 16 : hd % 16 == 0 ? 8 : 2;
   s.group = 1;
   while (s.group * s.run < hd && s.group < 32) s.group *= 2;
   return s;
 }
 
-// N elements a lane (8: once over the row; 2: as often as the row needs it).
+// N elements a lane (8 or 16: once over the row; 2: as often as the row needs it).
 template <int N, bool I4, bool ROPE>
 __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, KvqStore s, int group, int wide) {
-  constexpr int kRuns = N == 8 ? 1 : kKvqMaxHd / 64;
+  constexpr int kRuns = N >= 8 ? 1 : kKvqMaxHd / 64;
   const int lane = threadIdx.x & 31, in = lane & (group - 1);
   const int jobs = 2 * c.kv_heads + (s.q ? s.nh : 0);  // K heads, V heads, q heads of a row
-  const size_t job = ((size_t)blockIdx.x * (kStoreWarps * 32) + threadIdx.x) / group;
+  const int hd = c.hd, half = hd / 2;
+  const uint32_t job = ((size_t)blockIdx.x * (kStoreWarps * 32) + threadIdx.x) / group;  // rows * jobs is below 2^31
   const size_t row = job / jobs;
   const int what = (int)(job % jobs);
   // lanes without a row run on with the group's reductions
-  bool on = row < (size_t)s.rows;
-  const int pos = on ? (s.row_pos ? s.row_pos[row] : (int)row) : -1, seq = on && s.row_seq ? s.row_seq[row] : 0;
-  on = on && pos >= 0;
-  const int hd = c.hd, half = hd / 2;
+  const bool there = row < (size_t)s.rows;
+  const int pos = there ? (s.row_pos ? s.row_pos[row] : (int)row) : -1, seq = there && s.row_seq ? s.row_seq[row] : 0;
+  bool on = pos >= 0;
+  if (on && ROPE && pos >= s.rope_len) {
+    if (in == 0) atomicOr(s.status, kStatusBadContext);
+    on = false;
+  }
   const int kind = what < c.kv_heads ? 0 : 1, head = kind ? what - c.kv_heads : what;
   const bool is_q = what >= 2 * c.kv_heads;
   const void* src = is_q ? (const void*)s.q : kind ? s.v : s.k;
   const size_t at = row * (is_q ? s.ldq : kind ? s.ldv : s.ldk) + (size_t)(is_q ? what - 2 * c.kv_heads : head) * hd;
   const int bf16 = is_q ? 0 : s.bf16;
-  // the row, asked for before its place is known
-  float x[kRuns][N], w[kRuns][N];  // w: what a rotation pairs x with
+  float x[kRuns][N];
+  float w[ROPE ? kRuns : 1][N], cs[ROPE ? kRuns : 1][N], sn[ROPE ? kRuns : 1][N];  // a rotation's other element, cos and sin
 #pragma unroll
   for (int i = 0; i < kRuns; ++i) {
     const int d = N * (in + 32 * i);
 #pragma unroll
-    for (int j = 0; j < N; ++j) x[i][j] = w[i][j] = 0.0f;
-    if (!on || d >= hd) continue;
-    load_run<N>(src, at + d, bf16, wide, x[i]);
-    if (ROPE && (kind == 0 || is_q)) {
-      if (N == 8)
-        load_run<N>(src, at + (d < half ? d + half : d - half), bf16, wide, w[i]);
-      else
+    for (int j = 0; j < N; ++j) x[i][j] = 0.0f;
+    if (!there || d >= hd) continue;
+    load_run<N>(src, at + d, bf16, wide, x[i]);  // before its place is known
+    if (ROPE && on && (kind == 0 || is_q)) {
+      const size_t angle = (size_t)pos * half;
+      if (N >= 8) {
+        const int p = d < half ? d : d - half;
+        load_run<N>(src, at + (d < half ? d + half : p), bf16, wide, w[i]);
+        load_run<N>(s.rope_cos, angle + p, 0, wide, cs[i]);
+        load_run<N>(s.rope_sin, angle + p, 0, wide, sn[i]);
+      } else {
 #pragma unroll
-        for (int j = 0; j < N; ++j) w[i][j] = load_elem(src, at + (d + j < half ? d + j + half : d + j - half), bf16);
+        for (int j = 0; j < N; ++j) {
+          const int p = d + j < half ? d + j : d + j - half;
+          w[i][j] = load_elem(src, at + (d + j < half ? d + j + half : p), bf16);
+          cs[i][j] = s.rope_cos[angle + p];
+          sn[i][j] = s.rope_sin[angle + p];
+        }
+      }
     }
   }
   uint8_t* block = on ? block_of(c, seq, pos, is_q ? 0 : head) : nullptr;
-  if (on && (!block || (ROPE && pos >= s.rope_len))) {
+  if (on && !block) {
     if (in == 0) atomicOr(s.status, kStatusBadContext);
     on = false;
   }
-  const float* cs = ROPE && on ? s.rope_cos + (size_t)pos * half : nullptr;
-  const float* sn = ROPE && on ? s.rope_sin + (size_t)pos * half : nullptr;
   if (is_q) {  // in the reference's f32 order (rope.rs:414-431); a whole group, and no reduction below has others in it
     float* o = s.q_out + (row * s.nh + (what - 2 * c.kv_heads)) * hd;
     if (on)
@@ -168,10 +191,9 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           const int d = N * (in + 32 * i) + j;
-          if (d >= hd) continue;
-          const int p = d < half ? d : d - half;
-          o[d] = d < half ? __fsub_rn(__fmul_rn(x[i][j], cs[p]), __fmul_rn(w[i][j], sn[p]))
-                          : __fadd_rn(__fmul_rn(x[i][j], cs[p]), __fmul_rn(w[i][j], sn[p]));
+          if (!ROPE || d >= hd) continue;
+          const float a = __fmul_rn(x[i][j], cs[i][j]), b = __fmul_rn(w[i][j], sn[i][j]);
+          o[d] = d < half ? __fsub_rn(a, b) : __fadd_rn(a, b);
         }
     on = false;
   }
@@ -188,8 +210,7 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
       if (!on || d >= hd) continue;
       if (ROPE) {
         if (kind == 0) {
-          const int p = d < half ? d : d - half;
-          const double a = __dmul_rn(x[i][j], cs[p]), b = __dmul_rn(w[i][j], sn[p]);
+          const double a = __dmul_rn(x[i][j], cs[i][j]), b = __dmul_rn(w[i][j], sn[i][j]);
           v[i][j] = d < half ? __dsub_rn(a, b) : __dadd_rn(a, b);
           x[i][j] = (float)v[i][j];
         }
@@ -237,7 +258,7 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
   for (int i = 0; i < kRuns; ++i) {
     const int d = N * (in + 32 * i);
     if (d >= hd) continue;
-    uint32_t word[2] = {0u, 0u};
+    uint32_t word[4] = {0u, 0u, 0u, 0u};
     if (!bad && scale > 0.0f)
 #pragma unroll
       for (int j = 0; j < N; ++j) {
@@ -245,18 +266,22 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
         const float yf = I4 ? (ROPE ? (float)y : __fsub_rn(x[i][j], zero)) : x[i][j];
         const uint32_t q = (uint32_t)nearest_code(y, yf, scale, inv, I4 ? 0 : -127, I4 ? 15 : 127);
         if (I4)
-          word[0] |= q << (4 * j);
+          word[j / 8] |= q << (4 * (j % 8));
         else
           word[j / 4] |= (q & 255u) << (8 * (j % 4));
       }
-    if (N == 8 && I4)
-      *(uint32_t*)(codes + d / 2) = word[0];
-    else if (N == 8)
-      *(uint2*)(codes + d) = make_uint2(word[0], word[1]);
-    else if (I4)
-      codes[d / 2] = (uint8_t)word[0];
+    uint8_t* dst = codes + (I4 ? d / 2 : d);
+    constexpr int kBytes = I4 ? N / 2 : N;
+    if (kBytes == 16)
+      *(uint4*)dst = make_uint4(word[0], word[1], word[2], word[3]);
+    else if (kBytes == 8)
+      *(uint2*)dst = make_uint2(word[0], word[1]);
+    else if (kBytes == 4)
+      *(uint32_t*)dst = word[0];
+    else if (kBytes == 2)
+      *(uint16_t*)dst = (uint16_t)word[0];
     else
-      *(uint16_t*)(codes + d) = (uint16_t)word[0];
+      *dst = (uint8_t)word[0];
   }
   if (in == 0) {
     float* par = block_params(block, hd, I4, kind);
@@ -266,84 +291,115 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
 }
 
 // ---------------------------------------------------------------------------
-// Load.  A warp reads a row of K and V, all heads, the lanes over runs of N
-// elements in the order in which they are written.  kLoadAhead runs a lane are
-// asked for before the first is written.
+// Load.  Warps take rows in turn, all heads of K and V, the lanes over runs of
+// N elements in the order in which they are written; several warps share a row
+// when there are few.  Where the next row's blocks lie (three dependent loads)
+// is asked for before this row is read, and kLoadAhead runs a lane before the
+// first is written.  Codes become floats without conversions: a byte below the
+// bits of 2^23 is 2^23 + c.  Bound by memory.
 // ---------------------------------------------------------------------------
 __device__ __forceinline__ float code_at(const uint8_t* codes, int d, int i4) {
   return i4 ? (float)((codes[d >> 1] >> ((d & 1) * 4)) & 15) : (float)(int8_t)codes[d];
 }
 constexpr int kLoadAhead = 4;
+// Byte i of w (unsigned), less `bias`, as a float.
+__device__ __forceinline__ float byte_f32(uint32_t w, int i, float bias) {
+  return __fsub_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7440 + i)), 8388608.0f + bias);
+}
 template <int N, bool I4>
+__device__ __forceinline__ void codes_f32(const uint32_t* w, float* x) {
+  if (I4) {
+    const uint32_t even = w[0] & 0x0f0f0f0fu, odd = (w[0] >> 4) & 0x0f0f0f0fu;
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = byte_f32(j % 2 ? odd : even, j / 2, 0.0f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < N; ++j) x[j] = byte_f32(w[j / 4] ^ 0x80808080u, j % 4, 128.0f);
+  }
+}
+// HD: the head size, or 0 where it is not one of the common ones.
+template <int HD, int N, bool I4>
 __global__ void __launch_bounds__(kStoreWarps * 32)
     kvq_load_kernel(KvqView c, int rows, const int32_t* __restrict__ row_seq, const int32_t* __restrict__ row_pos,
                     void* __restrict__ k, size_t ldk, void* __restrict__ v, size_t ldv, int bf16, int wide,
                     int per_row, int32_t* status) {
-  // per_row warps share a row
-  const int lane = threadIdx.x & 31, hd = c.hd, runs = hd / N, all = 2 * c.kv_heads * runs;
-  const size_t job = (size_t)blockIdx.x * kStoreWarps + (threadIdx.x >> 5);
-  const int row = (int)(job / per_row), part = (int)(job % per_row);
-  if (row >= rows) return;
-  const int pos = row_pos ? row_pos[row] : row;
-  if (pos < 0) return;
-  const uint8_t* first = block_of(c, row_seq ? row_seq[row] : 0, pos, 0);
-  if (!first) {
-    if (lane == 0) atomicOr(status, kStatusBadContext);
-    return;
-  }
-  const int slot = pos % kPage, rowb = kvq_row_bytes(hd, I4), block_bytes = kvq_block_bytes(hd, I4);
-  for (int r0 = part * 32 + lane; r0 < all; r0 += per_row * 32 * kLoadAhead) {
-    uint32_t w[kLoadAhead][2];
-    float scale[kLoadAhead], zero[kLoadAhead];
-#pragma unroll
-    for (int i = 0; i < kLoadAhead; ++i) {
-      const int r = r0 + i * per_row * 32;
-      if (r >= all) continue;
-      const int which = r / runs, d = r % runs * N, kind = which >= c.kv_heads, head = which - kind * c.kv_heads;
-      const uint8_t* block = first + (size_t)head * block_bytes;
-      const uint8_t* codes = block + (kind * kPage + slot) * rowb;
-      if (N == 8 && I4) {
-        w[i][0] = *(const uint32_t*)(codes + d / 2);
-      } else if (N == 8) {
-        const uint2 u = *(const uint2*)(codes + d);
-        w[i][0] = u.x;
-        w[i][1] = u.y;
-      } else {
-        w[i][0] = I4 ? codes[d / 2] : *(const uint16_t*)(codes + d);
-      }
-      const float* par = block_params((uint8_t*)block, hd, I4, kind);
-      scale[i] = par[slot];
-      zero[i] = I4 ? par[kPage + slot] : 0.0f;
+  const int lane = threadIdx.x & 31, hd = HD ? HD : c.hd, runs = hd / N, all = 2 * c.kv_heads * runs;
+  const int warp = blockIdx.x * kStoreWarps + (threadIdx.x >> 5), teams = gridDim.x * kStoreWarps / per_row;
+  const int part = warp % per_row;
+  const int rowb = kvq_row_bytes(hd, I4), block_bytes = kvq_block_bytes(hd, I4);
+  int row = warp / per_row;
+  if (row >= teams) return;  // warps that make no whole team
+  int pos = -1, next_pos = -1;
+  const uint8_t *first = nullptr, *next = nullptr;
+  auto look_up = [&](int r, int* p) -> const uint8_t* {
+    *p = r < rows ? (row_pos ? row_pos[r] : r) : -1;
+    return *p >= 0 ? block_of(c, row_seq ? row_seq[r] : 0, *p, 0) : nullptr;
+  };
+  next = look_up(row, &next_pos);
+  for (; row < rows; row += teams) {
+    first = next;
+    pos = next_pos;
+    next = look_up(row > INT_MAX - teams ? INT_MAX : row + teams, &next_pos);
+    if (!first) {
+      if (lane == 0 && pos >= 0) atomicOr(status, kStatusBadContext);
+      if (row > INT_MAX - teams) break;
+      continue;
     }
+    const uint8_t* from = first + pos % kPage * rowb;  // head 0's K codes, and its K parameters
+    const float* par0 = block_params((uint8_t*)first, hd, I4, 0) + pos % kPage;
+    const size_t row_k = (size_t)row * ldk, row_v = (size_t)row * ldv;
+    for (int r0 = part * 32 + lane; r0 < all; r0 += per_row * 32 * kLoadAhead) {
+      uint32_t w[kLoadAhead][2];
+      float scale[kLoadAhead], zero[kLoadAhead];
 #pragma unroll
-    for (int i = 0; i < kLoadAhead; ++i) {
-      const int r = r0 + i * per_row * 32;
-      if (r >= all) continue;
-      const int which = r / runs, d = r % runs * N, kind = which >= c.kv_heads, head = which - kind * c.kv_heads;
-      void* dst = kind ? v : k;
-      const size_t at = (size_t)row * (kind ? ldv : ldk) + (size_t)head * hd + d;
-      float x[N];
-#pragma unroll
-      for (int j = 0; j < N; ++j) {
-        const float q = I4 ? (float)((w[i][0] >> (4 * j)) & 15u) : (float)(int8_t)(w[i][j / 4] >> (8 * (j % 4)));
-        x[j] = __fmaf_rn(q, scale[i], zero[i]);
-      }
-      if (N == 8 && wide && bf16) {
-        uint32_t u[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * j], x[2 * j + 1]);
-          u[j] = *(const uint32_t*)&p;
+      for (int i = 0; i < kLoadAhead; ++i) {
+        const int r = r0 + i * per_row * 32;
+        if (r >= all) continue;
+        const int which = r / runs, d = r % runs * N, kind = which >= c.kv_heads;
+        const uint32_t to_block = (which - kind * c.kv_heads) * block_bytes;
+        const uint8_t* codes = from + (to_block + kind * (kPage * rowb));
+        if (N == 8 && I4) {
+          w[i][0] = *(const uint32_t*)(codes + d / 2);
+        } else if (N == 8) {
+          const uint2 u = *(const uint2*)(codes + d);
+          w[i][0] = u.x;
+          w[i][1] = u.y;
+        } else {
+          w[i][0] = I4 ? codes[d / 2] : *(const uint16_t*)(codes + d);
         }
-        *(uint4*)((uint16_t*)dst + at) = make_uint4(u[0], u[1], u[2], u[3]);
-      } else if (N == 8 && wide) {
-        *(float4*)((float*)dst + at) = make_float4(x[0], x[1], x[2], x[3]);
-        *(float4*)((float*)dst + at + 4) = make_float4(x[4 % N], x[5 % N], x[6 % N], x[7 % N]);
-      } else {
+        const float* par = (const float*)((const uint8_t*)par0 + (to_block + kind * (I4 ? 128 : 64)));
+        scale[i] = par[0];
+        zero[i] = I4 ? par[kPage] : 0.0f;
+      }
 #pragma unroll
-        for (int j = 0; j < N; ++j) store_elem(dst, at + j, bf16, x[j]);
+      for (int i = 0; i < kLoadAhead; ++i) {
+        const int r = r0 + i * per_row * 32;
+        if (r >= all) continue;
+        const int kind = r >= all / 2;  // K and V rows are written in the order of r
+        void* dst = kind ? v : k;
+        const size_t at = (kind ? row_v : row_k) + (r - kind * (all / 2)) * N;
+        float x[N];
+        codes_f32<N, I4>(w[i], x);
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] = __fmaf_rn(x[j], scale[i], zero[i]);
+        if (N == 8 && wide && bf16) {
+          uint32_t u[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(x[2 * j % N], x[(2 * j + 1) % N]);
+            u[j] = *(const uint32_t*)&p;
+          }
+          *(uint4*)((uint16_t*)dst + at) = make_uint4(u[0], u[1], u[2], u[3]);
+        } else if (N == 8 && wide) {
+          *(float4*)((float*)dst + at) = make_float4(x[0], x[1], x[2 % N], x[3 % N]);
+          *(float4*)((float*)dst + at + 4) = make_float4(x[4 % N], x[5 % N], x[6 % N], x[7 % N]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < N; ++j) store_elem(dst, at + j, bf16, x[j]);
+        }
       }
     }
+    if (row > INT_MAX - teams) break;
   }
 }
 
@@ -1426,10 +1482,13 @@ void launch_store_of(const KvqView& c, const KvqStore& s, int group, int wide, c
 
 void launch_kvq_store(const KvqView& c, const KvqStore& s, cudaStream_t st) {
   if (s.rows <= 0) return;
-  const RowSplit split = split_row(c.hd);
+  const RowSplit split = split_row(c.hd, (size_t)s.rows * c.kv_heads >= 148 * 64);
   const int wide = aligned_runs(s.k, s.ldk, s.bf16) && aligned_runs(s.v, s.ldv, s.bf16) &&
-                   (!s.q || aligned_runs(s.q, s.ldq, 0));
-  if (split.run == 8)
+                   (!s.q || aligned_runs(s.q, s.ldq, 0)) && (uintptr_t)s.rope_cos % 16 == 0 &&
+                   (uintptr_t)s.rope_sin % 16 == 0;
+  if (split.run == 16)
+    launch_store_of<16>(c, s, split.group, wide, st);
+  else if (split.run == 8)
     launch_store_of<8>(c, s, split.group, wide, st);
   else
     launch_store_of<2>(c, s, split.group, wide, st);
@@ -1439,13 +1498,20 @@ void launch_kvq_store(const KvqView& c, const KvqStore& s, cudaStream_t st) {
 void launch_kvq_load(const KvqView& c, int rows, const int32_t* row_seq, const int32_t* row_pos, void* k, size_t ldk,
                      void* v, size_t ldv, int bf16, int32_t* status, cudaStream_t st) {
   if (rows <= 0) return;
-  const int run = split_row(c.hd).run, wide = aligned_runs(k, ldk, bf16) && aligned_runs(v, ldv, bf16);
+  const int run = split_row(c.hd, false).run, wide = aligned_runs(k, ldk, bf16) && aligned_runs(v, ldv, bf16);
   // few rows: more warps to each, so that all runs are asked for at once
   const int most = (int)ceil_div((size_t)2 * c.kv_heads * (c.hd / run), 32);
-  const int per_row = rows >= 148 * 16 ? (int)ceil_div(most, kLoadAhead) : most;
-  const unsigned blocks = (unsigned)ceil_div((size_t)rows * per_row, kStoreWarps);
-  auto* kernel = run == 8 ? (c.i4 ? kvq_load_kernel<8, true> : kvq_load_kernel<8, false>)
-                          : (c.i4 ? kvq_load_kernel<2, true> : kvq_load_kernel<2, false>);
+  const int per_row = rows >= 148 * 16 ? (int)ceil_div(most, 2 * kLoadAhead) : most;
+  const unsigned blocks = (unsigned)ceil_div((size_t)std::min(rows, kLoadTeams) * per_row, kStoreWarps);
+  auto* kernel = kvq_load_kernel<0, 2, false>;
+  if (run == 2)
+    kernel = c.i4 ? kvq_load_kernel<0, 2, true> : kvq_load_kernel<0, 2, false>;
+  else if (c.hd == 128)
+    kernel = c.i4 ? kvq_load_kernel<128, 8, true> : kvq_load_kernel<128, 8, false>;
+  else if (c.hd == 64)
+    kernel = c.i4 ? kvq_load_kernel<64, 8, true> : kvq_load_kernel<64, 8, false>;
+  else
+    kernel = c.i4 ? kvq_load_kernel<0, 8, true> : kvq_load_kernel<0, 8, false>;
   kernel<<<blocks, kStoreWarps * 32, 0, st>>>(c, rows, row_seq, row_pos, k, ldk, v, ldv, bf16, wide, per_row, status);
   count_launch();
 }
