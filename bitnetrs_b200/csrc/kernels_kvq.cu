@@ -1,7 +1,6 @@
 // kernels_kvq.cu — the quantised paged key-value cache: rows quantised into
-// their slots, rows read back, and GQA attention split over the context.
-#include "async.cuh"
-#include "kvq.cuh"
+// their slots, and rows read back.
+#include "kvq_device.cuh"
 
 #include <algorithm>
 #include <climits>
@@ -23,28 +22,6 @@ KvqView kvq_layer(const KvGeom& g, const int32_t* table, int seqs, int layer) {
 
 namespace {
 
-// The block of (position, head) of a sequence; null when the sequence, the
-// position or the page that the table names lies outside the cache.
-__device__ __forceinline__ uint8_t* block_of(const KvqView& c, int seq, int pos, int head) {
-  if ((unsigned)seq >= (unsigned)c.seqs || pos < 0 || pos / kPage >= c.per_seq) return nullptr;
-  const int page = c.table[(size_t)seq * c.per_seq + pos / kPage];
-  if ((unsigned)page >= (unsigned)c.pages) return nullptr;
-  return c.pool + ((size_t)page * c.kv_heads + head) * kvq_block_bytes(c.hd, c.i4);
-}
-// Parameters of a kind (0 K, 1 V): 16 scales, then for I4 16 zeros.
-__device__ __forceinline__ float* block_params(uint8_t* block, int hd, int i4, int kind) {
-  return (float*)(block + 2 * kPage * kvq_row_bytes(hd, i4)) + kind * kPage * (i4 ? 2 : 1);
-}
-
-__device__ __forceinline__ float load_elem(const void* x, size_t i, int bf16) {
-  return bf16 ? bf16_bits_to_f32(((const uint16_t*)x)[i]) : ((const float*)x)[i];
-}
-__device__ __forceinline__ void store_elem(void* x, size_t i, int bf16, float v) {
-  if (bf16)
-    ((uint16_t*)x)[i] = f32_to_bf16_bits(v);
-  else
-    ((float*)x)[i] = v;
-}
 // ---------------------------------------------------------------------------
 // Store.  A group of GROUP lanes (a power of two) quantises one row of one
 // head, N neighbouring elements a lane: the largest magnitude (I8) or the
@@ -298,9 +275,6 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
 // first is written.  Codes become floats without conversions: a byte below the
 // bits of 2^23 is 2^23 + c.  Bound by memory.
 // ---------------------------------------------------------------------------
-__device__ __forceinline__ float code_at(const uint8_t* codes, int d, int i4) {
-  return i4 ? (float)((codes[d >> 1] >> ((d & 1) * 4)) & 15) : (float)(int8_t)codes[d];
-}
 constexpr int kLoadAhead = 4;
 // Byte i of w (unsigned), less `bias`, as a float.
 __device__ __forceinline__ float byte_f32(uint32_t w, int i, float bias) {
@@ -403,1062 +377,6 @@ __global__ void __launch_bounds__(kStoreWarps * 32)
   }
 }
 
-// ---------------------------------------------------------------------------
-// Attention.  A unit is the (up to kMaxHeads) query heads of one row that share
-// a kv head; its work is the pages of the row's context.  The pages of all
-// units form one line, row by row and unit by unit, that is cut into equal
-// shares, one a CTA, so that a long context and a ragged batch load the GPU
-// evenly without the host knowing the lengths.  A unit that lies inside one
-// share is finished there.  One that is cut leaves a partial result (running
-// maximum, sum, unnormalised output) in each share it touches; a second kernel
-// joins them in the line's order, so a result depends on the lengths alone.
-// A share holds at most two partial units: its first (slot 0) and its last
-// (slot 1; a share inside one unit uses slot 0).
-// ---------------------------------------------------------------------------
-constexpr int kMaxHeads = 8;
-constexpr int kAttendCtas = 148 * 4;
-struct ShareMeta {
-  int row, unit;  // the unit that begins in this share and ends in a later one (row < 0: none)
-  int ends;       // whether the unit of slot 0 ends in this share
-  int pad;
-};
-
-struct Units {
-  int per_row, per_kv, heads;  // units a row, units a kv head, heads a unit
-};
-__host__ __device__ inline Units units_of(int nh, int kv_heads) {
-  const int group = nh / kv_heads;
-  Units u;
-  u.per_kv = (group + kMaxHeads - 1) / kMaxHeads;
-  u.heads = (group + u.per_kv - 1) / u.per_kv;
-  u.per_row = kv_heads * u.per_kv;
-  return u;
-}
-// The query heads of unit u: [first, first + n).
-__device__ __forceinline__ void unit_heads(const Units& us, int nh, int kv_heads, int u, int* kvh, int* first, int* n) {
-  const int group = nh / kv_heads, part = u % us.per_kv;
-  *kvh = u / us.per_kv;
-  *first = *kvh * group + part * us.heads;
-  *n = min(us.heads, group - part * us.heads);
-}
-
-// What row r sees: its sequence and how many positions (-1: the row belongs to no run).
-__device__ __forceinline__ int row_context(const KvqView& c, const KvqRows& R, int r, int max_len, int* seq,
-                                           int32_t* status) {
-  int len;
-  if (R.runs) {
-    if (r < R.cu[0] || r >= R.cu[R.runs]) return -1;
-    int lo = 0, hi = R.runs;  // cu[lo] <= r < cu[hi]
-    while (hi - lo > 1) {
-      const int mid = (lo + hi) / 2;
-      if (R.cu[mid] <= r)
-        lo = mid;
-      else
-        hi = mid;
-    }
-    *seq = R.seq_ids[lo];
-    len = R.starts[lo] + (r - R.cu[lo]) + 1;
-  } else {
-    *seq = R.row_seq[r];
-    len = R.row_len[r] + R.len_bias;
-  }
-  if (len <= 0) return 0;
-  if ((unsigned)*seq >= (unsigned)c.seqs) {
-    atomicOr(status, kStatusBadContext);
-    return 0;
-  }
-  if (len > max_len) {
-    atomicOr(status, kStatusBadContext);
-    len = max_len;
-  }
-  return len;
-}
-
-__device__ __forceinline__ float* share_slot(void* space, int shares, int share, int slot, int hd, const Units& us) {
-  return (float*)((ShareMeta*)space + shares) + ((size_t)share * 2 + slot) * (us.heads * (hd + 2));
-}
-
-// A partial result that a warp of the tensor-core kernel leaves for its CTA's
-// join, behind the shares' slots; rows padded like the ring's.
-__device__ __forceinline__ float* warp_slot(void* space, int shares, int warp, int hd, const Units& us) {
-  const size_t slots = (size_t)shares * 2 * (us.heads * (hd + 2));
-  return (float*)((ShareMeta*)space + shares) + (slots + 3) / 4 * 4 + (size_t)warp * (us.heads * (hd + 4));
-}
-
-__device__ void write_empty_row(const KvqAttend& a, int hd, int r) {
-  for (int i = threadIdx.x; i < a.nh * hd; i += blockDim.x) store_elem(a.out, (size_t)r * a.ldo + i, a.bf16, 0.0f);
-  if (a.lse)
-    for (int i = threadIdx.x; i < a.nh; i += blockDim.x) a.lse[(size_t)r * a.nh + i] = -INFINITY;
-}
-
-// One head's joined result (m in units of log2): output and log-sum-exp.
-__device__ __forceinline__ float lse_of(float m, float l) {
-  return l > 0.0f || isnan(l) ? __fmul_rn(__fadd_rn(m, log2f(l)), 0.69314718055994530942f) : -INFINITY;
-}
-
-constexpr int kPlainWarps = 4;
-
-// The simple form, for every head size: a warp takes whole pages; lanes share
-// a score as 16 positions x 2 halves of the dimensions, then own dimensions of
-// the output.
-__global__ void __launch_bounds__(kPlainWarps * 32)
-    kvq_attend_plain_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len) {
-  extern __shared__ float sm[];
-  __shared__ int found[4];
-  __shared__ long long total_sh, base_sh;
-  const int hd = c.hd, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const Units us = units_of(a.nh, c.kv_heads);
-  float* qs = sm;                                   // [heads][hd], scaled
-  float* part = qs + us.heads * hd;                 // [warps][heads][hd]
-  float* ml = part + kPlainWarps * us.heads * hd;   // [warps][heads][2]
-  const int shares = gridDim.x, share = blockIdx.x;
-  ShareMeta* meta = (ShareMeta*)a.space;
-  // the line's length, and rows that see nothing
-  if (tid == 0) {
-    total_sh = 0;
-    found[0] = -1;
-  }
-  __syncthreads();
-  long long mine = 0;
-  for (int r = tid; r < R.rows; r += blockDim.x) {
-    int seq;
-    const int len = row_context(c, R, r, max_len, &seq, a.status);
-    if (len > 0) mine += (len + kPage - 1) / kPage;
-  }
-  atomicAdd((unsigned long long*)&total_sh, (unsigned long long)mine);
-  for (int r = share; r < R.rows; r += shares) {
-    int seq;
-    if (row_context(c, R, r, max_len, &seq, a.status) == 0) write_empty_row(a, hd, r);
-  }
-  __syncthreads();
-  const long long total = total_sh * us.per_row;
-  const long long cuts = min((long long)shares, (total + kPlainWarps - 1) / kPlainWarps);
-  if (tid == 0) meta[share] = ShareMeta{-1, 0, 0, 0};
-  if (share >= cuts) return;
-  long long at = total * share / cuts;
-  const long long end = total * (share + 1) / cuts;
-  // the row in which the share begins
-  if (tid == 0) {
-    long long base = 0;
-    for (int r = 0; r < R.rows; ++r) {
-      int seq;
-      const int len = row_context(c, R, r, max_len, &seq, a.status);
-      const long long n = len > 0 ? (long long)((len + kPage - 1) / kPage) * us.per_row : 0;
-      if (at < base + n) {
-        found[0] = r;
-        base_sh = base;
-        break;
-      }
-      base += n;
-    }
-  }
-  __syncthreads();
-  int r = found[0];
-  long long base = base_sh;
-  const float qscale = __fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)hd));
-  while (at < end && r < R.rows) {
-    int seq = 0;
-    const int len = row_context(c, R, r, max_len, &seq, a.status);
-    const int pages = len > 0 ? (len + kPage - 1) / kPage : 0;
-    if (at >= base + (long long)pages * us.per_row) {
-      base += (long long)pages * us.per_row;
-      ++r;
-      continue;
-    }
-    const int u = (int)((at - base) / pages), first_page = (int)((at - base) % pages);
-    const int n_pages = (int)min((long long)(pages - first_page), end - at);
-    int kvh, h0, heads;
-    unit_heads(us, a.nh, c.kv_heads, u, &kvh, &h0, &heads);
-    __syncthreads();
-    for (int i = tid; i < heads * hd; i += blockDim.x)
-      qs[i] = __fmul_rn(load_elem(a.q, (size_t)r * a.ldq + (size_t)h0 * hd + i, a.bf16), qscale);
-    __syncthreads();
-    float m[kMaxHeads], l[kMaxHeads], acc[kMaxHeads][kKvqMaxHd / 32];
-#pragma unroll
-    for (int h = 0; h < kMaxHeads; ++h) {
-      m[h] = -INFINITY;
-      l[h] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < kKvqMaxHd / 32; ++i) acc[h][i] = 0.0f;
-    }
-    for (int p = first_page + warp; p < first_page + n_pages; p += kPlainWarps) {
-      uint8_t* block = block_of(c, seq, p * kPage, kvh);
-      if (!block) {
-        if (lane == 0) atomicOr(a.status, kStatusBadContext);
-        continue;
-      }
-      const int slot = lane & 15, rowb = kvq_row_bytes(hd, c.i4);
-      const bool live = p * kPage + slot < len;
-      const float* kp = block_params(block, hd, c.i4, 0);
-      const float* vp = block_params(block, hd, c.i4, 1);
-      const float ks = kp[slot], kz = c.i4 ? kp[kPage + slot] : 0.0f;
-      const float vs = live ? vp[slot] : 0.0f, vz = c.i4 && live ? vp[kPage + slot] : 0.0f;
-      const uint8_t* kc = block + (size_t)slot * rowb;
-#pragma unroll
-      for (int h = 0; h < kMaxHeads; ++h) {
-        if (h >= heads) continue;
-        float dot = 0.0f;
-        for (int d = lane >> 4; d < hd; d += 2) dot = __fmaf_rn(qs[h * hd + d], __fmaf_rn(code_at(kc, d, c.i4), ks, kz), dot);
-        dot = __fadd_rn(dot, __shfl_xor_sync(0xffffffffu, dot, 16));
-        if (!live) dot = -INFINITY;
-        float top = dot;
-#pragma unroll
-        for (int o = 8; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        const float mn = fmaxf(m[h], top), keep = exp2f(__fsub_rn(m[h], mn));
-        const float w = live ? exp2f(__fsub_rn(dot, mn)) : 0.0f;
-        m[h] = mn;
-        float sum = w;
-#pragma unroll
-        for (int o = 8; o; o >>= 1) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
-        l[h] = __fmaf_rn(l[h], keep, sum);
-#pragma unroll
-        for (int i = 0; i < kKvqMaxHd / 32; ++i) acc[h][i] = __fmul_rn(acc[h][i], keep);
-        for (int j = 0; j < kPage && p * kPage + j < len; ++j) {
-          const float wj = __shfl_sync(0xffffffffu, w, j);
-          const float s = __shfl_sync(0xffffffffu, vs, j), z = __shfl_sync(0xffffffffu, vz, j);
-          const uint8_t* vc = block + (size_t)(kPage + j) * rowb;
-#pragma unroll
-          for (int i = 0; i < kKvqMaxHd / 32; ++i)
-            if (lane + 32 * i < hd)
-              acc[h][i] = __fmaf_rn(wj, __fmaf_rn(code_at(vc, lane + 32 * i, c.i4), s, z), acc[h][i]);
-        }
-      }
-    }
-#pragma unroll
-    for (int h = 0; h < kMaxHeads; ++h) {
-      if (h >= heads) continue;
-#pragma unroll
-      for (int i = 0; i < kKvqMaxHd / 32; ++i)
-        if (lane + 32 * i < hd) part[(warp * us.heads + h) * hd + lane + 32 * i] = acc[h][i];
-      if (lane == 0) {
-        ml[(warp * us.heads + h) * 2] = m[h];
-        ml[(warp * us.heads + h) * 2 + 1] = l[h];
-      }
-    }
-    __syncthreads();
-    const bool begins = first_page == 0, ends = first_page + n_pages == pages;
-    float* slot = share_slot(a.space, shares, share, begins && !ends ? 1 : 0, hd, us);
-    for (int i = tid; i < heads * hd; i += blockDim.x) {
-      const int h = i / hd, d = i % hd;
-      float M = -INFINITY, L = 0.0f, o = 0.0f;
-      for (int w = 0; w < kPlainWarps; ++w) M = fmaxf(M, ml[(w * us.heads + h) * 2]);
-      for (int w = 0; w < kPlainWarps; ++w) {
-        const float mw = ml[(w * us.heads + h) * 2], lw = ml[(w * us.heads + h) * 2 + 1];
-        if (lw == 0.0f) continue;  // a warp without pages
-        const float f = exp2f(__fsub_rn(mw, M));
-        L = __fmaf_rn(lw, f, L);
-        o = __fmaf_rn(part[(w * us.heads + h) * hd + d], f, o);
-      }
-      if (begins && ends) {
-        store_elem(a.out, (size_t)r * a.ldo + (size_t)h0 * hd + i, a.bf16, __fdiv_rn(o, L));
-        if (a.lse && d == 0) a.lse[(size_t)r * a.nh + h0 + h] = lse_of(M, L);
-      } else {
-        slot[h * (hd + 2) + d] = o;
-        if (d == 0) {
-          slot[h * (hd + 2) + hd] = M;
-          slot[h * (hd + 2) + hd + 1] = L;
-        }
-      }
-    }
-    if (tid == 0) {
-      if (begins && !ends) {
-        meta[share].row = r;
-        meta[share].unit = u;
-      }
-      if (!begins) meta[share].ends = ends;
-    }
-    at += n_pages;
-  }
-}
-
-// ---------------------------------------------------------------------------
-// The tensor-core form, for head sizes of 64, 96 and 128 (I4: 64, 128).
-//
-// One warp multiplies a page (two of them in turn), its 16 positions (scores) or 16
-// dimensions (output) being the M of a product, and four heads its N.
-//   S[pos][head] = K codes . q        m16n8k32, 8-bit integers
-//   O[dim][head] += V codes^T . w     m16n8k16, fp16 with f32 sums
-// Scores: codes go into the product as they lie in memory.  q is held as a
-// 31-bit integer a dimension (relative to the head's largest element) in four
-// balanced digits of base 256, one column each, so that the integer products
-// are exact and a head's four columns, two in each of two products, are the
-// score.  The scale of a K row multiplies it.
-// Output: codes are exact in fp16.  A weight is not, so it is the sum of two
-// fp16 terms (22 bits), in neighbouring columns; a lane's pair of sums belongs
-// to one head.  The scale of a V row multiplies its weight before that is
-// split.  An I4 zero enters scores (times the sum of q) and output as a sum of
-// its own.
-// The weights are multiplied by a power of two a warp so that the largest
-// scale of V seen is near 2^5 and at most 2^9 (rescaled like the sums when a
-// larger one comes; a weight is at most 2^kSlack): a second term then still
-// holds 2^-30 of the largest weight.
-//
-// Each warp has a ring of pages of its own in shared memory.  One lane fetches
-// a page with two copies of the asynchronous copy engine, the codes as a tile
-// of 128-byte lines with their 16-byte pieces exchanged (128-byte swizzle), so
-// that loads of 8 rows x 16 bytes meet no bank twice, and the parameters as
-// they are.
-// Measured on a batch of 256 contexts of 128 to 4096 (I8), with the same bytes
-// asked for ahead: copies by each lane (cp.async) stop at 4.0 TB/s, since a
-// load that goes through L1 needs an entry there until it lands.
-//
-// Here the line of pages is cut into equal shares for the warps, not the
-// CTAs, so that no warp waits for another before its share is done.  The warps
-// of a CTA hold neighbouring shares: at the end the CTA joins the units that
-// its warps cut, and leaves to the join kernel those that CTAs cut.
-//
-// The order of dimensions inside a product is free, so a lane fetches wide
-// pieces of a row for its K operand (HD/4 codes of two rows, the four lanes of
-// a row side by side) and its V operand (HD/8 codes of four rows).  They come
-// by cp.async into a ring that only the same lane reads, so a warp waits for
-// its own copies alone.
-// ---------------------------------------------------------------------------
-constexpr int kMmaMaxWarps = 8;
-constexpr int kMmaShares = 296;  // two CTAs an SM with up to four heads a unit, else one
-// How far a score may exceed the running maximum before the sums are rescaled
-// (log2): rescaling then all but stops after a unit's first pages.
-constexpr float kSlack = 6.0f;
-
-template <int HD, bool I4, int NT>
-struct MmaTile {
-  static constexpr int kRow = I4 ? HD / 2 : HD;         // bytes of a row's codes
-  static constexpr int kChunks = kRow / 16;             // 16-byte pieces of a row
-  static constexpr int kCodes = 2 * kPage * kRow;         // bytes of a page's codes
-  static constexpr int kTile = (kCodes + 1023) / 1024 * 1024;
-  static constexpr int kParams = I4 ? 256 : 128;
-  // Warps a CTA and stages (of two pages) a warp: what shared memory holds
-  // twice an SM (once with NT = 2).
-  static constexpr int kWarps = NT == 1 && kTile > 3 * 1024 ? 6 : kMmaMaxWarps;
-  static constexpr int kStages = NT == 2 ? 3 : kTile <= 1024 ? 4 : kRow == 64 && !I4 ? 3 : 2;
-  static constexpr int kRing = kStages * 2 * kTile;  // a warp's tiles
-  static constexpr int kSmem = kWarps * kStages * 2 * (kTile + kParams);
-  static constexpr int kKSteps = HD / 32, kMTiles = HD / 16;
-  static constexpr int kPartStride = HD + 4;  // floats a head of a warp's partial result
-};
-
-// Where byte x of a tile lies: 16-byte pieces of a 128-byte line are exchanged by the line's number.
-__device__ __forceinline__ int swizzled(int x) { return x ^ ((x >> 3) & 0x70); }
-
-// A tile of one block's codes, lines of 128 bytes, swizzled as above.
-__device__ __forceinline__ void tma_codes(uint32_t dst, const CUtensorMap* map, int block, uint32_t bar) {
-  asm volatile(
-      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes"
-      " [%0], [%1, {%2, %2, %3}], [%4];\n" ::"r"(dst),
-      "l"((uint64_t)map), "r"(0), "r"(block), "r"(bar)
-      : "memory");
-}
-__device__ __forceinline__ void tma_bytes(uint32_t dst, const void* src, uint32_t bytes, uint32_t bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];\n" ::"r"(dst),
-               "l"((uint64_t)src), "r"(bytes), "r"(bar)
-               : "memory");
-}
-// N (2 or 4) matrices of 8 rows x 16 bytes, whose row addresses the lanes
-// 8 i .. 8 i + 7 hold for matrix i.  A lane gets bytes 4t .. 4t + 3 of row g;
-// transposed (as 16-bit elements) bytes 2g, 2g + 1 of rows 2t and 2t + 1.
-template <int N, bool TRANS>
-__device__ __forceinline__ void load_matrices(uint32_t addr, uint32_t* w) {
-  if constexpr (N == 4 && TRANS)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];\n"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                 : "r"(addr));
-  else if constexpr (N == 4)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];\n"
-                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
-                 : "r"(addr));
-  else if constexpr (TRANS)
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.trans.shared.b16 {%0, %1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
-  else
-    asm volatile("ldmatrix.sync.aligned.m8n8.x2.shared.b16 {%0, %1}, [%2];\n" : "=r"(w[0]), "=r"(w[1]) : "r"(addr));
-}
-// All pieces of 16 rows: w[2 c + h] is piece c of rows 8 h .. 8 h + 7.
-template <int CHUNKS, bool TRANS>
-__device__ __forceinline__ void load_rows(uint32_t tile, const int* at, uint32_t* w) {
-#pragma unroll
-  for (int c = 0; c < CHUNKS; c += 2) {
-    if (c + 1 < CHUNKS)
-      load_matrices<4, TRANS>(tile + at[c / 2], w + 2 * c);
-    else
-      load_matrices<2, TRANS>(tile + at[c / 2], w + 2 * c);
-  }
-}
-// c += product, fp16
-__device__ __forceinline__ void mma_f16(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                        uint32_t b1) {
-  asm(
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-// c = product (START) or c += product
-template <bool START>
-__device__ __forceinline__ void mma_s8(int (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
-  if constexpr (START)
-    asm(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%10, %10, %10, %10};\n"
-        : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "r"(0));
-  else
-    asm(
-        "mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};\n"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
-  uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;\n" : "=r"(y) : "r"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;\n" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-__device__ __forceinline__ float f16_lo(uint32_t h) {
-  float r;
-  asm("{ .reg .f16 a, b; mov.b32 {a, b}, %1; cvt.f32.f16 %0, a; }\n" : "=f"(r) : "r"(h));
-  return r;
-}
-__device__ __forceinline__ float f16_hi(uint32_t h) {
-  float r;
-  asm("{ .reg .f16 a, b; mov.b32 {a, b}, %1; cvt.f32.f16 %0, b; }\n" : "=f"(r) : "r"(h));
-  return r;
-}
-__device__ __forceinline__ uint32_t add_f16x2(uint32_t a, uint32_t b) {
-  uint32_t r;
-  asm("add.rn.f16x2 %0, %1, %2;\n" : "=r"(r) : "r"(a), "r"(b));
-  return r;
-}
-__device__ __forceinline__ uint32_t fma_f16x2(uint32_t a, uint32_t b, uint32_t c) {
-  uint32_t r;
-  asm("fma.rn.f16x2 %0, %1, %2, %3;\n" : "=r"(r) : "r"(a), "r"(b), "r"(c));
-  return r;
-}
-__device__ __forceinline__ float exp2_approx(float x) {  // within 2^-22; results below 2^-126 are 0
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;\n" : "=f"(r) : "f"(x));
-  return r;
-}
-// x as two fp16 terms, the larger in the low half.
-__device__ __forceinline__ uint32_t two_terms(float x) {
-  const uint32_t h = pack_f16(x, 0.0f);
-  return pack_f16(f16_lo(h), __fsub_rn(x, f16_lo(h)));
-}
-// (x & mask) ^ bits, and (x & mask) | bits, in one instruction each
-__device__ __forceinline__ uint32_t and_xor(uint32_t x, uint32_t mask, uint32_t bits) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0x6a;\n" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
-  return r;
-}
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
-  return r;
-}
-// Four signed bytes of w as fp16 pairs: elements (0, 2) and (1, 3).  A byte with
-// its sign flipped, below the bits of 1024, is 1152 + c.
-__device__ __forceinline__ void bytes_f16(uint32_t w, uint32_t* even, uint32_t* odd) {
-  *even = add_f16x2(and_xor(w, 0x00ff00ffu, 0x64806480u), 0xe480e480u);
-  *odd = add_f16x2(and_xor(w >> 8, 0x00ff00ffu, 0x64806480u), 0xe480e480u);
-}
-// Eight nibbles of w as fp16 pairs: x[i] = elements (i, i + 4).
-__device__ __forceinline__ void nibbles_f16(uint32_t w, uint32_t* x) {
-  const uint32_t v = w >> 8;
-  x[0] = add_f16x2(and_or(w, 0x000f000fu, 0x64006400u), 0xe400e400u);               // 1024 + c - 1024
-  x[1] = fma_f16x2(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd400d400u);  // (1024 + 16 c) / 16 - 64
-  x[2] = add_f16x2(and_or(v, 0x000f000fu, 0x64006400u), 0xe400e400u);
-  x[3] = fma_f16x2(and_or(v, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd400d400u);
-}
-// x as balanced base-256 digits, the least in the lowest byte (|x| <= 2^30).
-__device__ __forceinline__ uint32_t digits(int x) { return ((uint32_t)x + 0x80808080u) ^ 0x80808080u; }
-// Byte `i` of four words.
-__device__ __forceinline__ uint32_t gather_byte(uint32_t a, uint32_t b, uint32_t c, uint32_t d, int i) {
-  const uint32_t sel = (uint32_t)(i | ((i + 4) << 4));
-  return __byte_perm(__byte_perm(a, b, sel), __byte_perm(c, d, sel), 0x5410);
-}
-
-// The line of work as every CTA sees it: thread t of the CTA sums a run of
-// `each` rows, and before[t] is the line up to that run.
-template <int THREADS>
-struct Line {
-  long long before[THREADS + 1];
-  long long warp_sum[THREADS / 32];
-};
-__device__ __forceinline__ int row_pages(const KvqView& c, const KvqRows& R, int r, int max_len, int32_t* status) {
-  int seq;
-  const int len = row_context(c, R, r, max_len, &seq, status);
-  return len > 0 ? (len + kPage - 1) / kPage : 0;
-}
-// A unit weighs its pages and kUnitCost more: what q, the first copies and the
-// result of a unit cost a warp, in pages.
-constexpr int kUnitCost = 2;
-template <int THREADS>
-__device__ void measure_line(Line<THREADS>& line, const KvqView& c, const KvqRows& R, int max_len, int per_row, int each,
-                             int32_t* status) {
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-  const int r0 = min(tid * each, R.rows), r1 = min(r0 + each, R.rows);
-  long long mine = 0;
-  for (int r = r0; r < r1; ++r) {
-    const int pages = row_pages(c, R, r, max_len, status);
-    if (pages) mine += (long long)(pages + kUnitCost) * per_row;
-  }
-  long long upto = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long long v = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += v;
-  }
-  if (lane == 31) line.warp_sum[warp] = upto;
-  __syncthreads();
-  long long first = 0;
-  for (int w = 0; w < warp; ++w) first += line.warp_sum[w];
-  line.before[tid + 1] = first + upto;
-  if (tid == 0) line.before[0] = 0;
-  __syncthreads();
-}
-
-// What a warp leaves for the CTA's join: the unit that begins in its share and
-// does not end there (in its ring), and the part of an earlier one (in its
-// ring, or in the workspace when the warp went on after it).
-struct WarpNote {
-  int row, unit;        // row < 0: none begins here and ends later
-  int has0, ends0, far0;
-};
-
-template <int HD, bool I4, int NT>
-__global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 : 1)
-    kvq_attend_mma_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int min_weight, int wide_q,
-                          const __grid_constant__ CUtensorMap tmap) {
-  using T = MmaTile<HD, I4, NT>;
-  constexpr int kMmaWarps = T::kWarps, kThreads = kMmaWarps * 32;
-  extern __shared__ __align__(1024) uint8_t ring[];
-  __shared__ __align__(8) uint64_t full[kMmaWarps][T::kStages];
-  __shared__ int gave_up;
-  __shared__ Line<kThreads> line;
-  __shared__ float ml[kMmaWarps][2][kMaxHeads][2];  // of a warp's slots 0 and 1
-  __shared__ WarpNote notes[kMmaWarps];
-  pdl_launch_dependents();
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-  const Units us = units_of(a.nh, c.kv_heads);
-  const int shares = gridDim.x, share = blockIdx.x;
-  for (int r = share; r < R.rows; r += shares) {
-    int seq;
-    if (row_context(c, R, r, max_len, &seq, a.status) == 0) write_empty_row(a, HD, r);
-  }
-  if (lane == 0) {
-    for (int i = 0; i < T::kStages; ++i) mbar_init(smem_u32(&full[warp][i]), 1);
-    asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
-  }
-  if (tid == 0) gave_up = 0;
-  const int each = (R.rows + kThreads - 1) / kThreads;
-  measure_line<kThreads>(line, c, R, max_len, us.per_row, each, a.status);
-  const long long total = line.before[kThreads];
-  const long long cuts = min((long long)shares * kMmaWarps, (total + min_weight - 1) / min_weight);
-  const long long mine_at = (long long)share * kMmaWarps + warp;
-  long long at = mine_at < cuts ? total * mine_at / cuts : 0;
-  const long long end = mine_at < cuts ? total * (mine_at + 1) / cuts : 0;
-  int lo = 0, hi = kThreads;  // before[lo] <= at < before[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (line.before[mid] <= at)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  int r = lo * each;
-  long long base = line.before[lo];
-  WarpNote note{-1, 0, 0, 0, 0};
-  uint8_t* const mine = ring + warp * T::kRing;
-  uint8_t* const params = ring + kMmaWarps * T::kRing + warp * (T::kStages * 2 * T::kParams);
-  const uint32_t mine_s = smem_u32(mine), params_s = smem_u32(params), bar_s = smem_u32(&full[warp][0]);
-  const float qscale = __fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)HD));
-  // the rows that this lane names for the loads of K and V
-  int at_k[(T::kChunks + 1) / 2], at_v[(T::kChunks + 1) / 2];
-#pragma unroll
-  for (int c = 0; c < T::kChunks; c += 2) {
-    const int row = lane & 15, piece = min(c + (lane >> 4), T::kChunks - 1);
-    at_k[c / 2] = swizzled(row * T::kRow + piece * 16);
-    at_v[c / 2] = swizzled((kPage + row) * T::kRow + piece * 16);
-  }
-  int fill = 0, take = 0;      // stages, the next to fetch into and the next to use
-  uint32_t parity = 0;         // of the copies that `take` waits for
-
-  while (at < end && r < R.rows) {
-    int seq = 0;
-    const int len = row_context(c, R, r, max_len, &seq, a.status);
-    const int pages = len > 0 ? (len + kPage - 1) / kPage : 0;
-    const int weight = pages ? pages + kUnitCost : 0;
-    if (at >= base + (long long)weight * us.per_row) {
-      base += (long long)weight * us.per_row;
-      ++r;
-      continue;
-    }
-    const int u = (int)((at - base) / weight);
-    const long long first = base + (long long)u * weight + kUnitCost;  // where the unit's pages begin
-    const int p0 = (int)max(at - first, 0LL), p1 = (int)min(end - first, (long long)pages);
-    at = first + pages;
-    if (p1 <= p0) continue;
-    int kvh, h0, heads;
-    unit_heads(us, a.nh, c.kv_heads, u, &kvh, &h0, &heads);
-    const int n_pages = p1 - p0;
-    const int32_t* row_table = c.table + (size_t)seq * c.per_seq + p0;
-
-    // the copies of pages i and i + 1; lane l of the ids holds page (block of 32) + l
-    int ids = 0;
-    auto fetch = [&](int i) {
-      if (i >= n_pages) return;
-      if ((i & 31) == 0) {
-        ids = i + lane < n_pages ? row_table[i + lane] : 0;
-        if ((unsigned)ids >= (unsigned)c.pages) {
-          atomicOr(a.status, kStatusBadContext);
-          ids = 0;
-        }
-      }
-      const int first_block = __shfl_sync(0xffffffffu, ids, i & 31) * c.kv_heads + kvh;
-      const int second_block = __shfl_sync(0xffffffffu, ids, (i + 1) & 31) * c.kv_heads + kvh;
-      if (lane == 0) {
-        const uint32_t bar = bar_s + fill * 8, tile = mine_s + fill * (2 * T::kTile);
-        const uint32_t par = params_s + fill * (2 * T::kParams);
-        const bool both = i + 1 < n_pages;
-        mbar_expect_tx(bar, (T::kCodes + T::kParams) << both);
-        tma_codes(tile, &tmap, first_block, bar);
-        tma_bytes(par, c.pool + (size_t)first_block * (T::kCodes + T::kParams) + T::kCodes, T::kParams, bar);
-        if (both) {
-          tma_codes(tile + T::kTile, &tmap, second_block, bar);
-          tma_bytes(par + T::kParams, c.pool + (size_t)second_block * (T::kCodes + T::kParams) + T::kCodes,
-                    T::kParams, bar);
-        }
-      }
-      fill = fill + 1 == T::kStages ? 0 : fill + 1;
-    };
-    __syncwarp();
-#pragma unroll 1
-    for (int i = 0; i < T::kStages; ++i) fetch(2 * i);
-
-    // q: this lane's columns are head g / 2 of each tile of four, digits 3 - g % 2 and 1 - g % 2
-    uint32_t qf[NT][T::kKSteps][2][2];
-    float qs[NT], qsum[NT];  // of the heads whose sums this lane holds (t of each tile)
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      // of every 32 dimensions a lane's K codes are (I8) 4t .. 4t + 3 and 16 more, (I4) 8t .. 8t + 7
-      float x[HD / 4];
-      const int h = nt * 4 + (g >> 1);
-      const size_t src = (size_t)r * a.ldq + (size_t)(h0 + min(h, heads - 1)) * HD + t * (I4 ? 8 : 4);
-#pragma unroll
-      for (int i = 0; i < HD / 4; i += 4) {
-        const size_t at_q = src + i / 8 * 32 + i % 8 * (I4 ? 1 : 4);
-        if (wide_q) {
-          const float4 v = *(const float4*)((const float*)a.q + at_q);
-          x[i] = v.x;
-          x[i + 1] = v.y;
-          x[i + 2] = v.z;
-          x[i + 3] = v.w;
-        } else {
-#pragma unroll
-          for (int j = 0; j < 4; ++j) x[i + j] = load_elem(a.q, at_q + j, a.bf16);
-        }
-      }
-      float top = 0.0f, sum = 0.0f, zero = 0.0f;
-#pragma unroll
-      for (int i = 0; i < HD / 4; ++i) {
-        top = fmaxf(top, fabsf(x[i]));
-        if constexpr (I4) sum = __fadd_rn(sum, x[i]);
-        zero = __fmaf_rn(x[i], 0.0f, zero);  // NaN when an element is not finite
-      }
-#pragma unroll
-      for (int o = 1; o < 4; o <<= 1) {
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if constexpr (I4) sum = __fadd_rn(sum, __shfl_xor_sync(0xffffffffu, sum, o));
-        zero = __fadd_rn(zero, __shfl_xor_sync(0xffffffffu, zero, o));
-      }
-      // 2^29 / 2^floor(log2 top), the exponents kept within what a float and its inverse can hold
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 30), 254);
-      const float up = __uint_as_float((uint32_t)(283 - e) << 23), down = __uint_as_float((uint32_t)(e - 29) << 23);
-      const int d3 = 3 - (g & 1), d1 = 1 - (g & 1);
-#pragma unroll
-      for (int s = 0; s < T::kKSteps; ++s)
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          // the lane's elements of this half step, in the order in which the codes lie in a word
-          const int d = I4 ? 8 * s + k : 8 * s + 4 * k, skip = I4 ? 2 : 1;
-          uint32_t w[4];
-#pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = digits(__float2int_rn(__fmul_rn(x[d + j * skip], up)));
-          qf[nt][s][0][k] = gather_byte(w[0], w[1], w[2], w[3], d3);
-          qf[nt][s][1][k] = gather_byte(w[0], w[1], w[2], w[3], d1);
-        }
-      // a q that is not finite makes its head NaN
-      const float f = __fadd_rn(__fmul_rn(qscale, down), zero);
-      qs[nt] = __shfl_sync(0xffffffffu, f, 8 * t);
-      qsum[nt] = I4 ? __shfl_sync(0xffffffffu, __fmul_rn(sum, up), 8 * t) : 0.0f;
-    }
-
-    // Scores stay in the units of the integer products times their scales;
-    // qs (> 0) takes them to log2.  m is a maximum of theirs that lies at most
-    // kSlack / qs below the true one, mq = m * qs.
-    float m[NT], mq[NT], limit[NT], l[NT], zsum[NT], o[NT][T::kMTiles][4];
-    float vf = __uint_as_float(247u << 23);  // the weights' power of two
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      m[nt] = mq[nt] = limit[nt] = -INFINITY;
-      l[nt] = zsum[nt] = 0.0f;
-#pragma unroll
-      for (int i = 0; i < T::kMTiles; ++i)
-#pragma unroll
-        for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.0f;
-    }
-
-    for (int i = 0; i < n_pages; i += 2) {
-      if (!mbar_wait(bar_s + take * 8, parity, &gave_up)) {
-        give_up(&gave_up, a.status);
-        at = end;  // nothing more is asked for
-        break;
-      }
-      const uint32_t src = mine_s + take * (2 * T::kTile);
-      const float* par = (const float*)(params + take * (2 * T::kParams)) + g;
-      // live positions from the first page on; with an odd number of pages the
-      // second tile of the last pair holds what was there before
-      const int left = min(len - (p0 + i) * kPage, (n_pages - i) * kPage);
-      constexpr int kParFloats = T::kParams / 4, vpar = I4 ? 32 : 16;
-      float raw[2][NT][2], vs[2][2], vz[2][2];  // [page][..][slot g or g + 8]
-#pragma unroll
-      for (int pg = 0; pg < 2; ++pg) {
-        // scores
-        int sc[NT][2][4];
-        uint32_t kw[2 * T::kChunks];
-        load_rows<T::kChunks, false>(src + pg * T::kTile, at_k, kw);
-#pragma unroll
-        for (int s = 0; s < T::kKSteps; ++s) {
-          uint32_t x[2], y[2];  // rows g and g + 8
-          if constexpr (I4) {
-            x[0] = kw[2 * s] & 0x0f0f0f0fu;
-            x[1] = (kw[2 * s] >> 4) & 0x0f0f0f0fu;
-            y[0] = kw[2 * s + 1] & 0x0f0f0f0fu;
-            y[1] = (kw[2 * s + 1] >> 4) & 0x0f0f0f0fu;
-          } else {
-            x[0] = kw[4 * s];
-            y[0] = kw[4 * s + 1];
-            x[1] = kw[4 * s + 2];
-            y[1] = kw[4 * s + 3];
-          }
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-              if (s == 0)
-                mma_s8<true>(sc[nt][j], x[0], y[0], x[1], y[1], qf[nt][s][j][0], qf[nt][s][j][1]);
-              else
-                mma_s8<false>(sc[nt][j], x[0], y[0], x[1], y[1], qf[nt][s][j][0], qf[nt][s][j][1]);
-            }
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const float* pp = par + pg * kParFloats + 8 * k;
-          const float ks = pp[0], kz = I4 ? pp[16] : 0.0f;
-          vs[pg][k] = pp[vpar];
-          vz[pg][k] = I4 ? pp[vpar + 16] : 0.0f;
-#pragma unroll
-          for (int nt = 0; nt < NT; ++nt) {
-            // digits 3 and 2, 1 and 0: sums of at most 2^29
-            const float x = __fmaf_rn((float)(sc[nt][0][2 * k] * 256 + sc[nt][0][2 * k + 1]), 65536.0f,
-                                      (float)(sc[nt][1][2 * k] * 256 + sc[nt][1][2 * k + 1]));
-            raw[pg][nt][k] = I4 ? __fmaf_rn(qsum[nt], kz, __fmul_rn(x, ks)) : __fmul_rn(x, ks);
-          }
-        }
-      }
-      if (left < 2 * kPage) {  // behind the context the bytes may be anything: no scale of theirs is used
-#pragma unroll
-        for (int pg = 0; pg < 2; ++pg)
-#pragma unroll
-          for (int k = 0; k < 2; ++k)
-            if (pg * kPage + 8 * k + g >= left) {
-              vs[pg][k] = vz[pg][k] = 0.0f;
-#pragma unroll
-              for (int nt = 0; nt < NT; ++nt) raw[pg][nt][k] = -INFINITY;
-            }
-      }
-      float vtop = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
-      bool again = false;
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-        again |= fmaxf(fmaxf(raw[0][nt][0], raw[0][nt][1]), fmaxf(raw[1][nt][0], raw[1][nt][1])) > limit[nt];
-      // a score above the slack, or a scale of V above what the weights' power of two allows
-      again |= __fmul_rn(vtop, vf) > 512.0f;
-      if (__any_sync(0xffffffffu, again)) {
-#pragma unroll
-        for (int b = 4; b < 32; b <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, b));
-        float f = 1.0f;
-        if (__fmul_rn(vtop, vf) > 512.0f) {
-          const int e = min(max((int)(__float_as_uint(vtop) >> 23), 18), 255);
-          const float nf = __uint_as_float((uint32_t)(259 - e) << 23);
-          f = __fdiv_rn(nf, vf);
-          vf = nf;
-        }
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-          float top = fmaxf(fmaxf(raw[0][nt][0], raw[0][nt][1]), fmaxf(raw[1][nt][0], raw[1][nt][1]));
-#pragma unroll
-          for (int b = 4; b < 32; b <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
-          float keep = 1.0f;
-          if (top > m[nt]) {
-            m[nt] = top;
-            const float nq = __fmul_rn(top, qs[nt]);
-            keep = exp2_approx(__fsub_rn(mq[nt], nq));
-            mq[nt] = nq;
-            limit[nt] = __fadd_rn(top, __fdiv_rn(kSlack, qs[nt]));
-          }
-          l[nt] = __fmul_rn(l[nt], keep);
-          zsum[nt] = __fmul_rn(zsum[nt], keep);
-          keep = __fmul_rn(keep, f);
-#pragma unroll
-          for (int k = 0; k < T::kMTiles; ++k)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[nt][k][j] = __fmul_rn(o[nt][k][j], keep);
-        }
-      }
-#pragma unroll
-      for (int pg = 0; pg < 2; ++pg) {
-        uint32_t wb[NT][2];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-          for (int k = 0; k < 2; ++k) {
-            const float w = exp2_approx(__fmaf_rn(raw[pg][nt][k], qs[nt], -mq[nt]));  // 0 behind the context
-            l[nt] = __fadd_rn(l[nt], w);
-            if constexpr (I4) zsum[nt] = __fmaf_rn(w, vz[pg][k], zsum[nt]);
-            wb[nt][k] = transpose8x8(two_terms(__fmul_rn(w, __fmul_rn(vs[pg][k], vf))));
-          }
-        // output
-        // a register of V holds two bytes each of two positions, so that a widened pair is one dimension at two
-        // positions: of dimensions 2g, 2g + 1 of every 16 (I8), or 4g .. 4g + 3 of every 32 (I4)
-        uint32_t vw[2 * T::kChunks];
-        load_rows<T::kChunks, true>(src + pg * T::kTile, at_v, vw);
-#pragma unroll
-        for (int w = 0; w < T::kChunks; ++w) {
-          if constexpr (I4) {
-            uint32_t x[4], y[4];
-            nibbles_f16(vw[2 * w], x);
-            nibbles_f16(vw[2 * w + 1], y);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) {
-              mma_f16(o[nt][2 * w], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
-              mma_f16(o[nt][2 * w + 1], x[2], x[3], y[2], y[3], wb[nt][0], wb[nt][1]);
-            }
-          } else {
-            uint32_t x[2], y[2];
-            bytes_f16(vw[2 * w], &x[0], &x[1]);
-            bytes_f16(vw[2 * w + 1], &y[0], &y[1]);
-#pragma unroll
-            for (int nt = 0; nt < NT; ++nt) mma_f16(o[nt][w], x[0], x[1], y[0], y[1], wb[nt][0], wb[nt][1]);
-          }
-        }
-      }
-      __syncwarp();  // every lane has read the stage
-      fetch(i + 2 * T::kStages);
-      if (++take == T::kStages) {
-        take = 0;
-        parity ^= 1;
-      }
-    }
-    if (gave_up) {
-      // copies still in flight land (or the wait for each runs out) before the CTA may go
-      while (take != fill) {
-        mbar_wait(bar_s + take * 8, parity, nullptr);
-        if (++take == T::kStages) {
-          take = 0;
-          parity ^= 1;
-        }
-      }
-      break;
-    }
-
-    const bool begins = p0 == 0, ends = p1 == pages;
-    const float back = __fdiv_rn(1.0f, vf);
-    const int slot = begins && !ends ? 1 : 0;
-    if (!begins) {
-      note.has0 = 1;
-      note.ends0 = ends;
-      note.far0 = at < end;  // the ring is needed again
-    } else if (!ends) {
-      note.row = r;
-      note.unit = u;
-    }
-    __syncwarp();
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-      const int h = nt * 4 + t;
-#pragma unroll
-      for (int b = 4; b < 32; b <<= 1) {
-        l[nt] = __fadd_rn(l[nt], __shfl_xor_sync(0xffffffffu, l[nt], b));
-        if constexpr (I4) zsum[nt] = __fadd_rn(zsum[nt], __shfl_xor_sync(0xffffffffu, zsum[nt], b));
-      }
-      if (h >= heads) continue;
-      // the lane's dimensions: kRun from g * kRun of every 8 * kRun
-      constexpr int kRun = I4 ? 4 : 2;
-      float x[HD / 8];
-#pragma unroll
-      for (int k = 0; k < T::kMTiles; ++k) {
-        x[2 * k] = __fmaf_rn(__fadd_rn(o[nt][k][0], o[nt][k][1]), back, zsum[nt]);
-        x[2 * k + 1] = __fmaf_rn(__fadd_rn(o[nt][k][2], o[nt][k][3]), back, zsum[nt]);
-      }
-      if (begins && ends) {
-        const float inv = __fdiv_rn(1.0f, l[nt]);
-        const size_t dst = (size_t)r * a.ldo + (size_t)(h0 + h) * HD + g * kRun;
-#pragma unroll
-        for (int k = 0; k < HD / 8; ++k)
-          store_elem(a.out, dst + k / kRun * (8 * kRun) + k % kRun, a.bf16, __fmul_rn(x[k], inv));
-        if (a.lse && g == 0) a.lse[(size_t)r * a.nh + h0 + h] = lse_of(mq[nt], l[nt]);
-      } else {
-        float* part = !begins && at < end ? warp_slot(a.space, shares, (int)mine_at, HD, us) : (float*)mine;
-        part += h * T::kPartStride + g * kRun;
-#pragma unroll
-        for (int k = 0; k < HD / 8; k += kRun) {
-          float* dst = part + k * 8;
-          if constexpr (I4)
-            *(float4*)dst = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
-          else
-            *(float2*)dst = make_float2(x[k], x[k + 1]);
-        }
-        if (g == 0) {
-          ml[warp][slot][h][0] = mq[nt];
-          ml[warp][slot][h][1] = l[nt];
-        }
-      }
-    }
-  }
-  if (lane == 0) notes[warp] = note;
-  __syncthreads();
-
-  // Join what the CTA's warps left.  Chain w is the unit that begins in warp
-  // w's share and ends later, chain -1 what came in from the share before; a
-  // warp joins one head of one chain at a time.
-  if (tid == 0) {
-    ShareMeta out{-1, 0, 0, 0};
-    for (int w = 0; w < kMmaWarps; ++w) {
-      if (notes[w].ends0) {
-        out.row = -1;  // what was open has ended
-        out.ends |= notes[0].has0;
-      }
-      if (notes[w].row >= 0) {
-        out.row = notes[w].row;
-        out.unit = notes[w].unit;
-      }
-    }
-    ((ShareMeta*)a.space)[share] = out;
-  }
-  for (int job = warp; job < (kMmaWarps + 1) * us.heads; job += kMmaWarps) {
-    const int chain = job / us.heads - 1, h = job % us.heads;
-    const bool head = chain < 0;
-    if (head ? !notes[0].has0 : notes[chain].row < 0) continue;
-    const int from = chain + 1;  // the warps whose slot 0 belongs to it: [from, to)
-    int to = from;
-    bool ends = false;
-    while (to < kMmaWarps && !ends) ends = notes[to++].ends0;
-    int kvh, h0 = 0, heads = us.heads;
-    if (!head) unit_heads(us, a.nh, c.kv_heads, notes[chain].unit, &kvh, &h0, &heads);
-    if (h >= heads) continue;
-    // piece 0 is the chain's own (none for the head), piece 1 + i warp from + i's slot 0
-    float M = head ? -INFINITY : ml[chain][1][h][0];
-    for (int w = from; w < to; ++w) M = fmaxf(M, ml[w][0][h][0]);
-    float L = 0.0f, sum[HD / 32], f[kMmaWarps + 1];
-    const float* part[kMmaWarps + 1];
-#pragma unroll
-    for (int i = 0; i <= kMmaWarps; ++i) {
-      const int w = from + i - 1;
-      const bool there = i ? w < to : !head;
-      part[i] = nullptr;
-      f[i] = 0.0f;
-      if (there) {
-        const float* v = ml[w][i ? 0 : 1][h];
-        f[i] = exp2_approx(__fsub_rn(v[0], M));
-        L = __fmaf_rn(v[1], f[i], L);
-        part[i] = (i && notes[w].far0 ? warp_slot(a.space, shares, share * kMmaWarps + w, HD, us)
-                                      : (const float*)(ring + w * T::kRing)) + h * T::kPartStride;
-      }
-    }
-#pragma unroll
-    for (int k = 0; k < HD / 32; ++k) sum[k] = 0.0f;
-#pragma unroll
-    for (int i = 0; i <= kMmaWarps; ++i)
-      if (part[i])
-#pragma unroll
-        for (int k = 0; k < HD / 32; ++k) sum[k] = __fmaf_rn(part[i][lane + 32 * k], f[i], sum[k]);
-    if (!head && ends) {
-      const float inv = __fdiv_rn(1.0f, L);
-      const size_t row = notes[chain].row;
-#pragma unroll
-      for (int k = 0; k < HD / 32; ++k)
-        store_elem(a.out, row * a.ldo + (size_t)(h0 + h) * HD + lane + 32 * k, a.bf16, __fmul_rn(sum[k], inv));
-      if (a.lse && lane == 0) a.lse[row * a.nh + h0 + h] = lse_of(M, L);
-    } else {
-      float* dst = share_slot(a.space, shares, share, head ? 0 : 1, HD, us) + h * (HD + 2);
-#pragma unroll
-      for (int k = 0; k < HD / 32; ++k) dst[lane + 32 * k] = sum[k];
-      if (lane == 0) {
-        dst[HD] = M;
-        dst[HD + 1] = L;
-      }
-    }
-  }
-}
-
-// Joins the partial results of the unit that begins in this CTA's share and ends
-// in a later one, one head a CTA (blockIdx.y): the factors of all pieces
-// first, by all threads at once, then the sums, each group of threads over a
-// share of the pieces.
-constexpr int kJoinThreads = 256;
-__global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(KvqView c, KvqAttend a, int shares) {
-  __shared__ float factor[kAttendCtas];
-  __shared__ float red[kJoinThreads / 32];
-  __shared__ float sums[kJoinThreads];
-  __shared__ int last_sh;
-  pdl_wait();
-  const ShareMeta* meta = (const ShareMeta*)after_wait((uint8_t*)a.space);
-  const int share = blockIdx.x, h = blockIdx.y, hd = c.hd, tid = threadIdx.x;
-  const ShareMeta own = meta[share];
-  if (own.row < 0) return;
-  const Units us = units_of(a.nh, c.kv_heads);
-  int kvh, h0, heads;
-  unit_heads(us, a.nh, c.kv_heads, own.unit, &kvh, &h0, &heads);
-  if (h >= heads) return;
-  if (tid == 0) last_sh = shares - 1;
-  __syncthreads();
-  for (int s = share + 1 + tid; s < shares; s += kJoinThreads)
-    if (meta[s].ends) {
-      atomicMin(&last_sh, s);
-      break;
-    }
-  __syncthreads();
-  const int n = last_sh - share + 1;  // pieces: slot 1 of this share, slot 0 of the later ones
-  auto piece = [&](int i) { return share_slot(a.space, shares, share + i, i == 0, hd, us) + h * (hd + 2); };
-  float M = -INFINITY;
-  for (int i = tid; i < n; i += kJoinThreads) M = fmaxf(M, piece(i)[hd]);
-  M = block_reduce(M, [](float x, float y) { return fmaxf(x, y); }, red);
-  float L = 0.0f;
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const float* p = piece(i);
-    const float f = p[hd + 1] == 0.0f ? 0.0f : exp2_approx(__fsub_rn(p[hd], M));
-    factor[i] = f;
-    L = __fmaf_rn(p[hd + 1], f, L);
-  }
-  __syncthreads();
-  L = block_reduce(L, [](float x, float y) { return __fadd_rn(x, y); }, red);
-  // threads over dimensions, and groups of threads over the pieces
-  static_assert(kJoinThreads >= kKvqMaxHd, "a thread a dimension");
-  const int groups = kJoinThreads / hd, d = tid % hd, grp = tid / hd;
-  float o = 0.0f;
-  if (grp < groups)
-#pragma unroll 8
-    for (int i = grp; i < n; i += groups) o = __fmaf_rn(piece(i)[d], factor[i], o);
-  sums[tid] = o;
-  __syncthreads();
-  if (tid < hd) {
-    for (int k = 1; k < groups; ++k) o = __fadd_rn(o, sums[k * hd + tid]);
-    store_elem(a.out, (size_t)own.row * a.ldo + (size_t)(h0 + h) * hd + d, a.bf16, __fdiv_rn(o, L));
-  }
-  if (a.lse && tid == 0) a.lse[(size_t)own.row * a.nh + h0 + h] = lse_of(M, L);
-}
-
 }  // namespace
 
 namespace {
@@ -1514,83 +432,6 @@ void launch_kvq_load(const KvqView& c, int rows, const int32_t* row_seq, const i
     kernel = c.i4 ? kvq_load_kernel<0, 8, true> : kvq_load_kernel<0, 8, false>;
   kernel<<<blocks, kStoreWarps * 32, 0, st>>>(c, rows, row_seq, row_pos, k, ldk, v, ldv, bf16, wide, per_row, status);
   count_launch();
-}
-
-size_t kvq_attend_space(int nh, int kv_heads, int hd) {
-  const Units us = units_of(nh, kv_heads);
-  const size_t plain = (size_t)kAttendCtas * (sizeof(ShareMeta) + 2 * us.heads * (hd + 2) * sizeof(float));
-  const size_t mma = (size_t)kMmaShares * (sizeof(ShareMeta) + 2 * us.heads * (hd + 2) * sizeof(float) +
-                                           kMmaMaxWarps * us.heads * (hd + 4) * sizeof(float)) + 16;
-  return std::max(plain, mma);
-}
-
-namespace {
-constexpr int kMinWeight = kUnitCost + 2;  // the least share of a warp
-
-// The codes of every block as a tensor of 128-byte lines: [blocks][lines][128].
-template <class T>
-bool codes_map(const KvqView& c, CUtensorMap* map) {
-  const cuuint64_t dims[3] = {128, T::kCodes / 128, (cuuint64_t)c.pages * c.kv_heads};
-  const cuuint64_t strides[2] = {128, T::kCodes + T::kParams};
-  const cuuint32_t box[3] = {128, T::kCodes / 128, 1};
-  const cuuint32_t estr[3] = {1, 1, 1};
-  return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c.pool, dims, strides, box, estr,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
-                              CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
-template <int HD, bool I4, int NT>
-bool launch_mma(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, int wide_q, cudaStream_t st) {
-  using T = MmaTile<HD, I4, NT>;
-  static_assert(T::kRing >= NT * 4 * T::kPartStride * 4, "a warp's ring holds its partial result");
-  CUtensorMap map;
-  if (!codes_map<T>(c, &map)) return false;
-  auto* kernel = kvq_attend_mma_kernel<HD, I4, NT>;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
-  const int shares = NT == 1 ? kMmaShares : kMmaShares / 2;
-  kernel<<<shares, T::kWarps * 32, T::kSmem, st>>>(c, r, a, max_len, kMinWeight, wide_q, map);
-  launch_pdl(kvq_join_kernel, dim3(shares, units_of(a.nh, c.kv_heads).heads), dim3(kJoinThreads), 0, st, c, a, shares);
-  count_launch(2);
-  return true;
-}
-using LaunchMma = bool (*)(const KvqView&, const KvqRows&, const KvqAttend&, int, int, cudaStream_t);
-// The tensor-core kernel for a cache and number of heads a unit, or null.
-template <int HD>
-LaunchMma mma_of(bool i4, bool two) {
-  return i4 ? (two ? launch_mma<HD, true, 2> : launch_mma<HD, true, 1>)
-            : (two ? launch_mma<HD, false, 2> : launch_mma<HD, false, 1>);
-}
-LaunchMma mma_for(const KvqView& c, int heads) {
-  if ((size_t)c.pages * c.kv_heads >= (1ull << 31) || !tensor_map_encoder()) return nullptr;
-  switch (c.hd) {
-    case 32:
-      return mma_of<32>(c.i4, heads > 4);
-    case 64:
-      return mma_of<64>(c.i4, heads > 4);
-    case 96:
-      return mma_of<96>(c.i4, heads > 4);
-    case 128:
-      return mma_of<128>(c.i4, heads > 4);
-  }
-  return nullptr;
-}
-}  // namespace
-
-const char* kvq_attend_kernel_name(const KvqView& c, int nh) {
-  return mma_for(c, units_of(nh, c.kv_heads).heads) ? "kvq_attend_mma_kernel" : "kvq_attend_plain_kernel";
-}
-
-void launch_kvq_attend(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st) {
-  if (r.rows <= 0) return;
-  const Units us = units_of(a.nh, c.kv_heads);
-  if (LaunchMma launch = mma_for(c, us.heads)) {
-    const int wide_q = !a.bf16 && (uintptr_t)a.q % 16 == 0 && a.ldq % 4 == 0;
-    if (launch(c, r, a, max_len, wide_q, st)) return;
-  }
-  const size_t smem = ((size_t)us.heads * c.hd + kPlainWarps * us.heads * (c.hd + 2)) * sizeof(float);
-  kvq_attend_plain_kernel<<<kAttendCtas, kPlainWarps * 32, smem, st>>>(c, r, a, max_len);
-  kvq_join_kernel<<<dim3(kAttendCtas, us.heads), kJoinThreads, 0, st>>>(c, a, kAttendCtas);
-  count_launch(2);
 }
 
 }  // namespace bitnet

@@ -1,0 +1,625 @@
+// kernels_kvq_prompt.cu — causal attention of prompts over the quantised paged
+// cache on the 5th-generation tensor cores.
+//
+// A CTA holds 128 rows, the heads of one unit for 128 / heads consecutive
+// tokens of a sequence (row = token * heads + head), and goes through the keys
+// in tiles of 64 with one pass of the softmax:
+//   S[row][key] = Q . K codes        tcgen05.mma, M 128, N 64
+//   O[row][dim] += W . V codes       tcgen05.mma, M 128, N head_dim
+// The pages of a tile come as they lie (one bulk copy each) and all threads
+// widen their codes to fp16, in which they are exact, into tiles of 128-byte
+// lines (128-byte swizzle).  One image serves both products: keys by
+// dimensions, the contraction along a line for S and across the lines for O.
+// The scale of a K row multiplies its column of S, the scale of a V row the
+// weight of its key; an I4 zero enters S times the sum of q, and the output as
+// a sum of its own.
+//
+// Q lies in tensor memory as fp16, multiplied by a power of two a row so that
+// its largest element is near 2^14: bf16 is exact there.  An f32 row is the sum
+// of two such terms (the second in shared memory), and its weights W too, each
+// product being two on the same sums; with bf16 rows a weight is rounded once
+// to fp16 (2^-11), which its output's bf16 does not show.
+//
+// Two threads share a row, 32 of a tile's keys each.  They read S, write W over
+// it as the A operand of the second product, and rescale O only when a score
+// passes the row's maximum by kSlack (log2) or a scale of V grows too much, as
+// in the single-token kernel; the weights' power of two is folded into the
+// maximum, so that it divides out of the result.  Two CTAs share an SM: one's
+// softmax runs beside the other's products.
+//
+// Every wait is bounded; a CTA that gives up records it, waits (bounded) for
+// its copies and products and frees its tensor memory.
+#include "kvq_device.cuh"
+
+#include <algorithm>
+#include <climits>
+#include <type_traits>
+
+namespace bitnet {
+
+namespace {
+
+constexpr int kPromptRows = 128, kPromptThreads = 256, kKeys = 64, kTilePages = kKeys / kPage;
+constexpr uint32_t kTmemCols = 256, kTmemO = 0, kTmemS = 128, kTmemQ = 192;
+
+template <int HD, bool I4, bool TWO>
+struct PromptTile {
+  static constexpr int kRow = I4 ? HD / 2 : HD;  // bytes of a row's codes
+  static constexpr int kBlock = 2 * kPage * kRow + (I4 ? 256 : 128);
+  static constexpr int kAtoms = (HD + 63) / 64;  // 64 elements of fp16 are a 128-byte line
+  static constexpr int kOperand = kAtoms * kKeys * 128;
+  static constexpr int kQ = TWO ? kAtoms * kPromptRows * 128 : 0;
+  static constexpr int kRaw = kTilePages * kBlock;
+  static constexpr int kSmem = 1024 + 2 * kOperand + kQ + 2 * kRaw;
+};
+
+// Shared-memory operand of 128-byte lines, 128-byte swizzle, groups of 8 lines
+// 1024 bytes apart; `lead` is the distance between two runs of 64 elements
+// where the lines lie across the contraction.
+__device__ __forceinline__ uint64_t operand(uint32_t addr, uint32_t lead) {
+  return (uint64_t)((addr >> 4) & 0x3fffu) | (uint64_t)((lead >> 4) & 0x3fffu) << 16 | (uint64_t)(1024 >> 4) << 32 |
+         (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// fp16 operands, f32 sums, M = 128; B's lines along (0) or across (1) the contraction.
+__device__ __forceinline__ constexpr uint32_t product(int n, int across) {
+  return (1u << 4) | ((uint32_t)across << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(kPromptRows >> 4) << 24);
+}
+__device__ __forceinline__ void mma_tmem_a(uint32_t d, uint32_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
+      "r"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_smem_a(uint32_t d, uint64_t a, uint64_t b, uint32_t desc, bool add) {
+  asm volatile(
+      "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+      " tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
+      "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
+      : "memory");
+}
+__device__ __forceinline__ void mma_commit(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ void before_sync() { asm volatile("tcgen05.fence::before_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void after_sync() { asm volatile("tcgen05.fence::after_thread_sync;\n" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;\n" ::: "memory"); }
+__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;\n" ::: "memory"); }
+// 16 columns of this warp's 32 lanes (without the wait).
+__device__ __forceinline__ void tmem_ld16(uint32_t at, uint32_t* r) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(at)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};\n" ::"r"(at),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t* r) {
+  asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(at), "r"(r[0]),
+               "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// The order in which 8 neighbouring dimensions of I4 codes are widened: pairs (i, i + 4).
+template <bool I4>
+__device__ __forceinline__ constexpr int widened(int i) {
+  return I4 ? i / 2 + (i % 2) * 4 : i;
+}
+
+// 16 bytes of codes to fp16, 16-byte pieces p[0 ..].
+template <bool I4>
+__device__ __forceinline__ void widen(const uint4& raw, uint4* p) {
+  const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+  if constexpr (I4) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t x[4];
+      nibbles_f16(w[i], x);
+      p[i] = make_uint4(x[0], x[1], x[2], x[3]);
+    }
+  } else {
+    uint32_t x[8];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // a byte with its sign flipped, below the bits of 1024, is 1152 + c
+      const uint32_t u = w[i] ^ 0x80808080u;
+      x[2 * i] = add_f16x2(__byte_perm(u, 0x64646464u, 0x4140), 0xe480e480u);
+      x[2 * i + 1] = add_f16x2(__byte_perm(u, 0x64646464u, 0x4342), 0xe480e480u);
+    }
+    p[0] = make_uint4(x[0], x[1], x[2], x[3]);
+    p[1] = make_uint4(x[4], x[5], x[6], x[7]);
+  }
+}
+
+template <int HD, bool I4, bool TWO>
+__global__ void __launch_bounds__(kPromptThreads, 2)
+    kvq_prompt_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int wide_q, int wide_out) {
+  using T = PromptTile<HD, I4, TWO>;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ __align__(8) uint64_t raw_full[2], s_full, o_full, drained;
+  __shared__ uint32_t tmem_slot;
+  __shared__ int gave_up, found_run, found_tile;
+  __shared__ __align__(16) float par[2][4][kKeys];  // of a tile's keys: K scale and zero, V scale and zero
+  __shared__ float pair_a[2][kPromptRows], pair_b[2][kPromptRows], pair_c[2][kPromptRows];
+  const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  const int half = warp >> 2, row = (warp & 3) * 32 + lane;
+  const Units us = units_of(a.nh, c.kv_heads);
+  const int tokens_cta = kPromptRows / us.heads;
+
+  // which tile: all units of the last tokens of the first run, then of those before them, and so on
+  if (warp == 0) {
+    int left = blockIdx.x / us.per_row, run = -1;
+    for (int r0 = 0; r0 < R.runs && run < 0; r0 += 32) {
+      int n = 0;
+      if (r0 + lane < R.runs) {
+        const int lo = max(R.cu[r0 + lane], 0), hi = min(R.cu[r0 + lane + 1], R.rows);
+        n = hi > lo ? (hi - lo + tokens_cta - 1) / tokens_cta : 0;
+      }
+      int upto = n;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const unsigned hit = __ballot_sync(0xffffffffu, left < upto);
+      if (hit) {
+        const int at = __ffs(hit) - 1;
+        run = r0 + at;
+        const int n_at = __shfl_sync(0xffffffffu, n, at), upto_at = __shfl_sync(0xffffffffu, upto, at);
+        left = n_at - 1 - (left - (upto_at - n_at));
+      } else {
+        left -= __shfl_sync(0xffffffffu, upto, 31);
+      }
+    }
+    if (lane == 0) {
+      found_run = run;
+      found_tile = left;
+      gave_up = 0;
+      mbar_init(smem_u32(&raw_full[0]), 1);
+      mbar_init(smem_u32(&raw_full[1]), 1);
+      mbar_init(smem_u32(&s_full), 1);
+      mbar_init(smem_u32(&o_full), 1);
+      mbar_init(smem_u32(&drained), 1);
+      asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
+    }
+  }
+  __syncthreads();
+  const int run = found_run;
+  if (run < 0) return;
+  const int first_row = max(R.cu[run], 0), rows_run = min(R.cu[run + 1], R.rows) - first_row;
+  const int token0 = found_tile * tokens_cta, tokens = min(tokens_cta, rows_run - token0);
+  int kvh, h0, heads;
+  unit_heads(us, a.nh, c.kv_heads, blockIdx.x % us.per_row, &kvh, &h0, &heads);
+  const int seq = R.seq_ids[run];
+  // positions that are seen: by the CTA's last token, and by this thread's row
+  const long long start64 = (long long)R.starts[run] + (first_row - R.cu[run]) + token0;
+  const int start = (int)min(max(start64, -(1LL << 30)), (long long)INT_MAX - 2 * kPromptRows);
+  int seen = start + tokens;
+  const int token = row / us.heads, head = row % us.heads;
+  int limit_pos = start + token + 1;
+  bool bad_place = (unsigned)seq >= (unsigned)c.seqs;
+  if (bad_place) seen = 0;
+  if (seen > max_len) {
+    bad_place = true;
+    seen = max_len;
+  }
+  if (bad_place && tid == 0) atomicOr(a.status, kStatusBadContext);
+  limit_pos = min(limit_pos, seen);
+  const bool live_row = token < tokens && head < heads;
+  const size_t out_row = (size_t)(first_row + token0 + token);
+  const size_t out_at = out_row * a.ldo + (size_t)(h0 + head) * HD + half * (HD / 2);
+  if (seen <= 0) {
+    if (live_row) {
+      for (int i = 0; i < HD / 2; ++i) store_elem(a.out, out_at + i, a.bf16, 0.0f);
+      if (a.lse && half == 0) a.lse[out_row * a.nh + h0 + head] = -INFINITY;
+    }
+    return;
+  }
+  const int tiles = (seen + kKeys - 1) / kKeys;
+
+  uint8_t* const base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  uint8_t *const k_tile = base, *const v_tile = base + T::kOperand, *const q_low = base + 2 * T::kOperand;
+  uint8_t* const raws = base + 2 * T::kOperand + T::kQ;
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_slot)),
+                 "r"(kTmemCols)
+                 : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
+  }
+  // one tile's pages, by warp 0
+  auto fetch = [&](int j) {
+    const int first = j * kTilePages, pages = min(kTilePages, (seen + kPage - 1) / kPage - first);
+    const uint32_t bar = smem_u32(&raw_full[j & 1]);
+    int page = 0;
+    if (lane < pages) {
+      page = c.table[(size_t)seq * c.per_seq + first + lane];
+      if ((unsigned)page >= (unsigned)c.pages) {
+        atomicOr(a.status, kStatusBadContext);
+        page = 0;
+      }
+    }
+    if (lane == 0) mbar_expect_tx(bar, pages * T::kBlock);
+    __syncwarp();
+    if (lane < pages)
+      tma_bytes(smem_u32(raws + (j & 1) * T::kRaw + lane * T::kBlock),
+                c.pool + ((size_t)page * c.kv_heads + kvh) * T::kBlock, T::kBlock, bar);
+  };
+  if (warp == 0) {
+    fetch(0);
+    if (tiles > 1) fetch(1);
+  }
+
+  // q: the row's largest element, its sum, and whether all are finite, from the two threads' halves
+  const size_t q_at = out_row * a.ldq + (size_t)(h0 + head) * HD + half * (HD / 2);
+  auto load_q = [&](int i, float* x) {  // dimensions i .. i + 7 of the half
+    if (!live_row) {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = 0.0f;
+    } else if (wide_q && !a.bf16) {
+      const float4 u = *(const float4*)((const float*)a.q + q_at + i), v = *(const float4*)((const float*)a.q + q_at + i + 4);
+      x[0] = u.x, x[1] = u.y, x[2] = u.z, x[3] = u.w, x[4] = v.x, x[5] = v.y, x[6] = v.z, x[7] = v.w;
+    } else if (wide_q) {
+      const uint4 u = *(const uint4*)((const uint16_t*)a.q + q_at + i);
+      x[0] = bf_lo(u.x), x[1] = bf_hi(u.x), x[2] = bf_lo(u.y), x[3] = bf_hi(u.y);
+      x[4] = bf_lo(u.z), x[5] = bf_hi(u.z), x[6] = bf_lo(u.w), x[7] = bf_hi(u.w);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 8; ++k) x[k] = load_elem(a.q, q_at + i + k, a.bf16);
+    }
+  };
+  float top = 0.0f, qsum = 0.0f, odd = 0.0f;
+#pragma unroll 2
+  for (int i = 0; i < HD / 2; i += 8) {
+    float x[8];
+    load_q(i, x);
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      top = fmaxf(top, fabsf(x[k]));
+      qsum = __fadd_rn(qsum, x[k]);
+      odd = __fmaf_rn(x[k], 0.0f, odd);  // NaN when an element is not finite
+    }
+  }
+  pair_a[half][row] = top;
+  pair_b[half][row] = qsum;
+  pair_c[half][row] = odd;
+  before_sync();
+  __syncthreads();
+  after_sync();
+  const uint32_t tmem = tmem_slot;
+  const uint32_t tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+  top = fmaxf(pair_a[0][row], pair_a[1][row]);
+  qsum = __fadd_rn(pair_b[0][row], pair_b[1][row]);
+  odd = __fadd_rn(pair_c[0][row], pair_c[1][row]);
+  // 2^14 / 2^floor(log2 top), the exponents kept within what a float and its inverse can hold
+  const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
+  const float up = __uint_as_float((uint32_t)(268 - e) << 23), down = __uint_as_float((uint32_t)(e - 14) << 23);
+  const float qs = __fadd_rn(__fmul_rn(__fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)HD)), down), odd);
+  qsum = __fmul_rn(qsum, up);
+#pragma unroll 1
+  for (int i = 0; i < HD / 2; i += 16) {
+    uint32_t hi[8];
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float x[8];
+      load_q(i + 8 * g, x);
+      uint32_t lo[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float u = __fmul_rn(x[widened<I4>(2 * k)], up), v = __fmul_rn(x[widened<I4>(2 * k + 1)], up);
+        hi[4 * g + k] = pack_f16(u, v);
+        if (TWO) lo[k] = pack_f16(__fsub_rn(u, f16_lo(hi[4 * g + k])), __fsub_rn(v, f16_hi(hi[4 * g + k])));
+      }
+      if (TWO) {
+        const int d = half * (HD / 2) + i + 8 * g, piece = (d % 64) / 8;
+        *(uint4*)(q_low + d / 64 * (kPromptRows * 128) + row * 128 + ((piece ^ (row & 7)) << 4)) =
+            make_uint4(lo[0], lo[1], lo[2], lo[3]);
+      }
+    }
+    __syncwarp();
+    tmem_st8(tlane + kTmemQ + half * (HD / 4) + i / 2, hi);
+  }
+  tmem_wait_st();
+
+  // the codes of K (0) or V (1) of the tile in `j`'s buffer, widened into an operand
+  auto widen_tile = [&](int j, int kind, uint8_t* dst) {
+    constexpr int kPieces = T::kRow / 16, kOut = I4 ? 4 : 2;  // 16-byte pieces of a row, and what each becomes
+    const uint8_t* raw = raws + (j & 1) * T::kRaw;
+#pragma unroll
+    for (int i = 0; i < (kKeys * kPieces + kPromptThreads - 1) / kPromptThreads; ++i) {
+      const int at = i * kPromptThreads + tid;
+      if (kKeys * kPieces % kPromptThreads != 0 && at >= kKeys * kPieces) break;
+      const int key = at / kPieces, piece = at % kPieces;
+      uint4 p[4];
+      widen<I4>(*(const uint4*)(raw + key / kPage * T::kBlock + (kind * kPage + key % kPage) * T::kRow + piece * 16), p);
+#pragma unroll
+      for (int k = 0; k < kOut; ++k) {
+        const int to = piece * kOut + k;  // 16-byte piece of the widened row
+        *(uint4*)(dst + to / 8 * (kKeys * 128) + key * 128 + (((to % 8) ^ (key & 7)) << 4)) = p[k];
+      }
+    }
+  };
+  auto stage_params = [&](int j) {
+    if (tid < kKeys) {
+      const float* p = (const float*)(raws + (j & 1) * T::kRaw + tid / kPage * T::kBlock + 2 * kPage * T::kRow) + tid % kPage;
+      // behind the context the bytes may be anything
+      const bool live = j * kKeys + tid < seen;
+      par[j & 1][0][tid] = live ? p[0] : 0.0f;
+      par[j & 1][1][tid] = I4 && live ? p[kPage] : 0.0f;
+      par[j & 1][2][tid] = live ? p[I4 ? 2 * kPage : kPage] : 0.0f;
+      par[j & 1][3][tid] = I4 && live ? p[3 * kPage] : 0.0f;
+    }
+  };
+  auto issue_scores = [&]() {
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k) {
+      const uint64_t b = operand(smem_u32(k_tile) + k / 4 * (kKeys * 128) + k % 4 * 32, 16);
+      mma_tmem_a(tmem + kTmemS, tmem + kTmemQ + 8 * k, b, product(kKeys, 0), k > 0);
+      if (TWO)
+        mma_smem_a(tmem + kTmemS, operand(smem_u32(q_low) + k / 4 * (kPromptRows * 128) + k % 4 * 32, 16), b,
+                   product(kKeys, 0), true);
+    }
+    mma_commit(smem_u32(&s_full));
+  };
+  auto issue_output = [&](bool add) {
+#pragma unroll
+    for (int k = 0; k < kKeys / 16; ++k) {
+      const uint64_t b = operand(smem_u32(v_tile) + k * 2048, kKeys * 128);
+      mma_tmem_a(tmem + kTmemO, tmem + kTmemS + 8 * k, b, product(HD, 1), add || k > 0);
+      if (TWO) mma_tmem_a(tmem + kTmemO, tmem + kTmemS + 32 + 8 * k, b, product(HD, 1), true);
+    }
+    mma_commit(smem_u32(&o_full));
+  };
+  auto publish = [&]() {  // this thread's shared and tensor memory for the products to come
+    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+    tmem_wait_st();
+    before_sync();
+  };
+
+  bool ok = mbar_wait(smem_u32(&raw_full[0]), 0, &gave_up);
+  widen_tile(0, 0, k_tile);
+  stage_params(0);
+  publish();
+  bool stop = __syncthreads_or(!ok);
+  if (!stop && tid == 0) {
+    after_sync();
+    issue_scores();
+  }
+
+  // m: a maximum of the row's scores (in the units of the products times their
+  // scales) at most kSlack / qs below the true one; mq: m * qs less the power
+  // of two of the weights
+  float m = -INFINITY, mq = -INFINITY, limit = -INFINITY, l = 0.0f, zsum = 0.0f;
+  int ev = 100;  // the weights are multiplied by 2^ev
+  for (int j = 0; j < tiles && !stop; ++j) {
+    if (j > 0) {
+      ok &= mbar_wait(smem_u32(&o_full), (j - 1) & 1, &gave_up);
+      after_sync();
+      if (tid == 0) issue_scores();
+    }
+    widen_tile(j, 1, v_tile);
+    ok &= mbar_wait(smem_u32(&s_full), j & 1, &gave_up);
+    __syncwarp();
+    after_sync();
+    float s[kKeys / 2];
+    tmem_ld16(tlane + kTmemS + half * 32, (uint32_t*)s);
+    tmem_ld16(tlane + kTmemS + half * 32 + 16, (uint32_t*)s + 16);
+    tmem_wait_ld();
+    const float(*pj)[kKeys] = par[j & 1];
+    const int key0 = j * kKeys + half * 32;
+#pragma unroll
+    for (int i = 0; i < 32; i += 4) {
+      const float4 ks = *(const float4*)&pj[0][half * 32 + i];
+      const float k4[4] = {ks.x, ks.y, ks.z, ks.w};
+      float z4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+      if constexpr (I4) {
+        const float4 kz = *(const float4*)&pj[1][half * 32 + i];
+        z4[0] = kz.x, z4[1] = kz.y, z4[2] = kz.z, z4[3] = kz.w;
+      }
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        s[i + k] = I4 ? __fmaf_rn(s[i + k], k4[k], __fmul_rn(qsum, z4[k])) : __fmul_rn(s[i + k], k4[k]);
+    }
+    const bool masked = key0 + 32 > min(start + 1, seen);  // keys that the CTA's first token does not see, or no one does
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 32; ++i)
+        if (key0 + i >= limit_pos) s[i] = -INFINITY;
+    }
+    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+    for (int i = 0; i < 32; ++i) tops[i % 4] = fmaxf(tops[i % 4], s[i]);
+    const float top_s = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    // a scale of V times 2^ev above 2^9, or a score above the slack
+    bool again = top_s > limit;
+    if (tid < kKeys) again |= __fmul_rn(pj[2][tid], __int_as_float((127 + ev) << 23)) > 512.0f;
+    before_sync();
+    const bool rescale = __syncthreads_or(again);  // and every score has been read
+    after_sync();
+    if (rescale) {
+      pair_a[half][row] = top_s;
+      float vtop = 0.0f;
+      for (int i = 0; i < kKeys; i += 4) {
+        const float4 v = *(const float4*)&pj[2][i];
+        vtop = fmaxf(vtop, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
+      }
+      if (__fmul_rn(vtop, __int_as_float((127 + ev) << 23)) > 512.0f)
+        ev = max(132 - (int)(__float_as_uint(vtop) >> 23), -100);  // the largest near 2^5
+      __syncthreads();
+      m = fmaxf(m, fmaxf(pair_a[0][row], pair_a[1][row]));
+      const float nq = __fsub_rn(__fmul_rn(m, qs), (float)ev);
+      const float keep = mq == nq || m == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(mq, nq));
+      mq = nq;
+      limit = __fadd_rn(m, __fdiv_rn(kSlack, qs));
+      l = __fmul_rn(l, keep);
+      zsum = __fmul_rn(zsum, keep);
+      if (j > 0) {
+#pragma unroll 1
+        for (int i = 0; i < HD / 2; i += 16) {
+          float o[16];
+          tmem_ld16(tlane + kTmemO + half * (HD / 2) + i, (uint32_t*)o);
+          tmem_wait_ld();
+#pragma unroll
+          for (int k = 0; k < 16; ++k) o[k] = __fmul_rn(o[k], keep);
+          tmem_st16(tlane + kTmemO + half * (HD / 2) + i, (const uint32_t*)o);
+        }
+      }
+    }
+    // weights, over the scores; a key that the row does not see weighs nothing, whatever its scale
+    uint32_t hi[16], lo[16];
+    auto weigh = [&](auto some_hidden) {
+#pragma unroll
+      for (int i = 0; i < 32; i += 4) {
+        const float4 vs = *(const float4*)&pj[2][half * 32 + i];
+        const float v4[4] = {vs.x, vs.y, vs.z, vs.w};
+        float z4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (I4) {
+          const float4 vz = *(const float4*)&pj[3][half * 32 + i];
+          z4[0] = vz.x, z4[1] = vz.y, z4[2] = vz.z, z4[3] = vz.w;
+        }
+        float p[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float w = exp2_approx(__fmaf_rn(s[i + k], qs, -mq));
+          l = __fadd_rn(l, w);
+          const bool hidden = decltype(some_hidden)::value && key0 + i + k >= limit_pos;
+          if constexpr (I4) zsum = hidden ? zsum : __fmaf_rn(w, z4[k], zsum);
+          p[k] = hidden ? 0.0f : __fmul_rn(w, v4[k]);
+        }
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const uint32_t h = pack_f16(p[2 * k], p[2 * k + 1]);
+          hi[i / 2 + k] = h;
+          if (TWO) lo[i / 2 + k] = pack_f16(__fsub_rn(p[2 * k], f16_lo(h)), __fsub_rn(p[2 * k + 1], f16_hi(h)));
+        }
+      }
+    };
+    if (masked)
+      weigh(std::true_type{});
+    else
+      weigh(std::false_type{});
+    tmem_st16(tlane + kTmemS + half * 16, hi);
+    if (TWO) tmem_st16(tlane + kTmemS + 32 + half * 16, lo);
+    if (j + 1 < tiles) {
+      ok &= mbar_wait(smem_u32(&raw_full[(j + 1) & 1]), ((j + 1) >> 1) & 1, &gave_up);
+      widen_tile(j + 1, 0, k_tile);
+      stage_params(j + 1);
+    }
+    publish();
+    stop = __syncthreads_or(!ok);
+    if (stop) break;
+    if (warp == 0) {
+      if (lane == 0) {
+        after_sync();
+        issue_output(j > 0);
+      }
+      __syncwarp();
+      if (j + 2 < tiles) fetch(j + 2);
+    }
+  }
+  if (stop) {
+    // what is in flight lands (or its wait runs out) before the CTA may go
+    if (tid == 0) {
+      give_up(&gave_up, a.status);
+      mma_commit(smem_u32(&drained));
+      mbar_wait(smem_u32(&drained), 0, nullptr);
+      mbar_wait(smem_u32(&raw_full[0]), 0, nullptr);
+      mbar_wait(smem_u32(&raw_full[1]), 0, nullptr);
+      mbar_wait(smem_u32(&raw_full[0]), 1, nullptr);
+      mbar_wait(smem_u32(&raw_full[1]), 1, nullptr);
+    }
+  } else {
+    stop = !mbar_wait(smem_u32(&o_full), (tiles - 1) & 1, &gave_up);
+    if (stop) give_up(&gave_up, a.status);
+    after_sync();
+  }
+  pair_b[half][row] = l;
+  pair_c[half][row] = zsum;
+  __syncthreads();
+  l = __fadd_rn(pair_b[0][row], pair_b[1][row]);
+  zsum = __fadd_rn(pair_c[0][row], pair_c[1][row]);
+  const bool sees = limit_pos > 0;
+  const float inv = sees ? __fdiv_rn(1.0f, l) : 0.0f;
+#pragma unroll 1
+  for (int i = 0; i < HD / 2; i += 16) {
+    float o[16], x[16];
+    __syncwarp();
+    tmem_ld16(tlane + kTmemO + half * (HD / 2) + i, (uint32_t*)o);
+    tmem_wait_ld();
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+      const float v = sees ? __fmul_rn(__fadd_rn(o[k], zsum), inv) : 0.0f;
+      x[k / 8 * 8 + widened<I4>(k % 8)] = v;
+    }
+    if (!live_row || stop) {
+    } else if (wide_out && a.bf16) {
+#pragma unroll
+      for (int k = 0; k < 16; k += 8) {
+        uint32_t u[4];
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+          const __nv_bfloat162 p = __floats2bfloat162_rn(x[k + 2 * n], x[k + 2 * n + 1]);
+          u[n] = *(const uint32_t*)&p;
+        }
+        *(uint4*)((uint16_t*)a.out + out_at + i + k) = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+    } else if (wide_out) {
+#pragma unroll
+      for (int k = 0; k < 16; k += 4)
+        *(float4*)((float*)a.out + out_at + i + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+    } else {
+#pragma unroll
+      for (int k = 0; k < 16; ++k) store_elem(a.out, out_at + i + k, a.bf16, x[k]);
+    }
+  }
+  if (live_row && !stop && a.lse && half == 0)
+    a.lse[out_row * a.nh + h0 + head] = sees ? lse_of(mq, l) : -INFINITY;
+  __syncwarp();
+  before_sync();
+  __syncthreads();
+  if (warp == 1) {
+    after_sync();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
+  }
+}
+
+template <int HD, bool I4, bool TWO>
+void launch_prompt(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st) {
+  using T = PromptTile<HD, I4, TWO>;
+  const Units us = units_of(a.nh, c.kv_heads);
+  const int tokens = kPromptRows / us.heads;
+  const unsigned ctas = (unsigned)(r.rows / tokens + r.runs) * us.per_row;
+  auto* kernel = kvq_prompt_kernel<HD, I4, TWO>;
+  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
+  const size_t run = a.bf16 ? 8 : 4;
+  const int wide_q = (uintptr_t)a.q % 16 == 0 && a.ldq % run == 0;
+  const int wide_out = (uintptr_t)a.out % 16 == 0 && a.ldo % run == 0;
+  kernel<<<ctas, kPromptThreads, T::kSmem, st>>>(c, r, a, max_len, wide_q, wide_out);
+  count_launch();
+}
+template <int HD>
+void launch_prompt_of(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st) {
+  if (c.i4)
+    a.bf16 ? launch_prompt<HD, true, false>(c, r, a, max_len, st) : launch_prompt<HD, true, true>(c, r, a, max_len, st);
+  else
+    a.bf16 ? launch_prompt<HD, false, false>(c, r, a, max_len, st) : launch_prompt<HD, false, true>(c, r, a, max_len, st);
+}
+
+}  // namespace
+
+bool kvq_prompt_supported(const KvqView& c) { return c.hd == 64 || c.hd == 128; }
+
+void launch_kvq_prompt(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st) {
+  if (r.rows <= 0 || r.runs <= 0) return;
+  if (c.hd == 64)
+    launch_prompt_of<64>(c, r, a, max_len, st);
+  else
+    launch_prompt_of<128>(c, r, a, max_len, st);
+}
+
+}  // namespace bitnet

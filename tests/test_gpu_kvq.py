@@ -551,3 +551,43 @@ def test_small_heads_run(cuda_backend):
     with pytest.raises((InvalidConfig, BackendError)):
         cfg = ModelConfig(64, 1024, 1, 2, 1, 64, 32, 10000.0, 1e-5)  # head_dim 512
         BitNetModel(synth.random_model(cfg, seed=4), cuda_backend, max_batch_tokens=4).new_kv_cache(4, kv_dtype=KV_I8)
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [128, 64, 32])
+def test_prompt_attention_later_keys_stay_hidden(cuda_backend, hd, kv):
+    """A key that is not a number, scale of K, of V or both, touches the rows that see it and no others; rows behind a
+    negative start see nothing."""
+    n = 200
+    b = bench(cuda_backend, kv, 2, hd, [n, n], seed=2)
+    for kind, pos in ((0, 150), (1, 70)):
+        b.c.params_view(kind)[int(b.c.table[0, pos // 16]), 0, :, pos % 16] = float("nan")
+    q = torch.randn(2 * n, 8 * hd, device=b.dev, generator=torch.Generator(device=b.dev).manual_seed(6))
+    out, lse = b.prompt(q, 8, [0, 1], [0, n, 2 * n], [0, -40])
+    o = out.view(2 * n, 8, hd)
+    assert torch.isnan(o[70:n, :4]).all() and torch.isfinite(o[:n, 4:]).all() and torch.isfinite(o[:70]).all()
+    assert torch.isnan(lse[150:n, :4]).all() and torch.isfinite(lse[:150]).all() and torch.isfinite(lse[:n, 4:]).all()
+    for i in (0, 31, 69):
+        check_row(b, q[i], 8, 0, i + 1, out[i], lse[i])
+    assert (out[n:n + 40] == 0).all() and (lse[n:n + 40] == -math.inf).all()
+    for i in (40, 41, 110, n - 1):
+        check_row(b, q[n + i], 8, 1, i - 39, out[n + i], lse[n + i])
+
+
+@pytest.mark.parametrize("hd", [128, 32])
+def test_prompt_attention_bad_places_are_reported(cuda_backend, hd):
+    b = bench(cuda_backend, KV_I8, 1, hd, [100, 100], seed=8)
+    q = torch.randn(100, 4 * hd, device=b.dev)
+    out, lse = b.prompt(q, 4, [0, 9], [0, 60, 100], [0, 5])
+    assert b.status.item() == 4
+    check_row(b, q[59], 4, 0, 60, out[59], lse[59])
+    assert (out[60:] == 0).all() and (lse[60:] == -math.inf).all()
+    b.status.zero_()
+    out, lse = b.prompt(q, 4, [0], [0, 100], [0], max_len=50)  # cut there
+    assert b.status.item() == 4
+    check_row(b, q[49], 4, 0, 50, out[49], lse[49])
+    check_row(b, q[80], 4, 0, 50, out[80], lse[80])
+    b.status.zero_()
+    b.c.table[1, 3] = 10**6
+    b.prompt(q[:60], 4, [1], [0, 60], [0])
+    assert b.status.item() == 4
