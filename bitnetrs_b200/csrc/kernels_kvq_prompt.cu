@@ -14,18 +14,23 @@
 // weight of its key; an I4 zero enters S times the sum of q, and the output as
 // a sum of its own.
 //
-// Q lies in tensor memory as fp16, multiplied by a power of two a row so that
-// its largest element is near 2^14: bf16 is exact there.  An f32 row is the sum
-// of two such terms (the second in shared memory), and its weights W too, each
-// product being two on the same sums; with bf16 rows a weight is rounded once
-// to fp16 (2^-11), which its output's bf16 does not show.
+// Q is fp16, multiplied by a power of two a row so that its largest element is
+// near 2^14: bf16 is exact there.  An f32 row is the sum of two such terms, and
+// its weights W too, each product being two on the same sums; with bf16 rows a
+// weight is rounded once to fp16 (2^-11), which its output's bf16 does not show.
 //
 // Two threads share a row, 32 of a tile's keys each.  They read S, write W over
 // it as the A operand of the second product, and rescale O only when a score
 // passes the row's maximum by kSlack (log2) or a scale of V grows too much, as
 // in the single-token kernel; the weights' power of two is folded into the
-// maximum, so that it divides out of the result.  Two CTAs share an SM: one's
-// softmax runs beside the other's products.
+// maximum, so that it divides out of the result.
+//
+// Two CTAs share an SM, so each has half of its tensor memory: O, S, and what
+// is left for Q (its first term).  Heads of 64 leave room for a second S, and
+// the scores of the next tile are computed while this tile's are weighed; with
+// heads of 128 each product runs beside the widening of the other's codes.
+// What a step costs besides is the way of its pages, some 2000 cycles: they are
+// asked for kStages tiles ahead, their numbers one tile before that.
 //
 // Every wait is bounded; a CTA that gives up records it, waits (bounded) for
 // its copies and products and frees its tensor memory.
@@ -40,7 +45,7 @@ namespace bitnet {
 namespace {
 
 constexpr int kPromptRows = 128, kPromptThreads = 256, kKeys = 64, kTilePages = kKeys / kPage;
-constexpr uint32_t kTmemCols = 256, kTmemO = 0, kTmemS = 128, kTmemQ = 192;
+constexpr uint32_t kTmemCols = 256;
 
 template <int HD, bool I4, bool TWO>
 struct PromptTile {
@@ -48,9 +53,13 @@ struct PromptTile {
   static constexpr int kBlock = 2 * kPage * kRow + (I4 ? 256 : 128);
   static constexpr int kAtoms = (HD + 63) / 64;  // 64 elements of fp16 are a 128-byte line
   static constexpr int kOperand = kAtoms * kKeys * 128;
-  static constexpr int kQ = TWO ? kAtoms * kPromptRows * 128 : 0;
+  static constexpr bool kTwoS = HD <= 64;  // two buffers of scores
+  static constexpr uint32_t kTmemS = HD, kTmemQ = HD + (kTwoS ? 2 : 1) * kKeys;  // O begins at 0
+  static_assert(kTmemQ + HD / 2 <= kTmemCols, "half of an SM's tensor memory");
+  static constexpr int kQ = TWO ? kAtoms * kPromptRows * 128 : 0;  // Q's second term
   static constexpr int kRaw = kTilePages * kBlock;
-  static constexpr int kSmem = 1024 + 2 * kOperand + kQ + 2 * kRaw;
+  static constexpr int kStages = TWO && HD > 64 && !I4 ? 2 : 4;  // tiles of pages
+  static constexpr int kSmem = 1024 + 2 * kOperand + kQ + kStages * kRaw;
 };
 
 // Shared-memory operand of 128-byte lines, 128-byte swizzle, groups of 8 lines
@@ -142,7 +151,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     kvq_prompt_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int wide_q, int wide_out) {
   using T = PromptTile<HD, I4, TWO>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t raw_full[2], s_full, o_full, drained;
+  __shared__ __align__(8) uint64_t raw_full[T::kStages], s_full, o_full, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up, found_run, found_tile;
   __shared__ __align__(16) float par[2][4][kKeys];  // of a tile's keys: K scale and zero, V scale and zero
@@ -181,8 +190,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       found_run = run;
       found_tile = left;
       gave_up = 0;
-      mbar_init(smem_u32(&raw_full[0]), 1);
-      mbar_init(smem_u32(&raw_full[1]), 1);
+      for (int i = 0; i < T::kStages; ++i) mbar_init(smem_u32(&raw_full[i]), 1);
       mbar_init(smem_u32(&s_full), 1);
       mbar_init(smem_u32(&o_full), 1);
       mbar_init(smem_u32(&drained), 1);
@@ -224,7 +232,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   const int tiles = (seen + kKeys - 1) / kKeys;
 
   uint8_t* const base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  uint8_t *const k_tile = base, *const v_tile = base + T::kOperand, *const q_low = base + 2 * T::kOperand;
+  uint8_t *const k_tile = base, *const v_tile = base + T::kOperand, *const q_tile = base + 2 * T::kOperand;
   uint8_t* const raws = base + 2 * T::kOperand + T::kQ;
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_slot)),
@@ -232,27 +240,33 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
-  // one tile's pages, by warp 0
-  auto fetch = [&](int j) {
-    const int first = j * kTilePages, pages = min(kTilePages, (seen + kPage - 1) / kPage - first);
-    const uint32_t bar = smem_u32(&raw_full[j & 1]);
-    int page = 0;
-    if (lane < pages) {
-      page = c.table[(size_t)seq * c.per_seq + first + lane];
-      if ((unsigned)page >= (unsigned)c.pages) {
+  // one tile's pages, by warp 0; next_page is the lane's page of the tile after the last one asked for
+  int next_page = 0;
+  auto look_up = [&](int j) {
+    const int at = j * kTilePages + lane;
+    next_page = 0;
+    if (lane < kTilePages && at * kPage < seen) {
+      next_page = c.table[(size_t)seq * c.per_seq + at];
+      if ((unsigned)next_page >= (unsigned)c.pages) {
         atomicOr(a.status, kStatusBadContext);
-        page = 0;
+        next_page = 0;
       }
     }
+  };
+  auto fetch = [&](int j) {
+    const int stage = j % T::kStages, pages = min(kTilePages, (seen + kPage - 1) / kPage - j * kTilePages);
+    const uint32_t bar = smem_u32(&raw_full[stage]);
+    const int page = next_page;
     if (lane == 0) mbar_expect_tx(bar, pages * T::kBlock);
     __syncwarp();
     if (lane < pages)
-      tma_bytes(smem_u32(raws + (j & 1) * T::kRaw + lane * T::kBlock),
+      tma_bytes(smem_u32(raws + stage * T::kRaw + lane * T::kBlock),
                 c.pool + ((size_t)page * c.kv_heads + kvh) * T::kBlock, T::kBlock, bar);
+    look_up(j + 1);
   };
   if (warp == 0) {
-    fetch(0);
-    if (tiles > 1) fetch(1);
+    look_up(0);
+    for (int j = 0; j < min(tiles, T::kStages); ++j) fetch(j);
   }
 
   // q: the row's largest element, its sum, and whether all are finite, from the two threads' halves
@@ -317,19 +331,19 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       }
       if (TWO) {
         const int d = half * (HD / 2) + i + 8 * g, piece = (d % 64) / 8;
-        *(uint4*)(q_low + d / 64 * (kPromptRows * 128) + row * 128 + ((piece ^ (row & 7)) << 4)) =
+        *(uint4*)(q_tile + d / 64 * (kPromptRows * 128) + row * 128 + ((piece ^ (row & 7)) << 4)) =
             make_uint4(lo[0], lo[1], lo[2], lo[3]);
       }
     }
     __syncwarp();
-    tmem_st8(tlane + kTmemQ + half * (HD / 4) + i / 2, hi);
+    tmem_st8(tlane + T::kTmemQ + half * (HD / 4) + i / 2, hi);
   }
   tmem_wait_st();
 
   // the codes of K (0) or V (1) of the tile in `j`'s buffer, widened into an operand
   auto widen_tile = [&](int j, int kind, uint8_t* dst) {
     constexpr int kPieces = T::kRow / 16, kOut = I4 ? 4 : 2;  // 16-byte pieces of a row, and what each becomes
-    const uint8_t* raw = raws + (j & 1) * T::kRaw;
+    const uint8_t* raw = raws + j % T::kStages * T::kRaw;
 #pragma unroll
     for (int i = 0; i < (kKeys * kPieces + kPromptThreads - 1) / kPromptThreads; ++i) {
       const int at = i * kPromptThreads + tid;
@@ -346,7 +360,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   };
   auto stage_params = [&](int j) {
     if (tid < kKeys) {
-      const float* p = (const float*)(raws + (j & 1) * T::kRaw + tid / kPage * T::kBlock + 2 * kPage * T::kRow) + tid % kPage;
+      const float* p = (const float*)(raws + j % T::kStages * T::kRaw + tid / kPage * T::kBlock + 2 * kPage * T::kRow) + tid % kPage;
       // behind the context the bytes may be anything
       const bool live = j * kKeys + tid < seen;
       par[j & 1][0][tid] = live ? p[0] : 0.0f;
@@ -355,23 +369,26 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       par[j & 1][3][tid] = I4 && live ? p[3 * kPage] : 0.0f;
     }
   };
-  auto issue_scores = [&]() {
+  auto scores_at = [&](int j) -> uint32_t { return T::kTmemS + (T::kTwoS && (j & 1) ? kKeys : 0); };
+  auto issue_scores = [&](int j) {
+    const uint32_t d = tmem + scores_at(j);
 #pragma unroll
     for (int k = 0; k < HD / 16; ++k) {
       const uint64_t b = operand(smem_u32(k_tile) + k / 4 * (kKeys * 128) + k % 4 * 32, 16);
-      mma_tmem_a(tmem + kTmemS, tmem + kTmemQ + 8 * k, b, product(kKeys, 0), k > 0);
+      mma_tmem_a(d, tmem + T::kTmemQ + 8 * k, b, product(kKeys, 0), k > 0);
       if (TWO)
-        mma_smem_a(tmem + kTmemS, operand(smem_u32(q_low) + k / 4 * (kPromptRows * 128) + k % 4 * 32, 16), b,
-                   product(kKeys, 0), true);
+        mma_smem_a(d, operand(smem_u32(q_tile) + k / 4 * (kPromptRows * 128) + k % 4 * 32, 16), b, product(kKeys, 0),
+                   true);
     }
     mma_commit(smem_u32(&s_full));
   };
-  auto issue_output = [&](bool add) {
+  auto issue_output = [&](int j) {
+    const uint32_t w = tmem + scores_at(j);
 #pragma unroll
     for (int k = 0; k < kKeys / 16; ++k) {
       const uint64_t b = operand(smem_u32(v_tile) + k * 2048, kKeys * 128);
-      mma_tmem_a(tmem + kTmemO, tmem + kTmemS + 8 * k, b, product(HD, 1), add || k > 0);
-      if (TWO) mma_tmem_a(tmem + kTmemO, tmem + kTmemS + 32 + 8 * k, b, product(HD, 1), true);
+      mma_tmem_a(tmem, w + 8 * k, b, product(HD, 1), j > 0 || k > 0);
+      if (TWO) mma_tmem_a(tmem, w + 32 + 8 * k, b, product(HD, 1), true);
     }
     mma_commit(smem_u32(&o_full));
   };
@@ -388,7 +405,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   bool stop = __syncthreads_or(!ok);
   if (!stop && tid == 0) {
     after_sync();
-    issue_scores();
+    issue_scores(0);
   }
 
   // m: a maximum of the row's scores (in the units of the products times their
@@ -396,19 +413,22 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   // of two of the weights
   float m = -INFINITY, mq = -INFINITY, limit = -INFINITY, l = 0.0f, zsum = 0.0f;
   int ev = 100;  // the weights are multiplied by 2^ev
+  // the next tile's K, and the parameters of its keys
+  auto next_keys = [&](int j) {
+    ok &= mbar_wait(smem_u32(&raw_full[(j + 1) % T::kStages]), (j + 1) / T::kStages & 1, &gave_up);
+    widen_tile(j + 1, 0, k_tile);
+    stage_params(j + 1);
+  };
   for (int j = 0; j < tiles && !stop; ++j) {
-    if (j > 0) {
-      ok &= mbar_wait(smem_u32(&o_full), (j - 1) & 1, &gave_up);
-      after_sync();
-      if (tid == 0) issue_scores();
-    }
-    widen_tile(j, 1, v_tile);
+    const bool more = j + 1 < tiles;
+    if (!T::kTwoS) widen_tile(j, 1, v_tile);  // beside the scores' product
     ok &= mbar_wait(smem_u32(&s_full), j & 1, &gave_up);
     __syncwarp();
     after_sync();
+    const uint32_t s_at = tlane + scores_at(j);
     float s[kKeys / 2];
-    tmem_ld16(tlane + kTmemS + half * 32, (uint32_t*)s);
-    tmem_ld16(tlane + kTmemS + half * 32 + 16, (uint32_t*)s + 16);
+    tmem_ld16(s_at + half * 32, (uint32_t*)s);
+    tmem_ld16(s_at + half * 32 + 16, (uint32_t*)s + 16);
     tmem_wait_ld();
     const float(*pj)[kKeys] = par[j & 1];
     const int key0 = j * kKeys + half * 32;
@@ -438,10 +458,22 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     // a scale of V times 2^ev above 2^9, or a score above the slack
     bool again = top_s > limit;
     if (tid < kKeys) again |= __fmul_rn(pj[2][tid], __int_as_float((127 + ev) << 23)) > 512.0f;
-    before_sync();
+    if (T::kTwoS && more) next_keys(j);
+    publish();
     const bool rescale = __syncthreads_or(again);  // and every score has been read
     after_sync();
+    if (!T::kTwoS && warp == 0 && j + T::kStages < tiles) fetch(j + T::kStages);  // this tile's have been widened
+    if (T::kTwoS && more && tid == 0) {
+      if (j > 0) ok &= mbar_wait(smem_u32(&o_full), (j - 1) & 1, &gave_up);  // the weights that lie there
+      after_sync();
+      issue_scores(j + 1);
+    }
     if (rescale) {
+      if (T::kTwoS && j > 0) {
+        ok &= mbar_wait(smem_u32(&o_full), (j - 1) & 1, &gave_up);
+        __syncwarp();
+        after_sync();
+      }
       pair_a[half][row] = top_s;
       float vtop = 0.0f;
       for (int i = 0; i < kKeys; i += 4) {
@@ -462,11 +494,11 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
 #pragma unroll 1
         for (int i = 0; i < HD / 2; i += 16) {
           float o[16];
-          tmem_ld16(tlane + kTmemO + half * (HD / 2) + i, (uint32_t*)o);
+          tmem_ld16(tlane + half * (HD / 2) + i, (uint32_t*)o);
           tmem_wait_ld();
 #pragma unroll
           for (int k = 0; k < 16; ++k) o[k] = __fmul_rn(o[k], keep);
-          tmem_st16(tlane + kTmemO + half * (HD / 2) + i, (const uint32_t*)o);
+          tmem_st16(tlane + half * (HD / 2) + i, (const uint32_t*)o);
         }
       }
     }
@@ -503,12 +535,15 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       weigh(std::true_type{});
     else
       weigh(std::false_type{});
-    tmem_st16(tlane + kTmemS + half * 16, hi);
-    if (TWO) tmem_st16(tlane + kTmemS + 32 + half * 16, lo);
-    if (j + 1 < tiles) {
-      ok &= mbar_wait(smem_u32(&raw_full[(j + 1) & 1]), ((j + 1) >> 1) & 1, &gave_up);
-      widen_tile(j + 1, 0, k_tile);
-      stage_params(j + 1);
+    __syncwarp();
+    tmem_st16(s_at + half * 16, hi);
+    if (TWO) tmem_st16(s_at + 32 + half * 16, lo);
+    if (T::kTwoS) {
+      if (j > 0) {
+        ok &= mbar_wait(smem_u32(&o_full), (j - 1) & 1, &gave_up);
+        after_sync();
+      }
+      widen_tile(j, 1, v_tile);
     }
     publish();
     stop = __syncthreads_or(!ok);
@@ -516,10 +551,19 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     if (warp == 0) {
       if (lane == 0) {
         after_sync();
-        issue_output(j > 0);
+        issue_output(j);
       }
       __syncwarp();
-      if (j + 2 < tiles) fetch(j + 2);
+      if (T::kTwoS && j + T::kStages < tiles) fetch(j + T::kStages);
+    }
+    if (!T::kTwoS && more) {
+      next_keys(j);  // beside the output's product
+      publish();
+      stop = __syncthreads_or(!ok);
+      if (stop) break;
+      ok &= mbar_wait(smem_u32(&o_full), j & 1, &gave_up);
+      after_sync();
+      if (tid == 0) issue_scores(j + 1);
     }
   }
   if (stop) {
@@ -528,10 +572,10 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       give_up(&gave_up, a.status);
       mma_commit(smem_u32(&drained));
       mbar_wait(smem_u32(&drained), 0, nullptr);
-      mbar_wait(smem_u32(&raw_full[0]), 0, nullptr);
-      mbar_wait(smem_u32(&raw_full[1]), 0, nullptr);
-      mbar_wait(smem_u32(&raw_full[0]), 1, nullptr);
-      mbar_wait(smem_u32(&raw_full[1]), 1, nullptr);
+      for (int i = 0; i < T::kStages; ++i) {  // one of the two is past
+        mbar_wait(smem_u32(&raw_full[i]), 0, nullptr);
+        mbar_wait(smem_u32(&raw_full[i]), 1, nullptr);
+      }
     }
   } else {
     stop = !mbar_wait(smem_u32(&o_full), (tiles - 1) & 1, &gave_up);
@@ -549,7 +593,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   for (int i = 0; i < HD / 2; i += 16) {
     float o[16], x[16];
     __syncwarp();
-    tmem_ld16(tlane + kTmemO + half * (HD / 2) + i, (uint32_t*)o);
+    tmem_ld16(tlane + half * (HD / 2) + i, (uint32_t*)o);
     tmem_wait_ld();
 #pragma unroll
     for (int k = 0; k < 16; ++k) {
