@@ -19,18 +19,25 @@
 // its weights W too, each product being two on the same sums; with bf16 rows a
 // weight is rounded once to fp16 (2^-11), which its output's bf16 does not show.
 //
-// Two threads share a row, 32 of a tile's keys each.  They read S, write W over
-// it as the A operand of the second product, and rescale O only when a score
+// Warps 0-3 weigh: a thread reads its row of S, writes W over it as the A
+// operand of the second product, and rescales its row of O only when a score
 // passes the row's maximum by kSlack (log2) or a scale of V grows too much, as
 // in the single-token kernel; the weights' power of two is folded into the
-// maximum, so that it divides out of the result.
-//
+// maximum, so that it divides out of the result.  Warps 4-6 widen the next
+// tile's K and this tile's V, and fetch pages kStages tiles ahead (their
+// numbers one tile before that).  Warp 7 issues the products.  They meet at
+// mbarriers only:
+//   keys_ready    K widened, and its keys' parameters staged    3 warps
+//   scores_full   S computed (K's tile is free)                 commit
+//   weights_ready W written                                     4 warps
+//   values_ready  V widened                                     3 warps
+//   output_full   O summed (V's tile, W and S are free)         commit
+//   pages_empty   a tile's pages have been widened              3 warps
+// The first three alternate between two barriers a kind: with one, a phase that
+// a warp has yet to look at could be followed by the next.
 // Two CTAs share an SM, so each has half of its tensor memory: O, S, and what
-// is left for Q (its first term).  Heads of 64 leave room for a second S, and
-// the scores of the next tile are computed while this tile's are weighed; with
-// heads of 128 each product runs beside the widening of the other's codes.
-// What a step costs besides is the way of its pages, some 2000 cycles: they are
-// asked for kStages tiles ahead, their numbers one tile before that.
+// is left for Q (its first term).  Heads of 64 leave room for a second S, which
+// is computed while the first is weighed.
 //
 // Every wait is bounded; a CTA that gives up records it, waits (bounded) for
 // its copies and products and frees its tensor memory.
@@ -44,7 +51,7 @@ namespace bitnet {
 
 namespace {
 
-constexpr int kPromptRows = 128, kPromptThreads = 256, kKeys = 64, kTilePages = kKeys / kPage;
+constexpr int kPromptRows = 128, kPromptThreads = 256, kWiden = 96, kKeys = 64, kTilePages = kKeys / kPage;
 constexpr uint32_t kTmemCols = 256;
 
 template <int HD, bool I4, bool TWO>
@@ -151,12 +158,14 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     kvq_prompt_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int wide_q, int wide_out) {
   using T = PromptTile<HD, I4, TWO>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t raw_full[T::kStages], s_full, o_full, drained;
+  __shared__ __align__(8) uint64_t pages_full[T::kStages], pages_empty[T::kStages];
+  __shared__ __align__(8) uint64_t keys_ready[2], scores_full[2], weights_ready[2], values_ready, output_full, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up, found_run, found_tile;
   __shared__ __align__(16) float par[2][4][kKeys];  // of a tile's keys: K scale and zero, V scale and zero
   __shared__ float pair_a[2][kPromptRows], pair_b[2][kPromptRows], pair_c[2][kPromptRows];
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+  // in the prologue two threads share a row of Q, half of it each
   const int half = warp >> 2, row = (warp & 3) * 32 + lane;
   const Units us = units_of(a.nh, c.kv_heads);
   const int tokens_cta = kPromptRows / us.heads;
@@ -190,9 +199,17 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       found_run = run;
       found_tile = left;
       gave_up = 0;
-      for (int i = 0; i < T::kStages; ++i) mbar_init(smem_u32(&raw_full[i]), 1);
-      mbar_init(smem_u32(&s_full), 1);
-      mbar_init(smem_u32(&o_full), 1);
+      for (int i = 0; i < T::kStages; ++i) {
+        mbar_init(smem_u32(&pages_full[i]), 1);
+        mbar_init(smem_u32(&pages_empty[i]), kWiden / 32);
+      }
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(smem_u32(&keys_ready[i]), kWiden / 32);
+        mbar_init(smem_u32(&scores_full[i]), 1);
+        mbar_init(smem_u32(&weights_ready[i]), 4);
+      }
+      mbar_init(smem_u32(&values_ready), kWiden / 32);
+      mbar_init(smem_u32(&output_full), 1);
       mbar_init(smem_u32(&drained), 1);
       asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
     }
@@ -221,11 +238,11 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   limit_pos = min(limit_pos, seen);
   const bool live_row = token < tokens && head < heads;
   const size_t out_row = (size_t)(first_row + token0 + token);
-  const size_t out_at = out_row * a.ldo + (size_t)(h0 + head) * HD + half * (HD / 2);
+  const size_t out_at = out_row * a.ldo + (size_t)(h0 + head) * HD;
   if (seen <= 0) {
-    if (live_row) {
-      for (int i = 0; i < HD / 2; ++i) store_elem(a.out, out_at + i, a.bf16, 0.0f);
-      if (a.lse && half == 0) a.lse[out_row * a.nh + h0 + head] = -INFINITY;
+    if (live_row && warp < 4) {
+      for (int i = 0; i < HD; ++i) store_elem(a.out, out_at + i, a.bf16, 0.0f);
+      if (a.lse) a.lse[out_row * a.nh + h0 + head] = -INFINITY;
     }
     return;
   }
@@ -234,13 +251,13 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   uint8_t* const base = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   uint8_t *const k_tile = base, *const v_tile = base + T::kOperand, *const q_tile = base + 2 * T::kOperand;
   uint8_t* const raws = base + 2 * T::kOperand + T::kQ;
-  if (warp == 1) {
+  if (warp == 7) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n" ::"r"(smem_u32(&tmem_slot)),
                  "r"(kTmemCols)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
-  // one tile's pages, by warp 0; next_page is the lane's page of the tile after the last one asked for
+  // one tile's pages, by warp 4; next_page is the lane's page of the tile after the last one asked for
   int next_page = 0;
   auto look_up = [&](int j) {
     const int at = j * kTilePages + lane;
@@ -255,7 +272,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   };
   auto fetch = [&](int j) {
     const int stage = j % T::kStages, pages = min(kTilePages, (seen + kPage - 1) / kPage - j * kTilePages);
-    const uint32_t bar = smem_u32(&raw_full[stage]);
+    const uint32_t bar = smem_u32(&pages_full[stage]);
     const int page = next_page;
     if (lane == 0) mbar_expect_tx(bar, pages * T::kBlock);
     __syncwarp();
@@ -264,7 +281,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
                 c.pool + ((size_t)page * c.kv_heads + kvh) * T::kBlock, T::kBlock, bar);
     look_up(j + 1);
   };
-  if (warp == 0) {
+  if (warp == 4) {
     look_up(0);
     for (int j = 0; j < min(tiles, T::kStages); ++j) fetch(j);
   }
@@ -345,9 +362,9 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     constexpr int kPieces = T::kRow / 16, kOut = I4 ? 4 : 2;  // 16-byte pieces of a row, and what each becomes
     const uint8_t* raw = raws + j % T::kStages * T::kRaw;
 #pragma unroll
-    for (int i = 0; i < (kKeys * kPieces + kPromptThreads - 1) / kPromptThreads; ++i) {
-      const int at = i * kPromptThreads + tid;
-      if (kKeys * kPieces % kPromptThreads != 0 && at >= kKeys * kPieces) break;
+    for (int i = 0; i < (kKeys * kPieces + kWiden - 1) / kWiden; ++i) {
+      const int at = i * kWiden + (tid - 128);
+      if (kKeys * kPieces % kWiden != 0 && at >= kKeys * kPieces) break;
       const int key = at / kPieces, piece = at % kPieces;
       uint4 p[4];
       widen<I4>(*(const uint4*)(raw + key / kPage * T::kBlock + (kind * kPage + key % kPage) * T::kRow + piece * 16), p);
@@ -359,14 +376,15 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     }
   };
   auto stage_params = [&](int j) {
-    if (tid < kKeys) {
-      const float* p = (const float*)(raws + j % T::kStages * T::kRaw + tid / kPage * T::kBlock + 2 * kPage * T::kRow) + tid % kPage;
+    const int key = tid - 128;
+    if (key < kKeys) {
+      const float* p = (const float*)(raws + j % T::kStages * T::kRaw + key / kPage * T::kBlock + 2 * kPage * T::kRow) + key % kPage;
       // behind the context the bytes may be anything
-      const bool live = j * kKeys + tid < seen;
-      par[j & 1][0][tid] = live ? p[0] : 0.0f;
-      par[j & 1][1][tid] = I4 && live ? p[kPage] : 0.0f;
-      par[j & 1][2][tid] = live ? p[I4 ? 2 * kPage : kPage] : 0.0f;
-      par[j & 1][3][tid] = I4 && live ? p[3 * kPage] : 0.0f;
+      const bool live = j * kKeys + key < seen;
+      par[j & 1][0][key] = live ? p[0] : 0.0f;
+      par[j & 1][1][key] = I4 && live ? p[kPage] : 0.0f;
+      par[j & 1][2][key] = live ? p[I4 ? 2 * kPage : kPage] : 0.0f;
+      par[j & 1][3][key] = I4 && live ? p[3 * kPage] : 0.0f;
     }
   };
   auto scores_at = [&](int j) -> uint32_t { return T::kTmemS + (T::kTwoS && (j & 1) ? kKeys : 0); };
@@ -380,7 +398,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
         mma_smem_a(d, operand(smem_u32(q_tile) + k / 4 * (kPromptRows * 128) + k % 4 * 32, 16), b, product(kKeys, 0),
                    true);
     }
-    mma_commit(smem_u32(&s_full));
+    mma_commit(smem_u32(&scores_full[j & 1]));
   };
   auto issue_output = [&](int j) {
     const uint32_t w = tmem + scores_at(j);
@@ -390,244 +408,230 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       mma_tmem_a(tmem, w + 8 * k, b, product(HD, 1), j > 0 || k > 0);
       if (TWO) mma_tmem_a(tmem, w + 32 + 8 * k, b, product(HD, 1), true);
     }
-    mma_commit(smem_u32(&o_full));
+    mma_commit(smem_u32(&output_full));
   };
-  auto publish = [&]() {  // this thread's shared and tensor memory for the products to come
-    asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-    tmem_wait_st();
-    before_sync();
+  // One arrival a warp, after its writes to shared memory (for the products) or to tensor memory.
+  auto arrive = [&](uint64_t& bar) {
+    __syncwarp();
+    if (lane == 0) mbar_arrive(smem_u32(&bar));
   };
-
-  bool ok = mbar_wait(smem_u32(&raw_full[0]), 0, &gave_up);
-  widen_tile(0, 0, k_tile);
-  stage_params(0);
-  publish();
-  bool stop = __syncthreads_or(!ok);
-  if (!stop && tid == 0) {
-    after_sync();
-    issue_scores(0);
-  }
+  auto wait = [&](uint64_t& bar, int phase) {
+    const bool ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&bar), phase & 1, &gave_up));
+    if (!ok) give_up(&gave_up, a.status);
+    return ok;
+  };
+  // Q is in place
+  asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+  tmem_wait_st();
+  before_sync();
+  __syncthreads();
+  after_sync();
 
   // m: a maximum of the row's scores (in the units of the products times their
   // scales) at most kSlack / qs below the true one; mq: m * qs less the power
   // of two of the weights
   float m = -INFINITY, mq = -INFINITY, limit = -INFINITY, l = 0.0f, zsum = 0.0f;
-  int ev = 100;  // the weights are multiplied by 2^ev
-  // the next tile's K, and the parameters of its keys
-  auto next_keys = [&](int j) {
-    ok &= mbar_wait(smem_u32(&raw_full[(j + 1) % T::kStages]), (j + 1) / T::kStages & 1, &gave_up);
-    widen_tile(j + 1, 0, k_tile);
-    stage_params(j + 1);
-  };
-  for (int j = 0; j < tiles && !stop; ++j) {
-    const bool more = j + 1 < tiles;
-    if (!T::kTwoS) widen_tile(j, 1, v_tile);  // beside the scores' product
-    ok &= mbar_wait(smem_u32(&s_full), j & 1, &gave_up);
-    __syncwarp();
-    after_sync();
-    const uint32_t s_at = tlane + scores_at(j);
-    float s[kKeys / 2];
-    tmem_ld16(s_at + half * 32, (uint32_t*)s);
-    tmem_ld16(s_at + half * 32 + 16, (uint32_t*)s + 16);
-    tmem_wait_ld();
-    const float(*pj)[kKeys] = par[j & 1];
-    const int key0 = j * kKeys + half * 32;
-#pragma unroll
-    for (int i = 0; i < 32; i += 4) {
-      const float4 ks = *(const float4*)&pj[0][half * 32 + i];
-      const float k4[4] = {ks.x, ks.y, ks.z, ks.w};
-      float z4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-      if constexpr (I4) {
-        const float4 kz = *(const float4*)&pj[1][half * 32 + i];
-        z4[0] = kz.x, z4[1] = kz.y, z4[2] = kz.z, z4[3] = kz.w;
-      }
-#pragma unroll
-      for (int k = 0; k < 4; ++k)
-        s[i + k] = I4 ? __fmaf_rn(s[i + k], k4[k], __fmul_rn(qsum, z4[k])) : __fmul_rn(s[i + k], k4[k]);
-    }
-    const bool masked = key0 + 32 > min(start + 1, seen);  // keys that the CTA's first token does not see, or no one does
-    if (masked) {
-#pragma unroll
-      for (int i = 0; i < 32; ++i)
-        if (key0 + i >= limit_pos) s[i] = -INFINITY;
-    }
-    float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-    for (int i = 0; i < 32; ++i) tops[i % 4] = fmaxf(tops[i % 4], s[i]);
-    const float top_s = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    // a scale of V times 2^ev above 2^9, or a score above the slack
-    bool again = top_s > limit;
-    if (tid < kKeys) again |= __fmul_rn(pj[2][tid], __int_as_float((127 + ev) << 23)) > 512.0f;
-    if (T::kTwoS && more) next_keys(j);
-    publish();
-    const bool rescale = __syncthreads_or(again);  // and every score has been read
-    after_sync();
-    if (!T::kTwoS && warp == 0 && j + T::kStages < tiles) fetch(j + T::kStages);  // this tile's have been widened
-    if (T::kTwoS && more && tid == 0) {
-      if (j > 0) ok &= mbar_wait(smem_u32(&o_full), (j - 1) & 1, &gave_up);  // the weights that lie there
+  if (warp == 7) {
+    // ---- products ----
+    // scores of tile j into the buffer that held the weights of tile j - 2 (two buffers) or j - 1
+    auto scores = [&](int j) {
+      constexpr int kBack = T::kTwoS ? 2 : 1;
+      if (!wait(keys_ready[j & 1], j / 2) || (j >= kBack && !wait(output_full, j - kBack))) return false;
       after_sync();
-      issue_scores(j + 1);
-    }
-    if (rescale) {
-      if (T::kTwoS && j > 0) {
-        ok &= mbar_wait(smem_u32(&o_full), (j - 1) & 1, &gave_up);
-        __syncwarp();
-        after_sync();
-      }
-      pair_a[half][row] = top_s;
-      float vtop = 0.0f;
-      for (int i = 0; i < kKeys; i += 4) {
-        const float4 v = *(const float4*)&pj[2][i];
-        vtop = fmaxf(vtop, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)));
-      }
-      if (__fmul_rn(vtop, __int_as_float((127 + ev) << 23)) > 512.0f)
-        ev = max(132 - (int)(__float_as_uint(vtop) >> 23), -100);  // the largest near 2^5
-      __syncthreads();
-      m = fmaxf(m, fmaxf(pair_a[0][row], pair_a[1][row]));
-      const float nq = __fsub_rn(__fmul_rn(m, qs), (float)ev);
-      const float keep = mq == nq || m == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(mq, nq));
-      mq = nq;
-      limit = __fadd_rn(m, __fdiv_rn(kSlack, qs));
-      l = __fmul_rn(l, keep);
-      zsum = __fmul_rn(zsum, keep);
-      if (j > 0) {
-#pragma unroll 1
-        for (int i = 0; i < HD / 2; i += 16) {
-          float o[16];
-          tmem_ld16(tlane + half * (HD / 2) + i, (uint32_t*)o);
-          tmem_wait_ld();
-#pragma unroll
-          for (int k = 0; k < 16; ++k) o[k] = __fmul_rn(o[k], keep);
-          tmem_st16(tlane + half * (HD / 2) + i, (const uint32_t*)o);
-        }
-      }
-    }
-    // weights, over the scores; a key that the row does not see weighs nothing, whatever its scale
-    uint32_t hi[16], lo[16];
-    auto weigh = [&](auto some_hidden) {
-#pragma unroll
-      for (int i = 0; i < 32; i += 4) {
-        const float4 vs = *(const float4*)&pj[2][half * 32 + i];
-        const float v4[4] = {vs.x, vs.y, vs.z, vs.w};
-        float z4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        if constexpr (I4) {
-          const float4 vz = *(const float4*)&pj[3][half * 32 + i];
-          z4[0] = vz.x, z4[1] = vz.y, z4[2] = vz.z, z4[3] = vz.w;
-        }
-        float p[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const float w = exp2_approx(__fmaf_rn(s[i + k], qs, -mq));
-          l = __fadd_rn(l, w);
-          const bool hidden = decltype(some_hidden)::value && key0 + i + k >= limit_pos;
-          if constexpr (I4) zsum = hidden ? zsum : __fmaf_rn(w, z4[k], zsum);
-          p[k] = hidden ? 0.0f : __fmul_rn(w, v4[k]);
-        }
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const uint32_t h = pack_f16(p[2 * k], p[2 * k + 1]);
-          hi[i / 2 + k] = h;
-          if (TWO) lo[i / 2 + k] = pack_f16(__fsub_rn(p[2 * k], f16_lo(h)), __fsub_rn(p[2 * k + 1], f16_hi(h)));
-        }
-      }
-    };
-    if (masked)
-      weigh(std::true_type{});
-    else
-      weigh(std::false_type{});
-    __syncwarp();
-    tmem_st16(s_at + half * 16, hi);
-    if (TWO) tmem_st16(s_at + 32 + half * 16, lo);
-    if (T::kTwoS) {
-      if (j > 0) {
-        ok &= mbar_wait(smem_u32(&o_full), (j - 1) & 1, &gave_up);
-        after_sync();
-      }
-      widen_tile(j, 1, v_tile);
-    }
-    publish();
-    stop = __syncthreads_or(!ok);
-    if (stop) break;
-    if (warp == 0) {
-      if (lane == 0) {
-        after_sync();
-        issue_output(j);
-      }
+      if (lane == 0) issue_scores(j);
       __syncwarp();
-      if (T::kTwoS && j + T::kStages < tiles) fetch(j + T::kStages);
-    }
-    if (!T::kTwoS && more) {
-      next_keys(j);  // beside the output's product
-      publish();
-      stop = __syncthreads_or(!ok);
-      if (stop) break;
-      ok &= mbar_wait(smem_u32(&o_full), j & 1, &gave_up);
+      return true;
+    };
+    bool ok = scores(0);
+    for (int j = 0; j < tiles && ok; ++j) {
+      if (T::kTwoS && j + 1 < tiles && !scores(j + 1)) break;
+      if (!wait(values_ready, j) || !wait(weights_ready[j & 1], j / 2)) break;
       after_sync();
-      if (tid == 0) issue_scores(j + 1);
+      if (lane == 0) issue_output(j);
+      __syncwarp();
+      if (!T::kTwoS && j + 1 < tiles) ok = scores(j + 1);
     }
-  }
-  if (stop) {
-    // what is in flight lands (or its wait runs out) before the CTA may go
-    if (tid == 0) {
-      give_up(&gave_up, a.status);
-      mma_commit(smem_u32(&drained));
-      mbar_wait(smem_u32(&drained), 0, nullptr);
-      for (int i = 0; i < T::kStages; ++i) {  // one of the two is past
-        mbar_wait(smem_u32(&raw_full[i]), 0, nullptr);
-        mbar_wait(smem_u32(&raw_full[i]), 1, nullptr);
+  } else if (warp >= 4) {
+    // ---- widening ----
+    for (int j = 0; j < tiles; ++j) {
+      const int stage = j % T::kStages, use = j / T::kStages;
+      if (!wait(pages_full[stage], use) || (j > 0 && !wait(scores_full[(j - 1) & 1], (j - 1) / 2))) break;
+      stage_params(j);
+      widen_tile(j, 0, k_tile);
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      arrive(keys_ready[j & 1]);
+      if (j > 0 && !wait(output_full, j - 1)) break;
+      widen_tile(j, 1, v_tile);
+      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+      arrive(values_ready);
+      arrive(pages_empty[stage]);
+      if (warp == 4 && j + T::kStages < tiles) {
+        if (!wait(pages_empty[stage], use)) break;
+        fetch(j + T::kStages);
       }
     }
   } else {
-    stop = !mbar_wait(smem_u32(&o_full), (tiles - 1) & 1, &gave_up);
-    if (stop) give_up(&gave_up, a.status);
-    after_sync();
-  }
-  pair_b[half][row] = l;
-  pair_c[half][row] = zsum;
-  __syncthreads();
-  l = __fadd_rn(pair_b[0][row], pair_b[1][row]);
-  zsum = __fadd_rn(pair_c[0][row], pair_c[1][row]);
-  const bool sees = limit_pos > 0;
-  const float inv = sees ? __fdiv_rn(1.0f, l) : 0.0f;
-#pragma unroll 1
-  for (int i = 0; i < HD / 2; i += 16) {
-    float o[16], x[16];
-    __syncwarp();
-    tmem_ld16(tlane + half * (HD / 2) + i, (uint32_t*)o);
-    tmem_wait_ld();
+    // ---- weighing ----
+    int ev = 100;  // the weights are multiplied by 2^ev
+    for (int j = 0; j < tiles; ++j) {
+      if (!wait(keys_ready[j & 1], j / 2) || !wait(scores_full[j & 1], j / 2)) break;
+      after_sync();
+      const uint32_t s_at = tlane + scores_at(j);
+      float s[kKeys];
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
-      const float v = sees ? __fmul_rn(__fadd_rn(o[k], zsum), inv) : 0.0f;
-      x[k / 8 * 8 + widened<I4>(k % 8)] = v;
-    }
-    if (!live_row || stop) {
-    } else if (wide_out && a.bf16) {
+      for (int i = 0; i < kKeys; i += 16) tmem_ld16(s_at + i, (uint32_t*)s + i);
+      tmem_wait_ld();
+      const float(*pj)[kKeys] = par[j & 1];
+      const int key0 = j * kKeys;
 #pragma unroll
-      for (int k = 0; k < 16; k += 8) {
-        uint32_t u[4];
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-          const __nv_bfloat162 p = __floats2bfloat162_rn(x[k + 2 * n], x[k + 2 * n + 1]);
-          u[n] = *(const uint32_t*)&p;
+      for (int i = 0; i < kKeys; i += 4) {
+        const float4 ks = *(const float4*)&pj[0][i];
+        const float k4[4] = {ks.x, ks.y, ks.z, ks.w};
+        float z4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        if constexpr (I4) {
+          const float4 kz = *(const float4*)&pj[1][i];
+          z4[0] = kz.x, z4[1] = kz.y, z4[2] = kz.z, z4[3] = kz.w;
         }
-        *(uint4*)((uint16_t*)a.out + out_at + i + k) = make_uint4(u[0], u[1], u[2], u[3]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+          s[i + k] = I4 ? __fmaf_rn(s[i + k], k4[k], __fmul_rn(qsum, z4[k])) : __fmul_rn(s[i + k], k4[k]);
       }
-    } else if (wide_out) {
+      const bool masked = key0 + kKeys > min(start + 1, seen);  // keys that the CTA's first token does not see, or no one does
+      if (masked) {
 #pragma unroll
-      for (int k = 0; k < 16; k += 4)
-        *(float4*)((float*)a.out + out_at + i + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
-    } else {
+        for (int i = 0; i < kKeys; ++i)
+          if (key0 + i >= limit_pos) s[i] = -INFINITY;
+      }
+      float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int k = 0; k < 16; ++k) store_elem(a.out, out_at + i + k, a.bf16, x[k]);
+      for (int i = 0; i < kKeys; ++i) tops[i % 4] = fmaxf(tops[i % 4], s[i]);
+      const float top_s = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+      // a score above the slack, or a scale of V times 2^ev above 2^9
+      const float vtop = fmaxf(pj[2][lane], pj[2][lane + 32]);
+      if (__any_sync(0xffffffffu, top_s > limit || __fmul_rn(vtop, __int_as_float((127 + ev) << 23)) > 512.0f)) {
+        float v = vtop;
+#pragma unroll
+        for (int b = 1; b < 32; b <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, b));
+        if (__fmul_rn(v, __int_as_float((127 + ev) << 23)) > 512.0f)
+          ev = max(132 - (int)(__float_as_uint(v) >> 23), -100);  // the largest near 2^5
+        m = fmaxf(m, top_s);
+        const float nq = __fsub_rn(__fmul_rn(m, qs), (float)ev);
+        const float keep = mq == nq || m == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(mq, nq));
+        mq = nq;
+        limit = __fadd_rn(m, __fdiv_rn(kSlack, qs));
+        l = __fmul_rn(l, keep);
+        zsum = __fmul_rn(zsum, keep);
+        if (j > 0) {
+          if (!wait(output_full, j - 1)) break;
+          after_sync();
+#pragma unroll 1
+          for (int i = 0; i < HD; i += 16) {
+            float o[16];
+            tmem_ld16(tlane + i, (uint32_t*)o);
+            tmem_wait_ld();
+#pragma unroll
+            for (int k = 0; k < 16; ++k) o[k] = __fmul_rn(o[k], keep);
+            tmem_st16(tlane + i, (const uint32_t*)o);
+          }
+        }
+      }
+      // weights, over the scores; a key that the row does not see weighs nothing, whatever its scale
+      auto weigh = [&](auto some_hidden) {
+#pragma unroll
+        for (int i = 0; i < kKeys; i += 16) {
+          uint32_t hi[8], lo[8];
+#pragma unroll
+          for (int n = 0; n < 16; n += 4) {
+            const float4 vs = *(const float4*)&pj[2][i + n];
+            const float v4[4] = {vs.x, vs.y, vs.z, vs.w};
+            float z4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if constexpr (I4) {
+              const float4 vz = *(const float4*)&pj[3][i + n];
+              z4[0] = vz.x, z4[1] = vz.y, z4[2] = vz.z, z4[3] = vz.w;
+            }
+            float p[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              const float w = exp2_approx(__fmaf_rn(s[i + n + k], qs, -mq));
+              l = __fadd_rn(l, w);
+              const bool hidden = decltype(some_hidden)::value && key0 + i + n + k >= limit_pos;
+              if constexpr (I4) zsum = hidden ? zsum : __fmaf_rn(w, z4[k], zsum);
+              p[k] = hidden ? 0.0f : __fmul_rn(w, v4[k]);
+            }
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              const uint32_t h = pack_f16(p[2 * k], p[2 * k + 1]);
+              hi[n / 2 + k] = h;
+              if (TWO) lo[n / 2 + k] = pack_f16(__fsub_rn(p[2 * k], f16_lo(h)), __fsub_rn(p[2 * k + 1], f16_hi(h)));
+            }
+          }
+          tmem_st8(s_at + i / 2, hi);
+          if (TWO) tmem_st8(s_at + 32 + i / 2, lo);
+        }
+      };
+      if (masked)
+        weigh(std::true_type{});
+      else
+        weigh(std::false_type{});
+      tmem_wait_st();
+      before_sync();
+      arrive(weights_ready[j & 1]);
     }
+    wait(output_full, tiles - 1);
+    after_sync();
+    const bool sees = limit_pos > 0, good = *(volatile int*)&gave_up == 0;
+    const float inv = sees ? __fdiv_rn(1.0f, l) : 0.0f;
+#pragma unroll 1
+    for (int i = 0; i < HD; i += 16) {
+      float o[16], x[16];
+      __syncwarp();
+      tmem_ld16(tlane + i, (uint32_t*)o);
+      tmem_wait_ld();
+#pragma unroll
+      for (int k = 0; k < 16; ++k) {
+        const float v = sees ? __fmul_rn(__fadd_rn(o[k], zsum), inv) : 0.0f;
+        x[k / 8 * 8 + widened<I4>(k % 8)] = v;
+      }
+      if (!live_row || !good) {
+      } else if (wide_out && a.bf16) {
+#pragma unroll
+        for (int k = 0; k < 16; k += 8) {
+          uint32_t u[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(x[k + 2 * n], x[k + 2 * n + 1]);
+            u[n] = *(const uint32_t*)&p;
+          }
+          *(uint4*)((uint16_t*)a.out + out_at + i + k) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+      } else if (wide_out) {
+#pragma unroll
+        for (int k = 0; k < 16; k += 4)
+          *(float4*)((float*)a.out + out_at + i + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) store_elem(a.out, out_at + i + k, a.bf16, x[k]);
+      }
+    }
+    if (live_row && good && a.lse) a.lse[out_row * a.nh + h0 + head] = sees ? lse_of(mq, l) : -INFINITY;
+    __syncwarp();
   }
-  if (live_row && !stop && a.lse && half == 0)
-    a.lse[out_row * a.nh + h0 + head] = sees ? lse_of(mq, l) : -INFINITY;
-  __syncwarp();
   before_sync();
   __syncthreads();
-  if (warp == 1) {
+  if (warp == 7) {
     after_sync();
+    if (gave_up) {
+      // what is in flight lands (or its wait runs out) before the CTA may go
+      if (lane == 0) {
+        mma_commit(smem_u32(&drained));
+        mbar_wait(smem_u32(&drained), 0, nullptr);
+        for (int i = 0; i < T::kStages; ++i) {  // one of the two is past
+          mbar_wait(smem_u32(&pages_full[i]), 0, nullptr);
+          mbar_wait(smem_u32(&pages_full[i]), 1, nullptr);
+        }
+      }
+      __syncwarp();
+    }
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;\n" ::"r"(tmem), "r"(kTmemCols) : "memory");
   }
 }
