@@ -394,11 +394,11 @@ template <int THREADS>
 struct Line {
   long long before[THREADS + 1];
   long long warp_sum[THREADS / 32];
+  int len[THREADS], seq[THREADS];  // of the rows, where there is one a thread
 };
-__device__ __forceinline__ int row_pages(const KvqView& c, const KvqRows& R, int r, int max_len, int32_t* status) {
-  int seq;
-  const int len = row_context(c, R, r, max_len, &seq, status);
-  return len > 0 ? (len + kPage - 1) / kPage : 0;
+// x / d, in 32 bits where that is enough (a 64-bit division takes some 100 instructions).
+__device__ __forceinline__ long long div_fast(long long x, int d) {
+  return (x >> 32) == 0 ? (long long)((uint32_t)x / (uint32_t)d) : x / d;
 }
 // A unit weighs its pages and kUnitCost more: what q, the first copies and the
 // result of a unit cost a warp, in pages.
@@ -410,8 +410,11 @@ __device__ void measure_line(Line<THREADS>& line, const KvqView& c, const KvqRow
   const int r0 = min(tid * each, R.rows), r1 = min(r0 + each, R.rows);
   long long mine = 0;
   for (int r = r0; r < r1; ++r) {
-    const int pages = row_pages(c, R, r, max_len, status);
-    if (pages) mine += (long long)(pages + kUnitCost) * per_row;
+    int seq = 0;
+    const int len = row_context(c, R, r, max_len, &seq, status);
+    line.len[tid] = len;
+    line.seq[tid] = seq;
+    if (len > 0) mine += (long long)((len + kPage - 1) / kPage + kUnitCost) * per_row;
   }
   long long upto = mine;
 #pragma unroll
@@ -452,22 +455,33 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
   const Units us = units_of(a.nh, c.kv_heads);
   const int shares = gridDim.x, share = blockIdx.x;
-  for (int r = share; r < R.rows; r += shares) {
-    int seq;
-    if (row_context(c, R, r, max_len, &seq, a.status) == 0) write_empty_row(a, HD, r);
-  }
   if (lane == 0) {
     for (int i = 0; i < T::kStages; ++i) mbar_init(smem_u32(&full[warp][i]), 1);
     asm volatile("fence.mbarrier_init.release.cluster;\n" ::: "memory");
   }
-  if (tid == 0) gave_up = 0;
+  if (tid == 0) {
+    gave_up = 0;
+    asm volatile("prefetch.tensormap [%0];\n" ::"l"((uint64_t)&tmap) : "memory");
+  }
   const int each = (R.rows + kThreads - 1) / kThreads;
   measure_line<kThreads>(line, c, R, max_len, us.per_row, each, a.status);
+  // a row's sequence and length: with a row a thread they are here already
+  auto context = [&](int r, int* seq) {
+    if (each > 1) return row_context(c, R, r, max_len, seq, a.status);
+    *seq = line.seq[r];
+    return line.len[r];
+  };
+  for (int r = share; r < R.rows; r += shares) {
+    int seq;
+    if (context(r, &seq) == 0) write_empty_row(a, HD, r);
+  }
+  // shares of `quot` or one more
   const long long total = line.before[kThreads];
-  const long long cuts = min((long long)shares * kMmaWarps, (total + min_weight - 1) / min_weight);
+  const long long cuts = min((long long)shares * kMmaWarps, div_fast(total + min_weight - 1, min_weight));
+  const long long quot = cuts ? div_fast(total, (int)cuts) : 0, over = total - quot * cuts;
   const long long mine_at = (long long)share * kMmaWarps + warp;
-  long long at = mine_at < cuts ? total * mine_at / cuts : 0;
-  const long long end = mine_at < cuts ? total * (mine_at + 1) / cuts : 0;
+  long long at = mine_at < cuts ? quot * mine_at + min(mine_at, over) : 0;
+  const long long end = mine_at < cuts ? at + quot + (mine_at < over) : 0;
   int lo = 0, hi = kThreads;  // before[lo] <= at < before[hi]
   while (hi - lo > 1) {
     const int mid = (lo + hi) / 2;
@@ -496,7 +510,7 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
 
   while (at < end && r < R.rows) {
     int seq = 0;
-    const int len = row_context(c, R, r, max_len, &seq, a.status);
+    const int len = context(r, &seq);
     const int pages = len > 0 ? (len + kPage - 1) / kPage : 0;
     const int weight = pages ? pages + kUnitCost : 0;
     if (at >= base + (long long)weight * us.per_row) {
@@ -504,7 +518,7 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
       ++r;
       continue;
     }
-    const int u = (int)((at - base) / weight);
+    const int u = (int)div_fast(at - base, weight);
     const long long first = base + (long long)u * weight + kUnitCost;  // where the unit's pages begin
     const int p0 = (int)max(at - first, 0LL), p1 = (int)min(end - first, (long long)pages);
     at = first + pages;
@@ -914,60 +928,81 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
 }
 
 // Joins the partial results of the unit that begins in this CTA's share and ends
-// in a later one, one head a CTA (blockIdx.y): the factors of all pieces
-// first, by all threads at once, then the sums, each group of threads over a
-// share of the pieces.
-constexpr int kJoinThreads = 256;
-__global__ void __launch_bounds__(kJoinThreads) kvq_join_kernel(KvqView c, KvqAttend a, int shares) {
-  __shared__ float factor[kAttendCtas];
-  __shared__ float red[kJoinThreads / 32];
-  __shared__ float sums[kJoinThreads];
-  __shared__ int last_sh;
+// in a later one.  The CTA's warps are dealt to the unit's heads, several to a
+// head, which take its pieces in turn and meet once in shared memory.  What
+// the join costs is its three trips to L2, one after the other: the notes of
+// the shares, the pieces' maxima, the pieces.
+constexpr int kJoinWarps = 16;
+__global__ void __launch_bounds__(kJoinWarps * 32) kvq_join_kernel(KvqView c, KvqAttend a, int shares) {
+  __shared__ float sums[kJoinWarps][kKvqMaxHd];
+  __shared__ float maxima[kJoinWarps], totals[kJoinWarps];
   pdl_wait();
   const ShareMeta* meta = (const ShareMeta*)after_wait((uint8_t*)a.space);
-  const int share = blockIdx.x, h = blockIdx.y, hd = c.hd, tid = threadIdx.x;
+  const int share = blockIdx.x, hd = c.hd, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const ShareMeta own = meta[share];
+  int at = share + 1;
+  unsigned ends = __ballot_sync(0xffffffffu, at + lane < shares && meta[min(at + lane, shares - 1)].ends);
   if (own.row < 0) return;
+  while (!ends && at + 32 < shares) {
+    at += 32;
+    ends = __ballot_sync(0xffffffffu, at + lane < shares && meta[min(at + lane, shares - 1)].ends);
+  }
+  // pieces: slot 1 of this share, slot 0 of the later ones
+  const int n = (ends ? at + __ffs(ends) - 1 : shares - 1) - share + 1;
   const Units us = units_of(a.nh, c.kv_heads);
   int kvh, h0, heads;
   unit_heads(us, a.nh, c.kv_heads, own.unit, &kvh, &h0, &heads);
-  if (h >= heads) return;
-  if (tid == 0) last_sh = shares - 1;
-  __syncthreads();
-  for (int s = share + 1 + tid; s < shares; s += kJoinThreads)
-    if (meta[s].ends) {
-      atomicMin(&last_sh, s);
-      break;
+  const int team = kJoinWarps / heads, h = warp / team, mine = warp % team;  // warps a head
+  const bool on = h < heads;
+  auto piece = [&](int i) { return share_slot(a.space, shares, share + i, i == 0, hd, us) + min(h, heads - 1) * (hd + 2); };
+  float M = -INFINITY, L = 0.0f, o[kKvqMaxHd / 32];
+#pragma unroll
+  for (int k = 0; k < kKvqMaxHd / 32; ++k) o[k] = 0.0f;
+  // this warp's pieces: mine, mine + team, ... up to 32 of them at a time
+  for (int i0 = mine; i0 < n && on; i0 += 32 * team) {
+    const int i = i0 + lane * team;
+    const float m = i < n ? piece(i)[hd] : -INFINITY, l = i < n ? piece(i)[hd + 1] : 0.0f;
+    float top = m;
+#pragma unroll
+    for (int b = 16; b; b >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, b));
+    const float mn = fmaxf(M, top), keep = M == mn ? 1.0f : exp2_approx(__fsub_rn(M, mn));
+    const float f = l == 0.0f ? 0.0f : exp2_approx(__fsub_rn(m, mn));
+    M = mn;
+    L = __fmaf_rn(L, keep, __fmul_rn(l, f));  // a lane's part
+#pragma unroll
+    for (int k = 0; k < kKvqMaxHd / 32; ++k) o[k] = __fmul_rn(o[k], keep);
+    const int here = min(32, (n - i0 + team - 1) / team);
+#pragma unroll 4
+    for (int j = 0; j < here; ++j) {
+      const float* p = piece(i0 + j * team);
+      const float fj = __shfl_sync(0xffffffffu, f, j);
+#pragma unroll
+      for (int k = 0; k < kKvqMaxHd / 32; ++k)
+        if (lane + 32 * k < hd) o[k] = __fmaf_rn(p[lane + 32 * k], fj, o[k]);
     }
-  __syncthreads();
-  const int n = last_sh - share + 1;  // pieces: slot 1 of this share, slot 0 of the later ones
-  auto piece = [&](int i) { return share_slot(a.space, shares, share + i, i == 0, hd, us) + h * (hd + 2); };
-  float M = -INFINITY;
-  for (int i = tid; i < n; i += kJoinThreads) M = fmaxf(M, piece(i)[hd]);
-  M = block_reduce(M, [](float x, float y) { return fmaxf(x, y); }, red);
-  float L = 0.0f;
-  for (int i = tid; i < n; i += kJoinThreads) {
-    const float* p = piece(i);
-    const float f = p[hd + 1] == 0.0f ? 0.0f : exp2_approx(__fsub_rn(p[hd], M));
-    factor[i] = f;
-    L = __fmaf_rn(p[hd + 1], f, L);
+  }
+#pragma unroll
+  for (int b = 16; b; b >>= 1) L = __fadd_rn(L, __shfl_xor_sync(0xffffffffu, L, b));
+#pragma unroll
+  for (int k = 0; k < kKvqMaxHd / 32; ++k)
+    if (lane + 32 * k < hd) sums[warp][lane + 32 * k] = o[k];
+  if (lane == 0) {
+    maxima[warp] = M;
+    totals[warp] = L;
   }
   __syncthreads();
-  L = block_reduce(L, [](float x, float y) { return __fadd_rn(x, y); }, red);
-  // threads over dimensions, and groups of threads over the pieces
-  static_assert(kJoinThreads >= kKvqMaxHd, "a thread a dimension");
-  const int groups = kJoinThreads / hd, d = tid % hd, grp = tid / hd;
-  float o = 0.0f;
-  if (grp < groups)
-#pragma unroll 8
-    for (int i = grp; i < n; i += groups) o = __fmaf_rn(piece(i)[d], factor[i], o);
-  sums[tid] = o;
-  __syncthreads();
-  if (tid < hd) {
-    for (int k = 1; k < groups; ++k) o = __fadd_rn(o, sums[k * hd + tid]);
-    store_elem(a.out, (size_t)own.row * a.ldo + (size_t)(h0 + h) * hd + d, a.bf16, __fdiv_rn(o, L));
+  for (int d = threadIdx.x; d < heads * hd; d += kJoinWarps * 32) {
+    const int head = d / hd, first = head * team;
+    float top = -INFINITY, sum = 0.0f, total = 0.0f;
+    for (int w = first; w < first + min(team, n); ++w) top = fmaxf(top, maxima[w]);
+    for (int w = first; w < first + min(team, n); ++w) {
+      const float f = totals[w] == 0.0f ? 0.0f : exp2_approx(__fsub_rn(maxima[w], top));
+      sum = __fmaf_rn(sums[w][d - head * hd], f, sum);
+      total = __fmaf_rn(totals[w], f, total);
+    }
+    store_elem(a.out, (size_t)own.row * a.ldo + (size_t)h0 * hd + d, a.bf16, __fdiv_rn(sum, total));
+    if (a.lse && d == head * hd) a.lse[(size_t)own.row * a.nh + h0 + head] = lse_of(top, total);
   }
-  if (a.lse && tid == 0) a.lse[(size_t)own.row * a.nh + h0 + h] = lse_of(M, L);
 }
 
 }  // namespace
@@ -981,7 +1016,7 @@ size_t kvq_attend_space(int nh, int kv_heads, int hd) {
 }
 
 namespace {
-constexpr int kMinWeight = kUnitCost + 2;  // the least share of a warp
+constexpr int kMinWeight = kUnitCost + 1;  // the least share of a warp
 
 // The codes of every block as a tensor of 128-byte lines: [blocks][lines][128].
 template <class T>
@@ -1005,7 +1040,7 @@ bool launch_mma(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
   const int shares = NT == 1 ? kMmaShares : kMmaShares / 2;
   kernel<<<shares, T::kWarps * 32, T::kSmem, st>>>(c, r, a, max_len, kMinWeight, wide_q, map);
-  launch_pdl(kvq_join_kernel, dim3(shares, units_of(a.nh, c.kv_heads).heads), dim3(kJoinThreads), 0, st, c, a, shares);
+  launch_pdl(kvq_join_kernel, dim3(shares), dim3(kJoinWarps * 32), 0, st, c, a, shares);
   count_launch(2);
   return true;
 }
@@ -1049,7 +1084,7 @@ void launch_kvq_attend(const KvqView& c, const KvqRows& r, const KvqAttend& a, i
   }
   const size_t smem = ((size_t)us.heads * c.hd + kPlainWarps * us.heads * (c.hd + 2)) * sizeof(float);
   kvq_attend_plain_kernel<<<kAttendCtas, kPlainWarps * 32, smem, st>>>(c, r, a, max_len);
-  kvq_join_kernel<<<dim3(kAttendCtas, us.heads), kJoinThreads, 0, st>>>(c, a, kAttendCtas);
+  kvq_join_kernel<<<kAttendCtas, kJoinWarps * 32, 0, st>>>(c, a, kAttendCtas);
   count_launch(2);
 }
 
