@@ -276,8 +276,9 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // Each warp has a ring of pages of its own in shared memory.  One lane fetches
 // a page with two copies of the asynchronous copy engine, the codes as a tile
 // of 128-byte lines with their 16-byte pieces exchanged (128-byte swizzle), so
-// that loads of 8 rows x 16 bytes meet no bank twice, and the parameters as
-// they are.
+// that loads of 8 rows x 16 bytes meet no bank twice, and the parameters with
+// them or by themselves.  An SM's engine takes some 65 cycles a copy however
+// small it is, which is what bounded I4 heads of 128 with two copies a page.
 // Measured on a batch of 256 contexts of 128 to 4096 (I8), with the same bytes
 // asked for ahead: copies by each lane (cp.async) stop at 4.0 TB/s, since a
 // load that goes through L1 needs an entry there until it lands.
@@ -300,14 +301,19 @@ struct MmaTile {
   static constexpr int kRow = I4 ? HD / 2 : HD;         // bytes of a row's codes
   static constexpr int kChunks = kRow / 16;             // 16-byte pieces of a row
   static constexpr int kCodes = 2 * kPage * kRow;         // bytes of a page's codes
-  static constexpr int kTile = (kCodes + 1023) / 1024 * 1024;
   static constexpr int kParams = I4 ? 256 : 128;
+  // The parameters come with the codes, as further lines of the tile, where
+  // tiles rounded up to 1024 bytes leave room for them; else by themselves.
+  static constexpr bool kWhole = kCodes + kParams <= 3 * 1024;
+  static constexpr int kTile = (kCodes + (kWhole ? kParams : 0) + 1023) / 1024 * 1024;
+  static constexpr int kApart = kWhole ? 0 : kParams;
+  static constexpr int kLines = (kCodes + (kWhole ? kParams : 0)) / 128;
   // Warps a CTA and stages (of two pages) a warp: what shared memory holds
   // twice an SM (once with NT = 2).
   static constexpr int kWarps = NT == 1 && kTile > 3 * 1024 ? 6 : kMmaMaxWarps;
-  static constexpr int kStages = NT == 2 ? 3 : kTile <= 1024 ? 4 : kRow == 64 && !I4 ? 3 : 2;
+  static constexpr int kStages = NT == 2 ? 3 : kTile <= 1024 ? 4 : kTile <= 2048 ? 3 : 2;
   static constexpr int kRing = kStages * 2 * kTile;  // a warp's tiles
-  static constexpr int kSmem = kWarps * kStages * 2 * (kTile + kParams);
+  static constexpr int kSmem = kWarps * kStages * 2 * (kTile + kApart);
   static constexpr int kKSteps = HD / 32, kMTiles = HD / 16;
   static constexpr int kPartStride = HD + 4;  // floats a head of a warp's partial result
 };
@@ -441,7 +447,7 @@ struct WarpNote {
 
 template <int HD, bool I4, int NT>
 __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 : 1)
-    kvq_attend_mma_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int min_weight, int wide_q,
+    kvq_attend_mma_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int min_weight, int wide_q, int whole_units,
                           const __grid_constant__ CUtensorMap tmap) {
   using T = MmaTile<HD, I4, NT>;
   constexpr int kMmaWarps = T::kWarps, kThreads = kMmaWarps * 32;
@@ -464,37 +470,56 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
     asm volatile("prefetch.tensormap [%0];\n" ::"l"((uint64_t)&tmap) : "memory");
   }
   const int each = (R.rows + kThreads - 1) / kThreads;
-  measure_line<kThreads>(line, c, R, max_len, us.per_row, each, a.status);
+  if (!whole_units) measure_line<kThreads>(line, c, R, max_len, us.per_row, each, a.status);
   // a row's sequence and length: with a row a thread they are here already
   auto context = [&](int r, int* seq) {
-    if (each > 1) return row_context(c, R, r, max_len, seq, a.status);
+    if (each > 1 || whole_units) return row_context(c, R, r, max_len, seq, a.status);
     *seq = line.seq[r];
     return line.len[r];
   };
-  for (int r = share; r < R.rows; r += shares) {
+  long long at, end, base;
+  int r;
+  if (whole_units) {
+    // a CTA to a unit, whose pages its warps share
+    r = share / us.per_row;
+    base = 0;
     int seq;
-    if (context(r, &seq) == 0) write_empty_row(a, HD, r);
+    const int len = row_context(c, R, r, max_len, &seq, a.status);
+    if (len == 0 && share % us.per_row == 0) write_empty_row(a, HD, r);
+    const int pages = len > 0 ? (len + kPage - 1) / kPage : 0;
+    const long long first = (long long)(share % us.per_row) * (pages + kUnitCost) + kUnitCost;
+    const int takers = max(min(pages, kMmaWarps), 1);  // neighbours, a page or more each
+    at = first + (long long)pages * min(warp, takers) / takers;
+    end = first + (long long)pages * min(warp + 1, takers) / takers;
+    __syncthreads();  // the barriers are initialised
+  } else {
+    for (r = share; r < R.rows; r += shares) {
+      int seq;
+      if (context(r, &seq) == 0) write_empty_row(a, HD, r);
+    }
+    // shares of `quot` or one more
+    const long long total = line.before[kThreads];
+    const long long cuts = min((long long)shares * kMmaWarps, div_fast(total + min_weight - 1, min_weight));
+    const long long quot = cuts ? div_fast(total, (int)cuts) : 0, over = total - quot * cuts;
+    const long long nth = (long long)share * kMmaWarps + warp;
+    at = nth < cuts ? quot * nth + min(nth, over) : 0;
+    end = nth < cuts ? at + quot + (nth < over) : 0;
+    int lo = 0, hi = kThreads;  // before[lo] <= at < before[hi]
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) / 2;
+      if (line.before[mid] <= at)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    r = lo * each;
+    base = line.before[lo];
   }
-  // shares of `quot` or one more
-  const long long total = line.before[kThreads];
-  const long long cuts = min((long long)shares * kMmaWarps, div_fast(total + min_weight - 1, min_weight));
-  const long long quot = cuts ? div_fast(total, (int)cuts) : 0, over = total - quot * cuts;
-  const long long mine_at = (long long)share * kMmaWarps + warp;
-  long long at = mine_at < cuts ? quot * mine_at + min(mine_at, over) : 0;
-  const long long end = mine_at < cuts ? at + quot + (mine_at < over) : 0;
-  int lo = 0, hi = kThreads;  // before[lo] <= at < before[hi]
-  while (hi - lo > 1) {
-    const int mid = (lo + hi) / 2;
-    if (line.before[mid] <= at)
-      lo = mid;
-    else
-      hi = mid;
-  }
-  int r = lo * each;
-  long long base = line.before[lo];
   WarpNote note{-1, 0, 0, 0, 0};
   uint8_t* const mine = ring + warp * T::kRing;
-  uint8_t* const params = ring + kMmaWarps * T::kRing + warp * (T::kStages * 2 * T::kParams);
+  // where the parameters are: behind a tile's codes, or in a ring of their own
+  uint8_t* const params = T::kWhole ? mine + T::kCodes : ring + kMmaWarps * T::kRing + warp * (T::kStages * 2 * T::kParams);
+  constexpr int kParStride = T::kWhole ? T::kTile : T::kParams;
   const uint32_t mine_s = smem_u32(mine), params_s = smem_u32(params), bar_s = smem_u32(&full[warp][0]);
   const float qscale = __fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)HD));
   // the rows that this lane names for the loads of K and V
@@ -543,15 +568,17 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
       const int second_block = __shfl_sync(0xffffffffu, ids, (i + 1) & 31) * c.kv_heads + kvh;
       if (lane == 0) {
         const uint32_t bar = bar_s + fill * 8, tile = mine_s + fill * (2 * T::kTile);
-        const uint32_t par = params_s + fill * (2 * T::kParams);
+        const uint32_t par = params_s + fill * (2 * kParStride);
         const bool both = i + 1 < n_pages;
         mbar_expect_tx(bar, (T::kCodes + T::kParams) << both);
         tma_codes(tile, &tmap, first_block, bar);
-        tma_bytes(par, c.pool + (size_t)first_block * (T::kCodes + T::kParams) + T::kCodes, T::kParams, bar);
+        if (!T::kWhole)
+          tma_bytes(par, c.pool + (size_t)first_block * (T::kCodes + T::kParams) + T::kCodes, T::kParams, bar);
         if (both) {
           tma_codes(tile + T::kTile, &tmap, second_block, bar);
-          tma_bytes(par + T::kParams, c.pool + (size_t)second_block * (T::kCodes + T::kParams) + T::kCodes,
-                    T::kParams, bar);
+          if (!T::kWhole)
+            tma_bytes(par + T::kParams, c.pool + (size_t)second_block * (T::kCodes + T::kParams) + T::kCodes,
+                      T::kParams, bar);
         }
       }
       fill = fill + 1 == T::kStages ? 0 : fill + 1;
@@ -640,11 +667,10 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
         break;
       }
       const uint32_t src = mine_s + take * (2 * T::kTile);
-      const float* par = (const float*)(params + take * (2 * T::kParams)) + g;
+      const uint8_t* par = params + take * (2 * kParStride);
       // live positions from the first page on; with an odd number of pages the
       // second tile of the last pair holds what was there before
       const int left = min(len - (p0 + i) * kPage, (n_pages - i) * kPage);
-      constexpr int kParFloats = T::kParams / 4, vpar = I4 ? 32 : 16;
       float raw[2][NT][2], vs[2][2], vz[2][2];  // [page][..][slot g or g + 8]
 #pragma unroll
       for (int pg = 0; pg < 2; ++pg) {
@@ -678,10 +704,15 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
         }
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
-          const float* pp = par + pg * kParFloats + 8 * k;
-          const float ks = pp[0], kz = I4 ? pp[16] : 0.0f;
-          vs[pg][k] = pp[vpar];
-          vz[pg][k] = I4 ? pp[vpar + 16] : 0.0f;
+          // parameter `kind` (K scale, [K zero,] V scale, [V zero]) of slot g + 8 k
+          auto param = [&](int kind) {
+            const int x = 64 * kind + 32 * k, line = (T::kCodes + x) / 128;
+            const int turned = T::kWhole ? (line & 7) << 4 : 0;
+            return *(const float*)(par + pg * kParStride + (x & ~127) + (((x & 127) ^ (turned & 96)) | ((4 * g) ^ (turned & 16))));
+          };
+          const float ks = param(0), kz = I4 ? param(1) : 0.0f;
+          vs[pg][k] = param(I4 ? 2 : 1);
+          vz[pg][k] = I4 ? param(3) : 0.0f;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             // digits 3 and 2, 1 and 0: sums of at most 2^29
@@ -834,7 +865,7 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
           store_elem(a.out, dst + k / kRun * (8 * kRun) + k % kRun, a.bf16, __fmul_rn(x[k], inv));
         if (a.lse && g == 0) a.lse[(size_t)r * a.nh + h0 + h] = lse_of(mq[nt], l[nt]);
       } else {
-        float* part = !begins && at < end ? warp_slot(a.space, shares, (int)mine_at, HD, us) : (float*)mine;
+        float* part = !begins && at < end ? warp_slot(a.space, shares, share * kMmaWarps + warp, HD, us) : (float*)mine;
         part += h * T::kPartStride + g * kRun;
 #pragma unroll
         for (int k = 0; k < HD / 8; k += kRun) {
@@ -1016,14 +1047,18 @@ size_t kvq_attend_space(int nh, int kv_heads, int hd) {
 }
 
 namespace {
+// Units of at most this many positions, and no more of them than CTAs, are taken
+// by a CTA each: its warps' pages take less time than a second kernel, which
+// joins what several CTAs leave (some 4 us against 0.35 us a page and warp).
+constexpr int kWholeUnits = 1024;
 constexpr int kMinWeight = kUnitCost + 1;  // the least share of a warp
 
 // The codes of every block as a tensor of 128-byte lines: [blocks][lines][128].
 template <class T>
 bool codes_map(const KvqView& c, CUtensorMap* map) {
-  const cuuint64_t dims[3] = {128, T::kCodes / 128, (cuuint64_t)c.pages * c.kv_heads};
+  const cuuint64_t dims[3] = {128, T::kLines, (cuuint64_t)c.pages * c.kv_heads};
   const cuuint64_t strides[2] = {128, T::kCodes + T::kParams};
-  const cuuint32_t box[3] = {128, T::kCodes / 128, 1};
+  const cuuint32_t box[3] = {128, T::kLines, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   return tensor_map_encoder()(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c.pool, dims, strides, box, estr,
                               CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
@@ -1038,10 +1073,15 @@ bool launch_mma(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_
   if (!codes_map<T>(c, &map)) return false;
   auto* kernel = kvq_attend_mma_kernel<HD, I4, NT>;
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
-  const int shares = NT == 1 ? kMmaShares : kMmaShares / 2;
-  kernel<<<shares, T::kWarps * 32, T::kSmem, st>>>(c, r, a, max_len, kMinWeight, wide_q, map);
+  int shares = NT == 1 ? kMmaShares : kMmaShares / 2;
+  const size_t units = (size_t)r.rows * units_of(a.nh, c.kv_heads).per_row;
+  const bool whole = max_len <= kWholeUnits && units <= (size_t)shares;
+  if (whole) shares = (int)units;
+  kernel<<<shares, T::kWarps * 32, T::kSmem, st>>>(c, r, a, max_len, kMinWeight, wide_q, whole, map);
+  count_launch();
+  if (whole) return true;
   launch_pdl(kvq_join_kernel, dim3(shares), dim3(kJoinWarps * 32), 0, st, c, a, shares);
-  count_launch(2);
+  count_launch();
   return true;
 }
 using LaunchMma = bool (*)(const KvqView&, const KvqRows&, const KvqAttend&, int, int, cudaStream_t);
