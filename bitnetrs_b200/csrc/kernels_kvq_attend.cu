@@ -60,14 +60,14 @@ __device__ __forceinline__ int row_context(const KvqView& c, const KvqRows& R, i
 }
 
 __device__ __forceinline__ float* share_slot(void* space, int shares, int share, int slot, int hd, const Units& us) {
-  return (float*)((ShareMeta*)space + shares) + ((size_t)share * 2 + slot) * (us.heads * (hd + 2));
+  return (float*)((ShareMeta*)space + shares) + ((size_t)share * 2 + slot) * (us.heads * (hd + 4));
 }
 
 // A partial result that a warp of the tensor-core kernel leaves for its CTA's
 // join, behind the shares' slots; rows padded like the ring's.
 __device__ __forceinline__ float* warp_slot(void* space, int shares, int warp, int hd, const Units& us) {
-  const size_t slots = (size_t)shares * 2 * (us.heads * (hd + 2));
-  return (float*)((ShareMeta*)space + shares) + (slots + 3) / 4 * 4 + (size_t)warp * (us.heads * (hd + 4));
+  const size_t slots = (size_t)shares * 2 * (us.heads * (hd + 4));
+  return (float*)((ShareMeta*)space + shares) + slots + (size_t)warp * (us.heads * (hd + 4));
 }
 
 __device__ void write_empty_row(const KvqAttend& a, int hd, int r) {
@@ -233,10 +233,10 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
         store_elem(a.out, (size_t)r * a.ldo + (size_t)h0 * hd + i, a.bf16, __fdiv_rn(o, L));
         if (a.lse && d == 0) a.lse[(size_t)r * a.nh + h0 + h] = lse_of(M, L);
       } else {
-        slot[h * (hd + 2) + d] = o;
+        slot[h * (hd + 4) + d] = o;
         if (d == 0) {
-          slot[h * (hd + 2) + hd] = M;
-          slot[h * (hd + 2) + hd + 1] = L;
+          slot[h * (hd + 4) + hd] = M;
+          slot[h * (hd + 4) + hd + 1] = L;
         }
       }
     }
@@ -277,8 +277,7 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // a page with two copies of the asynchronous copy engine, the codes as a tile
 // of 128-byte lines with their 16-byte pieces exchanged (128-byte swizzle), so
 // that loads of 8 rows x 16 bytes meet no bank twice, and the parameters with
-// them or by themselves.  An SM's engine takes some 65 cycles a copy however
-// small it is, which is what bounded I4 heads of 128 with two copies a page.
+// them or by themselves.
 // Measured on a batch of 256 contexts of 128 to 4096 (I8), with the same bytes
 // asked for ahead: copies by each lane (cp.async) stop at 4.0 TB/s, since a
 // load that goes through L1 needs an entry there until it lands.
@@ -304,14 +303,15 @@ struct MmaTile {
   static constexpr int kParams = I4 ? 256 : 128;
   // The parameters come with the codes, as further lines of the tile, where
   // tiles rounded up to 1024 bytes leave room for them; else by themselves.
-  static constexpr bool kWhole = kCodes + kParams <= 3 * 1024;
+  static constexpr bool kWhole = kCodes + kParams <= 2 * 1024;
   static constexpr int kTile = (kCodes + (kWhole ? kParams : 0) + 1023) / 1024 * 1024;
   static constexpr int kApart = kWhole ? 0 : kParams;
   static constexpr int kLines = (kCodes + (kWhole ? kParams : 0)) / 128;
   // Warps a CTA and stages (of two pages) a warp: what shared memory holds
   // twice an SM (once with NT = 2).
   static constexpr int kWarps = NT == 1 && kTile > 3 * 1024 ? 6 : kMmaMaxWarps;
-  static constexpr int kStages = NT == 2 ? 3 : kTile <= 1024 ? 4 : kTile <= 2048 ? 3 : 2;
+  static constexpr int kPair = kWarps * 2 * (kTile + kApart);
+  static constexpr int kStages = NT == 2 ? 3 : 4 * kPair <= 104 * 1024 ? 4 : 104 * 1024 / kPair;
   static constexpr int kRing = kStages * 2 * kTile;  // a warp's tiles
   static constexpr int kSmem = kWarps * kStages * 2 * (kTile + kApart);
   static constexpr int kKSteps = HD / 32, kMTiles = HD / 16;
@@ -885,71 +885,71 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
   if (lane == 0) notes[warp] = note;
   __syncthreads();
 
-  // Join what the CTA's warps left.  Chain w is the unit that begins in warp
-  // w's share and ends later, chain -1 what came in from the share before; a
-  // warp joins one head of one chain at a time.
+  // Join what the CTA's warps left.  Chain w + 1 is the unit that begins in
+  // warp w's share and ends later, chain 0 what came in from the share before;
+  // its pieces are that warp's slot 1 and the slots 0 of the warps behind it.
+  // A warp joins one head of one chain at a time, a lane first to a piece, then
+  // to dimensions.  (The code runs once a CTA, so what it costs is its length:
+  // instructions that no warp has met yet come from L2.)
+  const WarpNote left = notes[min(lane, kMmaWarps - 1)];
+  const unsigned begun = __ballot_sync(0xffffffffu, lane < kMmaWarps && left.row >= 0);
+  const unsigned ended = __ballot_sync(0xffffffffu, lane < kMmaWarps && left.ends0);
+  const unsigned far = __ballot_sync(0xffffffffu, lane < kMmaWarps && left.far0);
+  const bool came_in = notes[0].has0;
   if (tid == 0) {
-    ShareMeta out{-1, 0, 0, 0};
-    for (int w = 0; w < kMmaWarps; ++w) {
-      if (notes[w].ends0) {
-        out.row = -1;  // what was open has ended
-        out.ends |= notes[0].has0;
-      }
-      if (notes[w].row >= 0) {
-        out.row = notes[w].row;
-        out.unit = notes[w].unit;
-      }
-    }
-    ((ShareMeta*)a.space)[share] = out;
+    const int last = 31 - __clz(begun);  // -1: none
+    const bool open = begun && !(ended >> last >> 1);
+    ((ShareMeta*)a.space)[share] =
+        ShareMeta{open ? notes[last].row : -1, open ? notes[last].unit : 0, came_in && ended, 0};
   }
   for (int job = warp; job < (kMmaWarps + 1) * us.heads; job += kMmaWarps) {
-    const int chain = job / us.heads - 1, h = job % us.heads;
-    const bool head = chain < 0;
-    if (head ? !notes[0].has0 : notes[chain].row < 0) continue;
-    const int from = chain + 1;  // the warps whose slot 0 belongs to it: [from, to)
-    int to = from;
-    bool ends = false;
-    while (to < kMmaWarps && !ends) ends = notes[to++].ends0;
+    const int chain = job / us.heads, h = job - chain * us.heads;
+    if (chain ? !(begun >> (chain - 1) & 1) : !came_in) continue;
+    const unsigned ends_at = ended >> chain;
+    const int to = ends_at ? chain + __ffs(ends_at) : kMmaWarps;  // slots 0 of the warps [chain, to)
+    const int own = chain ? 1 : 0, pieces = own + to - chain;
     int kvh, h0 = 0, heads = us.heads;
-    if (!head) unit_heads(us, a.nh, c.kv_heads, notes[chain].unit, &kvh, &h0, &heads);
+    if (chain) unit_heads(us, a.nh, c.kv_heads, notes[chain - 1].unit, &kvh, &h0, &heads);
     if (h >= heads) continue;
-    // piece 0 is the chain's own (none for the head), piece 1 + i warp from + i's slot 0
-    float M = head ? -INFINITY : ml[chain][1][h][0];
-    for (int w = from; w < to; ++w) M = fmaxf(M, ml[w][0][h][0]);
-    float L = 0.0f, sum[HD / 32], f[kMmaWarps + 1];
-    const float* part[kMmaWarps + 1];
+    // lane i: piece i, which warp `of` left
+    const int of = min(chain - own + lane, kMmaWarps - 1);
+    const bool first = own && lane == 0, there = lane < pieces;
+    const float mp = there ? ml[of][first][h][0] : -INFINITY, lp = there ? ml[of][first][h][1] : 0.0f;
+    float M = mp;
 #pragma unroll
-    for (int i = 0; i <= kMmaWarps; ++i) {
-      const int w = from + i - 1;
-      const bool there = i ? w < to : !head;
-      part[i] = nullptr;
-      f[i] = 0.0f;
-      if (there) {
-        const float* v = ml[w][i ? 0 : 1][h];
-        f[i] = exp2_approx(__fsub_rn(v[0], M));
-        L = __fmaf_rn(v[1], f[i], L);
-        part[i] = (i && notes[w].far0 ? warp_slot(a.space, shares, share * kMmaWarps + w, HD, us)
-                                      : (const float*)(ring + w * T::kRing)) + h * T::kPartStride;
-      }
+    for (int b = 8; b; b >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, b));
+    const float f = there ? exp2_approx(__fsub_rn(mp, M)) : 0.0f;
+    float L = there ? __fmul_rn(lp, f) : 0.0f;
+#pragma unroll
+    for (int b = 8; b; b >>= 1) L = __fadd_rn(L, __shfl_xor_sync(0xffffffffu, L, b));
+    M = __shfl_sync(0xffffffffu, M, 0);
+    L = __shfl_sync(0xffffffffu, L, 0);
+    constexpr int kRun = HD / 32;  // a lane's dimensions
+    float sum[kRun];
+#pragma unroll
+    for (int k = 0; k < kRun; ++k) sum[k] = 0.0f;
+#pragma unroll 3
+    for (int i = 0; i < pieces; ++i) {
+      const int w = chain - own + i;
+      const bool in_ring = (own && i == 0) || !(far >> w & 1);
+      const float* part = in_ring ? (const float*)(ring + w * T::kRing)
+                                  : warp_slot(a.space, shares, share * kMmaWarps + w, HD, us);
+      part += h * T::kPartStride + lane * kRun;
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+#pragma unroll
+      for (int k = 0; k < kRun; ++k) sum[k] = __fmaf_rn(part[k], fi, sum[k]);
     }
-#pragma unroll
-    for (int k = 0; k < HD / 32; ++k) sum[k] = 0.0f;
-#pragma unroll
-    for (int i = 0; i <= kMmaWarps; ++i)
-      if (part[i])
-#pragma unroll
-        for (int k = 0; k < HD / 32; ++k) sum[k] = __fmaf_rn(part[i][lane + 32 * k], f[i], sum[k]);
-    if (!head && ends) {
+    if (own && ends_at) {
       const float inv = __fdiv_rn(1.0f, L);
-      const size_t row = notes[chain].row;
+      const size_t row = notes[chain - 1].row;
 #pragma unroll
-      for (int k = 0; k < HD / 32; ++k)
-        store_elem(a.out, row * a.ldo + (size_t)(h0 + h) * HD + lane + 32 * k, a.bf16, __fmul_rn(sum[k], inv));
+      for (int k = 0; k < kRun; ++k)
+        store_elem(a.out, row * a.ldo + (size_t)(h0 + h) * HD + lane * kRun + k, a.bf16, __fmul_rn(sum[k], inv));
       if (a.lse && lane == 0) a.lse[row * a.nh + h0 + h] = lse_of(M, L);
     } else {
-      float* dst = share_slot(a.space, shares, share, head ? 0 : 1, HD, us) + h * (HD + 2);
+      float* dst = share_slot(a.space, shares, share, own, HD, us) + h * (HD + 4);
 #pragma unroll
-      for (int k = 0; k < HD / 32; ++k) dst[lane + 32 * k] = sum[k];
+      for (int k = 0; k < kRun; ++k) dst[lane * kRun + k] = sum[k];
       if (lane == 0) {
         dst[HD] = M;
         dst[HD + 1] = L;
@@ -985,10 +985,12 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kvq_join_kernel(KvqView c, Kv
   unit_heads(us, a.nh, c.kv_heads, own.unit, &kvh, &h0, &heads);
   const int team = kJoinWarps / heads, h = warp / team, mine = warp % team;  // warps a head
   const bool on = h < heads;
-  auto piece = [&](int i) { return share_slot(a.space, shares, share + i, i == 0, hd, us) + min(h, heads - 1) * (hd + 2); };
-  float M = -INFINITY, L = 0.0f, o[kKvqMaxHd / 32];
+  auto piece = [&](int i) { return share_slot(a.space, shares, share + i, i == 0, hd, us) + min(h, heads - 1) * (hd + 4); };
+  // a lane's dimensions: four from 4 * lane, and four 128 further on
+  float M = -INFINITY, L = 0.0f, o[8];
 #pragma unroll
-  for (int k = 0; k < kKvqMaxHd / 32; ++k) o[k] = 0.0f;
+  for (int k = 0; k < 8; ++k) o[k] = 0.0f;
+  const bool fours = hd % 4 == 0;
   // this warp's pieces: mine, mine + team, ... up to 32 of them at a time
   for (int i0 = mine; i0 < n && on; i0 += 32 * team) {
     const int i = i0 + lane * team;
@@ -1001,22 +1003,42 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kvq_join_kernel(KvqView c, Kv
     M = mn;
     L = __fmaf_rn(L, keep, __fmul_rn(l, f));  // a lane's part
 #pragma unroll
-    for (int k = 0; k < kKvqMaxHd / 32; ++k) o[k] = __fmul_rn(o[k], keep);
+    for (int k = 0; k < 8; ++k) o[k] = __fmul_rn(o[k], keep);
     const int here = min(32, (n - i0 + team - 1) / team);
-#pragma unroll 4
+#pragma unroll 8
     for (int j = 0; j < here; ++j) {
       const float* p = piece(i0 + j * team);
       const float fj = __shfl_sync(0xffffffffu, f, j);
-#pragma unroll
-      for (int k = 0; k < kKvqMaxHd / 32; ++k)
-        if (lane + 32 * k < hd) o[k] = __fmaf_rn(p[lane + 32 * k], fj, o[k]);
+      if (fours) {
+        if (4 * lane < hd) {
+          const float4 v = *(const float4*)(p + 4 * lane);
+          o[0] = __fmaf_rn(v.x, fj, o[0]);
+          o[1] = __fmaf_rn(v.y, fj, o[1]);
+          o[2] = __fmaf_rn(v.z, fj, o[2]);
+          o[3] = __fmaf_rn(v.w, fj, o[3]);
+        }
+        if (4 * lane + 128 < hd) {
+          const float4 v = *(const float4*)(p + 4 * lane + 128);
+          o[4] = __fmaf_rn(v.x, fj, o[4]);
+          o[5] = __fmaf_rn(v.y, fj, o[5]);
+          o[6] = __fmaf_rn(v.z, fj, o[6]);
+          o[7] = __fmaf_rn(v.w, fj, o[7]);
+        }
+      } else {
+        for (int k = 0; k < 8; ++k) {
+          const int d = 4 * lane + k % 4 + k / 4 * 128;
+          if (d < hd) o[k] = __fmaf_rn(p[d], fj, o[k]);
+        }
+      }
     }
   }
 #pragma unroll
   for (int b = 16; b; b >>= 1) L = __fadd_rn(L, __shfl_xor_sync(0xffffffffu, L, b));
 #pragma unroll
-  for (int k = 0; k < kKvqMaxHd / 32; ++k)
-    if (lane + 32 * k < hd) sums[warp][lane + 32 * k] = o[k];
+  for (int k = 0; k < 8; ++k) {
+    const int d = 4 * lane + k % 4 + k / 4 * 128;
+    if (d < hd) sums[warp][d] = o[k];
+  }
   if (lane == 0) {
     maxima[warp] = M;
     totals[warp] = L;
@@ -1040,8 +1062,8 @@ __global__ void __launch_bounds__(kJoinWarps * 32) kvq_join_kernel(KvqView c, Kv
 
 size_t kvq_attend_space(int nh, int kv_heads, int hd) {
   const Units us = units_of(nh, kv_heads);
-  const size_t plain = (size_t)kAttendCtas * (sizeof(ShareMeta) + 2 * us.heads * (hd + 2) * sizeof(float));
-  const size_t mma = (size_t)kMmaShares * (sizeof(ShareMeta) + 2 * us.heads * (hd + 2) * sizeof(float) +
+  const size_t plain = (size_t)kAttendCtas * (sizeof(ShareMeta) + 2 * us.heads * (hd + 4) * sizeof(float));
+  const size_t mma = (size_t)kMmaShares * (sizeof(ShareMeta) + 2 * us.heads * (hd + 4) * sizeof(float) +
                                            kMmaMaxWarps * us.heads * (hd + 4) * sizeof(float)) + 16;
   return std::max(plain, mma);
 }
