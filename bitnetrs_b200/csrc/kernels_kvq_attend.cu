@@ -1129,14 +1129,15 @@ LaunchMma mma_for(const KvqView& c, int heads) {
 }
 }  // namespace
 
-const char* kvq_attend_kernel_name(const KvqView& c, int nh) {
+const char* kvq_attend_kernel_name(const KvqView& c, const KvqRows& r, int nh) {
+  if (kvq_prompt_pays(c, r, nh)) return "kvq_prompt_kernel";
   return mma_for(c, units_of(nh, c.kv_heads).heads) ? "kvq_attend_mma_kernel" : "kvq_attend_plain_kernel";
 }
 
 void launch_kvq_attend(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st) {
   if (r.rows <= 0) return;
   const Units us = units_of(a.nh, c.kv_heads);
-  if (r.runs && kvq_prompt_supported(c) && r.rows >= 16 * r.runs) {
+  if (kvq_prompt_pays(c, r, a.nh)) {
     launch_kvq_prompt(c, r, a, max_len, st);
     return;
   }

@@ -66,9 +66,10 @@ struct bitnet_cuda_model {
   uint32_t *tokens = nullptr, *next = nullptr;
   uint32_t* hist = nullptr;  // [max_position_embeddings] tokens of the sequence being sampled
   int32_t *tok_pos = nullptr, *tok_seq = nullptr, *last_row = nullptr, *order = nullptr, *status = nullptr;
+  int32_t* runs = nullptr;  // of a step's sequences: ids [Tmax], first positions [Tmax], first rows [Tmax + 1]
   DevBuf partial;
   // pinned staging
-  int32_t* h_meta = nullptr;  // [4 * Tmax]: pos, seq, last_row, order (tokens by descending position)
+  int32_t* h_meta = nullptr;  // [4 * Tmax]: pos, seq, last_row, order (tokens by descending position); then `runs`
   uint32_t* h_tokens = nullptr;
   // captured decode graphs, keyed by (kv, batch, timed), with their kernel
   // counts and (when timed) the event pairs recorded around each launch
@@ -407,6 +408,23 @@ void tp_row_split(bitnet_cuda_model* m, const uint32_t* W, int K, float ws, int 
   launch_acc_epilogue(m->tp_acc, T, H, ws, m->amax, Epi::Residual, m->h, H, st);
 }
 
+// The rows of a step over a quantised cache: a token a sequence, or runs of them.
+KvqRows kvq_rows(const bitnet_cuda_model* m, int T, int n_seqs) {
+  KvqRows r;
+  r.rows = T;
+  if (T == n_seqs) {
+    r.row_seq = m->tok_seq;
+    r.row_len = m->tok_pos;
+    r.len_bias = 1;  // a token sees its own position too
+  } else {
+    r.runs = n_seqs;
+    r.seq_ids = m->runs;
+    r.starts = m->runs + m->Tmax;
+    r.cu = m->runs + 2 * m->Tmax;
+  }
+  return r;
+}
+
 // Run the transformer over T tokens whose metadata (tokens, tok_pos, tok_seq,
 // last_row) is already on the device.  n_out rows of final hidden state
 // (selected by last_row) go through final norm, lm_head and argmax.
@@ -465,11 +483,7 @@ void run_forward(bitnet_cuda_model* m, bitnet_cuda_kv* kv, int T, int n_out, int
     float* attn_out = m->tp ? m->tp_gath + (size_t)m->tp_rank * T * qd : m->attn;
     timed(m, kAttn, st, [&] {
       if (kv->g.quant) {
-        KvqRows r;
-        r.rows = T;
-        r.row_seq = m->tok_seq;
-        r.row_len = m->tok_pos;
-        r.len_bias = 1;  // a token sees its own position too
+        const KvqRows r = kvq_rows(m, T, n_out);
         KvqAttend a;
         a.q = m->qrot;
         a.out = attn_out;
@@ -617,7 +631,8 @@ int copy_logits(bitnet_cuda_model* m, int n_out, float* dst, cudaMemcpyKind kind
 
 // Name of the attention kernel run_forward launches for T tokens (same tests).
 const char* attention_kernel_name(const bitnet_cuda_model* m, const bitnet_cuda_kv* kv, int T, int max_ctx) {
-  if (kv->g.quant) return kvq_attend_kernel_name(kvq_layer(kv->g, kv->d_table, kv->max_seqs, 0), m->nh);
+  if (kv->g.quant)  // T tokens of one sequence
+    return kvq_attend_kernel_name(kvq_layer(kv->g, kv->d_table, kv->max_seqs, 0), kvq_rows(m, T, 1), m->nh);
   if (use_decode1(m, kv, T, max_ctx)) return "decode1_kernel";
   if (use_exact_attention(m, T) && use_x4_attention(m, kv, max_ctx)) return "attn_qk_softmax_kernel+attn_pv_kernel";
   if (use_exact_attention(m, T) && use_exact3_attention(m, kv, max_ctx)) return "paged_attention_exact3_kernel";
@@ -676,6 +691,11 @@ int prepare_batch(bitnet_cuda_model* m, bitnet_cuda_kv* kv, size_t n_seqs, const
       m->h_meta[m->Tmax + t] = (int32_t)s;
     }
     m->h_meta[2 * m->Tmax + i] = (int32_t)(t - 1);
+    int32_t* run = m->h_meta + 4 * m->Tmax + i;
+    run[0] = (int32_t)s;
+    run[m->Tmax] = (int32_t)start;
+    run[2 * m->Tmax] = (int32_t)(t - counts[i]);
+    run[2 * m->Tmax + 1] = (int32_t)t;
     max_ctx = std::max<int>(max_ctx, (int)end);
   }
   // attention CTAs start in this order: the longest contexts first
@@ -687,11 +707,13 @@ int prepare_batch(bitnet_cuda_model* m, bitnet_cuda_kv* kv, size_t n_seqs, const
   return BITNET_OK;
 }
 
-int upload_meta(bitnet_cuda_model* m, int T, int n_out, cudaStream_t st) {
+int upload_meta(bitnet_cuda_model* m, const bitnet_cuda_kv* kv, int T, int n_out, cudaStream_t st) {
   BN_CUDA(cudaMemcpyAsync(m->tok_pos, m->h_meta, T * 4, cudaMemcpyHostToDevice, st));
   BN_CUDA(cudaMemcpyAsync(m->tok_seq, m->h_meta + m->Tmax, T * 4, cudaMemcpyHostToDevice, st));
   BN_CUDA(cudaMemcpyAsync(m->last_row, m->h_meta + 2 * m->Tmax, n_out * 4, cudaMemcpyHostToDevice, st));
   BN_CUDA(cudaMemcpyAsync(m->order, m->h_meta + 3 * m->Tmax, T * 4, cudaMemcpyHostToDevice, st));
+  if (kv->g.quant && T != n_out)
+    BN_CUDA(cudaMemcpyAsync(m->runs, m->h_meta + 4 * m->Tmax, (3 * (size_t)m->Tmax + 1) * 4, cudaMemcpyHostToDevice, st));
   return BITNET_OK;
 }
 
@@ -989,6 +1011,7 @@ int model_create_impl(bitnet_cuda_ctx* ctx, const bitnet_cuda_config* cfg, const
   if ((rc = m->alloc(&m->tok_seq, T))) return fail(rc);
   if ((rc = m->alloc(&m->last_row, T))) return fail(rc);
   if ((rc = m->alloc(&m->order, T))) return fail(rc);
+  if ((rc = m->alloc(&m->runs, 3 * T + 1))) return fail(rc);
   if ((rc = m->alloc(&m->hist, cfg->max_position_embeddings))) return fail(rc);
   if ((rc = m->alloc(&m->status, 16))) return fail(rc);
   if (tp) {
@@ -1002,7 +1025,7 @@ int model_create_impl(bitnet_cuda_ctx* ctx, const bitnet_cuda_config* cfg, const
     if ((rc = m->alloc(&m->tp_lgath, R * G * m->Vs))) return fail(rc);
     if ((rc = m->alloc(&m->tp_logits, R * G * m->Vs))) return fail(rc);
   }
-  cudaError_t e = cudaMallocHost(&m->h_meta, 4 * T * sizeof(int32_t));
+  cudaError_t e = cudaMallocHost(&m->h_meta, (7 * T + 1) * sizeof(int32_t));
   if (e != cudaSuccess) return fail(cuda_error(e, "cudaMallocHost"));
   e = cudaMallocHost(&m->h_tokens, T * sizeof(uint32_t));
   if (e != cudaSuccess) return fail(cuda_error(e, "cudaMallocHost"));
@@ -1270,7 +1293,7 @@ static int forward_common(bitnet_cuda_model* m, bitnet_cuda_kv* kv, size_t n_seq
   BN_TRY(ensure_partial(m, kv, T, max_ctx));
   std::memcpy(m->h_tokens, tokens, (size_t)T * 4);
   BN_CUDA(cudaMemcpyAsync(m->tokens, m->h_tokens, (size_t)T * 4, cudaMemcpyHostToDevice, st));
-  BN_TRY(upload_meta(m, T, (int)n_seqs, st));
+  BN_TRY(upload_meta(m, kv, T, (int)n_seqs, st));
   run_forward(m, kv, T, (int)n_seqs, max_ctx, st);
   BN_CUDA(cudaGetLastError());
   if (logits) BN_TRY(copy_logits(m, (int)n_seqs, logits, cudaMemcpyDeviceToHost, st));
@@ -1327,7 +1350,7 @@ static int decode_graph(bitnet_cuda_model* m, bitnet_cuda_kv* kv, size_t batch, 
   // contexts grow; splits past a token's context exit immediately.
   const int cap_ctx = (int)kv->capacity();
   BN_TRY(ensure_partial(m, kv, T, cap_ctx));
-  BN_TRY(upload_meta(m, T, T, st));
+  BN_TRY(upload_meta(m, kv, T, T, st));
   if (src_on_host) {
     std::memcpy(m->h_tokens, src, (size_t)T * 4);
     BN_CUDA(cudaMemcpyAsync(m->tokens, m->h_tokens, (size_t)T * 4, cudaMemcpyHostToDevice, st));

@@ -336,7 +336,8 @@ def test_attention_in_a_graph_and_on_another_stream(cuda_backend):
 
 @pytest.mark.parametrize("io", ["f32", "bf16"])
 @pytest.mark.parametrize("kv", KINDS)
-@pytest.mark.parametrize("nh,heads,hd", [(20, 5, 128), (16, 2, 64), (4, 2, 32), (3, 3, 96), (9, 1, 128)])
+@pytest.mark.parametrize("nh,heads,hd", [(20, 5, 128), (16, 2, 64), (4, 2, 32), (3, 3, 96), (9, 1, 128), (32, 8, 128),
+                                         (32, 16, 64), (24, 8, 64), (40, 4, 128), (7, 7, 128)])
 def test_prompt_attention(cuda_backend, nh, heads, hd, kv, io):
     counts, starts, seqs = [70, 0, 1, 33, 129], [0, 5, 40, 100, 17], [2, 0, 4, 1, 3]
     lens = [0] * 5
@@ -465,7 +466,7 @@ def test_model_forward_over_a_quantised_cache(cuda_backend, one_layer, kv):
     toks = synth.uniform_u32(12, 7, 100, 0, cfg.vocab_size - 1).tolist()
     full = m.new_kv_cache(num_pages=40, kv_dtype=kv)
     a = m.forward(toks, 0, full)
-    assert m.attention_kernel(full, 1).startswith("kvq_")
+    assert m.attention_kernel(full, 1).startswith("kvq_attend")
     plain = m.new_kv_cache(num_pages=40)
     m.forward(toks, 0, plain)
     sh = (100, cfg.num_key_value_heads, cfg.head_dim())
@@ -527,6 +528,26 @@ def test_model_decode_batch_and_layer_view(cuda_backend, small, kv):
 
 
 @pytest.mark.parametrize("kv", KINDS)
+def test_model_packed_prefill(cuda_backend, kv):
+    """Ragged prompts packed into steps of 512 tokens run the prompt kernel (8 kv heads of 128), one of them split over
+    steps; each sequence's logits against the same prompt by itself in steps of 16 (the single-token kernel).  One
+    layer, so the codes are the same; the bound is that of test_model_forward_over_a_quantised_cache."""
+    cfg = ModelConfig(300, 2048, 1, 16, 8, 256, 700, 10000.0, 1e-5)
+    m = BitNetModel(synth.random_model(cfg, seed=3), cuda_backend, max_batch_tokens=512)
+    prompts = [synth.uniform_u32(4, i, n, 0, 299).tolist() for i, n in enumerate([333, 1, 400, 60])]
+    cache = m.new_kv_cache(num_pages=70, max_seqs=4, kv_dtype=kv)
+    assert m.attention_kernel(cache, 512) == "kvq_prompt_kernel"
+    _, logits = m.prefill_packed(cache, range(4), prompts, want_logits=True)
+    ref = m.new_kv_cache(num_pages=70, max_seqs=4, kv_dtype=kv)
+    for s, p in enumerate(prompts):
+        for at in range(0, len(p), 16):
+            r = m.forward(p[at:at + 16], at, ref, seq=s)
+        for x, y in zip(cache.read(s, len(p)), ref.read(s, len(p))):
+            np.testing.assert_array_equal(x, y)
+        assert np.max(np.abs(logits[s] - r)) <= 1e-2 * np.max(np.abs(r))
+
+
+@pytest.mark.parametrize("kv", KINDS)
 def test_model_generate_runs(cuda_backend, small, kv):
     cfg, w = small
     m = BitNetModel(w, cuda_backend, max_batch_tokens=32)
@@ -559,35 +580,37 @@ def test_prompt_attention_later_keys_stay_hidden(cuda_backend, hd, kv):
     """A key that is not a number, scale of K, of V or both, touches the rows that see it and no others; rows behind a
     negative start see nothing."""
     n = 200
-    b = bench(cuda_backend, kv, 2, hd, [n, n], seed=2)
+    b = bench(cuda_backend, kv, 6, hd, [n, n], seed=2)
     for kind, pos in ((0, 150), (1, 70)):
         b.c.params_view(kind)[int(b.c.table[0, pos // 16]), 0, :, pos % 16] = float("nan")
-    q = torch.randn(2 * n, 8 * hd, device=b.dev, generator=torch.Generator(device=b.dev).manual_seed(6))
-    out, lse = b.prompt(q, 8, [0, 1], [0, n, 2 * n], [0, -40])
-    o = out.view(2 * n, 8, hd)
+    nh = 24  # the first four share the kv head in question
+    q = torch.randn(2 * n, nh * hd, device=b.dev, generator=torch.Generator(device=b.dev).manual_seed(6))
+    out, lse = b.prompt(q, nh, [0, 1], [0, n, 2 * n], [0, -40])
+    o = out.view(2 * n, nh, hd)
     assert torch.isnan(o[70:n, :4]).all() and torch.isfinite(o[:n, 4:]).all() and torch.isfinite(o[:70]).all()
     assert torch.isnan(lse[150:n, :4]).all() and torch.isfinite(lse[:150]).all() and torch.isfinite(lse[:n, 4:]).all()
     for i in (0, 31, 69):
-        check_row(b, q[i], 8, 0, i + 1, out[i], lse[i])
+        check_row(b, q[i], nh, 0, i + 1, out[i], lse[i])
     assert (out[n:n + 40] == 0).all() and (lse[n:n + 40] == -math.inf).all()
     for i in (40, 41, 110, n - 1):
-        check_row(b, q[n + i], 8, 1, i - 39, out[n + i], lse[n + i])
+        check_row(b, q[n + i], nh, 1, i - 39, out[n + i], lse[n + i])
 
 
 @pytest.mark.parametrize("hd", [128, 32])
 def test_prompt_attention_bad_places_are_reported(cuda_backend, hd):
-    b = bench(cuda_backend, KV_I8, 1, hd, [100, 100], seed=8)
-    q = torch.randn(100, 4 * hd, device=b.dev)
-    out, lse = b.prompt(q, 4, [0, 9], [0, 60, 100], [0, 5])
+    nh = 48
+    b = bench(cuda_backend, KV_I8, 12, hd, [100, 100], seed=8)
+    q = torch.randn(100, nh * hd, device=b.dev)
+    out, lse = b.prompt(q, nh, [0, 9], [0, 60, 100], [0, 5])
     assert b.status.item() == 4
-    check_row(b, q[59], 4, 0, 60, out[59], lse[59])
+    check_row(b, q[59], nh, 0, 60, out[59], lse[59])
     assert (out[60:] == 0).all() and (lse[60:] == -math.inf).all()
     b.status.zero_()
-    out, lse = b.prompt(q, 4, [0], [0, 100], [0], max_len=50)  # cut there
+    out, lse = b.prompt(q, nh, [0], [0, 100], [0], max_len=50)  # cut there
     assert b.status.item() == 4
-    check_row(b, q[49], 4, 0, 50, out[49], lse[49])
-    check_row(b, q[80], 4, 0, 50, out[80], lse[80])
+    check_row(b, q[49], nh, 0, 50, out[49], lse[49])
+    check_row(b, q[80], nh, 0, 50, out[80], lse[80])
     b.status.zero_()
     b.c.table[1, 3] = 10**6
-    b.prompt(q[:60], 4, [1], [0, 60], [0])
+    b.prompt(q, nh, [1], [0, 100], [0])
     assert b.status.item() == 4
