@@ -624,7 +624,7 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
         zero = __fadd_rn(zero, __shfl_xor_sync(0xffffffffu, zero, o));
       }
       // 2^29 / 2^floor(log2 top), the exponents kept within what a float and its inverse can hold
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 30), 254);
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 36), 254);
       const float up = __uint_as_float((uint32_t)(283 - e) << 23), down = __uint_as_float((uint32_t)(e - 29) << 23);
       const int d3 = 3 - (g & 1), d1 = 1 - (g & 1);
 #pragma unroll
@@ -640,9 +640,9 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
           qf[nt][s][1][k] = gather_byte(w[0], w[1], w[2], w[3], d1);
         }
       // a q that is not finite makes its head NaN
-      const float f = __fadd_rn(__fmul_rn(qscale, down), zero);
+      const float f = __fadd_rn(__fmul_rn(I4 ? qscale / 16 : qscale, down), zero);
       qs[nt] = __shfl_sync(0xffffffffu, f, 8 * t);
-      qsum[nt] = I4 ? __shfl_sync(0xffffffffu, __fmul_rn(sum, up), 8 * t) : 0.0f;
+      qsum[nt] = I4 ? __shfl_sync(0xffffffffu, __fmul_rn(sum, __fmul_rn(up, 16.0f)), 8 * t) : 0.0f;
     }
 
     // Scores stay in the units of the integer products times their scales;
@@ -682,10 +682,11 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
         for (int s = 0; s < T::kKSteps; ++s) {
           uint32_t x[2], y[2];  // rows g and g + 8
           if constexpr (I4) {
-            x[0] = kw[2 * s] & 0x0f0f0f0fu;
-            x[1] = (kw[2 * s] >> 4) & 0x0f0f0f0fu;
-            y[0] = kw[2 * s + 1] & 0x0f0f0f0fu;
-            y[1] = (kw[2 * s + 1] >> 4) & 0x0f0f0f0fu;
+            // 16 (c - 8) as signed bytes
+            x[0] = and_xor(kw[2 * s] << 4, 0xf0f0f0f0u, 0x80808080u);
+            x[1] = and_xor(kw[2 * s], 0xf0f0f0f0u, 0x80808080u);
+            y[0] = and_xor(kw[2 * s + 1] << 4, 0xf0f0f0f0u, 0x80808080u);
+            y[1] = and_xor(kw[2 * s + 1], 0xf0f0f0f0u, 0x80808080u);
           } else {
             x[0] = kw[4 * s];
             y[0] = kw[4 * s + 1];
@@ -710,9 +711,9 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
             const int turned = T::kWhole ? (line & 7) << 4 : 0;
             return *(const float*)(par + pg * kParStride + (x & ~127) + (((x & 127) ^ (turned & 96)) | ((4 * g) ^ (turned & 16))));
           };
-          const float ks = param(0), kz = I4 ? param(1) : 0.0f;
+          const float ks = param(0), kz = I4 ? __fmaf_rn(8.0f, ks, param(1)) : 0.0f;
           vs[pg][k] = param(I4 ? 2 : 1);
-          vz[pg][k] = I4 ? param(3) : 0.0f;
+          vz[pg][k] = I4 ? __fmaf_rn(kNibbleMid, vs[pg][k], param(3)) : 0.0f;
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
             // digits 3 and 2, 1 and 0: sums of at most 2^29
@@ -829,7 +830,7 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
     }
 
     const bool begins = p0 == 0, ends = p1 == pages;
-    const float back = __fdiv_rn(1.0f, vf);
+    const float back = __fdiv_rn(I4 ? 1.0f / kNibbleUnit : 1.0f, vf);
     const int slot = begins && !ends ? 1 : 0;
     if (!begins) {
       note.has0 = 1;

@@ -53,6 +53,7 @@ namespace {
 
 constexpr int kPromptRows = 128, kPromptThreads = 256, kWiden = 96, kKeys = 64, kTilePages = kKeys / kPage;
 constexpr uint32_t kTmemCols = 256;
+constexpr int kSumTiles = 8;  // f32 rows: tiles that are summed in tensor memory
 
 template <int HD, bool I4, bool TWO>
 struct PromptTile {
@@ -120,6 +121,19 @@ __device__ __forceinline__ void tmem_st16(uint32_t at, const uint32_t* r) {
 __device__ __forceinline__ void tmem_st8(uint32_t at, const uint32_t* r) {
   asm volatile("tcgen05.st.sync.aligned.32x32b.x8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"r"(at), "r"(r[0]),
                "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// 32 bytes at a time: a thread's accesses are a row from its neighbours', so each is a line of its own.
+__device__ __forceinline__ void load_f32x8(const float* p, float* x) {
+  asm volatile("ld.global.v8.f32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];\n"
+               : "=f"(x[0]), "=f"(x[1]), "=f"(x[2]), "=f"(x[3]), "=f"(x[4]), "=f"(x[5]), "=f"(x[6]), "=f"(x[7])
+               : "l"(p)
+               : "memory");
+}
+__device__ __forceinline__ void store_f32x8(float* p, const float* x) {
+  asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
+               "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
                : "memory");
 }
 
@@ -330,8 +344,9 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   // 2^14 / 2^floor(log2 top), the exponents kept within what a float and its inverse can hold
   const int e = min(max((int)(__float_as_uint(top) >> 23), 20), 254);
   const float up = __uint_as_float((uint32_t)(268 - e) << 23), down = __uint_as_float((uint32_t)(e - 14) << 23);
-  const float qs = __fadd_rn(__fmul_rn(__fdiv_rn(1.4426950408889634f, __fsqrt_rn((float)HD)), down), odd);
-  qsum = __fmul_rn(qsum, up);
+  constexpr float kUnit = I4 ? kNibbleUnit : 1.0f;  // of the widened codes
+  const float qs = __fadd_rn(__fmul_rn(__fdiv_rn(1.4426950408889634f / kUnit, __fsqrt_rn((float)HD)), down), odd);
+  qsum = __fmul_rn(qsum, __fmul_rn(up, kUnit));
 #pragma unroll 1
   for (int i = 0; i < HD / 2; i += 16) {
     uint32_t hi[8];
@@ -382,32 +397,37 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       // behind the context the bytes may be anything
       const bool live = j * kKeys + key < seen;
       par[j & 1][0][key] = live ? p[0] : 0.0f;
-      par[j & 1][1][key] = I4 && live ? p[kPage] : 0.0f;
+      par[j & 1][1][key] = I4 && live ? __fmaf_rn(kNibbleMid, p[0], p[kPage]) : 0.0f;
       par[j & 1][2][key] = live ? p[I4 ? 2 * kPage : kPage] : 0.0f;
-      par[j & 1][3][key] = I4 && live ? p[3 * kPage] : 0.0f;
+      par[j & 1][3][key] = I4 && live ? __fmaf_rn(kNibbleMid, p[2 * kPage], p[3 * kPage]) : 0.0f;
     }
   };
   auto scores_at = [&](int j) -> uint32_t { return T::kTmemS + (T::kTwoS && (j & 1) ? kKeys : 0); };
+  // The second terms first: the sums are cut, not rounded, to f32, each time by
+  // what they have grown to.
   auto issue_scores = [&](int j) {
     const uint32_t d = tmem + scores_at(j);
+    auto k_at = [&](int k) { return operand(smem_u32(k_tile) + k / 4 * (kKeys * 128) + k % 4 * 32, 16); };
+    if (TWO)
 #pragma unroll
-    for (int k = 0; k < HD / 16; ++k) {
-      const uint64_t b = operand(smem_u32(k_tile) + k / 4 * (kKeys * 128) + k % 4 * 32, 16);
-      mma_tmem_a(d, tmem + T::kTmemQ + 8 * k, b, product(kKeys, 0), k > 0);
-      if (TWO)
-        mma_smem_a(d, operand(smem_u32(q_tile) + k / 4 * (kPromptRows * 128) + k % 4 * 32, 16), b, product(kKeys, 0),
-                   true);
-    }
+      for (int k = 0; k < HD / 16; ++k)
+        mma_smem_a(d, operand(smem_u32(q_tile) + k / 4 * (kPromptRows * 128) + k % 4 * 32, 16), k_at(k),
+                   product(kKeys, 0), k > 0);
+#pragma unroll
+    for (int k = 0; k < HD / 16; ++k)
+      mma_tmem_a(d, tmem + T::kTmemQ + 8 * k, k_at(k), product(kKeys, 0), TWO || k > 0);
     mma_commit(smem_u32(&scores_full[j & 1]));
   };
   auto issue_output = [&](int j) {
     const uint32_t w = tmem + scores_at(j);
+    const bool adds = TWO ? j % kSumTiles != 0 : j > 0;
+    auto v_at = [&](int k) { return operand(smem_u32(v_tile) + k * 2048, kKeys * 128); };
+    if (TWO)
 #pragma unroll
-    for (int k = 0; k < kKeys / 16; ++k) {
-      const uint64_t b = operand(smem_u32(v_tile) + k * 2048, kKeys * 128);
-      mma_tmem_a(tmem, w + 8 * k, b, product(HD, 1), j > 0 || k > 0);
-      if (TWO) mma_tmem_a(tmem, w + 32 + 8 * k, b, product(HD, 1), true);
-    }
+      for (int k = 0; k < kKeys / 16; ++k) mma_tmem_a(tmem, w + 32 + 8 * k, v_at(k), product(HD, 1), adds || k > 0);
+#pragma unroll
+    for (int k = 0; k < kKeys / 16; ++k)
+      mma_tmem_a(tmem, w + 8 * k, v_at(k), product(HD, 1), TWO || adds || k > 0);
     mma_commit(smem_u32(&output_full));
   };
   // One arrival a warp, after its writes to shared memory (for the products) or to tensor memory.
@@ -473,6 +493,54 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   } else {
     // ---- weighing ----
     int ev = 100;  // the weights are multiplied by 2^ev
+    float kept = 1.0f;  // what m's growth has left of the sums that are in the output's place
+    // 16 elements of the row's output, in the order in which they lie in o
+    auto load_sums = [&](int i, float* o) {
+      const float* p = (const float*)a.out + out_at + i;
+      float x[16];
+      if (wide_out == 2) {
+        load_f32x8(p, x);
+        load_f32x8(p + 8, x + 8);
+      } else if (wide_out) {
+#pragma unroll
+        for (int k = 0; k < 16; k += 4) {
+          const float4 u = *(const float4*)(p + k);
+          x[k] = u.x, x[k + 1] = u.y, x[k + 2] = u.z, x[k + 3] = u.w;
+        }
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) x[k] = p[k];
+      }
+#pragma unroll
+      for (int k = 0; k < 16; ++k) o[k] = __fmaf_rn(x[k / 8 * 8 + widened<I4>(k % 8)], kept, o[k]);
+    };
+    auto store_out = [&](int i, const float* o) {
+      float x[16];
+#pragma unroll
+      for (int k = 0; k < 16; ++k) x[k / 8 * 8 + widened<I4>(k % 8)] = o[k];
+      if (!TWO && wide_out) {
+#pragma unroll
+        for (int k = 0; k < 16; k += 8) {
+          uint32_t u[4];
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const __nv_bfloat162 p = __floats2bfloat162_rn(x[k + 2 * n], x[k + 2 * n + 1]);
+            u[n] = *(const uint32_t*)&p;
+          }
+          *(uint4*)((uint16_t*)a.out + out_at + i + k) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
+      } else if (wide_out == 2) {
+        store_f32x8((float*)a.out + out_at + i, x);
+        store_f32x8((float*)a.out + out_at + i + 8, x + 8);
+      } else if (wide_out) {
+#pragma unroll
+        for (int k = 0; k < 16; k += 4)
+          *(float4*)((float*)a.out + out_at + i + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
+      } else {
+#pragma unroll
+        for (int k = 0; k < 16; ++k) store_elem(a.out, out_at + i + k, !TWO, x[k]);
+      }
+    };
     for (int j = 0; j < tiles; ++j) {
       if (!wait(keys_ready[j & 1], j / 2) || !wait(scores_full[j & 1], j / 2)) break;
       after_sync();
@@ -495,6 +563,23 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
 #pragma unroll
         for (int k = 0; k < 4; ++k)
           s[i + k] = I4 ? __fmaf_rn(s[i + k], k4[k], __fmul_rn(qsum, z4[k])) : __fmul_rn(s[i + k], k4[k]);
+      }
+      if (TWO && j > 0 && j % kSumTiles == 0) {  // the sums so far, to the output's place
+        if (!wait(output_full, j - 1)) break;
+        after_sync();
+#pragma unroll 1
+        for (int i = 0; i < HD; i += 16) {
+          float o[16];
+          __syncwarp();
+          tmem_ld16(tlane + i, (uint32_t*)o);
+          tmem_wait_ld();
+          if (live_row) {
+            if (j > kSumTiles) load_sums(i, o);
+            store_out(i, o);
+          }
+        }
+        __syncwarp();
+        kept = 1.0f;
       }
       const bool masked = key0 + kKeys > min(start + 1, seen);  // keys that the CTA's first token does not see, or no one does
       if (masked) {
@@ -521,7 +606,8 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
         limit = __fadd_rn(m, __fdiv_rn(kSlack, qs));
         l = __fmul_rn(l, keep);
         zsum = __fmul_rn(zsum, keep);
-        if (j > 0) {
+        kept = __fmul_rn(kept, keep);
+        if (TWO ? j % kSumTiles != 0 : j > 0) {
           if (!wait(output_full, j - 1)) break;
           after_sync();
 #pragma unroll 1
@@ -536,6 +622,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
         }
       }
       // weights, over the scores; a key that the row does not see weighs nothing, whatever its scale
+      float l_tile = 0.0f, z_tile = 0.0f;  // a tile's sums by themselves: a long context's would lose their small terms
       auto weigh = [&](auto some_hidden) {
 #pragma unroll
         for (int i = 0; i < kKeys; i += 16) {
@@ -553,9 +640,9 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               const float w = exp2_approx(__fmaf_rn(s[i + n + k], qs, -mq));
-              l = __fadd_rn(l, w);
+              l_tile = __fadd_rn(l_tile, w);
               const bool hidden = decltype(some_hidden)::value && key0 + i + n + k >= limit_pos;
-              if constexpr (I4) zsum = hidden ? zsum : __fmaf_rn(w, z4[k], zsum);
+              if constexpr (I4) z_tile = hidden ? z_tile : __fmaf_rn(w, z4[k], z_tile);
               p[k] = hidden ? 0.0f : __fmul_rn(w, v4[k]);
             }
 #pragma unroll
@@ -573,6 +660,8 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
         weigh(std::true_type{});
       else
         weigh(std::false_type{});
+      l = __fadd_rn(l, l_tile);
+      zsum = __fadd_rn(zsum, z_tile);
       tmem_wait_st();
       before_sync();
       arrive(weights_ready[j & 1]);
@@ -583,34 +672,15 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     const float inv = sees ? __fdiv_rn(1.0f, l) : 0.0f;
 #pragma unroll 1
     for (int i = 0; i < HD; i += 16) {
-      float o[16], x[16];
+      float o[16];
       __syncwarp();
       tmem_ld16(tlane + i, (uint32_t*)o);
       tmem_wait_ld();
+      if (live_row && good) {
+        if (TWO && tiles > kSumTiles) load_sums(i, o);
 #pragma unroll
-      for (int k = 0; k < 16; ++k) {
-        const float v = sees ? __fmul_rn(__fadd_rn(o[k], zsum), inv) : 0.0f;
-        x[k / 8 * 8 + widened<I4>(k % 8)] = v;
-      }
-      if (!live_row || !good) {
-      } else if (wide_out && a.bf16) {
-#pragma unroll
-        for (int k = 0; k < 16; k += 8) {
-          uint32_t u[4];
-#pragma unroll
-          for (int n = 0; n < 4; ++n) {
-            const __nv_bfloat162 p = __floats2bfloat162_rn(x[k + 2 * n], x[k + 2 * n + 1]);
-            u[n] = *(const uint32_t*)&p;
-          }
-          *(uint4*)((uint16_t*)a.out + out_at + i + k) = make_uint4(u[0], u[1], u[2], u[3]);
-        }
-      } else if (wide_out) {
-#pragma unroll
-        for (int k = 0; k < 16; k += 4)
-          *(float4*)((float*)a.out + out_at + i + k) = make_float4(x[k], x[k + 1], x[k + 2], x[k + 3]);
-      } else {
-#pragma unroll
-        for (int k = 0; k < 16; ++k) store_elem(a.out, out_at + i + k, a.bf16, x[k]);
+        for (int k = 0; k < 16; ++k) o[k] = sees ? __fmul_rn(I4 ? __fmaf_rn(o[k], 1.0f / kUnit, zsum) : o[k], inv) : 0.0f;
+        store_out(i, o);
       }
     }
     if (live_row && good && a.lse) a.lse[out_row * a.nh + h0 + head] = sees ? lse_of(mq, l) : -INFINITY;
@@ -646,7 +716,8 @@ void launch_prompt(const KvqView& c, const KvqRows& r, const KvqAttend& a, int m
   cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
   const size_t run = a.bf16 ? 8 : 4;
   const int wide_q = (uintptr_t)a.q % 16 == 0 && a.ldq % run == 0;
-  const int wide_out = (uintptr_t)a.out % 16 == 0 && a.ldo % run == 0;
+  // 16 bytes of the output at a time, or 32 (f32)
+  const int wide_out = (uintptr_t)a.out % 16 || a.ldo % run ? 0 : a.bf16 || (uintptr_t)a.out % 32 || a.ldo % 8 ? 1 : 2;
   kernel<<<ctas, kPromptThreads, T::kSmem, st>>>(c, r, a, max_len, wide_q, wide_out);
   count_launch();
 }

@@ -103,15 +103,10 @@ __device__ __forceinline__ uint32_t two_terms(float x) {
   const uint32_t h = pack_f16(x, 0.0f);
   return pack_f16(f16_lo(h), __fsub_rn(x, f16_lo(h)));
 }
-// (x & mask) ^ bits, and (x & mask) | bits, in one instruction each
+// (x & mask) ^ bits in one instruction
 __device__ __forceinline__ uint32_t and_xor(uint32_t x, uint32_t mask, uint32_t bits) {
   uint32_t r;
   asm("lop3.b32 %0, %1, %2, %3, 0x6a;\n" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
-  return r;
-}
-__device__ __forceinline__ uint32_t and_or(uint32_t x, uint32_t mask, uint32_t bits) {
-  uint32_t r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;\n" : "=r"(r) : "r"(x), "r"(mask), "r"(bits));
   return r;
 }
 // Four signed bytes of w as fp16 pairs: elements (0, 2) and (1, 3).  A byte with
@@ -120,13 +115,19 @@ __device__ __forceinline__ void bytes_f16(uint32_t w, uint32_t* even, uint32_t* 
   *even = add_f16x2(and_xor(w, 0x00ff00ffu, 0x64806480u), 0xe480e480u);
   *odd = add_f16x2(and_xor(w >> 8, 0x00ff00ffu, 0x64806480u), 0xe480e480u);
 }
-// Eight nibbles of w as fp16 pairs: x[i] = elements (i, i + 4).
+// Eight nibbles c of w as fp16 pairs (c - 7.5) / 512: x[i] = elements (i, i + 4).
+// With codes on both sides of 0, and zero + 7.5 scale for the zero, neither of
+// the two sums that make an I4 value's product outgrows it.  A nibble alone in
+// its 16 bits is the subnormal c / 2^24 (or c / 2^20), so one product and sum,
+// both exact, widens a pair.
+constexpr float kNibbleMid = 7.5f, kNibbleUnit = 1.0f / 512;
 __device__ __forceinline__ void nibbles_f16(uint32_t w, uint32_t* x) {
+  constexpr uint32_t kLow = 0x78007800u, kHigh = 0x68006800u, kMid = 0xa380a380u;  // 2^15, 2^11, -7.5 / 512
   const uint32_t v = w >> 8;
-  x[0] = add_f16x2(and_or(w, 0x000f000fu, 0x64006400u), 0xe400e400u);               // 1024 + c - 1024
-  x[1] = fma_f16x2(and_or(w, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd400d400u);  // (1024 + 16 c) / 16 - 64
-  x[2] = add_f16x2(and_or(v, 0x000f000fu, 0x64006400u), 0xe400e400u);
-  x[3] = fma_f16x2(and_or(v, 0x00f000f0u, 0x64006400u), 0x2c002c00u, 0xd400d400u);
+  x[0] = fma_f16x2(w & 0x000f000fu, kLow, kMid);
+  x[1] = fma_f16x2(w & 0x00f000f0u, kHigh, kMid);
+  x[2] = fma_f16x2(v & 0x000f000fu, kLow, kMid);
+  x[3] = fma_f16x2(v & 0x00f000f0u, kHigh, kMid);
 }
 }  // namespace
 }  // namespace bitnet
