@@ -23,6 +23,7 @@ KV_I8 = 2
 KV_I4 = 3
 STATUS_NON_FINITE = 1
 STATUS_BAD_CONTEXT = 4
+STATUS_WAIT_TIMEOUT = 8
 
 
 class PagedKV:

@@ -488,12 +488,20 @@ int bitnet_cuda_model_attention_kernel(bitnet_cuda_model* model, bitnet_cuda_kv*
  *
  * The entry points below take device addresses, return without synchronising
  * and can be captured into a graph.  They leave the calling thread's current
- * device as it was.  What the host cannot see is checked on the device: a
- * sequence, position, length or page outside the cache is not accessed, and
- * sets a bit of *status (device int32, which the caller zeroes and reads):
- * BITNET_STATUS_NON_FINITE or BITNET_STATUS_BAD_CONTEXT. */
+ * device as it was.  Outputs overlap no input, each other or the pool.  What
+ * the host cannot see is checked on the device, and sets a bit of *status
+ * (device int32, which the caller zeroes and reads):
+ * BITNET_STATUS_NON_FINITE   a row to store holds a NaN or an infinity.
+ * BITNET_STATUS_BAD_CONTEXT  a sequence, position, length or page outside the
+ *   cache.  It is not accessed: a store skips the row and a load leaves its
+ *   outputs as they were; attention gives zeros for a bad sequence, cuts a
+ *   long length, and reads another page in a bad one's place, so that such a
+ *   row's result means nothing.
+ * BITNET_STATUS_WAIT_TIMEOUT  a kernel's own wait for its copies or products
+ *   ran out; the call's results mean nothing. */
 #define BITNET_STATUS_NON_FINITE 1
 #define BITNET_STATUS_BAD_CONTEXT 4
+#define BITNET_STATUS_WAIT_TIMEOUT 8
 typedef struct {
   void* pool;                /* 16-byte aligned */
   const int32_t* page_table; /* [seqs][pages_per_seq] */
@@ -537,9 +545,10 @@ int bitnet_cuda_kv_attention_workspace(const bitnet_cuda_kv_pages* cache, size_t
  *   lse[r][h] = log sum_j exp(q . k_j / sqrt(head_dim))   (optional, f32 [rows][n_heads]).
  * A row of length 0 (or less) gives zeros and -inf.  Several rows may name one
  * sequence.  No length may exceed max_len (a longer one is cut there and sets
- * the status).  Scores, softmax and sums are held to f32 accuracy; with bf16
+ * the status).  Scores, softmax and sums are held to f32 accuracy, for keys
+ * and values of up to 2^80 (above, they may overflow to infinities); with bf16
  * q and out (x_is_bf16 != 0) only the output is rounded.  The context is split
- * over the GPU by the lengths alone, so equal lengths give equal bits. */
+ * over the GPU by the lengths alone, so a call repeated gives the same bits. */
 int bitnet_cuda_kv_attention_device(bitnet_cuda_ctx* ctx, const bitnet_cuda_kv_pages* cache, const void* q, size_t ldq,
                                     int x_is_bf16, size_t rows, size_t n_heads, const int32_t* row_seq,
                                     const int32_t* row_len, size_t max_len, void* out, size_t ldo, float* lse,
@@ -551,7 +560,8 @@ int bitnet_cuda_kv_attention_device(bitnet_cuda_ctx* ctx, const bitnet_cuda_kv_p
  * n_seqs and n_seqs; cu_rows does not decrease and stays within `rows`), and
  * each attends to the positions up to its own.  Rows outside every range are
  * left as they were.  max_len bounds starts[i] + the rows of i.  The rest is as
- * above. */
+ * above, but that with bf16 rows a softmax weight may be rounded once to fp16
+ * (by 2^-11 at most) where many rows share the work. */
 int bitnet_cuda_kv_prompt_attention_device(bitnet_cuda_ctx* ctx, const bitnet_cuda_kv_pages* cache, const void* q,
                                            size_t ldq, int x_is_bf16, size_t rows, size_t n_heads, size_t n_seqs,
                                            const int32_t* seq_ids, const int32_t* cu_rows, const int32_t* starts,

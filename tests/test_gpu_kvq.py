@@ -614,3 +614,137 @@ def test_prompt_attention_bad_places_are_reported(cuda_backend, hd):
     b.c.table[1, 3] = 10**6
     b.prompt(q, nh, [1], [0, 100], [0])
     assert b.status.item() == 4
+
+
+# ---- many rows, long sums, extremes, graphs ---------------------------------------------
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("rope", [False, True])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [32, 64, 96, 128, 256, 80])
+def test_store_many_rows_as_few(cuda_backend, hd, kv, rope, io):
+    """A store of many rows (more elements a lane) writes what stores of a few rows each write, which are tested above."""
+    heads, n = 6, 1700
+    one = bench(cuda_backend, kv, heads, hd, [n], seed=3, fill="noise")
+    few = bench(cuda_backend, kv, heads, hd, [n], seed=3, fill="noise")
+    g = torch.Generator(device=one.dev).manual_seed(hd)
+    x = torch.randn(n, 2 * heads * hd, device=one.dev, generator=g)
+    x[5] = torch.randint(-9, 10, (x.shape[1],), device=one.dev, generator=g).float()  # ties
+    x[6] *= 1e-41
+    x[7] = 0.25
+    x[8, 3] = float("inf")
+    k, v = x.to(DT[io]).split(heads * hd, 1)
+    cos, sin = (torch.randn(n, hd // 2, device=one.dev, generator=g) for _ in range(2))
+    angles = (cos.data_ptr(), sin.data_ptr(), n) if rope else None
+    pos = torch.randperm(n, device=one.dev, generator=g).tolist()
+    one.store(k, v, [0] * n, pos, angles)
+    for i in range(0, n, 100):
+        few.store(k[i:i + 100], v[i:i + 100], [0] * 100, pos[i:i + 100], angles)
+    torch.cuda.synchronize()
+    assert one.status.item() == few.status.item() == 1
+    torch.testing.assert_close(one.c.pool, few.c.pool, rtol=0, atol=0)
+
+
+def far(got, ref):
+    return ((got.double() - ref).norm() / ref.norm()).item()
+
+
+@pytest.mark.parametrize("shift", [0, 4, 8, 2])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("nh,heads,hd", [(32, 8, 128), (24, 12, 64)])
+def test_long_sums_keep_their_accuracy(cuda_backend, nh, heads, hd, kv, shift):
+    """f32 rows over long contexts, both kernels, with the output at every alignment of 4 bytes.
+
+    Tensor cores cut their f32 sums.  Up to 64 such additions follow one another before a sum is added, rounded, to the
+    rest: each cuts 2^-24 of the sum on average, and the sum is on average half of what it becomes, so a block is off
+    by 64 * 2^-25 = 2^-19, and blocks, like their sums, add as independent terms.  The scores' 2 * hd / 16 additions
+    and the weights' roundings are within 2^-20 together.  Below 2^-18.4 = 3e-6; a sum left in the tensor cores over
+    1300 positions would be off by 5e-6 and more."""
+    n, start = 90, 1250
+    b = bench(cuda_backend, kv, heads, hd, [start + n, 700], seed=4)
+    g = torch.Generator(device=b.dev).manual_seed(5)
+    q = torch.randn(n + 600, nh * hd, device=b.dev, generator=g)
+    wide = torch.full((n + 600, nh * hd + 12), 9.0, device=b.dev)
+    out = wide[:, shift:shift + nh * hd] if shift != 8 else torch.zeros_like(q)
+    a, c, s = b.ints([0, 1]), b.ints([0, n, n + 600]), b.ints([start, 100])
+    sp, lse = b.space(nh), torch.zeros(n + 600, nh, device=b.dev)
+    b.kv.prompt_attention(q.data_ptr(), out.data_ptr(), n + 600, nh, 2, a.data_ptr(), c.data_ptr(), s.data_ptr(),
+                          start + n, sp.data_ptr(), sp.numel(), b.status.data_ptr(), ldo=out.stride(0),
+                          lse=lse.data_ptr(), stream=1)
+    torch.cuda.synchronize()
+    assert b.status.item() == 0
+    rows = [(0, 0, start + 1), (n // 2, 0, start + n // 2 + 1), (n - 1, 0, start + n), (n, 1, 101), (n + 410, 1, 511),
+            (n + 411, 1, 512), (n + 412, 1, 513), (n + 599, 1, 700)]
+    ref = []
+    for r, seq, length in rows:
+        check_row(b, q[r], nh, seq, length, out[r], lse[r])
+        ref.append(R.attention(b.c, q[r].double().view(nh, hd), seq, length)[0].flatten())
+    at = [r[0] for r in rows]
+    assert far(out[at], torch.stack(ref)) < 3e-6
+    one, _ = b.attend(q[at].contiguous(), nh, [r[1] for r in rows], [r[2] for r in rows])
+    assert far(one, torch.stack(ref)) < 3e-6
+    if shift != 8:
+        assert (wide[:, :shift] == 9.0).all() and (wide[:, shift + nh * hd:] == 9.0).all()
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [128, 64, 32, 80])
+def test_attention_of_large_keys_and_values(cuda_backend, hd, kv):
+    """Keys near 2^72 under queries near 2^-72, values near 2^78: only powers of two against the ordinary case."""
+    heads, nh, n = 8, 32, 300
+    b = bench(cuda_backend, kv, heads, hd, [n], seed=12)
+    b.c.params_view(0).mul_(2.0**72)
+    b.c.params_view(1).mul_(2.0**78)
+    q = torch.randn(n, nh * hd, device=b.dev, generator=torch.Generator(device=b.dev).manual_seed(1)) * 2.0**-72
+    out, lse = b.prompt(q, nh, [0], [0, n], [0])
+    one, lse1 = b.attend(q, nh, [0] * n, list(range(1, n + 1)))
+    for i in (0, 77, 299):
+        check_row(b, q[i], nh, 0, i + 1, out[i], lse[i])
+        check_row(b, q[i], nh, 0, i + 1, one[i], lse1[i])
+
+
+@pytest.mark.parametrize("kv", KINDS)
+def test_store_prompt_load_in_a_graph(cuda_backend, kv):
+    """A prompt's store, attention and read-back captured together and replayed for another prompt, shorter, of
+    another sequence, with padding rows behind it."""
+    heads, nh, hd, n = 8, 32, 128, 200
+    b = bench(cuda_backend, kv, heads, hd, [n, n], fill="zeros")
+    g = torch.Generator(device=b.dev).manual_seed(3)
+    x = torch.randn(n, (nh + 2 * heads) * hd, device=b.dev, generator=g)
+    q, k, v = x.split([nh * hd, heads * hd, heads * hd], 1)
+    out, lse = torch.full((n, nh * hd), 7.0, device=b.dev), torch.full((n, nh), 7.0, device=b.dev)
+    kb, vb = torch.full((n, heads * hd), 7.0, device=b.dev), torch.full((n, heads * hd), 7.0, device=b.dev)
+    seq, pos = b.ints([0] * n), b.ints(range(n))
+    run, cu, start = b.ints([0]), b.ints([0, n]), b.ints([0])
+    sp = b.space(nh)
+
+    def call(stream):
+        b.kv.store(k.data_ptr(), v.data_ptr(), n, seq.data_ptr(), pos.data_ptr(), b.status.data_ptr(), ldk=x.stride(0),
+                   ldv=x.stride(0), stream=stream)
+        b.kv.prompt_attention(q.data_ptr(), out.data_ptr(), n, nh, 1, run.data_ptr(), cu.data_ptr(), start.data_ptr(),
+                              n, sp.data_ptr(), sp.numel(), b.status.data_ptr(), ldq=x.stride(0), lse=lse.data_ptr(),
+                              stream=stream)
+        b.kv.load(kb.data_ptr(), vb.data_ptr(), n, seq.data_ptr(), pos.data_ptr(), b.status.data_ptr(), stream=stream)
+
+    torch.cuda.synchronize()
+    graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream(b.dev)
+    with torch.cuda.graph(graph, stream=side):
+        call(torch.cuda.current_stream().cuda_stream)
+    for s, m in ((0, n), (1, 133)):
+        x.normal_(generator=g)
+        for t in (out, lse, kb, vb):
+            t.fill_(7.0)
+        seq.fill_(s)
+        pos[m:] = -1
+        run.fill_(s)
+        cu[1] = m
+        graph.replay()
+        torch.cuda.synchronize()
+        assert b.status.item() == 0
+        for i in (0, 63, 64, m - 1):
+            check_row(b, q[i], nh, s, i + 1, out[i], lse[i])
+        for kind, t in ((0, kb), (1, vb)):
+            torch.testing.assert_close(t[:m], b.c.rows(kind, s, list(range(m))).flatten(1).float(), rtol=0, atol=0)
+        for t in (out, lse, kb, vb):
+            assert (t[m:] == 7.0).all()
