@@ -95,6 +95,13 @@ __device__ __forceinline__ void mma_smem_a(uint32_t d, uint64_t a, uint64_t b, u
       "l"(a), "l"(b), "r"(desc), "r"((uint32_t)add)
       : "memory");
 }
+// One lane of a whole warp, known as such to the compiler: operands of what it
+// issues stay in uniform registers.
+__device__ __forceinline__ bool elected() {
+  uint32_t is;
+  asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}\n" : "=r"(is));
+  return is != 0;
+}
 __device__ __forceinline__ void mma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n" ::"r"(bar) : "memory");
 }
@@ -135,6 +142,39 @@ __device__ __forceinline__ void store_f32x8(float* p, const float* x) {
   asm volatile("st.global.v8.f32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};\n" ::"l"(p), "f"(x[0]), "f"(x[1]), "f"(x[2]), "f"(x[3]),
                "f"(x[4]), "f"(x[5]), "f"(x[6]), "f"(x[7])
                : "memory");
+}
+
+// Two f32 operations in one instruction, on neighbouring registers; each rounds
+// as the plain one does.
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};\n" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ float2 unpair(uint64_t x) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;\n" : "=f"(r.x), "=f"(r.y) : "l"(x));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;\n" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;\n" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;\n" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 // The order in which 8 neighbouring dimensions of I4 codes are widened: pairs (i, i + 4).
@@ -336,7 +376,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   before_sync();
   __syncthreads();
   after_sync();
-  const uint32_t tmem = tmem_slot;
+  const uint32_t tmem = __shfl_sync(0xffffffffu, tmem_slot, 0);
   const uint32_t tlane = tmem + ((uint32_t)((warp & 3) * 32) << 16);
   top = fmaxf(pair_a[0][row], pair_a[1][row]);
   qsum = __fadd_rn(pair_b[0][row], pair_b[1][row]);
@@ -458,7 +498,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       constexpr int kBack = T::kTwoS ? 2 : 1;
       if (!wait(keys_ready[j & 1], j / 2) || (j >= kBack && !wait(output_full, j - kBack))) return false;
       after_sync();
-      if (lane == 0) issue_scores(j);
+      if (elected()) issue_scores(j);
       __syncwarp();
       return true;
     };
@@ -467,7 +507,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       if (T::kTwoS && j + 1 < tiles && !scores(j + 1)) break;
       if (!wait(values_ready, j) || !wait(weights_ready[j & 1], j / 2)) break;
       after_sync();
-      if (lane == 0) issue_output(j);
+      if (elected()) issue_output(j);
       __syncwarp();
       if (!T::kTwoS && j + 1 < tiles) ok = scores(j + 1);
     }
@@ -553,16 +593,18 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       const int key0 = j * kKeys;
 #pragma unroll
       for (int i = 0; i < kKeys; i += 4) {
-        const float4 ks = *(const float4*)&pj[0][i];
-        const float k4[4] = {ks.x, ks.y, ks.z, ks.w};
-        float z4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        const ulonglong2 ks = *(const ulonglong2*)&pj[0][i];
+        uint64_t u = pair(s[i], s[i + 1]), v = pair(s[i + 2], s[i + 3]);
         if constexpr (I4) {
-          const float4 kz = *(const float4*)&pj[1][i];
-          z4[0] = kz.x, z4[1] = kz.y, z4[2] = kz.z, z4[3] = kz.w;
+          const ulonglong2 kz = *(const ulonglong2*)&pj[1][i];
+          u = fma2(u, ks.x, mul2(pair(qsum, qsum), kz.x));
+          v = fma2(v, ks.y, mul2(pair(qsum, qsum), kz.y));
+        } else {
+          u = mul2(u, ks.x);
+          v = mul2(v, ks.y);
         }
-#pragma unroll
-        for (int k = 0; k < 4; ++k)
-          s[i + k] = I4 ? __fmaf_rn(s[i + k], k4[k], __fmul_rn(qsum, z4[k])) : __fmul_rn(s[i + k], k4[k]);
+        const float2 x = unpair(u), y = unpair(v);
+        s[i] = x.x, s[i + 1] = x.y, s[i + 2] = y.x, s[i + 3] = y.y;
       }
       if (TWO && j > 0 && j % kSumTiles == 0) {  // the sums so far, to the output's place
         if (!wait(output_full, j - 1)) break;
@@ -589,7 +631,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       }
       float tops[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int i = 0; i < kKeys; ++i) tops[i % 4] = fmaxf(tops[i % 4], s[i]);
+      for (int i = 0; i < kKeys; i += 2) tops[i / 2 % 4] = max3(tops[i / 2 % 4], s[i], s[i + 1]);
       const float top_s = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       // a score above the slack, or a scale of V times 2^ev above 2^9
       const float vtop = fmaxf(pj[2][lane], pj[2][lane + 32]);
@@ -622,34 +664,38 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
         }
       }
       // weights, over the scores; a key that the row does not see weighs nothing, whatever its scale
-      float l_tile = 0.0f, z_tile = 0.0f;  // a tile's sums by themselves: a long context's would lose their small terms
+      uint64_t l_tile = 0, z_tile = 0;  // a tile's sums by themselves: a long context's would lose their small terms
       auto weigh = [&](auto some_hidden) {
 #pragma unroll
         for (int i = 0; i < kKeys; i += 16) {
           uint32_t hi[8], lo[8];
 #pragma unroll
           for (int n = 0; n < 16; n += 4) {
-            const float4 vs = *(const float4*)&pj[2][i + n];
-            const float v4[4] = {vs.x, vs.y, vs.z, vs.w};
-            float z4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-            if constexpr (I4) {
-              const float4 vz = *(const float4*)&pj[3][i + n];
-              z4[0] = vz.x, z4[1] = vz.y, z4[2] = vz.z, z4[3] = vz.w;
-            }
-            float p[4];
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-              const float w = exp2_approx(__fmaf_rn(s[i + n + k], qs, -mq));
-              l_tile = __fadd_rn(l_tile, w);
-              const bool hidden = decltype(some_hidden)::value && key0 + i + n + k >= limit_pos;
-              if constexpr (I4) z_tile = hidden ? z_tile : __fmaf_rn(w, z4[k], z_tile);
-              p[k] = hidden ? 0.0f : __fmul_rn(w, v4[k]);
-            }
+            const ulonglong2 vs = *(const ulonglong2*)&pj[2][i + n];
+            ulonglong2 vz = make_ulonglong2(0, 0);
+            if constexpr (I4) vz = *(const ulonglong2*)&pj[3][i + n];
 #pragma unroll
             for (int k = 0; k < 2; ++k) {
-              const uint32_t h = pack_f16(p[2 * k], p[2 * k + 1]);
+              const int at = i + n + 2 * k;
+              const float2 x = unpair(fma2(pair(s[at], s[at + 1]), pair(qs, qs), pair(-mq, -mq)));
+              const uint64_t w = pair(exp2_approx(x.x), exp2_approx(x.y));
+              l_tile = add2(l_tile, w);
+              uint64_t scale = k ? vs.y : vs.x, zero = k ? vz.y : vz.x;
+              if constexpr (decltype(some_hidden)::value) {
+                const bool h0 = key0 + at >= limit_pos, h1 = key0 + at + 1 >= limit_pos;
+                const float2 a = unpair(scale), b = unpair(zero);
+                scale = pair(h0 ? 0.0f : a.x, h1 ? 0.0f : a.y);
+                zero = pair(h0 ? 0.0f : b.x, h1 ? 0.0f : b.y);
+              }
+              if constexpr (I4) z_tile = fma2(w, zero, z_tile);
+              const uint64_t p = mul2(w, scale);
+              const float2 f = unpair(p);
+              const uint32_t h = pack_f16(f.x, f.y);
               hi[n / 2 + k] = h;
-              if (TWO) lo[n / 2 + k] = pack_f16(__fsub_rn(p[2 * k], f16_lo(h)), __fsub_rn(p[2 * k + 1], f16_hi(h)));
+              if (TWO) {
+                const float2 r = unpair(add2(p, pair(-f16_lo(h), -f16_hi(h))));
+                lo[n / 2 + k] = pack_f16(r.x, r.y);
+              }
             }
           }
           tmem_st8(s_at + i / 2, hi);
@@ -660,8 +706,9 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
         weigh(std::true_type{});
       else
         weigh(std::false_type{});
-      l = __fadd_rn(l, l_tile);
-      zsum = __fadd_rn(zsum, z_tile);
+      const float2 lt = unpair(l_tile), zt = unpair(z_tile);
+      l = __fadd_rn(l, __fadd_rn(lt.x, lt.y));
+      if (I4) zsum = __fadd_rn(zsum, __fadd_rn(zt.x, zt.y));
       tmem_wait_st();
       before_sync();
       arrive(weights_ready[j & 1]);
