@@ -421,11 +421,15 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       const int at = i * kWiden + (tid - 128);
       if (kKeys * kPieces % kWiden != 0 && at >= kKeys * kPieces) break;
       const int key = at / kPieces, piece = at % kPieces;
-      uint4 p[4];
-      widen<I4>(*(const uint4*)(raw + key / kPage * T::kBlock + (kind * kPage + key % kPage) * T::kRow + piece * 16), p);
+      uint4 p[4], u = *(const uint4*)(raw + key / kPage * T::kBlock + (kind * kPage + key % kPage) * T::kRow + piece * 16);
+      // lanes whose pieces go to the second 64 elements write the halves of their output the other way round: eight
+      // lanes then write to eight places of a line, not to four
+      const bool turn = HD > 64 && piece >= kPieces / 2;
+      if (turn) u = make_uint4(u.z, u.w, u.x, u.y);
+      widen<I4>(u, p);
 #pragma unroll
       for (int k = 0; k < kOut; ++k) {
-        const int to = piece * kOut + k;  // 16-byte piece of the widened row
+        const int to = piece * kOut + (turn ? k ^ (kOut / 2) : k);  // 16-byte piece of the widened row
         *(uint4*)(dst + to / 8 * (kKeys * 128) + key * 128 + (((to % 8) ^ (key & 7)) << 4)) = p[k];
       }
     }
