@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     kvq_prompt_kernel(KvqView c, KvqRows R, KvqAttend a, int max_len, int wide_q, int wide_out) {
   using T = PromptTile<HD, I4, TWO>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ __align__(8) uint64_t pages_full[T::kStages], pages_empty[T::kStages];
+  __shared__ __align__(8) uint64_t pages_full[T::kStages];
   __shared__ __align__(8) uint64_t keys_ready[2], scores_full[2], weights_ready[2], values_ready, output_full, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up, found_run, found_tile;
@@ -253,10 +253,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       found_run = run;
       found_tile = left;
       gave_up = 0;
-      for (int i = 0; i < T::kStages; ++i) {
-        mbar_init(smem_u32(&pages_full[i]), 1);
-        mbar_init(smem_u32(&pages_empty[i]), kWiden / 32);
-      }
+      for (int i = 0; i < T::kStages; ++i) mbar_init(smem_u32(&pages_full[i]), 1);
       for (int i = 0; i < 2; ++i) {
         mbar_init(smem_u32(&keys_ready[i]), kWiden / 32);
         mbar_init(smem_u32(&scores_full[i]), 1);
@@ -311,22 +308,20 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
                  : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;\n" ::: "memory");
   }
-  // one tile's pages, by warp 4; next_page is the lane's page of the tile after the last one asked for
+  // one tile's pages, by warp 7; next_page is the lane's page of the tile after the last one asked for
   int next_page = 0;
   auto look_up = [&](int j) {
     const int at = j * kTilePages + lane;
     next_page = 0;
-    if (lane < kTilePages && at * kPage < seen) {
-      next_page = c.table[(size_t)seq * c.per_seq + at];
-      if ((unsigned)next_page >= (unsigned)c.pages) {
-        atomicOr(a.status, kStatusBadContext);
-        next_page = 0;
-      }
-    }
+    if (lane < kTilePages && at * kPage < seen) next_page = c.table[(size_t)seq * c.per_seq + at];
   };
   auto fetch = [&](int j) {
     const int stage = j % T::kStages, pages = min(kTilePages, (seen + kPage - 1) / kPage - j * kTilePages);
     const uint32_t bar = smem_u32(&pages_full[stage]);
+    if ((unsigned)next_page >= (unsigned)c.pages) {  // looked at here, where it is used: the load has had a tile's time
+      atomicOr(a.status, kStatusBadContext);
+      next_page = 0;
+    }
     const int page = next_page;
     if (lane == 0) mbar_expect_tx(bar, pages * T::kBlock);
     __syncwarp();
@@ -335,7 +330,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
                 c.pool + ((size_t)page * c.kv_heads + kvh) * T::kBlock, T::kBlock, bar);
     look_up(j + 1);
   };
-  if (warp == 4) {
+  if (warp == 7) {
     look_up(0);
     for (int j = 0; j < min(tiles, T::kStages); ++j) fetch(j);
   }
@@ -509,7 +504,9 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     bool ok = scores(0);
     for (int j = 0; j < tiles && ok; ++j) {
       if (T::kTwoS && j + 1 < tiles && !scores(j + 1)) break;
-      if (!wait(values_ready, j) || !wait(weights_ready[j & 1], j / 2)) break;
+      if (!wait(values_ready, j)) break;
+      if (j + T::kStages < tiles) fetch(j + T::kStages);  // the tile's codes have been widened
+      if (!wait(weights_ready[j & 1], j / 2)) break;
       after_sync();
       if (elected()) issue_output(j);
       __syncwarp();
@@ -528,11 +525,6 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       widen_tile(j, 1, v_tile);
       asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
       arrive(values_ready);
-      arrive(pages_empty[stage]);
-      if (warp == 4 && j + T::kStages < tiles) {
-        if (!wait(pages_empty[stage], use)) break;
-        fetch(j + T::kStages);
-      }
     }
   } else {
     // ---- weighing ----
