@@ -24,20 +24,24 @@
 // passes the row's maximum by kSlack (log2) or a scale of V grows too much, as
 // in the single-token kernel; the weights' power of two is folded into the
 // maximum, so that it divides out of the result.  Warps 4-6 widen the next
-// tile's K and this tile's V, and fetch pages kStages tiles ahead (their
-// numbers one tile before that).  Warp 7 issues the products.  They meet at
+// tile's K and this tile's V.  Warp 7 issues the products, and fetches pages
+// kStages tiles ahead (their numbers one tile before that).  They meet at
 // mbarriers only:
 //   keys_ready    K widened, and its keys' parameters staged    3 warps
 //   scores_full   S computed (K's tile is free)                 commit
 //   weights_ready W written                                     4 warps
 //   values_ready  V widened                                     3 warps
 //   output_full   O summed (V's tile, W and S are free)         commit
-//   pages_empty   a tile's pages have been widened              3 warps
-// The first three alternate between two barriers a kind: with one, a phase that
+// The first three have several barriers a kind, in turn: with one, a phase that
 // a warp has yet to look at could be followed by the next.
-// Two CTAs share an SM, so each has half of its tensor memory: O, S, and what
-// is left for Q (its first term).  Heads of 64 leave room for a second S, which
-// is computed while the first is weighed.
+// Two CTAs share an SM, so each has half of its tensor memory.  With a second S
+// the next tile's scores are computed while a tile is weighed, K's widening
+// running a tile ahead of V's.  Heads of 64 have room for it beside O and Q
+// (its first term).  Heads of 128 have it where Q is one term and the codes are
+// small enough that Q fits into shared memory beside four tiles of pages (with
+// two tiles, as I8 would have, pages come too late: 275 against 267 us for 4
+// ragged prompts of 6 to 9 thousand rows; I4 gains, 281 to 258 us, and heads of
+// 64 232 to 195 us).
 //
 // Every wait is bounded; a CTA that gives up records it, waits (bounded) for
 // its copies and products and frees its tensor memory.
@@ -61,12 +65,15 @@ struct PromptTile {
   static constexpr int kBlock = 2 * kPage * kRow + (I4 ? 256 : 128);
   static constexpr int kAtoms = (HD + 63) / 64;  // 64 elements of fp16 are a 128-byte line
   static constexpr int kOperand = kAtoms * kKeys * 128;
-  static constexpr bool kTwoS = HD <= 64;  // two buffers of scores
+  static constexpr bool kTwoS = HD <= 64 || (I4 && !TWO);  // two buffers of scores
+  static constexpr bool kSharedQ = HD > 64 && kTwoS;       // Q (its one term) in shared memory
   static constexpr uint32_t kTmemS = HD, kTmemQ = HD + (kTwoS ? 2 : 1) * kKeys;  // O begins at 0
-  static_assert(kTmemQ + HD / 2 <= kTmemCols, "half of an SM's tensor memory");
-  static constexpr int kQ = TWO ? kAtoms * kPromptRows * 128 : 0;  // Q's second term
+  static_assert(kTmemQ + (kSharedQ ? 0 : HD / 2) <= kTmemCols, "half of an SM's tensor memory");
+  static constexpr int kQ = TWO || kSharedQ ? kAtoms * kPromptRows * 128 : 0;  // Q's second term, or Q
   static constexpr int kRaw = kTilePages * kBlock;
   static constexpr int kStages = TWO && HD > 64 && !I4 ? 2 : 4;  // tiles of pages
+  static constexpr int kLag = kTwoS ? 1 : 0;                     // tiles by which V is widened behind K
+  static constexpr int kTurns = kTwoS ? 4 : 2;                   // tiles whose parameters, or K's barrier, are kept apart
   static constexpr int kSmem = 1024 + 2 * kOperand + kQ + kStages * kRaw;
 };
 
@@ -213,10 +220,10 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   using T = PromptTile<HD, I4, TWO>;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   __shared__ __align__(8) uint64_t pages_full[T::kStages];
-  __shared__ __align__(8) uint64_t keys_ready[2], scores_full[2], weights_ready[2], values_ready, output_full, drained;
+  __shared__ __align__(8) uint64_t keys_ready[T::kTurns], scores_full[2], weights_ready[2], values_ready, output_full, drained;
   __shared__ uint32_t tmem_slot;
   __shared__ int gave_up, found_run, found_tile;
-  __shared__ __align__(16) float par[2][4][kKeys];  // of a tile's keys: K scale and zero, V scale and zero
+  __shared__ __align__(16) float par[T::kTurns][4][kKeys];  // of a tile's keys: K scale and zero, V scale and zero
   __shared__ float pair_a[2][kPromptRows], pair_b[2][kPromptRows], pair_c[2][kPromptRows];
   const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
   // in the prologue two threads share a row of Q, half of it each
@@ -254,8 +261,8 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       found_tile = left;
       gave_up = 0;
       for (int i = 0; i < T::kStages; ++i) mbar_init(smem_u32(&pages_full[i]), 1);
+      for (int i = 0; i < T::kTurns; ++i) mbar_init(smem_u32(&keys_ready[i]), kWiden / 32);
       for (int i = 0; i < 2; ++i) {
-        mbar_init(smem_u32(&keys_ready[i]), kWiden / 32);
         mbar_init(smem_u32(&scores_full[i]), 1);
         mbar_init(smem_u32(&weights_ready[i]), 4);
       }
@@ -396,14 +403,15 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
         hi[4 * g + k] = pack_f16(u, v);
         if (TWO) lo[k] = pack_f16(__fsub_rn(u, f16_lo(hi[4 * g + k])), __fsub_rn(v, f16_hi(hi[4 * g + k])));
       }
-      if (TWO) {
+      if (TWO || T::kSharedQ) {
         const int d = half * (HD / 2) + i + 8 * g, piece = (d % 64) / 8;
+        const uint32_t* x16 = TWO ? lo : hi + 4 * g;
         *(uint4*)(q_tile + d / 64 * (kPromptRows * 128) + row * 128 + ((piece ^ (row & 7)) << 4)) =
-            make_uint4(lo[0], lo[1], lo[2], lo[3]);
+            make_uint4(x16[0], x16[1], x16[2], x16[3]);
       }
     }
     __syncwarp();
-    tmem_st8(tlane + T::kTmemQ + half * (HD / 4) + i / 2, hi);
+    if (!T::kSharedQ) tmem_st8(tlane + T::kTmemQ + half * (HD / 4) + i / 2, hi);
   }
   tmem_wait_st();
 
@@ -435,10 +443,10 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       const float* p = (const float*)(raws + j % T::kStages * T::kRaw + key / kPage * T::kBlock + 2 * kPage * T::kRow) + key % kPage;
       // behind the context the bytes may be anything
       const bool live = j * kKeys + key < seen;
-      par[j & 1][0][key] = live ? p[0] : 0.0f;
-      par[j & 1][1][key] = I4 && live ? __fmaf_rn(kNibbleMid, p[0], p[kPage]) : 0.0f;
-      par[j & 1][2][key] = live ? p[I4 ? 2 * kPage : kPage] : 0.0f;
-      par[j & 1][3][key] = I4 && live ? __fmaf_rn(kNibbleMid, p[2 * kPage], p[3 * kPage]) : 0.0f;
+      par[j % T::kTurns][0][key] = live ? p[0] : 0.0f;
+      par[j % T::kTurns][1][key] = I4 && live ? __fmaf_rn(kNibbleMid, p[0], p[kPage]) : 0.0f;
+      par[j % T::kTurns][2][key] = live ? p[I4 ? 2 * kPage : kPage] : 0.0f;
+      par[j % T::kTurns][3][key] = I4 && live ? __fmaf_rn(kNibbleMid, p[2 * kPage], p[3 * kPage]) : 0.0f;
     }
   };
   auto scores_at = [&](int j) -> uint32_t { return T::kTmemS + (T::kTwoS && (j & 1) ? kKeys : 0); };
@@ -447,14 +455,15 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   auto issue_scores = [&](int j) {
     const uint32_t d = tmem + scores_at(j);
     auto k_at = [&](int k) { return operand(smem_u32(k_tile) + k / 4 * (kKeys * 128) + k % 4 * 32, 16); };
-    if (TWO)
+    if (TWO || T::kSharedQ)
 #pragma unroll
       for (int k = 0; k < HD / 16; ++k)
         mma_smem_a(d, operand(smem_u32(q_tile) + k / 4 * (kPromptRows * 128) + k % 4 * 32, 16), k_at(k),
                    product(kKeys, 0), k > 0);
+    if (!T::kSharedQ)
 #pragma unroll
-    for (int k = 0; k < HD / 16; ++k)
-      mma_tmem_a(d, tmem + T::kTmemQ + 8 * k, k_at(k), product(kKeys, 0), TWO || k > 0);
+      for (int k = 0; k < HD / 16; ++k)
+        mma_tmem_a(d, tmem + T::kTmemQ + 8 * k, k_at(k), product(kKeys, 0), TWO || k > 0);
     mma_commit(smem_u32(&scores_full[j & 1]));
   };
   auto issue_output = [&](int j) {
@@ -495,7 +504,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     // scores of tile j into the buffer that held the weights of tile j - 2 (two buffers) or j - 1
     auto scores = [&](int j) {
       constexpr int kBack = T::kTwoS ? 2 : 1;
-      if (!wait(keys_ready[j & 1], j / 2) || (j >= kBack && !wait(output_full, j - kBack))) return false;
+      if (!wait(keys_ready[j % T::kTurns], j / T::kTurns) || (j >= kBack && !wait(output_full, j - kBack))) return false;
       after_sync();
       if (elected()) issue_scores(j);
       __syncwarp();
@@ -514,17 +523,21 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     }
   } else if (warp >= 4) {
     // ---- widening ----
-    for (int j = 0; j < tiles; ++j) {
-      const int stage = j % T::kStages, use = j / T::kStages;
-      if (!wait(pages_full[stage], use) || (j > 0 && !wait(scores_full[(j - 1) & 1], (j - 1) / 2))) break;
-      stage_params(j);
-      widen_tile(j, 0, k_tile);
-      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      arrive(keys_ready[j & 1]);
-      if (j > 0 && !wait(output_full, j - 1)) break;
-      widen_tile(j, 1, v_tile);
-      asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
-      arrive(values_ready);
+    for (int j = 0; j < tiles + T::kLag; ++j) {
+      if (j < tiles) {
+        if (!wait(pages_full[j % T::kStages], j / T::kStages) || (j > 0 && !wait(scores_full[(j - 1) & 1], (j - 1) / 2))) break;
+        stage_params(j);
+        widen_tile(j, 0, k_tile);
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        arrive(keys_ready[j % T::kTurns]);
+      }
+      const int v = j - T::kLag;
+      if (v >= 0) {
+        if (v > 0 && !wait(output_full, v - 1)) break;
+        widen_tile(v, 1, v_tile);
+        asm volatile("fence.proxy.async.shared::cta;\n" ::: "memory");
+        arrive(values_ready);
+      }
     }
   } else {
     // ---- weighing ----
@@ -578,14 +591,14 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       }
     };
     for (int j = 0; j < tiles; ++j) {
-      if (!wait(keys_ready[j & 1], j / 2) || !wait(scores_full[j & 1], j / 2)) break;
+      if (!wait(keys_ready[j % T::kTurns], j / T::kTurns) || !wait(scores_full[j & 1], j / 2)) break;
       after_sync();
       const uint32_t s_at = tlane + scores_at(j);
       float s[kKeys];
 #pragma unroll
       for (int i = 0; i < kKeys; i += 16) tmem_ld16(s_at + i, (uint32_t*)s + i);
       tmem_wait_ld();
-      const float(*pj)[kKeys] = par[j & 1];
+      const float(*pj)[kKeys] = par[j % T::kTurns];
       const int key0 = j * kKeys;
 #pragma unroll
       for (int i = 0; i < kKeys; i += 4) {
