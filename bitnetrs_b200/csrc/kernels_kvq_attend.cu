@@ -1130,15 +1130,15 @@ LaunchMma mma_for(const KvqView& c, int heads) {
 }
 }  // namespace
 
-const char* kvq_attend_kernel_name(const KvqView& c, const KvqRows& r, int nh) {
-  if (kvq_prompt_pays(c, r, nh)) return "kvq_prompt_kernel";
+const char* kvq_attend_kernel_name(const KvqView& c, const KvqRows& r, int nh, bool bf16) {
+  if (kvq_prompt_pays(c, r, nh, bf16)) return "kvq_prompt_kernel";
   return mma_for(c, units_of(nh, c.kv_heads).heads) ? "kvq_attend_mma_kernel" : "kvq_attend_plain_kernel";
 }
 
 void launch_kvq_attend(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st) {
   if (r.rows <= 0) return;
   const Units us = units_of(a.nh, c.kv_heads);
-  if (kvq_prompt_pays(c, r, a.nh)) {
+  if (kvq_prompt_pays(c, r, a.nh, a.bf16)) {
     launch_kvq_prompt(c, r, a, max_len, st);
     return;
   }

@@ -33,15 +33,20 @@
 //   values_ready  V widened                                     3 warps
 //   output_full   O summed (V's tile, W and S are free)         commit
 // The first three have several barriers a kind, in turn: with one, a phase that
-// a warp has yet to look at could be followed by the next.
+// a warp has yet to look at could be followed by the next.  A wait for a
+// phase must begin after the phase before has ended and before the next one can
+// end.  Every warp waits for each phase in turn, but for output_full the warps
+// that weigh: before they arrive with the weights of tile j, O of tile j cannot
+// be complete, and O of tile j - 1 (one buffer of S) or j - 2 (two) is, for S of
+// tile j was issued after it.
 // Two CTAs share an SM, so each has half of its tensor memory.  With a second S
 // the next tile's scores are computed while a tile is weighed, K's widening
 // running a tile ahead of V's.  Heads of 64 have room for it beside O and Q
 // (its first term).  Heads of 128 have it where Q is one term and the codes are
 // small enough that Q fits into shared memory beside four tiles of pages (with
 // two tiles, as I8 would have, pages come too late: 275 against 267 us for 4
-// ragged prompts of 6 to 9 thousand rows; I4 gains, 281 to 258 us, and heads of
-// 64 232 to 195 us).
+// ragged prompts, 6600 rows in all; I4 gains, 281 to 270 us, and heads of
+// 64 232 to 195 us, before the wait that the last tile then needs).
 //
 // Every wait is bounded; a CTA that gives up records it, waits (bounded) for
 // its copies and products and frees its tensor memory.
@@ -720,6 +725,9 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       if (I4) zsum = __fadd_rn(zsum, __fadd_rn(zt.x, zt.y));
       tmem_wait_st();
       before_sync();
+      // the last wait below must not take the phase before the last for its own; that one cannot end
+      // before this arrival, and the one before it has ended
+      if (T::kTwoS && j > 0 && j == tiles - 1 && !wait(output_full, j - 1)) break;
       arrive(weights_ready[j & 1]);
     }
     wait(output_full, tiles - 1);
@@ -789,16 +797,16 @@ void launch_prompt_of(const KvqView& c, const KvqRows& r, const KvqAttend& a, in
 
 // Runs of rows are taken here where that is the faster way.  For 64 positions
 // of every row's context a CTA of this kernel takes 1.6 us by itself and an SM
-// with two of them 1.3 us a CTA; the single-token kernel takes 64 positions of
-// one unit in 1.9 ns of the whole GPU (heads of 128, up to four a unit).
-// Measured: 1024 tokens of a fresh prompt with 5 units 51 against 135 us, 32
-// tokens behind 8000 positions 242 against some 60 us.
-bool kvq_prompt_pays(const KvqView& c, const KvqRows& r, int nh) {
+// with two of them 1.2 us a CTA (f32 rows 2.4 and 2.1 us); the single-token
+// kernel takes 64 positions of one unit in 1.9 ns of the whole GPU (heads of
+// 128, up to four a unit).  Measured: 1024 f32 rows of a fresh prompt with 5
+// units 48 against 135 us; 32 rows behind 8000 positions 242 against some 60 us.
+bool kvq_prompt_pays(const KvqView& c, const KvqRows& r, int nh, bool bf16) {
   if (!r.runs || (c.hd != 64 && c.hd != 128)) return false;
   const Units us = units_of(nh, c.kv_heads);
   const double ctas = ((double)r.rows / (kPromptRows / us.heads) + r.runs) * us.per_row;
   if (ctas > (double)INT_MAX) return false;
-  return std::max(1.6, 1.3 * ctas / 148) < 1.9e-3 * r.rows * us.per_row;
+  return std::max(bf16 ? 1.6 : 2.4, (bf16 ? 1.2 : 2.1) * ctas / 148) < 1.9e-3 * r.rows * us.per_row;
 }
 
 void launch_kvq_prompt(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st) {

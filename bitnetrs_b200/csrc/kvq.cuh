@@ -82,8 +82,8 @@ size_t kvq_attend_space(int nh, int kv_heads, int hd);
 void launch_kvq_attend(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st);
 // Runs of rows on the tensor cores, 128 / (heads a unit) tokens a CTA
 // (kernels_kvq_prompt.cu); launch_kvq_attend chooses it.
-bool kvq_prompt_pays(const KvqView& c, const KvqRows& r, int nh);
+bool kvq_prompt_pays(const KvqView& c, const KvqRows& r, int nh, bool bf16);
 void launch_kvq_prompt(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st);
-const char* kvq_attend_kernel_name(const KvqView& c, const KvqRows& r, int nh);
+const char* kvq_attend_kernel_name(const KvqView& c, const KvqRows& r, int nh, bool bf16);
 
 }  // namespace bitnet

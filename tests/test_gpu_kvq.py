@@ -688,6 +688,28 @@ def test_long_sums_keep_their_accuracy(cuda_backend, nh, heads, hd, kv, shift):
         assert (wide[:, :shift] == 9.0).all() and (wide[:, shift + nh * hd:] == 9.0).all()
 
 
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [128, 64])
+def test_prompt_attention_repeats_itself(cuda_backend, hd, kv, io):
+    """A prompt of many more CTAs than the GPU holds, whose warps get in one another's way, gives the same bits every
+    time, and every row what the single-token operator gives (bf16: within a weight's fp16 and the output's bf16)."""
+    nh, heads, n = 32, 8, 2500
+    b = bench(cuda_backend, kv, heads, hd, [n], seed=3)
+    q = torch.randn(n, nh * hd, device=b.dev, generator=torch.Generator(device=b.dev).manual_seed(5)).to(DT[io])
+    first, lse = b.prompt(q, nh, [0], [0, n], [0])
+    for _ in range(25):
+        again, lse2 = b.prompt(q, nh, [0], [0, n], [0])
+        assert torch.equal(first, again) and torch.equal(lse, lse2)
+    one, _ = b.attend(q, nh, [0] * n, list(range(1, n + 1)))
+    # f32: both within 32-bit sums of the same, below 2^-15 of max |v|; bf16: a step of each output, and the weights' 2^-11
+    vmax = b.c.rows(1, 0, list(range(n))).abs().max().item()
+    off = (first.double() - one.double()).abs() - 2.0**-15 * vmax
+    if io == "bf16":
+        off = off - 2.0**-7 * one.double().abs() - 2.0**-11 * vmax
+    assert (off <= 0).all()
+
+
 @pytest.mark.parametrize("kv", KINDS)
 @pytest.mark.parametrize("hd", [128, 64, 32, 80])
 def test_attention_of_large_keys_and_values(cuda_backend, hd, kv):
