@@ -252,13 +252,15 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 }
 
 // ---------------------------------------------------------------------------
-// The tensor-core form, for head sizes of 64, 96 and 128 (I4: 64, 128).
+// The tensor-core form, for heads of 32, 64, 96 and 128.
 //
 // One warp multiplies a page (two of them in turn), its 16 positions (scores) or 16
 // dimensions (output) being the M of a product, and four heads its N.
 //   S[pos][head] = K codes . q        m16n8k32, 8-bit integers
 //   O[dim][head] += V codes^T . w     m16n8k16, fp16 with f32 sums
-// Scores: codes go into the product as they lie in memory.  q is held as a
+// Scores: codes go into the product as they lie in memory (I4: as 16 (c - 8),
+// with zero + 8 scale for the zero, so that neither part of a score outgrows
+// it).  q is held as a
 // 31-bit integer a dimension (relative to the head's largest element) in four
 // balanced digits of base 256, one column each, so that the integer products
 // are exact and a head's four columns, two in each of two products, are the
@@ -278,20 +280,21 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // of 128-byte lines with their 16-byte pieces exchanged (128-byte swizzle), so
 // that loads of 8 rows x 16 bytes meet no bank twice, and the parameters with
 // them or by themselves.
-// Measured on a batch of 256 contexts of 128 to 4096 (I8), with the same bytes
-// asked for ahead: copies by each lane (cp.async) stop at 4.0 TB/s, since a
-// load that goes through L1 needs an entry there until it lands.
+// Measured on a batch of 256 contexts of 128 to 4096 (20 heads over 5, heads of
+// 128, I8), with the same bytes asked for ahead: copies by each lane (cp.async)
+// stop at 4.0 TB/s, since a load that goes through L1 needs an entry there
+// until it lands; the ring takes 129 us, 5.2 TB/s, and 100003 positions of one
+// sequence as I4 43 us, 2.7 TB/s, where instructions and the ends are the bound.
 //
 // Here the line of pages is cut into equal shares for the warps, not the
 // CTAs, so that no warp waits for another before its share is done.  The warps
 // of a CTA hold neighbouring shares: at the end the CTA joins the units that
 // its warps cut, and leaves to the join kernel those that CTAs cut.
 //
-// The order of dimensions inside a product is free, so a lane fetches wide
-// pieces of a row for its K operand (HD/4 codes of two rows, the four lanes of
-// a row side by side) and its V operand (HD/8 codes of four rows).  They come
-// by cp.async into a ring that only the same lane reads, so a warp waits for
-// its own copies alone.
+// The order of dimensions inside a product is free, so the words that ldmatrix
+// leaves in a lane (V's transposed: two positions' bytes of a dimension) go into
+// the products as they are; q, and the output as it is written, are in the order
+// that this gives.
 // ---------------------------------------------------------------------------
 constexpr int kMmaMaxWarps = 8;
 constexpr int kMmaShares = 296;  // two CTAs an SM with up to four heads a unit, else one

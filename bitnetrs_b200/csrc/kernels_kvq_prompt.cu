@@ -45,7 +45,7 @@
 // (its first term).  Heads of 128 have it where Q is one term and the codes are
 // small enough that Q fits into shared memory beside four tiles of pages (with
 // two tiles, as I8 would have, pages come too late: 275 against 267 us for 4
-// ragged prompts, 6600 rows in all; I4 gains, 281 to 270 us, and heads of
+// ragged prompts, 4500 rows in all; I4 gains, 281 to 270 us, and heads of
 // 64 232 to 195 us, before the wait that the last tile then needs).
 //
 // Every wait is bounded; a CTA that gives up records it, waits (bounded) for
