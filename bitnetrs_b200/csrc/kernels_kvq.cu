@@ -32,7 +32,7 @@ namespace {
 // t = x / scale is off by less than 127 * 3 * 2^-24 < 2^-15, so rint(t) is the
 // code unless t lies that close to a border; there the quotient is taken in 64
 // bits, and the remainder of the code it gives (one fma, exact at a border)
-// decides.  A rotated element is held in 64 bits: its two products are exact
+// decides.  Away from borders t is at most the largest code and a rounding.  A rotated element is held in 64 bits: its two products are exact
 // there and their sum is rounded once.
 //
 // Bound by memory for many rows (the rows read once, the codes written once)
@@ -48,12 +48,26 @@ __device__ __noinline__ int border_code(double x, double scale, int least, int m
     c -= 1.0;
   return min(max((int)c, least), most);
 }
-// `x` is what is divided: an element (I8), or an element less the zero (I4).
-__device__ __forceinline__ int nearest_code(double x, float xf, float scale, float inv, int least, int most) {
-  const float t = __fmul_rn(xf, inv), c = rintf(t);
-  // a scale so small that its reciprocal is not finite, or t, also goes the long way
-  if (!(fabsf(__fsub_rn(t, c)) < 0.4999f)) return border_code(x, scale, least, most);
-  return min(max((int)c, least), most);
+// x / scale as the sum with 1.5 * 2^23, whose rounding is that to the nearest
+// integer, ties to even: the code is in its low bits.  *off is raised to the
+// quotient's distance from it, or becomes NaN (a scale so small that its
+// reciprocal is not finite): unless it stays below 0.4999 the codes are looked
+// at again.
+constexpr uint32_t kCodeBits = 0x4b400000u;
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ float min_nan(float a, float b) {
+  float r;
+  asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t code_bits(float x, float inv, float* off) {
+  const float t = __fmul_rn(x, inv), f = __fadd_rn(t, __uint_as_float(kCodeBits));
+  *off = max_nan(*off, fabsf(__fsub_rn(t, __fsub_rn(f, __uint_as_float(kCodeBits)))));
+  return __float_as_uint(f);
 }
 
 // N elements from x[i] on, in wide loads where `wide` says that they are aligned.
@@ -177,14 +191,14 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
   double v[ROPE ? kRuns : 1][N];  // elements in 64 bits, where 32 do not hold them
   float top = I4 ? -INFINITY : 0.0f, low = INFINITY;  // the largest x (I4) or |x| (I8), the least x
   double top64 = top, low64 = low;
-  bool finite = true;
+  int bad = 0;
 #pragma unroll
   for (int i = 0; i < kRuns; ++i)
 #pragma unroll
     for (int j = 0; j < N; ++j) {
-      const int d = N * (in + 32 * i) + j;
+      const int run = N * (in + 32 * i), d = run + j;
       if (ROPE) v[i][j] = x[i][j];
-      if (!on || d >= hd) continue;
+      if (!on || run >= hd) continue;  // runs lie in a row whole
       if (ROPE) {
         if (kind == 0) {
           const double a = __dmul_rn(x[i][j], cs[i][j]), b = __dmul_rn(w[i][j], sn[i][j]);
@@ -193,26 +207,26 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
         }
         top64 = fmax(top64, I4 ? v[i][j] : fabs(v[i][j]));
         if (I4) low64 = fmin(low64, v[i][j]);
+        bad |= !isfinite(x[i][j]);
       } else {
-        top = fmaxf(top, I4 ? x[i][j] : fabsf(x[i][j]));
-        if (I4) low = fminf(low, x[i][j]);
+        top = max_nan(top, I4 ? x[i][j] : fabsf(x[i][j]));
+        if (I4) low = min_nan(low, x[i][j]);
       }
-      finite &= isfinite(x[i][j]) != 0;
     }
   float zero = 0.0f, scale;
-  int bad = !finite;
   for (int o = group / 2; o; o >>= 1) {
-    bad |= __shfl_xor_sync(0xffffffffu, bad, o);
     if (ROPE) {
+      bad |= __shfl_xor_sync(0xffffffffu, bad, o);
       top64 = fmax(top64, __shfl_xor_sync(0xffffffffu, top64, o));
       if (I4) low64 = fmin(low64, __shfl_xor_sync(0xffffffffu, low64, o));
     } else {
-      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-      if (I4) low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
+      top = max_nan(top, __shfl_xor_sync(0xffffffffu, top, o));
+      if (I4) low = min_nan(low, __shfl_xor_sync(0xffffffffu, low, o));
     }
   }
   if (!on) return;
   if (!ROPE) {
+    bad = !isfinite(top) || (I4 && !isfinite(low));
     top64 = top;
     low64 = low;
   }
@@ -236,17 +250,32 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
     const int d = N * (in + 32 * i);
     if (d >= hd) continue;
     uint32_t word[4] = {0u, 0u, 0u, 0u};
-    if (!bad && scale > 0.0f)
+    if (!bad && scale > 0.0f) {
+      // what is divided: an element (I8), or an element less the zero (I4)
+      auto part = [&](int j) { return I4 ? (ROPE ? (float)(v[i][j] - (double)zero) : __fsub_rn(x[i][j], zero)) : x[i][j]; };
+      uint32_t bits[N];
+      float off = 0.0f;
+#pragma unroll
+      for (int j = 0; j < N; ++j) bits[j] = code_bits(part(j), inv, &off);
+      if (!(off < 0.4999f)) {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          float mine = 0.0f;
+          code_bits(part(j), inv, &mine);
+          if (!(mine < 0.4999f))
+            bits[j] = kCodeBits + border_code((ROPE ? v[i][j] : (double)x[i][j]) - (double)zero, scale, I4 ? 0 : -127, I4 ? 15 : 127);
+        }
+      }
 #pragma unroll
       for (int j = 0; j < N; ++j) {
-        const double y = ROPE ? v[i][j] - (double)zero : (double)x[i][j] - (double)zero;
-        const float yf = I4 ? (ROPE ? (float)y : __fsub_rn(x[i][j], zero)) : x[i][j];
-        const uint32_t q = (uint32_t)nearest_code(y, yf, scale, inv, I4 ? 0 : -127, I4 ? 15 : 127);
         if (I4)
-          word[j / 8] |= q << (4 * (j % 8));
-        else
-          word[j / 4] |= (q & 255u) << (8 * (j % 4));
+          word[j / 8] += (bits[j] << (4 * (j % 8))) - (kCodeBits << (4 * (j % 8)));
+        else if (j % 4 == 3)
+          word[j / 4] = __byte_perm(__byte_perm(bits[j - 3], bits[j - 2], 0x0040), __byte_perm(bits[j - 1], bits[j], 0x0040), 0x5410);
+        else if (N == 2 && j == 1)
+          word[0] = __byte_perm(bits[0], bits[1], 0x0040);
       }
+    }
     uint8_t* dst = codes + (I4 ? d / 2 : d);
     constexpr int kBytes = I4 ? N / 2 : N;
     if (kBytes == 16)
