@@ -70,6 +70,15 @@ __device__ __forceinline__ uint32_t code_bits(float x, float inv, float* off) {
   return __float_as_uint(f);
 }
 
+// x / 15 rounded to 32 bits.  The product with 1 / 15 is within 2^-51 of it, so
+// the division is made only where that could matter.
+__device__ __noinline__ float fifteenth_slow(double x) { return (float)(x / 15.0); }
+__device__ __forceinline__ float fifteenth(double x) {
+  const double y = x * (1.0 / 15.0), e = y * 0x1p-50;
+  const float low = (float)(y - e), high = (float)(y + e);
+  return low == high ? low : fifteenth_slow(x);
+}
+
 // N elements from x[i] on, in wide loads where `wide` says that they are aligned.
 template <int N>
 __device__ __forceinline__ void load_run(const void* x, size_t i, int bf16, bool wide, float* v) {
@@ -126,9 +135,11 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
   const int lane = threadIdx.x & 31, in = lane & (group - 1);
   const int jobs = 2 * c.kv_heads + (s.q ? s.nh : 0);  // K heads, V heads, q heads of a row
   const int hd = c.hd, half = hd / 2;
-  const uint32_t job = ((size_t)blockIdx.x * (kStoreWarps * 32) + threadIdx.x) / group;  // rows * jobs is below 2^31
-  const size_t row = job / jobs;
-  const int what = (int)(job % jobs);
+  const int lg = 31 - __clz(group);  // group is a power of two
+  const uint32_t job = blockIdx.x * (uint32_t)(kStoreWarps * 32 >> lg) + (threadIdx.x >> lg);  // rows * jobs is below 2^31
+  const uint32_t row32 = job / (uint32_t)jobs;
+  const size_t row = row32;
+  const int what = (int)(job - row32 * (uint32_t)jobs);
   // lanes without a row run on with the group's reductions
   const bool there = row < (size_t)s.rows;
   const int pos = there ? (s.row_pos ? s.row_pos[row] : (int)row) : -1, seq = there && s.row_seq ? s.row_seq[row] : 0;
@@ -232,7 +243,7 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
   }
   if (I4) {
     zero = __fadd_rn((float)low64, 0.0f);  // never -0
-    scale = __fadd_rn((float)((top64 - (double)zero) / 15.0), 0.0f);
+    scale = __fadd_rn(fifteenth(top64 - (double)zero), 0.0f);
   } else {
     scale = ROPE ? (float)(top64 / 127.0) : __fdiv_rn(top, 127.0f);
   }
