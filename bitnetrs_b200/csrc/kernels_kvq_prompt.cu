@@ -41,12 +41,21 @@
 // tile j was issued after it.
 // Two CTAs share an SM, so each has half of its tensor memory.  With a second S
 // the next tile's scores are computed while a tile is weighed, K's widening
-// running a tile ahead of V's.  Heads of 64 have room for it beside O and Q
-// (its first term).  Heads of 128 have it where Q is one term and the codes are
-// small enough that Q fits into shared memory beside four tiles of pages (with
-// two tiles, as I8 would have, pages come too late: 275 against 267 us for 4
-// ragged prompts, 4500 rows in all; I4 gains, 281 to 270 us, and heads of
-// 64 232 to 195 us, before the wait that the last tile then needs).
+// running a tile ahead of V's.  Heads of up to 64 have room for it beside O and
+// Q (its first term).  Heads of 96 and 128 have it where Q is one term and the
+// codes are small enough that Q fits into shared memory beside four tiles of
+// pages.  With two tiles, as I8 would have, pages come too late: 275 against
+// 267 us for 4 ragged prompts, 4500 rows in all of 32 heads of 128 over 8 (bf16)
+// behind up to 1900 positions; I4 gains, 281 to 265 us, and heads of 64 232 to
+// 195 us.  The same as f32 rows over I4 take 470 us, and 1024 f32 rows of 20
+// heads over 5 (I8) 49 us.
+//
+// What bounds it: the handshakes of a tile, S, weights, O, one after the other
+// (some 3000 cycles by itself, 2200 a CTA with two on an SM), with half of the
+// SM's issue slots in use and a fifth of the tensor cores' time.  Not faster
+// were: the weights by eight warps (305 to 325 us), rows spread over
+// four lanes so that a key's parameters serve four of them (307 to 324 us), and
+// f32 sums brought to the output 32 or 64 dimensions at a time (470 to 509 us).
 //
 // Every wait is bounded; a CTA that gives up records it, waits (bounded) for
 // its copies and products and frees its tensor memory.
@@ -802,7 +811,7 @@ void launch_prompt_of(const KvqView& c, const KvqRows& r, const KvqAttend& a, in
 // 128, up to four a unit).  Measured: 1024 f32 rows of a fresh prompt with 5
 // units 48 against 135 us; 32 rows behind 8000 positions 242 against some 60 us.
 bool kvq_prompt_pays(const KvqView& c, const KvqRows& r, int nh, bool bf16) {
-  if (!r.runs || (c.hd != 64 && c.hd != 128)) return false;
+  if (!r.runs || (c.hd != 32 && c.hd != 64 && c.hd != 96 && c.hd != 128)) return false;
   const Units us = units_of(nh, c.kv_heads);
   const double ctas = ((double)r.rows / (kPromptRows / us.heads) + r.runs) * us.per_row;
   if (ctas > (double)INT_MAX) return false;
@@ -811,10 +820,16 @@ bool kvq_prompt_pays(const KvqView& c, const KvqRows& r, int nh, bool bf16) {
 
 void launch_kvq_prompt(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_len, cudaStream_t st) {
   if (r.rows <= 0 || r.runs <= 0) return;
-  if (c.hd == 64)
-    launch_prompt_of<64>(c, r, a, max_len, st);
-  else
-    launch_prompt_of<128>(c, r, a, max_len, st);
+  switch (c.hd) {
+    case 32:
+      return launch_prompt_of<32>(c, r, a, max_len, st);
+    case 64:
+      return launch_prompt_of<64>(c, r, a, max_len, st);
+    case 96:
+      return launch_prompt_of<96>(c, r, a, max_len, st);
+    case 128:
+      return launch_prompt_of<128>(c, r, a, max_len, st);
+  }
 }
 
 }  // namespace bitnet

@@ -72,9 +72,14 @@ def bench(be, kv, heads, hd, lens, **kw):
     return Bench(be, R.Cache(kv, heads, hd, lens, torch.device("cuda", be.device_id), **kw))
 
 
-def check_row(b, q_row, nh, seq, length, out_row, lse_row):
+def check_row(b, q_row, nh, seq, length, out_row, lse_row, fp16_weights=False):
+    """fp16_weights: each softmax weight w_j is rounded once to fp16, by at most half a step, 2^-11 w_j, where it
+    multiplies the codes' part of v_j: c * scale (I8), or (c - 7.5) * scale (I4), at most half the row's range.  Both are
+    at most max |v|, and the weights add up to 1, so the output is off by at most 2^-11 max |v| more."""
     hd = b.c.hd
     ref, lse, bound = R.attention(b.c, q_row.double().view(nh, hd), seq, length)
+    if fp16_weights and length > 0:
+        bound = bound + 2.0**-11 * b.c.rows(1, seq, range(length)).abs().max()
     got = out_row.double().view(nh, hd)
     if out_row.dtype == torch.bfloat16:
         bound = bound * (1 + 2.0**-8) + 2.0**-8 * ref.abs()
@@ -357,7 +362,7 @@ def test_prompt_attention(cuda_backend, nh, heads, hd, kv, io):
         for j in sorted({0, 1, 15, 16, 31, 32, 63, 64, counts[i] // 2, counts[i] - 2, counts[i] - 1}):
             if 0 <= j < counts[i]:
                 r = cu[i] + j
-                check_row(b, q[r], nh, s, starts[i] + j + 1, out[r], lse[r])
+                check_row(b, q[r], nh, s, starts[i] + j + 1, out[r], lse[r], fp16_weights=io == "bf16")
 
 
 @pytest.mark.parametrize("kv", KINDS)
@@ -770,3 +775,24 @@ def test_store_prompt_load_in_a_graph(cuda_backend, kv):
             torch.testing.assert_close(t[:m], b.c.rows(kind, s, list(range(m))).flatten(1).float(), rtol=0, atol=0)
         for t in (out, lse, kb, vb):
             assert (t[m:] == 7.0).all()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("nh,heads,hd", [(32, 8, 32), (24, 12, 32), (24, 8, 96), (27, 9, 96), (36, 6, 96), (16, 16, 32)])
+def test_prompt_attention_of_other_heads(cuda_backend, nh, heads, hd, kv, io):
+    test_prompt_attention(cuda_backend, nh, heads, hd, kv, io)
+
+
+@pytest.mark.parametrize("shift", [0, 8, 2])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("nh,heads,hd", [(24, 8, 96), (36, 12, 32)])
+def test_long_sums_of_other_heads(cuda_backend, nh, heads, hd, kv, shift):
+    test_long_sums_keep_their_accuracy(cuda_backend, nh, heads, hd, kv, shift)
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [96, 32])
+def test_prompt_attention_of_other_heads_repeats_itself(cuda_backend, hd, kv, io):
+    test_prompt_attention_repeats_itself(cuda_backend, hd, kv, io)
