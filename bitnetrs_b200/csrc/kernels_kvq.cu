@@ -37,8 +37,8 @@ namespace {
 //
 // Bound, for many rows, by the loads that a warp waits for and its instructions
 // (some 500 for 16 elements a lane), for few by three dependent loads (position,
-// page, and the row beside them).  Measured: 6600 rows of 8 kv heads of 128, bf16
-// to I4, 29 us (2.0 TB/s); one row of 5 heads, rotated, 4.8 us with its launch.
+// page, and the row beside them).  Measured: 6605 rows of 8 kv heads of 128, bf16
+// to I4, 20 us (1.7 TB/s); one row of 5 heads, rotated, 2.7 us with its launch.
 // Neither more warps an SM (fewer registers), nor CTAs that stay and take row
 // after row, nor reductions that do not wait for the row's page were faster.
 // ---------------------------------------------------------------------------
@@ -119,8 +119,8 @@ constexpr int kLoadTeams = 148 * 320;  // warps, at most: eight times what the S
 
 // Elements a lane, and lanes a row of one head.  A rotation pairs whole runs, so
 // half a row is a multiple of a run of 8 or 16.  With many rows 16 elements a
-// lane keep twice the bytes on the way (6600 rows of 8 kv heads, bf16 to I4: 35 us
-// with 8, 29 us with 16); with few there are more lanes to share the work.
+// lane keep twice the bytes on the way (6605 rows of 8 kv heads, bf16 to I4: 25 us
+// with 8, 20 us with 16); with few there are more lanes to share the work.
 struct RowSplit {
   int group, run;
 };
@@ -317,7 +317,8 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
 // when there are few.  Where the next row's blocks lie (three dependent loads)
 // is asked for before this row is read, and kLoadAhead runs a lane before the
 // first is written.  Codes become floats without conversions: a byte below the
-// bits of 2^23 is 2^23 + c.  Bound by memory.
+// bits of 2^23 is 2^23 + c.  Bound by memory: 130870 rows of 8 kv heads of 128,
+// I4 to bf16, 143 us (4.8 TB/s, most of it writes); 517 rows of 5, I8 to f32, 3 us.
 // ---------------------------------------------------------------------------
 constexpr int kLoadAhead = 4;
 // Byte i of w (unsigned), less `bias`, as a float.

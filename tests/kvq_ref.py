@@ -1,5 +1,5 @@
 """The quantised key-value cache and its attention in 64 bits (torch, any
-device), the checker of the kvq tests."""
+device), the reference of the kvq tests."""
 import math
 
 import torch
