@@ -1098,7 +1098,8 @@ bool launch_mma(const KvqView& c, const KvqRows& r, const KvqAttend& a, int max_
   CUtensorMap map;
   if (!codes_map<T>(c, &map)) return false;
   auto* kernel = kvq_attend_mma_kernel<HD, I4, NT>;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
+  static std::atomic<uint64_t> allowed{0};
+  allow_shared((const void*)kernel, T::kSmem, allowed);
   int shares = NT == 1 ? kMmaShares : kMmaShares / 2;
   const size_t units = (size_t)r.rows * units_of(a.nh, c.kv_heads).per_row;
   const bool whole = max_len <= kWholeUnits && units <= (size_t)shares;

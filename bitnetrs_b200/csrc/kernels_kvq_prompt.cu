@@ -786,7 +786,8 @@ void launch_prompt(const KvqView& c, const KvqRows& r, const KvqAttend& a, int m
   const int tokens = kPromptRows / us.heads;
   const unsigned ctas = (unsigned)(r.rows / tokens + r.runs) * us.per_row;
   auto* kernel = kvq_prompt_kernel<HD, I4, TWO>;
-  cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem);
+  static std::atomic<uint64_t> allowed{0};
+  allow_shared((const void*)kernel, T::kSmem, allowed);
   const size_t run = a.bf16 ? 8 : 4;
   const int wide_q = (uintptr_t)a.q % 16 == 0 && a.ldq % run == 0;
   // 16 bytes of the output at a time, or 32 (f32)

@@ -1,6 +1,8 @@
 // kvq_device.cuh — device helpers shared by the kernels of the quantised cache.
 #pragma once
 
+#include <atomic>
+
 #include "async.cuh"
 #include "kvq.cuh"
 
@@ -130,4 +132,14 @@ __device__ __forceinline__ void nibbles_f16(uint32_t w, uint32_t* x) {
   x[3] = fma_f16x2(v & 0x00f000f0u, kHigh, kMid);
 }
 }  // namespace
+// Lets a kernel have its dynamic shared memory, once a device and kernel: the
+// call costs the host a tenth of a small attention.
+inline void allow_shared(const void* kernel, int bytes, std::atomic<uint64_t>& done) {
+  int device = 0;
+  cudaGetDevice(&device);
+  const uint64_t bit = device < 64 ? 1ull << device : 0;
+  if (done.load(std::memory_order_acquire) & bit) return;
+  if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) == cudaSuccess) done.fetch_or(bit);
+}
+
 }  // namespace bitnet

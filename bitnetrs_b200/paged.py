@@ -40,6 +40,10 @@ class PagedKV:
         self._ref = C.byref(pages)
         self._kv_width = pages.kv_heads * pages.head_dim
         self._owner = owner  # keeps a model's cache alive
+        self._store = self._lib.bitnet_cuda_kv_store_device
+        self._load = self._lib.bitnet_cuda_kv_load_device
+        self._attention = self._lib.bitnet_cuda_kv_attention_device
+        self._prompt = self._lib.bitnet_cuda_kv_prompt_attention_device
 
     @classmethod
     def of_layer(cls, kv, layer: int) -> "PagedKV":
@@ -64,17 +68,21 @@ class PagedKV:
         (device int32 arrays).  ``rope`` = (cos, sin, length): K is rotated first."""
         cos, sin, length = rope if rope is not None else (None, None, 0)
         w = self._kv_width
-        check(self._lib.bitnet_cuda_kv_store_device(
+        code = self._store(
             self.backend._h, self._ref, k, w if ldk is None else ldk, v, w if ldv is None else ldv,
-            int(bf16), rows, row_seq, row_pos, cos, sin, length, status, stream or None))
+            int(bf16), rows, row_seq, row_pos, cos, sin, length, status, stream or None)
+        if code:
+            check(code)
 
     def load(self, k: int, v: int, rows: int, row_seq: int, row_pos: int, status: int, *, ldk: Optional[int] = None,
              ldv: Optional[int] = None, bf16: bool = False, stream: int = 0) -> None:
         """Read rows back into ``k`` and ``v``."""
         w = self._kv_width
-        check(self._lib.bitnet_cuda_kv_load_device(
+        code = self._load(
             self.backend._h, self._ref, rows, row_seq, row_pos, k, w if ldk is None else ldk, v,
-            w if ldv is None else ldv, int(bf16), status, stream or None))
+            w if ldv is None else ldv, int(bf16), status, stream or None)
+        if code:
+            check(code)
 
     def attention_workspace(self, n_heads: int) -> int:
         """Bytes of the workspace that one attention call in flight needs."""
@@ -87,10 +95,12 @@ class PagedKV:
                   ldo: Optional[int] = None, bf16: bool = False, lse: int = 0, stream: int = 0) -> None:
         """Attention of single tokens: row r sees the first ``row_len[r]`` positions of sequence ``row_seq[r]``."""
         w = n_heads * self._pages.head_dim
-        check(self._lib.bitnet_cuda_kv_attention_device(
+        code = self._attention(
             self.backend._h, self._ref, q, w if ldq is None else ldq, int(bf16), rows, n_heads,
             row_seq, row_len, max_len, out, w if ldo is None else ldo, lse or None, workspace, workspace_bytes, status,
-            stream or None))
+            stream or None)
+        if code:
+            check(code)
 
     def prompt_attention(self, q: int, out: int, rows: int, n_heads: int, n_seqs: int, seq_ids: int, cu_rows: int,
                          starts: int, max_len: int, workspace: int, workspace_bytes: int, status: int, *,
@@ -99,7 +109,9 @@ class PagedKV:
         """Causal attention of prompts whose K and V are in the cache: rows ``cu_rows[i]`` to ``cu_rows[i + 1]`` are
         the positions from ``starts[i]`` of sequence ``seq_ids[i]``."""
         w = n_heads * self._pages.head_dim
-        check(self._lib.bitnet_cuda_kv_prompt_attention_device(
+        code = self._prompt(
             self.backend._h, self._ref, q, w if ldq is None else ldq, int(bf16), rows, n_heads, n_seqs,
             seq_ids, cu_rows, starts, max_len, out, w if ldo is None else ldo, lse or None, workspace,
-            workspace_bytes, status, stream or None))
+            workspace_bytes, status, stream or None)
+        if code:
+            check(code)
