@@ -796,3 +796,76 @@ def test_long_sums_of_other_heads(cuda_backend, nh, heads, hd, kv, shift):
 @pytest.mark.parametrize("hd", [96, 32])
 def test_prompt_attention_of_other_heads_repeats_itself(cuda_backend, hd, kv, io):
     test_prompt_attention_repeats_itself(cuda_backend, hd, kv, io)
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [128, 64, 96, 32, 80])
+def test_queries_and_outputs_at_odd_places(cuda_backend, hd, kv, io):
+    """q and out that start on their element's size only, with odd row strides; both operators."""
+    nh, heads, n = 24, 8, 150
+    b = bench(cuda_backend, kv, heads, hd, [n], seed=6)
+    g = torch.Generator(device=b.dev).manual_seed(2)
+    big = torch.randn(n, nh * hd + 7, device=b.dev, generator=g).to(DT[io])
+    q = big[:, 3:3 + nh * hd]
+    wide = torch.full((n, nh * hd + 5), 9.0, device=b.dev, dtype=DT[io])
+    out = wide[:, 1:1 + nh * hd]
+    a, c, s, sp = b.ints([0]), b.ints([0, n]), b.ints([0]), b.space(nh)
+    b.kv.prompt_attention(q.data_ptr(), out.data_ptr(), n, nh, 1, a.data_ptr(), c.data_ptr(), s.data_ptr(), n,
+                          sp.data_ptr(), sp.numel(), b.status.data_ptr(), ldq=q.stride(0), ldo=out.stride(0),
+                          bf16=io == "bf16", stream=1)
+    torch.cuda.synchronize()
+    for i in (0, 1, 63, 64, n - 1):
+        check_row(b, q[i], nh, 0, i + 1, out[i], None, fp16_weights=io == "bf16")
+    assert (wide[:, :1] == 9.0).all() and (wide[:, 1 + nh * hd:] == 9.0).all()
+    wide.fill_(9.0)
+    one, _ = b.attend(q[:9], nh, [0] * 9, [1, 2, 15, 16, 17, 100, n, 0, 33], out=out[:9], lse=False)
+    for i, length in enumerate([1, 2, 15, 16, 17, 100, n, 0, 33]):
+        check_row(b, q[i], nh, 0, length, one[i], None)
+    assert b.status.item() == 0 and (wide[:, :1] == 9.0).all() and (wide[9:] == 9.0).all()
+
+
+@pytest.mark.parametrize("hd", [128, 96, 80])
+def test_nothing_to_attend_to(cuda_backend, hd):
+    """Lengths of zero everywhere (max_len 0 too), prompts behind negative starts, no runs, empty runs, no rows."""
+    nh, heads, n = 24, 8, 64
+    b = bench(cuda_backend, KV_I8, heads, hd, [n, n], seed=6)
+    q = torch.randn(n, nh * hd, device=b.dev)
+    for most in (0, n, None):
+        out, lse = b.attend(q, nh, [0, 1] * 32, [0] * n, max_len=most)
+        assert (out == 0).all() and (lse == -math.inf).all()
+    out, lse = b.attend(q, nh, [0, 1] * 32, [-5] * n)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    out, lse = b.prompt(q, nh, [0], [0, n], [-n], max_len=0)
+    assert (out == 0).all() and (lse == -math.inf).all()
+    out, lse = b.prompt(q, nh, [0, 1, 0], [5, 5, 5, 5], [0, 3, 9])
+    assert (out == 77.0).all() and (lse == 77.0).all()
+    out, lse = b.prompt(q, nh, [0, 1, 0, 1], [0, 0, 30, 30, 60], [0, 2, 9, 4])
+    assert (out[60:] == 77.0).all() and b.status.item() == 0
+    for r, seq, length in ((0, 1, 3), (29, 1, 32), (30, 1, 5), (59, 1, 34)):
+        check_row(b, q[r], nh, seq, length, out[r], lse[r])
+    assert b.attend(q[:0], nh, [], [])[0].shape[0] == 0
+
+
+@pytest.mark.parametrize("kv,spare", [(KV_I8, 140000), (KV_I4, 260000)])
+def test_pool_beyond_32_bits(cuda_backend, kv, spare):
+    """Pages at more than 2^32 bytes into the pool: stored, read back and attended to."""
+    nh, heads, hd, n = 32, 8, 128, 300
+    b = bench(cuda_backend, kv, heads, hd, [n, 20], fill="zeros", spare=spare)
+    assert b.c.pool.numel() > 2**32
+    b.c.table[0] = b.c.pages - 1 - torch.arange(b.c.per_seq, dtype=torch.int32, device=b.dev)
+    g = torch.Generator(device=b.dev).manual_seed(3)
+    k, v = (torch.randn(n, heads * hd, device=b.dev, generator=g) for _ in range(2))
+    q = torch.randn(n, nh * hd, device=b.dev, generator=g)
+    b.store(k, v, [0] * n, list(range(n)))
+    kb, vb = torch.zeros_like(k), torch.zeros_like(v)
+    b.load(kb, vb, [0] * n, list(range(n)))
+    out, lse = b.prompt(q, nh, [0], [0, n], [0])
+    one, lse1 = b.attend(q, nh, [0] * n, list(range(1, n + 1)))
+    assert b.status.item() == 0
+    for kind, t in ((0, kb), (1, vb)):
+        torch.testing.assert_close(t, b.c.rows(kind, 0, list(range(n))).flatten(1).float(), rtol=0, atol=0)
+    assert kb.abs().amax(1).min() > 0
+    for i in (0, 100, n - 1):
+        check_row(b, q[i], nh, 0, i + 1, out[i], lse[i])
+        check_row(b, q[i], nh, 0, i + 1, one[i], lse1[i])
