@@ -15,9 +15,11 @@
 // a sum of its own.
 //
 // Q is fp16, multiplied by a power of two a row so that its largest element is
-// near 2^14: bf16 is exact there.  An f32 row is the sum of two such terms, and
-// its weights W too, each product being two on the same sums; with bf16 rows a
-// weight is rounded once to fp16 (2^-11), which its output's bf16 does not show.
+// near 2^14: bf16 is exact there.  An f32 row is the sum of two such terms, as
+// the weights W are for both types, each product being two on the same sums.
+// Weights of one term (2^-11) move a result by some 2e-4, which a tenth and more
+// of the bf16 outputs show; the second term costs bf16 rows 309 against 268 us
+// (4 ragged prompts, I4, as below).
 //
 // Warps 0-3 weigh: a thread reads its row of S, writes W over it as the A
 // operand of the second product, and rescales its row of O only when a score
@@ -465,7 +467,9 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
   };
   auto scores_at = [&](int j) -> uint32_t { return T::kTmemS + (T::kTwoS && (j & 1) ? kKeys : 0); };
   // The second terms first: the sums are cut, not rounded, to f32, each time by
-  // what they have grown to.
+  // what they have grown to.  (2^-25 of the result an addition on average, eight
+  // of them a tile: f32 rows bring the sums out every kSumTiles tiles, bf16 rows
+  // have nowhere to bring them to and are off by 2^-22 a tile, 2^-13 at 32768 keys.)
   auto issue_scores = [&](int j) {
     const uint32_t d = tmem + scores_at(j);
     auto k_at = [&](int k) { return operand(smem_u32(k_tile) + k / 4 * (kKeys * 128) + k % 4 * 32, 16); };
@@ -484,12 +488,10 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     const uint32_t w = tmem + scores_at(j);
     const bool adds = TWO ? j % kSumTiles != 0 : j > 0;
     auto v_at = [&](int k) { return operand(smem_u32(v_tile) + k * 2048, kKeys * 128); };
-    if (TWO)
 #pragma unroll
-      for (int k = 0; k < kKeys / 16; ++k) mma_tmem_a(tmem, w + 32 + 8 * k, v_at(k), product(HD, 1), adds || k > 0);
+    for (int k = 0; k < kKeys / 16; ++k) mma_tmem_a(tmem, w + 32 + 8 * k, v_at(k), product(HD, 1), adds || k > 0);
 #pragma unroll
-    for (int k = 0; k < kKeys / 16; ++k)
-      mma_tmem_a(tmem, w + 8 * k, v_at(k), product(HD, 1), TWO || adds || k > 0);
+    for (int k = 0; k < kKeys / 16; ++k) mma_tmem_a(tmem, w + 8 * k, v_at(k), product(HD, 1), true);
     mma_commit(smem_u32(&output_full));
   };
   // One arrival a warp, after its writes to shared memory (for the products) or to tensor memory.
@@ -715,14 +717,12 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
               const float2 f = unpair(p);
               const uint32_t h = pack_f16(f.x, f.y);
               hi[n / 2 + k] = h;
-              if (TWO) {
-                const float2 r = unpair(add2(p, pair(-f16_lo(h), -f16_hi(h))));
-                lo[n / 2 + k] = pack_f16(r.x, r.y);
-              }
+              const float2 r = unpair(add2(p, pair(-f16_lo(h), -f16_hi(h))));
+              lo[n / 2 + k] = pack_f16(r.x, r.y);
             }
           }
           tmem_st8(s_at + i / 2, hi);
-          if (TWO) tmem_st8(s_at + 32 + i / 2, lo);
+          tmem_st8(s_at + 32 + i / 2, lo);
         }
       };
       if (masked)

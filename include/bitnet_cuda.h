@@ -560,8 +560,8 @@ int bitnet_cuda_kv_attention_device(bitnet_cuda_ctx* ctx, const bitnet_cuda_kv_p
  * n_seqs and n_seqs; cu_rows does not decrease and stays within `rows`), and
  * each attends to the positions up to its own.  Rows outside every range are
  * left as they were.  max_len bounds starts[i] + the rows of i.  The rest is as
- * above, but that with bf16 rows a softmax weight may be rounded once to fp16
- * (by 2^-11 at most) where many rows share the work. */
+ * above, but that with bf16 rows, where many share the work, sums over the keys
+ * are cut, not rounded, to f32: an output is off by some 2^-22 for every 64 keys. */
 int bitnet_cuda_kv_prompt_attention_device(bitnet_cuda_ctx* ctx, const bitnet_cuda_kv_pages* cache, const void* q,
                                            size_t ldq, int x_is_bf16, size_t rows, size_t n_heads, size_t n_seqs,
                                            const int32_t* seq_ids, const int32_t* cu_rows, const int32_t* starts,
