@@ -1,6 +1,7 @@
 // kernels_kvq_attend.cu — GQA attention over the quantised paged cache, split
 // over the context and joined.
 #include "kvq_device.cuh"
+#include "kvq_ring.h"
 
 #include <algorithm>
 
@@ -533,8 +534,8 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
     at_k[c / 2] = swizzled(row * T::kRow + piece * 16);
     at_v[c / 2] = swizzled((kPage + row) * T::kRow + piece * 16);
   }
-  int fill = 0, take = 0;      // stages, the next to fetch into and the next to use
-  uint32_t parity = 0;         // of the copies that `take` waits for
+  StageRing<T::kStages> copies;
+  bool failed = false;  // the same in all lanes
 
   while (at < end && r < R.rows) {
     int seq = 0;
@@ -570,8 +571,8 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
       const int first_block = __shfl_sync(0xffffffffu, ids, i & 31) * c.kv_heads + kvh;
       const int second_block = __shfl_sync(0xffffffffu, ids, (i + 1) & 31) * c.kv_heads + kvh;
       if (lane == 0) {
-        const uint32_t bar = bar_s + fill * 8, tile = mine_s + fill * (2 * T::kTile);
-        const uint32_t par = params_s + fill * (2 * kParStride);
+        const uint32_t bar = bar_s + copies.fill * 8, tile = mine_s + copies.fill * (2 * T::kTile);
+        const uint32_t par = params_s + copies.fill * (2 * kParStride);
         const bool both = i + 1 < n_pages;
         mbar_expect_tx(bar, (T::kCodes + T::kParams) << both);
         tma_codes(tile, &tmap, first_block, bar);
@@ -584,7 +585,7 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
                       T::kParams, bar);
         }
       }
-      fill = fill + 1 == T::kStages ? 0 : fill + 1;
+      copies.fetched();
     };
     __syncwarp();
 #pragma unroll 1
@@ -664,13 +665,14 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
     }
 
     for (int i = 0; i < n_pages; i += 2) {
-      if (!mbar_wait(bar_s + take * 8, parity, &gave_up)) {
+      // agreed on by the warp: what follows is done by all lanes together
+      if (!__all_sync(0xffffffffu, mbar_wait(bar_s + copies.take * 8, copies.parity, &gave_up))) {
         give_up(&gave_up, a.status);
-        at = end;  // nothing more is asked for
+        failed = true;
         break;
       }
-      const uint32_t src = mine_s + take * (2 * T::kTile);
-      const uint8_t* par = params + take * (2 * kParStride);
+      const uint32_t src = mine_s + copies.take * (2 * T::kTile);
+      const uint8_t* par = params + copies.take * (2 * kParStride);
       // live positions from the first page on; with an odd number of pages the
       // second tile of the last pair holds what was there before
       const int left = min(len - (p0 + i) * kPage, (n_pages - i) * kPage);
@@ -814,21 +816,16 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
         }
       }
       __syncwarp();  // every lane has read the stage
+      copies.used();
       fetch(i + 2 * T::kStages);
-      if (++take == T::kStages) {
-        take = 0;
-        parity ^= 1;
-      }
     }
-    if (gave_up) {
+    if (failed) {
       // copies still in flight land (or the wait for each runs out) before the CTA may go
-      while (take != fill) {
-        mbar_wait(bar_s + take * 8, parity, nullptr);
-        if (++take == T::kStages) {
-          take = 0;
-          parity ^= 1;
-        }
+      while (copies.flying) {
+        mbar_wait(bar_s + copies.take * 8, copies.parity, nullptr);
+        copies.used();
       }
+      __syncwarp();
       break;
     }
 
