@@ -23,9 +23,15 @@
 //
 // Warps 0-3 weigh: a thread reads its row of S, writes W over it as the A
 // operand of the second product, and rescales its row of O only when a score
-// passes the row's maximum by kSlack (log2) or a scale of V grows too much, as
-// in the single-token kernel; the weights' power of two is folded into the
-// maximum, so that it divides out of the result.  Warps 4-6 widen the next
+// passes the row's maximum by kSlack (log2) or a weight times its scale of V
+// grows too much.  A row's weights have a power of two of their own, by the
+// largest such product that the row has had (not by scales alone: a key that
+// the row does not see, or gives no weight, must not push the others below what
+// fp16 holds); it is folded into the maximum, so that it divides out of the
+// result.  The largest is between 2^-2 and 2^9 then (up to 2^15 with the slack),
+// so what two terms of fp16 lose of a smaller one is below 2^-23 of it.  While
+// the scales of a tile are within 2^6 of one another they tell that by
+// themselves; else a row's products are looked at.  Warps 4-6 widen the next
 // tile's K and this tile's V.  Warp 7 issues the products, and fetches pages
 // kStages tiles ahead (their numbers one tile before that).  They meet at
 // mbarriers only:
@@ -513,7 +519,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
 
   // m: a maximum of the row's scores (in the units of the products times their
   // scales) at most kSlack / qs below the true one; mq: m * qs less the power
-  // of two of the weights
+  // of two of the row's weights
   float m = -INFINITY, mq = -INFINITY, limit = -INFINITY, l = 0.0f, zsum = 0.0f;
   if (warp == 7) {
     // ---- products ----
@@ -557,7 +563,9 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     }
   } else {
     // ---- weighing ----
-    int ev = 100;  // the weights are multiplied by 2^ev
+    int ev = limit_pos > 0 ? 100 : -100;  // the row's weights are multiplied by 2^ev
+    float cap = 0.0f;                     // 2^(9 - the largest ev of the warp's rows)
+    float most = 0.0f;  // of the row's largest weight (relative to m) times scale of V: what it is at least
     float kept = 1.0f;  // what m's growth has left of the sums that are in the output's place
     // 16 elements of the row's output, in the order in which they lie in o
     auto load_sums = [&](int i, float* o) {
@@ -658,23 +666,41 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
 #pragma unroll
       for (int i = 0; i < kKeys; i += 2) tops[i / 2 % 4] = max3(tops[i / 2 % 4], s[i], s[i + 1]);
       const float top_s = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-      // a score above the slack, or a scale of V times 2^ev above 2^9
+      // a score above the slack, or a scale of V that some row's 2^ev takes above 2^9
       const float vtop = fmaxf(pj[2][lane], pj[2][lane + 32]);
-      if (__any_sync(0xffffffffu, top_s > limit || __fmul_rn(vtop, __int_as_float((127 + ev) << 23)) > 512.0f)) {
-        float v = vtop;
+      if (__any_sync(0xffffffffu, top_s > limit || vtop > cap)) {
+        const float m_new = fmaxf(m, top_s), m_at = __fmul_rn(m_new, qs);
+        // the tile's largest and least scale, as bits (not numbers: 0)
+        const uint32_t high = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vtop, 0.0f)));
+        const uint32_t low = __reduce_min_sync(
+            0xffffffffu, __float_as_uint(fminf(fmaxf(pj[2][lane], 0.0f), fmaxf(pj[2][lane + 32], 0.0f))));
+        if (m == -INFINITY) {
+          if (limit_pos > 0) ev = min(max(131 - (int)(high >> 23), -100), 100);  // the largest scale near 2^4
+        } else {
+          most = __fmul_rn(most, exp2_approx(__fsub_rn(__fmul_rn(m, qs), m_at)));
+        }
+        // a key with the largest score so far has a weight of 1
+        if (top_s >= m) most = fmaxf(most, __uint_as_float(low));
+        const float unit = __int_as_float((127 + ev) << 23);
+        const bool fits = __fmul_rn(__uint_as_float(high), unit) <= 512.0f && __fmul_rn(most, unit) >= 0.25f;
+        if (__any_sync(0xffffffffu, !fits && limit_pos > 0)) {
 #pragma unroll
-        for (int b = 1; b < 32; b <<= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, b));
-        if (__fmul_rn(v, __int_as_float((127 + ev) << 23)) > 512.0f)
-          ev = max(132 - (int)(__float_as_uint(v) >> 23), -100);  // the largest near 2^5
-        m = fmaxf(m, top_s);
-        const float nq = __fsub_rn(__fmul_rn(m, qs), (float)ev);
+          for (int i = 0; i < kKeys; ++i)  // (a product that is not a number is passed over)
+            most = fmaxf(most, __fmul_rn(exp2_approx(__fmaf_rn(s[i], qs, -m_at)), pj[2][i]));
+          const float now = __fmul_rn(most, unit);
+          if (!(now >= 0.25f && now <= 512.0f) && limit_pos > 0)
+            ev = min(max(129 - (int)(__float_as_uint(most) >> 23), -100), 100);  // near 2^2 (no product yet: as large as it may be)
+        }
+        cap = __int_as_float((136 - __reduce_max_sync(0xffffffffu, ev)) << 23);
+        m = m_new;
+        const float nq = __fsub_rn(m_at, (float)ev);
         const float keep = mq == nq || m == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(mq, nq));
         mq = nq;
         limit = __fadd_rn(m, __fdiv_rn(kSlack, qs));
         l = __fmul_rn(l, keep);
         zsum = __fmul_rn(zsum, keep);
         kept = __fmul_rn(kept, keep);
-        if (TWO ? j % kSumTiles != 0 : j > 0) {
+        if ((TWO ? j % kSumTiles != 0 : j > 0) && __any_sync(0xffffffffu, keep != 1.0f)) {
           if (!wait(output_full, j - 1)) break;
           after_sync();
 #pragma unroll 1

@@ -43,6 +43,58 @@ class Without:
         return self.whole.rows(kind, seq, [int(p) for p in pos if int(p) not in self.skip])
 
 
+# ---- values of very different size ------------------------------------------------------
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [128, 96, 64, 32])
+@pytest.mark.parametrize("power", [20, 40, 70])
+def test_prompt_rows_do_not_feel_the_size_of_later_values(cuda_backend, power, hd, kv, io):
+    """Values 2^power times as large at positions 70 and 197 onwards: rows before them, in the same tile of keys and the
+    same CTA, are as exact as without them (the bound counts the values that a row sees)."""
+    n, heads, nh = 200, 8, 32
+    b = bench(cuda_backend, kv, heads, hd, [n, n], seed=power)
+    scale_rows(b, 1, 0, [70], 2.0**power)
+    scale_rows(b, 1, 1, [197, 198, 199], 2.0**power)
+    q = normal(b, 1, 2 * n, nh * hd).to(DT[io])
+    out, lse = b.prompt(q, nh, [0, 1], [0, n, 2 * n], [0, 0])
+    assert b.status.item() == 0
+    for seq, rows in ((0, (0, 40, 63, 64, 65, 68, 69, 70, 71, 199)), (1, (0, 69, 128, 191, 192, 194, 196, 197, 199))):
+        for i in rows:
+            check_row(b, q[seq * n + i], nh, seq, i + 1, out[seq * n + i], lse[seq * n + i], fp16_weights=io == "bf16")
+
+
+def far_below(b, seq, pos, power):
+    """Makes position `pos` a key that every query with 4 in dimension 0 scores at most -4 * 1900 / sqrt(hd) < -470 (for
+    hd <= 256), some 450 below the others, with values 2^power times as large: its weight is below 2^-600, so nothing
+    of it may show in 32 bits, or in 64."""
+    x = torch.zeros(b.c.hd, dtype=torch.float64, device=b.dev)
+    x[0] = -2000
+    put_row(b, 0, seq, pos, x)
+    scale_rows(b, 1, seq, [pos], 2.0**power)
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [128, 96, 64, 32])
+@pytest.mark.parametrize("power", [30, 60])
+def test_prompt_rows_do_not_feel_the_size_of_values_without_weight(cuda_backend, power, hd, kv, io):
+    n, heads, nh = 200, 8, 32
+    b = bench(cuda_backend, kv, heads, hd, [n], seed=power)
+    skip = (3, 66, 150)
+    for p in skip:
+        far_below(b, 0, p, power)
+    q = normal(b, 2, n, nh, hd)
+    q[..., 0] = 4
+    q = q.flatten(1).to(DT[io])
+    out, lse = b.prompt(q, nh, [0], [0, n], [0])
+    assert b.status.item() == 0
+    for i in (2, 10, 63, 64, 70, 128, 149, 160, 199):
+        left = i + 1
+        check_row(Without(b, skip), q[i], nh, 0, left, out[i], lse[i], fp16_weights=io == "bf16")
+
+
 @pytest.mark.parametrize("kv", KINDS)
 @pytest.mark.parametrize("nh,heads,hd", [(32, 8, 128), (24, 8, 96), (32, 8, 64), (32, 8, 32)])
 def test_bf16_prompts_round_nothing_but_their_output(cuda_backend, nh, heads, hd, kv):
