@@ -567,6 +567,11 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
     float cap = 0.0f;                     // 2^(9 - the largest ev of the warp's rows)
     float most = 0.0f;  // of the row's largest weight (relative to m) times scale of V: what it is at least
     float kept = 1.0f;  // what m's growth has left of the sums that are in the output's place
+    // What a key's weight is multiplied with: the scale of V.  A zero (I4) goes into a sum of its own, in 32 bits; it
+    // counts 2^24 times less, so that it cannot overflow there (a scale that much smaller is lost in 32 bits anyway).
+    auto size_of = [&](const float(*p)[kKeys], int key) {
+      return I4 ? fmaxf(p[2][key], __fmul_rn(fabsf(p[3][key]), 0x1p-24f)) : p[2][key];
+    };
     // 16 elements of the row's output, in the order in which they lie in o
     auto load_sums = [&](int i, float* o) {
       const float* p = (const float*)a.out + out_at + i;
@@ -667,13 +672,13 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
       for (int i = 0; i < kKeys; i += 2) tops[i / 2 % 4] = max3(tops[i / 2 % 4], s[i], s[i + 1]);
       const float top_s = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
       // a score above the slack, or a scale of V that some row's 2^ev takes above 2^9
-      const float vtop = fmaxf(pj[2][lane], pj[2][lane + 32]);
+      const float size_a = size_of(pj, lane), size_b = size_of(pj, lane + 32), vtop = fmaxf(size_a, size_b);
       if (__any_sync(0xffffffffu, top_s > limit || vtop > cap)) {
         const float m_new = fmaxf(m, top_s), m_at = __fmul_rn(m_new, qs);
-        // the tile's largest and least scale, as bits (not numbers: 0)
+        // the tile's largest and least size, as bits (not numbers: 0)
         const uint32_t high = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(vtop, 0.0f)));
         const uint32_t low = __reduce_min_sync(
-            0xffffffffu, __float_as_uint(fminf(fmaxf(pj[2][lane], 0.0f), fmaxf(pj[2][lane + 32], 0.0f))));
+            0xffffffffu, __float_as_uint(fminf(fmaxf(size_a, 0.0f), fmaxf(size_b, 0.0f))));
         if (m == -INFINITY) {
           if (limit_pos > 0) ev = min(max(131 - (int)(high >> 23), -100), 100);  // the largest scale near 2^4
         } else {
@@ -686,7 +691,7 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
         if (__any_sync(0xffffffffu, !fits && limit_pos > 0)) {
 #pragma unroll
           for (int i = 0; i < kKeys; ++i)  // (a product that is not a number is passed over)
-            most = fmaxf(most, __fmul_rn(exp2_approx(__fmaf_rn(s[i], qs, -m_at)), pj[2][i]));
+            most = fmaxf(most, __fmul_rn(exp2_approx(__fmaf_rn(s[i], qs, -m_at)), size_of(pj, i)));
           const float now = __fmul_rn(most, unit);
           if (!(now >= 0.25f && now <= 512.0f) && limit_pos > 0)
             ev = min(max(129 - (int)(__float_as_uint(most) >> 23), -100), 100);  // near 2^2 (no product yet: as large as it may be)

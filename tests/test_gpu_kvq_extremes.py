@@ -95,6 +95,44 @@ def test_prompt_rows_do_not_feel_the_size_of_values_without_weight(cuda_backend,
         check_row(Without(b, skip), q[i], nh, 0, left, out[i], lse[i], fp16_weights=io == "bf16")
 
 
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("hd", [128, 96, 64, 32, 80])
+@pytest.mark.parametrize("zero,scale", [(22, None), (30, None), (54, None), (78, None), (60, -60), (40, 0), (-90, None)])
+def test_constant_and_nearly_constant_values(cuda_backend, zero, scale, hd, io):
+    """I4 rows of V whose elements are all equal, near 2^zero: their scale is 0 and the zero holds them.  Or with a scale
+    near 2^scale, far below the zero."""
+    heads, nh, n = 8, 32, 200
+    b = bench(cuda_backend, KV_I4, heads, hd, [n], seed=zero + 100)
+    par = b.c.params_view(1)
+    par[..., 1, :] = normal(b, 1, *par[..., 1, :].shape) * 2.0**zero
+    par[..., 0, :] = 0.0 if scale is None else (1 + torch.rand(par[..., 0, :].shape, device=b.dev)) * 2.0**scale
+    q = normal(b, 2, n, nh * hd).to(DT[io])
+    out, lse = b.prompt(q, nh, [0], [0, n], [0])
+    one, lse1 = b.attend(q, nh, [0] * n, list(range(1, n + 1)))
+    assert b.status.item() == 0
+    for i in (0, 1, 63, 64, 130, n - 1):
+        check_row(b, q[i], nh, 0, i + 1, out[i], lse[i], fp16_weights=io == "bf16")
+        check_row(b, q[i], nh, 0, i + 1, one[i], lse1[i])
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [128, 64])
+def test_values_that_are_all_zero_at_first(cuda_backend, hd, kv):
+    """The first 100 values are 0, the rest ordinary or near 2^-100."""
+    heads, nh, n = 8, 32, 300
+    for power in (0, -100):
+        b = bench(cuda_backend, kv, heads, hd, [n], seed=5)
+        b.c.params_view(1).mul_(2.0**power)
+        scale_rows(b, 1, 0, range(100), 0.0)
+        q = normal(b, 2, n, nh * hd)
+        out, lse = b.prompt(q, nh, [0], [0, n], [0])
+        one, lse1 = b.attend(q, nh, [0] * n, list(range(1, n + 1)))
+        assert (out[:100] == 0).all() and (one[:100] == 0).all() and b.status.item() == 0
+        for i in (100, 101, 127, 128, 200, 299):
+            check_row(b, q[i], nh, 0, i + 1, out[i], None)
+            check_row(b, q[i], nh, 0, i + 1, one[i], None)
+
+
 @pytest.mark.parametrize("kv", KINDS)
 @pytest.mark.parametrize("nh,heads,hd", [(32, 8, 128), (24, 8, 96), (32, 8, 64), (32, 8, 32)])
 def test_bf16_prompts_round_nothing_but_their_output(cuda_backend, nh, heads, hd, kv):
