@@ -271,10 +271,12 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // to one head.  The scale of a V row multiplies its weight before that is
 // split.  An I4 zero enters scores (times the sum of q) and output as a sum of
 // its own.
-// The weights are multiplied by a power of two a warp so that the largest
-// scale of V seen is near 2^5 and at most 2^9 (rescaled like the sums when a
-// larger one comes; a weight is at most 2^kSlack): a second term then still
-// holds 2^-30 of the largest weight.
+// The weights are multiplied by a power of two a head so that the largest
+// product of a weight and a scale of V that the head has had is between 2^-2 and
+// 2^9 (up to 2^15 with the slack; rescaled like the sums when a scale comes that
+// might exceed it): two terms then hold 2^-23 of it.  The scales alone do not
+// tell: a key with large values and no weight must not push the others below
+// what fp16 holds.
 //
 // Each warp has a ring of pages of its own in shared memory.  One lane fetches
 // a page with two copies of the asynchronous copy engine, the codes as a tile
@@ -653,9 +655,11 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
     // qs (> 0) takes them to log2.  m is a maximum of theirs that lies at most
     // kSlack / qs below the true one, mq = m * qs.
     float m[NT], mq[NT], limit[NT], l[NT], zsum[NT], o[NT][T::kMTiles][4];
-    float vf = __uint_as_float(247u << 23);  // the weights' power of two
+    float vf[NT], most[NT];  // the weights' power of two, and the largest weight (relative to m) times scale of V
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
+      vf[nt] = __uint_as_float(247u << 23);
+      most[nt] = 0.0f;
       m[nt] = mq[nt] = limit[nt] = -INFINITY;
       l[nt] = zsum[nt] = 0.0f;
 #pragma unroll
@@ -739,23 +743,15 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
               for (int nt = 0; nt < NT; ++nt) raw[pg][nt][k] = -INFINITY;
             }
       }
-      float vtop = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
+      const float vtop = fmaxf(fmaxf(vs[0][0], vs[0][1]), fmaxf(vs[1][0], vs[1][1]));
       bool again = false;
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int nt = 0; nt < NT; ++nt) {
+        // a score above the slack, or a scale of V above what the weights' power of two allows
         again |= fmaxf(fmaxf(raw[0][nt][0], raw[0][nt][1]), fmaxf(raw[1][nt][0], raw[1][nt][1])) > limit[nt];
-      // a score above the slack, or a scale of V above what the weights' power of two allows
-      again |= __fmul_rn(vtop, vf) > 512.0f;
+        again |= __fmul_rn(vtop, vf[nt]) > 512.0f;
+      }
       if (__any_sync(0xffffffffu, again)) {
-#pragma unroll
-        for (int b = 4; b < 32; b <<= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, b));
-        float f = 1.0f;
-        if (__fmul_rn(vtop, vf) > 512.0f) {
-          const int e = min(max((int)(__float_as_uint(vtop) >> 23), 18), 255);
-          const float nf = __uint_as_float((uint32_t)(259 - e) << 23);
-          f = __fdiv_rn(nf, vf);
-          vf = nf;
-        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
           float top = fmaxf(fmaxf(raw[0][nt][0], raw[0][nt][1]), fmaxf(raw[1][nt][0], raw[1][nt][1]));
@@ -768,6 +764,23 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
             keep = exp2_approx(__fsub_rn(mq[nt], nq));
             mq[nt] = nq;
             limit[nt] = __fadd_rn(top, __fdiv_rn(kSlack, qs[nt]));
+          }
+          float p = 0.0f;  // the largest product here (one that is not a number is passed over)
+#pragma unroll
+          for (int pg = 0; pg < 2; ++pg)
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+              p = fmaxf(p, __fmul_rn(exp2_approx(__fmaf_rn(raw[pg][nt][k], qs[nt], -mq[nt])), vs[pg][k]));
+#pragma unroll
+          for (int b = 4; b < 32; b <<= 1) p = fmaxf(p, __shfl_xor_sync(0xffffffffu, p, b));
+          most[nt] = fmaxf(__fmul_rn(most[nt], keep), p);
+          const float now = __fmul_rn(most[nt], vf[nt]);
+          float f = 1.0f;
+          if (most[nt] > 0.0f && !(now >= 0.25f && now <= 512.0f)) {
+            const int e = min(max((int)(__float_as_uint(most[nt]) >> 23), 15), 252);
+            const float nf = __uint_as_float((uint32_t)(256 - e) << 23);  // the product near 2^2
+            f = __fdiv_rn(nf, vf[nt]);
+            vf[nt] = nf;
           }
           l[nt] = __fmul_rn(l[nt], keep);
           zsum[nt] = __fmul_rn(zsum[nt], keep);
@@ -788,7 +801,7 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
             const float w = exp2_approx(__fmaf_rn(raw[pg][nt][k], qs[nt], -mq[nt]));  // 0 behind the context
             l[nt] = __fadd_rn(l[nt], w);
             if constexpr (I4) zsum[nt] = __fmaf_rn(w, vz[pg][k], zsum[nt]);
-            wb[nt][k] = transpose8x8(two_terms(__fmul_rn(w, __fmul_rn(vs[pg][k], vf))));
+            wb[nt][k] = transpose8x8(two_terms(__fmul_rn(__fmul_rn(w, vs[pg][k]), vf[nt])));
           }
         // output
         // a register of V holds two bytes each of two positions, so that a widened pair is one dimension at two
@@ -830,7 +843,6 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
     }
 
     const bool begins = p0 == 0, ends = p1 == pages;
-    const float back = __fdiv_rn(I4 ? 1.0f / kNibbleUnit : 1.0f, vf);
     const int slot = begins && !ends ? 1 : 0;
     if (!begins) {
       note.has0 = 1;
@@ -850,6 +862,7 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
         if constexpr (I4) zsum[nt] = __fadd_rn(zsum[nt], __shfl_xor_sync(0xffffffffu, zsum[nt], b));
       }
       if (h >= heads) continue;
+      const float back = __fdiv_rn(I4 ? 1.0f / kNibbleUnit : 1.0f, vf[nt]);
       // the lane's dimensions: kRun from g * kRun of every 8 * kRun
       constexpr int kRun = I4 ? 4 : 2;
       float x[HD / 8];

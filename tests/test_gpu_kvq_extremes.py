@@ -96,6 +96,50 @@ def test_prompt_rows_do_not_feel_the_size_of_values_without_weight(cuda_backend,
 
 
 @pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("nh,heads,hd", [(32, 8, 128), (8, 1, 128), (8, 2, 96), (16, 2, 64), (4, 2, 32), (6, 2, 80)])
+@pytest.mark.parametrize("power", [30, 60])
+def test_single_rows_do_not_feel_the_size_of_values_without_weight(cuda_backend, power, nh, heads, hd, kv, io):
+    lens = [300, 20, 700, 5]
+    b = bench(cuda_backend, kv, heads, hd, lens, seed=power + hd)
+    skip = (3, 17, 250)
+    for s, n in enumerate(lens):
+        for p in skip:
+            if p < n:
+                far_below(b, s, p, power)
+    q = normal(b, 3, len(lens), nh, hd)
+    q[..., 0] = 4
+    q = q.flatten(1).to(DT[io])
+    for most in (700, 16 * b.c.per_seq):
+        out, lse = b.attend(q, nh, range(len(lens)), lens, max_len=most)
+        assert b.status.item() == 0
+        for s, n in enumerate(lens):
+            check_row(Without(b, skip), q[s], nh, s, n, out[s], lse[s])
+
+
+@pytest.mark.parametrize("kv", KINDS)
+def test_one_head_of_a_group_sees_large_values(cuda_backend, kv):
+    """Heads that share a kv head, of which one alone gives its weight to a key with values 2^50 times as large."""
+    hd, nh = 128, 4
+    b = bench(cuda_backend, kv, 1, hd, [2000], seed=4)
+    x = torch.zeros(hd, dtype=torch.float64, device=b.dev)
+    x[0] = -2000
+    put_row(b, 0, 0, 1000, x)
+    scale_rows(b, 1, 0, [1000], 2.0**50)
+    q = normal(b, 3, 1, nh, hd)
+    q[..., 0] = 4
+    q[:, 2, 0] = -4
+    out, lse = b.attend(q.flatten(1), nh, [0], [2000])
+    # its weight is 1, held to 2^-22; an I4 value's two parts and the five roundings on the way are below 2^-20 more
+    v = b.c.rows(1, 0, [1000])[0, 0]
+    assert ((out.view(nh, hd)[2].double() - v).abs() <= 2.0**-19 * v.abs().max()).all()
+    one = Without(b, (1000,))
+    ref, _, bound = R.attention(one, q[0].double(), 0, 2000)
+    for h in (0, 1, 3):
+        assert ((out.view(nh, hd)[h].double() - ref[h]).abs() <= bound[h]).all()
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
 @pytest.mark.parametrize("hd", [128, 96, 64, 32, 80])
 @pytest.mark.parametrize("zero,scale", [(22, None), (30, None), (54, None), (78, None), (60, -60), (40, 0), (-90, None)])
 def test_constant_and_nearly_constant_values(cuda_backend, zero, scale, hd, io):
