@@ -299,6 +299,9 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // the products as they are; q, and the output as it is written, are in the order
 // that this gives.
 // ---------------------------------------------------------------------------
+// The tensor cores cut their f32 sums, 2^-25 of the result a page on average, so
+// every kSumPages pages they are added, rounded, to sums of a lane's own.
+constexpr int kSumPages = 32;
 constexpr int kMmaMaxWarps = 8;
 constexpr int kMmaShares = 296;  // two CTAs an SM with up to four heads a unit, else one
 template <int HD, bool I4, int NT>
@@ -654,7 +657,7 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
     // Scores stay in the units of the integer products times their scales;
     // qs (> 0) takes them to log2.  m is a maximum of theirs that lies at most
     // kSlack / qs below the true one, mq = m * qs.
-    float m[NT], mq[NT], limit[NT], l[NT], zsum[NT], o[NT][T::kMTiles][4];
+    float m[NT], mq[NT], limit[NT], l[NT], zsum[NT], o[NT][T::kMTiles][4], sum[NT][T::kMTiles][2];
     float vf[NT], most[NT];  // the weights' power of two, and the largest weight (relative to m) times scale of V
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -665,7 +668,7 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
 #pragma unroll
       for (int i = 0; i < T::kMTiles; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) o[nt][i][j] = 0.0f;
+        for (int j = 0; j < 4; ++j) o[nt][i][j] = sum[nt][i][j / 2] = 0.0f;
     }
 
     for (int i = 0; i < n_pages; i += 2) {
@@ -674,6 +677,17 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
         give_up(&gave_up, a.status);
         failed = true;
         break;
+      }
+      if (i % kSumPages == 0 && i > 0) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int k = 0; k < T::kMTiles; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+              sum[nt][k][j] = __fadd_rn(sum[nt][k][j], __fadd_rn(o[nt][k][2 * j], o[nt][k][2 * j + 1]));
+              o[nt][k][2 * j] = o[nt][k][2 * j + 1] = 0.0f;
+            }
       }
       const uint32_t src = mine_s + copies.take * (2 * T::kTile);
       const uint8_t* par = params + copies.take * (2 * kParStride);
@@ -789,6 +803,10 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
           for (int k = 0; k < T::kMTiles; ++k)
 #pragma unroll
             for (int j = 0; j < 4; ++j) o[nt][k][j] = __fmul_rn(o[nt][k][j], keep);
+#pragma unroll
+          for (int k = 0; k < T::kMTiles; ++k)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) sum[nt][k][j] = __fmul_rn(sum[nt][k][j], keep);
         }
       }
 #pragma unroll
@@ -868,8 +886,8 @@ __global__ void __launch_bounds__(MmaTile<HD, I4, NT>::kWarps * 32, NT == 1 ? 2 
       float x[HD / 8];
 #pragma unroll
       for (int k = 0; k < T::kMTiles; ++k) {
-        x[2 * k] = __fmaf_rn(__fadd_rn(o[nt][k][0], o[nt][k][1]), back, zsum[nt]);
-        x[2 * k + 1] = __fmaf_rn(__fadd_rn(o[nt][k][2], o[nt][k][3]), back, zsum[nt]);
+        x[2 * k] = __fmaf_rn(__fadd_rn(sum[nt][k][0], __fadd_rn(o[nt][k][0], o[nt][k][1])), back, zsum[nt]);
+        x[2 * k + 1] = __fmaf_rn(__fadd_rn(sum[nt][k][1], __fadd_rn(o[nt][k][2], o[nt][k][3])), back, zsum[nt]);
       }
       if (begins && ends) {
         const float inv = __fdiv_rn(1.0f, l[nt]);

@@ -177,6 +177,31 @@ def test_values_that_are_all_zero_at_first(cuda_backend, hd, kv):
             check_row(b, q[i], nh, 0, i + 1, one[i], None)
 
 
+# ---- long sums ----------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("nh,heads,hd", [(32, 8, 128), (64, 8, 128), (48, 12, 64), (16, 8, 32), (20, 10, 96)])
+def test_long_sums_of_many_rows_keep_their_accuracy(cuda_backend, nh, heads, hd, kv):
+    """So many rows that a warp of the single-token kernel has a whole context of 500 pages to itself.
+
+    Tensor cores cut their f32 sums by 2^-24 of the sum on average at each addition, and a sum is on average half of
+    what it becomes: 2^-25 a page.  At most 64 pages follow one another before a sum is added, rounded, to the rest, so a
+    result is off by 2^-19, and its scores and weights within 2^-20: below 2^-18.4 = 3e-6.  Left in the tensor cores
+    for 500 pages a sum would be off by 1.5e-5."""
+    rows, n = 2400 // heads, 8000
+    b = bench(cuda_backend, kv, heads, hd, [n], seed=4)
+    q = normal(b, 5, rows, nh * hd)
+    out, lse = b.attend(q, nh, [0] * rows, [n] * rows)
+    assert b.status.item() == 0
+    at = [0, 7, rows // 2, rows - 1]
+    ref = []
+    for r in at:
+        check_row(b, q[r], nh, 0, n, out[r], lse[r])
+        ref.append(R.attention(b.c, q[r].double().view(nh, hd), 0, n)[0].flatten())
+    assert far(out[at], torch.stack(ref)) < 3e-6
+
+
 @pytest.mark.parametrize("kv", KINDS)
 @pytest.mark.parametrize("nh,heads,hd", [(32, 8, 128), (24, 8, 96), (32, 8, 64), (32, 8, 32)])
 def test_bf16_prompts_round_nothing_but_their_output(cuda_backend, nh, heads, hd, kv):
