@@ -32,8 +32,13 @@ namespace {
 // t = x / scale is off by less than 127 * 3 * 2^-24 < 2^-15, so rint(t) is the
 // code unless t lies that close to a border; there the quotient is taken in 64
 // bits, and the remainder of the code it gives (one fma, exact at a border)
-// decides.  Away from borders t is at most the largest code and a rounding.  A rotated element is held in 64 bits: its two products are exact
-// there and their sum is rounded once.
+// decides.  Away from borders t is at least the least code and at most the
+// largest, and a rounding, but for I4 rows of rotated K: an element is held in
+// 64 bits there (its two products are exact and their sum is rounded once) and the
+// row's zero in 32, so an element may lie below the zero by half of the zero's
+// last place, which is many codes where a row is nearly constant.  A t outside
+// the codes is sent to the same second look, which ends at the least or the
+// largest code.
 //
 // Bound, for many rows, by the loads that a warp waits for and its instructions
 // (some 500 for 16 elements a lane), for few by three dependent loads (position,
@@ -68,9 +73,12 @@ __device__ __forceinline__ float min_nan(float a, float b) {
   asm("min.NaN.f32 %0, %1, %2;\n" : "=f"(r) : "f"(a), "f"(b));
   return r;
 }
+// With BELOW it is raised, too, to how far the quotient lies outside [0, 15].
+template <bool BELOW>
 __device__ __forceinline__ uint32_t code_bits(float x, float inv, float* off) {
   const float t = __fmul_rn(x, inv), f = __fadd_rn(t, __uint_as_float(kCodeBits));
   *off = max_nan(*off, fabsf(__fsub_rn(t, __fsub_rn(f, __uint_as_float(kCodeBits)))));
+  if (BELOW) *off = max_nan(*off, __fsub_rn(fabsf(__fsub_rn(t, 7.5f)), 7.5f));
   return __float_as_uint(f);
 }
 
@@ -271,12 +279,12 @@ __global__ void __launch_bounds__(kStoreWarps * 32) kvq_store_kernel(KvqView c, 
       uint32_t bits[N];
       float off = 0.0f;
 #pragma unroll
-      for (int j = 0; j < N; ++j) bits[j] = code_bits(part(j), inv, &off);
+      for (int j = 0; j < N; ++j) bits[j] = code_bits<I4 && ROPE>(part(j), inv, &off);
       if (!(off < 0.4999f)) {
 #pragma unroll
         for (int j = 0; j < N; ++j) {
           float mine = 0.0f;
-          code_bits(part(j), inv, &mine);
+          code_bits<I4 && ROPE>(part(j), inv, &mine);
           if (!(mine < 0.4999f))
             bits[j] = kCodeBits + border_code((ROPE ? v[i][j] : (double)x[i][j]) - (double)zero, scale, I4 ? 0 : -127, I4 ? 15 : 127);
         }

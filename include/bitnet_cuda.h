@@ -483,8 +483,10 @@ int bitnet_cuda_model_attention_kernel(bitnet_cuda_model* model, bitnet_cuda_kv*
  *   parameters scale[16], zero[16].  zero = min x, scale = (max x - zero) / 15,
  *   both rounded to f32, c = (x - zero) / scale to the nearest (ties to even),
  *   value zero + c * scale.
- * Codes are the exact nearest ones.  A row that holds a NaN or an infinity
- * reads back as NaN.
+ * Codes are the exact nearest ones of their range, 0 where the scale is not above
+ * 0.  (A rotated element is not rounded to f32 before, so it may lie below the
+ * zero, and all of a nearly constant row may.)  A row that holds a NaN or an
+ * infinity reads back as NaN.
  *
  * The entry points below take device addresses, return without synchronising
  * and can be captured into a graph.  They leave the calling thread's current

@@ -222,3 +222,38 @@ def test_bf16_prompts_round_nothing_but_their_output(cuda_backend, nh, heads, hd
         ref.append(R.attention(b.c, q[r].double().view(nh, hd), 0, r + 1)[0].flatten())
     same = out[rows].double() == torch.stack(ref).float().to(torch.bfloat16).double()
     assert (~same).double().mean().item() < 0.01
+
+
+# ---- rows that are nearly constant ------------------------------------------------------------
+
+
+@pytest.mark.parametrize("many", [False, True])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("heads,hd", [(6, 128), (6, 32), (6, 80), (6, 6)])
+def test_store_of_rotated_rows_that_are_nearly_constant(cuda_backend, heads, hd, kv, many):
+    """A rotated element is held in 64 bits and its row's zero in 32, so elements may lie below the zero: they are the
+    least code.  Rows of a spread of 0 to 20 steps of 32 bits around 1.3 and 100, rotated by angles whose sine is 0."""
+    n = 1700 if many else 80
+    b = bench(cuda_backend, kv, heads, hd, [n], seed=3, fill="zeros")
+    g = torch.Generator(device=b.dev).manual_seed(hd)
+    base = torch.tensor([1.3, 100.0], device=b.dev).repeat(n // 2)[:, None, None]
+    step = 2.0**-23 * torch.tensor([1.0, 64.0], device=b.dev).repeat(n // 2)[:, None, None]
+    spread = torch.randint(0, 21, (n, heads, 1), device=b.dev, generator=g)
+    k = base + step * torch.floor(torch.rand(n, heads, hd, device=b.dev, generator=g) * (spread + 1))
+    k = k.flatten(1).contiguous()
+    v = torch.randn(n, heads * hd, device=b.dev, generator=g)
+    cos = (0.6 + 0.3 * torch.rand(n, 1, device=b.dev, generator=g)).repeat(1, hd // 2).contiguous()
+    sin = torch.zeros(n, hd // 2, device=b.dev)
+    b.store(k, v, [0] * n, list(range(n)), (cos.data_ptr(), sin.data_ptr(), n))
+    torch.cuda.synchronize()
+    assert b.status.item() == 0
+    p = torch.arange(n, device=b.dev)
+    kr = R.rotate(k.double().view(n, heads, hd), cos.double(), sin.double())
+    below = kr.amin(-1) < kr.amin(-1).float().double()
+    assert below.double().mean() > 0.2  # rows whose zero lies above their least element are among them
+    for kind, val in ((0, kr), (1, v.double().view(n, heads, hd))):
+        c, s, z = R.quantise(kv, val)
+        page, slot = b.c.table[0, p // 16].long(), p % 16
+        torch.testing.assert_close(b.c.params_view(kind)[page, :, 0, slot], s[..., 0].float(), rtol=0, atol=0)
+        data = c.to(torch.int8).view(torch.uint8) if kv == KV_I8 else (c[..., 0::2] | (c[..., 1::2] << 4)).to(torch.uint8)
+        torch.testing.assert_close(b.c.codes_view(kind)[page, :, slot], data, rtol=0, atol=0)
