@@ -631,8 +631,9 @@ int copy_logits(bitnet_cuda_model* m, int n_out, float* dst, cudaMemcpyKind kind
 
 // Name of the attention kernel run_forward launches for T tokens (same tests).
 const char* attention_kernel_name(const bitnet_cuda_model* m, const bitnet_cuda_kv* kv, int T, int max_ctx) {
-  if (kv->g.quant)  // T tokens of one sequence
-    return kvq_attend_kernel_name(kvq_layer(kv->g, kv->d_table, kv->max_seqs, 0), kvq_rows(m, T, 1), m->nh, false);
+  if (kv->g.quant)  // a token a sequence if there are as many, else T tokens of one
+    return kvq_attend_kernel_name(kvq_layer(kv->g, kv->d_table, kv->max_seqs, 0),
+                                  kvq_rows(m, T, T <= kv->max_seqs ? T : 1), m->nh, false);
   if (use_decode1(m, kv, T, max_ctx)) return "decode1_kernel";
   if (use_exact_attention(m, T) && use_x4_attention(m, kv, max_ctx)) return "attn_qk_softmax_kernel+attn_pv_kernel";
   if (use_exact_attention(m, T) && use_exact3_attention(m, kv, max_ctx)) return "paged_attention_exact3_kernel";

@@ -283,7 +283,8 @@ class BitNetModel:
         check(self._lib.bitnet_cuda_model_set_kernel_timing(self._h, 1 if enable else 0))
 
     def attention_kernel(self, kv: "KVCache", tokens: int = 1) -> str:
-        """Name of the attention kernel a step of `tokens` query tokens over `kv` launches."""
+        """Name of the attention kernel a step of `tokens` query tokens over `kv` launches (over a quantised cache: a
+        decode step when `kv` has that many sequences, else a prompt's)."""
         buf = C.create_string_buffer(64)
         check(self._lib.bitnet_cuda_model_attention_kernel(self._h, kv.handle, tokens, buf, 64))
         return buf.value.decode()

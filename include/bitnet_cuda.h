@@ -462,7 +462,10 @@ int bitnet_cuda_model_check(bitnet_cuda_model* model);
 /* Diagnostics (no counterpart in the reference): writes into `name` (NUL
  * terminated, at most name_len bytes) the name of the attention kernel that a
  * step of `tokens` query tokens over `kv` launches under the current numerics
- * mode, for contexts up to the cache's capacity. */
+ * mode, for contexts up to the cache's capacity.  Over a quantised cache a
+ * decode step and a prompt's step of as many tokens may launch different
+ * kernels: the name is the decode step's when the cache has `tokens` sequences
+ * or more, else that of a prompt of `tokens` tokens. */
 int bitnet_cuda_model_attention_kernel(bitnet_cuda_model* model, bitnet_cuda_kv* kv, uint32_t tokens, char* name,
                                        size_t name_len);
 

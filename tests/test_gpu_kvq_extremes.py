@@ -257,3 +257,20 @@ def test_store_of_rotated_rows_that_are_nearly_constant(cuda_backend, heads, hd,
         torch.testing.assert_close(b.c.params_view(kind)[page, :, 0, slot], s[..., 0].float(), rtol=0, atol=0)
         data = c.to(torch.int8).view(torch.uint8) if kv == KV_I8 else (c[..., 0::2] | (c[..., 1::2] << 4)).to(torch.uint8)
         torch.testing.assert_close(b.c.codes_view(kind)[page, :, slot], data, rtol=0, atol=0)
+
+
+# ---- in a model ---------------------------------------------------------------------------------
+
+
+def test_the_attention_kernel_of_decode_batches_is_named(cuda_backend):
+    """As many tokens as the cache has sequences, or fewer, may be a decode step's, a token a sequence; more are a
+    prompt's."""
+    cfg = ModelConfig(300, 2048, 1, 16, 8, 256, 700, 10000.0, 1e-5)
+    m = BitNetModel(synth.random_model(cfg, seed=3), cuda_backend, max_batch_tokens=512)
+    for kv in KINDS:
+        cache = m.new_kv_cache(num_pages=300, max_seqs=256, kv_dtype=kv)
+        for tokens in (1, 2, 80, 256):
+            assert m.attention_kernel(cache, tokens) == "kvq_attend_mma_kernel"
+        for tokens in (257, 512):
+            assert m.attention_kernel(cache, tokens) == "kvq_prompt_kernel"
+        cache.close()
