@@ -82,8 +82,9 @@ int check_attend(const KvqView& c, const void* q, size_t ldq, int bf16, size_t r
                  KvqAttend* a, int* bound) {
   if (n_heads == 0 || n_heads % c.kv_heads != 0)
     return shape_error("n_heads a multiple of kv_heads (" + sz(c.kv_heads) + ")", sz(n_heads));
-  if (n_heads * (size_t)c.hd > (size_t)INT_MAX || rows > (size_t)INT_MAX)
-    return shape_error("rows and n_heads * head_dim below 2^31", "more");
+  // the kernels' 32-bit row numbers go on by up to a grid, or a CTA's tokens, behind the last row
+  if (n_heads * (size_t)c.hd > (size_t)INT_MAX || rows > (size_t)INT_MAX - 1024)
+    return shape_error("n_heads * head_dim below 2^31, rows below 2^31 - 1024", "more");
   const size_t width = n_heads * (size_t)c.hd;
   BN_TRY(check_matrix(q, ldq, width, bf16, "q"));
   BN_TRY(check_matrix(out, ldo, width, bf16, "out"));
@@ -225,7 +226,7 @@ int bitnet_cuda_kv_prompt_attention_device(bitnet_cuda_ctx* ctx, const bitnet_cu
   int bound = 0;
   BN_TRY(check_attend(c, q, ldq, x_is_bf16, rows, n_heads, max_len, out, ldo, lse, workspace, workspace_bytes, status,
                       &a, &bound));
-  if (n_seqs > (size_t)INT_MAX) return shape_error("n_seqs below 2^31", sz(n_seqs));
+  if (n_seqs >= (size_t)1 << 30) return shape_error("n_seqs below 2^30", sz(n_seqs));
   BN_TRY(check_words(seq_ids, "seq_ids"));
   BN_TRY(check_words(cu_rows, "cu_rows"));
   BN_TRY(check_words(starts, "starts"));
