@@ -71,6 +71,7 @@ struct bitnet_cuda_model {
   // pinned staging
   int32_t* h_meta = nullptr;  // [4 * Tmax]: pos, seq, last_row, order (tokens by descending position); then `runs`
   uint32_t* h_tokens = nullptr;
+  cudaEvent_t staged = nullptr;  // after a step's copies out of the staging memory: the next step may write it then
   // captured decode graphs, keyed by (kv, batch, timed), with their kernel
   // counts and (when timed) the event pairs recorded around each launch
   struct Graph {
@@ -189,7 +190,7 @@ int check_scale(float s, const char* what) {
   return BITNET_OK;
 }
 
-int model_wait(bitnet_cuda_model* m, cudaStream_t st);
+int model_wait(bitnet_cuda_model* m, cudaStream_t st, cudaEvent_t ev = nullptr);
 
 // Ensure sequence `seq` has pages for positions [0, end); update the device table.
 int kv_reserve(bitnet_cuda_kv* kv, uint32_t seq, size_t end, cudaStream_t st) {
@@ -346,20 +347,20 @@ void tp_abort(bitnet_cuda_model* m) {
   m->tp_dead = true;
 }
 
-// Waits for st.  For a tensor-parallel model the wait also watches the
+// Waits for st, or for `ev` on it.  For a tensor-parallel model the wait also watches the
 // communicator: an asynchronous NCCL error, or no completion within
 // tp_timeout_ms (a peer that left or stopped), aborts the communicator.
-int model_wait(bitnet_cuda_model* m, cudaStream_t st) {
+int model_wait(bitnet_cuda_model* m, cudaStream_t st, cudaEvent_t ev) {
   if (!m->tp) {
-    BN_CUDA(cudaStreamSynchronize(st));
+    BN_CUDA(ev ? cudaEventSynchronize(ev) : cudaStreamSynchronize(st));
     return BITNET_OK;
   }
   if (m->tp_dead) return backend_error("the tensor-parallel communicator was aborted after an earlier failure");
   const auto t0 = std::chrono::steady_clock::now();
   for (;;) {
-    const cudaError_t e = cudaStreamQuery(st);
+    const cudaError_t e = ev ? cudaEventQuery(ev) : cudaStreamQuery(st);
     if (e == cudaSuccess) return BITNET_OK;
-    if (e != cudaErrorNotReady) return cuda_error(e, "cudaStreamQuery");
+    if (e != cudaErrorNotReady) return cuda_error(e, ev ? "cudaEventQuery" : "cudaStreamQuery");
     ncclResult_t ae = ncclSuccess;
     m->nc->comm_get_async_error(m->comm, &ae);
     const bool late = std::chrono::steady_clock::now() - t0 > std::chrono::milliseconds(m->tp_timeout_ms);
@@ -678,6 +679,8 @@ int prepare_batch(bitnet_cuda_model* m, bitnet_cuda_kv* kv, size_t n_seqs, const
     T += counts[i];
   }
   if (T > (size_t)m->Tmax) return shape_error("batch tokens <= " + sz(m->Tmax), sz(T));
+  // a step issued before may still have to copy its own metadata
+  BN_TRY(model_wait(m, st, m->staged));
   int max_ctx = 1;
   size_t t = 0;
   for (size_t i = 0; i < n_seqs; ++i) {
@@ -772,6 +775,7 @@ static void model_release(bitnet_cuda_model* m) {
   for (void* p : m->allocs) cudaFree(p);
   if (m->h_meta) cudaFreeHost(m->h_meta);
   if (m->h_tokens) cudaFreeHost(m->h_tokens);
+  if (m->staged) cudaEventDestroy(m->staged);
   m->partial.release();
   delete m;
   ctx_release(c);
@@ -1030,6 +1034,8 @@ int model_create_impl(bitnet_cuda_ctx* ctx, const bitnet_cuda_config* cfg, const
   if (e != cudaSuccess) return fail(cuda_error(e, "cudaMallocHost"));
   e = cudaMallocHost(&m->h_tokens, T * sizeof(uint32_t));
   if (e != cudaSuccess) return fail(cuda_error(e, "cudaMallocHost"));
+  e = cudaEventCreateWithFlags(&m->staged, cudaEventDisableTiming);
+  if (e != cudaSuccess) return fail(cuda_error(e, "cudaEventCreateWithFlags"));
   e = cudaMemsetAsync(m->status, 0, 64, ctx->stream);
   if (e != cudaSuccess) return fail(cuda_error(e, "cudaMemset"));
   e = cudaStreamSynchronize(ctx->stream);
@@ -1295,6 +1301,7 @@ static int forward_common(bitnet_cuda_model* m, bitnet_cuda_kv* kv, size_t n_seq
   std::memcpy(m->h_tokens, tokens, (size_t)T * 4);
   BN_CUDA(cudaMemcpyAsync(m->tokens, m->h_tokens, (size_t)T * 4, cudaMemcpyHostToDevice, st));
   BN_TRY(upload_meta(m, kv, T, (int)n_seqs, st));
+  BN_CUDA(cudaEventRecord(m->staged, st));
   run_forward(m, kv, T, (int)n_seqs, max_ctx, st);
   BN_CUDA(cudaGetLastError());
   if (logits) BN_TRY(copy_logits(m, (int)n_seqs, logits, cudaMemcpyDeviceToHost, st));
@@ -1358,6 +1365,7 @@ static int decode_graph(bitnet_cuda_model* m, bitnet_cuda_kv* kv, size_t batch, 
   } else {
     BN_CUDA(cudaMemcpyAsync(m->tokens, src, (size_t)T * 4, cudaMemcpyDeviceToDevice, st));
   }
+  BN_CUDA(cudaEventRecord(m->staged, st));
   if (m->tp_dead) return backend_error("the tensor-parallel communicator was aborted after an earlier failure");
   auto key = std::make_tuple((void*)kv, T, m->timing ? 1 : 0);
   auto it = m->graphs.find(key);
