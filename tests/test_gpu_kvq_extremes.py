@@ -274,3 +274,80 @@ def test_the_attention_kernel_of_decode_batches_is_named(cuda_backend):
         for tokens in (257, 512):
             assert m.attention_kernel(cache, tokens) == "kvq_prompt_kernel"
         cache.close()
+
+
+# ---- forms that no other test meets -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [128, 64])
+def test_prompts_of_many_runs(cuda_backend, hd, kv, io):
+    """More runs than a warp has lanes, empty ones among them."""
+    heads, nh, runs = 8, 32, 75
+    counts = [(7 * i) % 40 if i % 9 else 0 for i in range(runs)]
+    starts = [(13 * i) % 90 for i in range(runs)]
+    seqs = [(31 * i) % runs for i in range(runs)]
+    lens = [0] * runs
+    for c, s, i in zip(counts, starts, seqs):
+        lens[i] = c + s
+    b = bench(cuda_backend, kv, heads, hd, lens, seed=hd)
+    cu = [0]
+    for c in counts:
+        cu.append(cu[-1] + c)
+    q = normal(b, 5, cu[-1], nh * hd).to(DT[io])
+    out, lse = b.prompt(q, nh, seqs, cu, starts)
+    assert b.status.item() == 0 and (out != 77.0).all()
+    for i in list(range(0, runs, 6)) + [31, 32, 33, 63, 64, 65, runs - 1]:
+        for j in sorted({0, counts[i] // 2, counts[i] - 1}):
+            if 0 <= j < counts[i]:
+                check_row(b, q[cu[i] + j], nh, seqs[i], starts[i] + j + 1, out[cu[i] + j], lse[cu[i] + j],
+                          fp16_weights=io == "bf16")
+
+
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("nh,heads,hd", [(8, 2, 100), (6, 3, 112), (4, 1, 256), (9, 1, 80)])
+def test_other_head_sizes(cuda_backend, nh, heads, hd, kv, io):
+    """Stored, read back and attended to with head sizes of the simple kernel, a prompt of 400 rows among them."""
+    n = 400
+    b = bench(cuda_backend, kv, heads, hd, [n, 77], fill="zeros")
+    k, v, q = normal(b, 1, n, heads * hd), normal(b, 2, n, heads * hd), normal(b, 3, n, nh * hd).to(DT[io])
+    b.store(k, v, [0] * n, list(range(n)))
+    b.store(v[:77], k[:77], [1] * 77, list(range(77)))
+    kb, vb = torch.zeros_like(k), torch.zeros_like(v)
+    b.load(kb, vb, [0] * n, list(range(n)))
+    out, lse = b.prompt(q, nh, [0], [0, n], [0])
+    one, lse1 = b.attend(q[:3], nh, [1, 0, 1], [77, 399, 16])
+    assert b.status.item() == 0
+    for kind, x, back in ((0, k, kb), (1, v, vb)):
+        c, s, z = R.quantise(kv, x.double().view(n, heads, hd))
+        torch.testing.assert_close(back, (c.double() * s + z).flatten(1).float(), rtol=0, atol=0)
+    for i in (0, 15, 16, 255, 330, n - 1):
+        check_row(b, q[i], nh, 0, i + 1, out[i], lse[i])
+    for i, (seq, length) in enumerate(((1, 77), (0, 399), (1, 16))):
+        check_row(b, q[i], nh, seq, length, one[i], lse1[i])
+
+
+@pytest.mark.parametrize("kv", KINDS)
+def test_tensor_parallel_rank_over_a_quantised_cache(cuda_backend, kv):
+    """The tensor-parallel form of the model's steps (a rank of one) over a quantised cache, bit for bit the plain one's."""
+    from bitnetrs_b200 import tp
+
+    cfg = ModelConfig(1000, 512, 2, 4, 2, 768, 256, 10000.0, 1e-5)
+    w = synth.random_model(cfg, seed=21)
+    prompts = [[(11 * i + 7 * j) % cfg.vocab_size for j in range(n)] for i, n in enumerate((5, 70, 9))]
+    got = []
+    for rank in (None, tp.TensorParallel(0, 1, tp.unique_id())):
+        m = BitNetModel(w, cuda_backend, max_batch_tokens=128, tp=rank)
+        cache = m.new_kv_cache(num_pages=64, max_seqs=3, kv_dtype=kv)
+        nxt, logits = m.prefill(cache, [0, 1, 2], prompts, want_logits=True)
+        got.append([logits, nxt])
+        for _ in range(4):
+            nxt, logits = m.decode_step(cache, [0, 1, 2], nxt, want_logits=True)
+            got[-1] += [logits, nxt]
+        got[-1] += list(cache.read(1, 74))
+        cache.close()
+        m.close()
+    for a, b in zip(*got):
+        np.testing.assert_array_equal(a, b)
