@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kPlainWarps * 32)
 // Measured on a batch of 256 contexts of 128 to 4096 (20 heads over 5, heads of
 // 128, I8), with the same bytes asked for ahead: copies by each lane (cp.async)
 // stop at 4.0 TB/s, since a load that goes through L1 needs an entry there
-// until it lands; the ring takes 129 us, 5.2 TB/s, and 100003 positions of one
+// until it lands; the ring takes 131 us, 5.1 TB/s, and 100003 positions of one
 // sequence as I4 43 us, 2.7 TB/s, where instructions and the ends are the bound.
 //
 // Here the line of pages is cut into equal shares for the warps, not the
@@ -1103,7 +1103,11 @@ size_t kvq_attend_space(int nh, int kv_heads, int hd) {
 namespace {
 // Units of at most this many positions, and no more of them than CTAs, are taken
 // by a CTA each: its warps' pages take less time than a second kernel, which
-// joins what several CTAs leave (some 4 us against 0.35 us a page and warp).
+// joins what several CTAs leave.  Measured (whole, cut; us): heads of 128, I8, 5
+// units of 1024 positions 16 and 18, of 2048 23 and 20; 40 units 14 and 23, 25 and
+// 25; 165 units 23 and 29, 33 and 39.  So whole units are the faster way up to 1024
+// positions always, and beyond where there are many of them, which this rule
+// leaves to the cut.
 constexpr int kWholeUnits = 1024;
 constexpr int kMinWeight = kUnitCost + 1;  // the least share of a warp
 

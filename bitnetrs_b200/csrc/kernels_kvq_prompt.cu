@@ -6,7 +6,7 @@
 // in tiles of 64 with one pass of the softmax:
 //   S[row][key] = Q . K codes        tcgen05.mma, M 128, N 64
 //   O[row][dim] += W . V codes       tcgen05.mma, M 128, N head_dim
-// The pages of a tile come as they lie (one bulk copy each) and all threads
+// The pages of a tile come as they lie (one bulk copy each) and three warps
 // widen their codes to fp16, in which they are exact, into tiles of 128-byte
 // lines (128-byte swizzle).  One image serves both products: keys by
 // dimensions, the contraction along a line for S and across the lines for O.
@@ -19,7 +19,7 @@
 // the weights W are for both types, each product being two on the same sums.
 // Weights of one term (2^-11) move a result by some 2e-4, which a tenth and more
 // of the bf16 outputs show; the second term costs bf16 rows 309 against 268 us
-// (4 ragged prompts, I4, as below).
+// (the 4 ragged prompts below, I4).
 //
 // Warps 0-3 weigh: a thread reads its row of S, writes W over it as the A
 // operand of the second product, and rescales its row of O only when a score
@@ -55,15 +55,16 @@
 // pages.  With two tiles, as I8 would have, pages come too late: 275 against
 // 267 us for 4 ragged prompts, 4500 rows in all of 32 heads of 128 over 8 (bf16)
 // behind up to 1900 positions; I4 gains, 281 to 265 us, and heads of 64 232 to
-// 195 us.  The same as f32 rows over I4 take 470 us, and 1024 f32 rows of 20
-// heads over 5 (I8) 49 us.
+// 195 us (all with weights of one term).  Those prompts take 310 us over I4, 294
+// over I8, 242 with heads of 64 and 489 as f32 rows; 1024 f32 rows of 20 heads
+// over 5 (I8) take 52 us.
 //
-// What bounds it: the handshakes of a tile, S, weights, O, one after the other
-// (some 3000 cycles by itself, 2200 a CTA with two on an SM), with half of the
-// SM's issue slots in use and a fifth of the tensor cores' time.  Not faster
-// were: the weights by eight warps (305 to 325 us), rows spread over
-// four lanes so that a key's parameters serve four of them (307 to 324 us), and
-// f32 sums brought to the output 32 or 64 dimensions at a time (470 to 509 us).
+// What bounds it: the handshakes of a tile, S, weights, O, one after the other,
+// with half of the SM's issue slots in use and three tenths of the tensor cores'
+// time.  Not faster were (weights of one term): the weights by eight warps (305
+// to 325 us), rows spread over four lanes so that a key's parameters serve four of
+// them (307 to 324 us), and f32 sums brought to the output 32 or 64 dimensions at
+// a time (470 to 509 us).
 //
 // Every wait is bounded; a CTA that gives up records it, waits (bounded) for
 // its copies and products and frees its tensor memory.
@@ -79,7 +80,10 @@ namespace {
 
 constexpr int kPromptRows = 128, kPromptThreads = 256, kWiden = 96, kKeys = 64, kTilePages = kKeys / kPage;
 constexpr uint32_t kTmemCols = 256;
-constexpr int kSumTiles = 8;  // f32 rows: tiles that are summed in tensor memory
+// f32 rows: tiles that are summed in tensor memory.  With 8 the error is 0.5 to 1.6
+// times that of f32 matrix products, with 4 it is 0.3 to 1.1 times and 1024 rows
+// take 72 against 64 us (cold caches).
+constexpr int kSumTiles = 8;
 
 template <int HD, bool I4, bool TWO>
 struct PromptTile {
@@ -839,9 +843,16 @@ void launch_prompt_of(const KvqView& c, const KvqRows& r, const KvqAttend& a, in
 // Runs of rows are taken here where that is the faster way.  For 64 positions
 // of every row's context a CTA of this kernel takes 1.6 us by itself and an SM
 // with two of them 1.2 us a CTA (f32 rows 2.4 and 2.1 us); the single-token
-// kernel takes 64 positions of one unit in 1.9 ns of the whole GPU (heads of
-// 128, up to four a unit).  Measured: 1024 f32 rows of a fresh prompt with 5
-// units 48 against 135 us; 32 rows behind 8000 positions 242 against some 60 us.
+// kernel takes 64 positions of one unit in 1.9 ns of the whole GPU.  These are
+// heads of 128, up to four a unit; smaller heads take less of both, so that the
+// two meet at about the same number of rows.  Measured (this kernel, the other;
+// 8 units, us): behind 8000 positions 64 rows 281 and 109, 128 rows 285 and 188,
+// 256 rows 293 and 352 (f32, I4, heads of 128), 64 rows 162 and 109, 128 rows 164
+// and 190 (bf16); fresh prompts of 64 rows 25 and 23 (f32), 21 and 25 (bf16), 512
+// rows 43 and 72 (f32).  128 rows behind 8000 positions with heads of 64 172 and
+// 125 (f32), 129 and 125 (bf16), with heads of 32 147 and 102, 129 and 102.  The
+// rule takes the faster of each but for bf16 rows: the fresh 64 (25) and the two
+// of 129.
 bool kvq_prompt_pays(const KvqView& c, const KvqRows& r, int nh, bool bf16) {
   if (!r.runs || (c.hd != 32 && c.hd != 64 && c.hd != 96 && c.hd != 128)) return false;
   const Units us = units_of(nh, c.kv_heads);

@@ -353,9 +353,9 @@ int bitnet_cuda_lm_head_i8_table(const uint16_t* embed_bf16, size_t rows, size_t
 /* Paged KV cache (replaces KVCache, model/src/lib.rs:118-315): num_pages pages
  * of 16 positions x all layers, shared by up to max_seqs sequences.  The
  * quantised types (no counterpart in the reference) take an even head_dim of
- * at most 256; attention over them runs split over the context in f32
- * accuracy under every numerics mode (the reference's operation order is
- * defined by its unquantised cache). */
+ * at most 256; attention over them runs split over the context under every
+ * numerics mode, with about the error of f32 sums (the reference's operation
+ * order is defined by its unquantised cache). */
 int bitnet_cuda_kv_create(bitnet_cuda_model* model, uint32_t num_pages, uint32_t max_seqs, int kv_dtype,
                           bitnet_cuda_kv** out);
 void bitnet_cuda_kv_destroy(bitnet_cuda_kv* kv);
@@ -550,10 +550,13 @@ int bitnet_cuda_kv_attention_workspace(const bitnet_cuda_kv_pages* cache, size_t
  *   lse[r][h] = log sum_j exp(q . k_j / sqrt(head_dim))   (optional, f32 [rows][n_heads]).
  * A row of length 0 (or less) gives zeros and -inf.  Several rows may name one
  * sequence.  No length may exceed max_len (a longer one is cut there and sets
- * the status).  Scores, softmax and sums are held to f32 accuracy, for keys
- * and values of up to 2^80 (above, they may overflow to infinities); with bf16
- * q and out (x_is_bf16 != 0) only the output is rounded.  The context is split
- * over the GPU by the lengths alone, so a call repeated gives the same bits. */
+ * the status).  Scores and weights are held to 22 bits or more, the softmax and
+ * the sums in f32: the error is about that of f32 matrix products (between a
+ * quarter and twice theirs, below 3e-6 of a result in norm), for keys and values
+ * of up to 2^80 (above, they may overflow to infinities) and results down to
+ * 2^-90 (below, they lose bits); with bf16 q and out (x_is_bf16 != 0) the output
+ * is rounded besides.  The context is split over the GPU by the lengths alone, so
+ * a call repeated gives the same bits. */
 int bitnet_cuda_kv_attention_device(bitnet_cuda_ctx* ctx, const bitnet_cuda_kv_pages* cache, const void* q, size_t ldq,
                                     int x_is_bf16, size_t rows, size_t n_heads, const int32_t* row_seq,
                                     const int32_t* row_len, size_t max_len, void* out, size_t ldo, float* lse,
