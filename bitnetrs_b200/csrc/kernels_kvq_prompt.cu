@@ -703,10 +703,15 @@ __global__ void __launch_bounds__(kPromptThreads, 2)
         cap = __int_as_float((136 - __reduce_max_sync(0xffffffffu, ev)) << 23);
         m = m_new;
         const float nq = __fsub_rn(m_at, (float)ev);
-        const float keep = mq == nq || m == -INFINITY ? 1.0f : exp2_approx(__fsub_rn(mq, nq));
+        const float step = __fsub_rn(mq, nq), keep = mq == nq || m == -INFINITY ? 1.0f : exp2_approx(step);
         mq = nq;
         limit = __fadd_rn(m, __fdiv_rn(kSlack, qs));
-        l = __fmul_rn(l, keep);
+        if (step < -100.0f) {  // values that grow so far leave nothing of the outputs before them, but their weights count
+          const float half_step = exp2_approx(__fmul_rn(0.5f, step));
+          l = __fmul_rn(__fmul_rn(l, half_step), half_step);
+        } else {
+          l = __fmul_rn(l, keep);
+        }
         zsum = __fmul_rn(zsum, keep);
         kept = __fmul_rn(kept, keep);
         if ((TWO ? j % kSumTiles != 0 : j > 0) && __any_sync(0xffffffffu, keep != 1.0f)) {

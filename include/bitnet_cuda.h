@@ -391,7 +391,9 @@ int bitnet_cuda_decode_step(bitnet_cuda_model* model, bitnet_cuda_kv* kv, size_t
 
 /* Device-resident decode step: seq_ids on the host (scheduler state),
  * tokens / next_tokens / logits in device memory.  next_tokens may alias
- * tokens.  Runs as one CUDA graph per batch size. */
+ * tokens.  Runs as one CUDA graph per batch size.  Returns before the step has
+ * run, but waits until the step before it has begun (its metadata and this
+ * step's go through one buffer). */
 int bitnet_cuda_decode_step_device(bitnet_cuda_model* model, bitnet_cuda_kv* kv, size_t batch,
                                    const uint32_t* seq_ids, const uint32_t* d_tokens, uint32_t* d_next_tokens,
                                    float* d_logits, void* stream);

@@ -177,6 +177,26 @@ def test_values_that_are_all_zero_at_first(cuda_backend, hd, kv):
             check_row(b, q[i], nh, 0, i + 1, one[i], None)
 
 
+@pytest.mark.parametrize("io", ["f32", "bf16"])
+@pytest.mark.parametrize("kv", KINDS)
+@pytest.mark.parametrize("hd", [128, 64, 32, 80])
+@pytest.mark.parametrize("at", [40, 64, 100])
+def test_values_that_grow_far(cuda_backend, at, hd, kv, io):
+    """Values near 2^-70 up to position `at`, near 2^75 from there on: the small ones no longer show in the output, but
+    their weights still share it."""
+    heads, nh, n = 8, 32, 200
+    b = bench(cuda_backend, kv, heads, hd, [n], seed=9)
+    scale_rows(b, 1, 0, range(at), 2.0**-70)
+    scale_rows(b, 1, 0, range(at, n), 2.0**75)
+    q = normal(b, 2, n, nh * hd).to(DT[io])
+    out, lse = b.prompt(q, nh, [0], [0, n], [0])
+    one, lse1 = b.attend(q, nh, [0] * n, list(range(1, n + 1)))
+    assert b.status.item() == 0
+    for i in (0, at - 1, at, at + 1, 127, 128, n - 1):
+        check_row(b, q[i], nh, 0, i + 1, out[i], lse[i], fp16_weights=io == "bf16")
+        check_row(b, q[i], nh, 0, i + 1, one[i], lse1[i])
+
+
 # ---- long sums ----------------------------------------------------------------------------
 
 
