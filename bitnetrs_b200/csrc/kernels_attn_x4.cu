@@ -156,7 +156,8 @@ __global__ void __launch_bounds__(kQkThreads, 3) attn_qk_softmax_kernel(
     for (int p0 = warp * 2; p0 < n; p0 += kQkRoundPages) {
       bool ok = mbar_wait(smem_u32(&full_bar[p0 % kQkSlots]), (p0 / kQkSlots) & 1, abort_p);
       if (ok && p0 + 1 < n) ok = mbar_wait(smem_u32(&full_bar[(p0 + 1) % kQkSlots]), ((p0 + 1) / kQkSlots) & 1, abort_p);
-      if (!ok) {
+      // agreed on by the warp, whose lanes go on together
+      if (!__all_sync(0xffffffffu, ok)) {
         give_up(abort_p, status);
         break;
       }
@@ -371,7 +372,7 @@ __global__ void __launch_bounds__(kPvThreads, 6) attn_pv_kernel(
     for (int h = 0; h < 4; ++h) o[h][0] = o[h][1] = 0.0f;
     for (int P = 0; P < n; ++P) {
       const int s = P % kPvSlots;
-      if (!mbar_wait(smem_u32(&full_bar[s]), (P / kPvSlots) & 1, abort_p)) {
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&full_bar[s]), (P / kPvSlots) & 1, abort_p))) {
         give_up(abort_p, status);
         break;
       }
